@@ -399,6 +399,39 @@ int mgs_delta_step(const void* q, const void* k, const void* v, const void* beta
                    const void* H_prev, void* y, void* H, int64_t B, int heads, int nh, int dk,
                    int dv, int dtype, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* Linear attention with a decay for each head (no counterpart in the
+ * reference). Per (batch, head), gamma_t = exp(log_gamma_t):
+ *   S_t = gamma_t S_{t-1} + k_t v_t^T,   y_t = S_t^T q_t,   S_0 = H0, H_T = S_T.
+ * Q, K (B, H, T, dk), V, y (B, H, T, dv) in the op dtype with any batch, head
+ * and time strides and a dense last dimension; log_gamma (B, H, T) fp32 with
+ * any strides, <= 0 (-inf: the state is wiped); H0, H_T (B, H, dk, dv) fp32,
+ * C-contiguous. H0 may be NULL (zeros).
+ * `strides` (host memory) holds batch, head and time strides in elements, three
+ * to a tensor: forward Q, K, V, log_gamma, y; backward Q, K, V, log_gamma, dy,
+ * dQ, dK, dV. Rows that start on 16 bytes and hold a multiple of 8 elements are
+ * read and written in vectors, others element by element.
+ * Envelope: dk, dv <= 128 for bf16, <= 64 for fp32 and fp16 (both dimensions
+ * are linear: a wider head is a sum over blocks of dk and a concatenation over
+ * blocks of dv). The size queries return 0 outside it, the entry points
+ * MGS_UNSUPPORTED.
+ * `saved` (mgs_linear_attn_saved_size bytes, 16-byte aligned) takes the states
+ * at the chunks' starts for the backward; NULL: no backward follows.        */
+size_t mgs_linear_attn_workspace_size(int64_t B, int H, int64_t T, int dk, int dv, int dtype);
+size_t mgs_linear_attn_saved_size(int64_t B, int H, int64_t T, int dk, int dv, int dtype);
+int mgs_linear_attn_fwd(const void* Q, const void* K, const void* V, const float* log_gamma,
+                        const float* H0, void* y, float* H_T, float* saved, const int64_t* strides,
+                        int64_t B, int H, int64_t T, int dk, int dv, int dtype, void* workspace,
+                        size_t workspace_bytes, void* stream);
+/* Backward: (dQ, dK, dV, dlog_gamma, dH0) of sum(y * dy) + sum(H_T * dH_T).
+ * dlog_gamma (B, H, T) fp32 C-contiguous; dH_T may be NULL (zeros), dH0 NULL
+ * (not wanted). */
+int mgs_linear_attn_bwd(const void* Q, const void* K, const void* V, const float* log_gamma,
+                        const float* saved, const void* dy, const float* dH_T, void* dQ, void* dK,
+                        void* dV, float* dlog_gamma, float* dH0, const int64_t* strides, int64_t B,
+                        int H, int64_t T, int dk, int dv, int dtype, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

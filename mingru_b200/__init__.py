@@ -7,6 +7,7 @@ B200 kernels of ``libmingru_scan.so`` through its C ABI
 fallback: CPU tensors raise.
 """
 
+from .attn_ops import linear_attention
 from .modules import (
     DeltaMinGRU,
     GivensMinGRU,
@@ -53,4 +54,5 @@ __all__ = [
     "parallel_scan_log",
     "raise_device_error",
     "take_device_error",
+    "linear_attention",
 ]

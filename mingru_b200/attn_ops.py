@@ -1,0 +1,232 @@
+"""Linear attention with a decay for each head, on the sm_100a kernels.
+
+Per (batch, head), with ``gamma_t = exp(log_gamma_t)``::
+
+    S_t = gamma_t S_{t-1} + k_t v_t^T        (d_k x d_v, fp32)
+    y_t = S_t^T q_t
+
+:func:`linear_attention` runs whole sequences (forward and backward);
+``step_ops.linear_attention_step`` is the same recurrence for single tokens.
+No counterpart in the reference, whose matrix-state mixer is the delta rule;
+this is the recurrence that rule is without its correction, ``k^T S`` taken
+from ``v``.
+
+As the scan ops: CUDA tensors only, ``ValueError`` for what is outside the
+kernels' envelope, ``torch.library`` custom ops for ``torch.compile``, no
+second-order autograd.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .scan_ops import _dense, _dtype_code, _ptr, _require_cuda, _stream, _workspace
+
+__all__ = ["linear_attention"]
+
+_OP = "linear_attention"
+_MAX_D = {torch.bfloat16: 128, torch.float32: 64, torch.float16: 64}  # d_k, d_v of one kernel call
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """A dense last dimension; the other strides are the kernels' business."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _strides(*ts: torch.Tensor):
+    flat = [s for t in ts for s in t.stride()[:3]]
+    return (ctypes.c_int64 * len(flat))(*flat)
+
+
+def _saved_floats(Q: torch.Tensor, V: torch.Tensor) -> int:
+    B, H, T, dk = Q.shape
+    return _lib.load().mgs_linear_attn_saved_size(B, H, T, dk, V.shape[3], _dtype_code(_OP, Q)) // 4
+
+
+def _forward(Q, K, V, lg, H0, save):
+    lib = _lib.load()
+    with torch.cuda.device(Q.device):  # sizes are queried on the launch device
+        Q, K, V = _rows(Q), _rows(K), _rows(V)
+        B, H, T, dk = Q.shape
+        dv = V.shape[3]
+        code = _dtype_code(_OP, Q)
+        y = torch.empty_like(V)
+        HT = torch.empty(B, H, dk, dv, dtype=torch.float32, device=Q.device)
+        saved = torch.empty(_saved_floats(Q, V) if save else 0, dtype=torch.float32, device=Q.device)
+        if T == 0:  # no token: the state passes through
+            HT.zero_() if H0 is None else HT.copy_(H0)
+            return y, HT, saved
+        if H0 is not None:
+            H0 = _dense(H0)
+        n = lib.mgs_linear_attn_workspace_size(B, H, T, dk, dv, code)
+        ws = _workspace(n, Q.device) if n else None
+        st = lib.mgs_linear_attn_fwd(
+            _ptr(Q), _ptr(K), _ptr(V), _ptr(lg), _ptr(H0), _ptr(y), _ptr(HT),
+            _ptr(saved) if save else None, _strides(Q, K, V, lg, y), B, H, T, dk, dv, code, _ptr(ws), n,
+            _stream(Q),
+        )
+        _lib.check(st, f"{_OP} forward")
+        return y, HT, saved
+
+
+@torch.library.custom_op("mingru_b200::linear_attn_fwd", mutates_args=())
+def _linear_attn_fwd(
+    Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, lg: torch.Tensor, H0: torch.Tensor | None,
+    save: bool,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _forward(Q, K, V, lg, H0, save)
+
+
+@_linear_attn_fwd.register_fake
+def _(Q, K, V, lg, H0, save):
+    B, H, T, dk = Q.shape
+    return (torch.empty_like(V), Q.new_empty((B, H, dk, V.shape[3]), dtype=torch.float32),
+            Q.new_empty((_saved_floats(Q, V) if save else 0,), dtype=torch.float32))
+
+
+@torch.library.custom_op("mingru_b200::linear_attn_bwd", mutates_args=())
+def _linear_attn_bwd(
+    Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, lg: torch.Tensor, saved: torch.Tensor,
+    dy: torch.Tensor, dHT: torch.Tensor | None, want_dH0: bool,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    lib = _lib.load()
+    with torch.cuda.device(Q.device):  # sizes are queried on the launch device
+        Q, K, V, dy = (_rows(x) for x in (Q, K, V, dy.to(Q.dtype)))
+        B, H, T, dk = Q.shape
+        dv = V.shape[3]
+        code = _dtype_code(_OP, Q)
+        dQ, dK, dV = (torch.empty_like(x) for x in (Q, K, V))
+        dlg = torch.empty(B, H, T, dtype=torch.float32, device=Q.device)
+        dH0 = torch.empty((B, H, dk, dv) if want_dH0 else (0,), dtype=torch.float32, device=Q.device)
+        if dHT is not None:
+            dHT = _dense(dHT.float())
+        if T == 0:
+            if want_dH0:
+                dH0.zero_() if dHT is None else dH0.copy_(dHT)
+            return dQ, dK, dV, dlg, dH0
+        n = lib.mgs_linear_attn_workspace_size(B, H, T, dk, dv, code)
+        ws = _workspace(n, Q.device) if n else None
+        st = lib.mgs_linear_attn_bwd(
+            _ptr(Q), _ptr(K), _ptr(V), _ptr(lg), _ptr(saved), _ptr(dy), _ptr(dHT), _ptr(dQ), _ptr(dK),
+            _ptr(dV), _ptr(dlg), _ptr(dH0) if want_dH0 else None,
+            _strides(Q, K, V, lg, dy, dQ, dK, dV), B, H, T, dk, dv, code, _ptr(ws), n, _stream(Q),
+        )
+        _lib.check(st, f"{_OP} backward")
+        return dQ, dK, dV, dlg, dH0
+
+
+@_linear_attn_bwd.register_fake
+def _(Q, K, V, lg, saved, dy, dHT, want_dH0):
+    B, H, T, dk = Q.shape
+    f32 = dict(dtype=torch.float32)
+    return (torch.empty_like(Q), torch.empty_like(K), torch.empty_like(V), Q.new_empty((B, H, T), **f32),
+            Q.new_empty((B, H, dk, V.shape[3]) if want_dH0 else (0,), **f32))
+
+
+def _setup(ctx, inputs, output):
+    Q, K, V, lg, H0, _save = inputs
+    ctx.save_for_backward(Q, K, V, lg, output[2])
+    ctx.has_h0 = H0 is not None
+    ctx.mark_non_differentiable(output[2])
+    ctx.set_materialize_grads(False)
+
+
+def _backward(ctx, dy, dHT, _gsaved):
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{_OP} does not support second-order autograd (create_graph=True)")
+    Q, K, V, lg, saved = ctx.saved_tensors
+    if dy is None and dHT is None:
+        return (None,) * 6
+    if dy is None:
+        dy = torch.zeros_like(V)
+    want = ctx.has_h0 and ctx.needs_input_grad[4]
+    dQ, dK, dV, dlg, dH0 = _linear_attn_bwd(Q, K, V, lg, saved, dy, dHT, want)
+    return dQ, dK, dV, dlg, dH0 if want else None, None
+
+
+torch.library.register_autograd("mingru_b200::linear_attn_fwd", _backward, setup_context=_setup)
+
+
+def _blocks(d: int, width: int):
+    return [slice(i, min(d, i + width)) for i in range(0, d, width)]
+
+
+def _run(Q, K, V, lg, H0):
+    dk, dv = Q.shape[3], V.shape[3]
+    wide = _MAX_D[Q.dtype]
+    if max(dk, dv) <= wide:
+        if torch.compiler.is_compiling() or (
+                torch.is_grad_enabled()
+                and any(t is not None and t.requires_grad for t in (Q, K, V, lg, H0))):
+            return _linear_attn_fwd(Q, K, V, lg, H0, True)[:2]
+        return _forward(Q, K, V, lg, H0, False)[:2]  # nothing to differentiate: no dispatcher
+    if Q.dtype != torch.float32:
+        # Blocks of 16-bit inputs run on fp32 copies, so that their partial
+        # outputs and gradients are added before the one rounding.
+        y, HT = _run(Q.float(), K.float(), V.float(), lg, H0)
+        return y.to(Q.dtype), HT
+    # The recurrence is linear in k and q and separate in the columns of v: y
+    # adds up over blocks of d_k, and value columns are independent.
+    ys, hts = [], []
+    for j in _blocks(dv, wide):
+        parts = [_run(Q[..., i], K[..., i], V[..., j], lg, None if H0 is None else H0[:, :, i, j])
+                 for i in _blocks(dk, wide)]
+        ys.append(sum((y for y, _ in parts[1:]), parts[0][0]))
+        hts.append(torch.cat([h for _, h in parts], 2))
+    return torch.cat(ys, -1), torch.cat(hts, -1)
+
+
+def linear_attention(
+    Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, log_gamma: torch.Tensor,
+    H0: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Linear attention with a decay for each head; returns ``(y, H_T)``.
+
+    ``Q``, ``K`` ``(B, n_heads, T, d_k)``, ``V`` ``(B, n_heads, T, d_v)`` in
+    fp32, bf16 or fp16, ``log_gamma`` ``(B, n_heads, T)`` or broadcastable to
+    it (``(1, n_heads, 1)``: one decay for each head), ``H0`` ``(B, n_heads,
+    d_k, d_v)`` or ``None`` (zeros). ``y`` ``(B, n_heads, T, d_v)`` has the
+    inputs' dtype and ``V``'s memory order; the state ``H_T`` is fp32.
+    Differentiable w.r.t. all five tensors.
+
+    Batch, head and time strides are free: views such as ``(B, T, n_heads,
+    d).transpose(1, 2)`` or slices of one projection are read in place, and
+    gradients come in the same order. Any ``d_k``, ``d_v`` (heads wider than
+    128 in bf16, or 64 in fp32 and fp16, run as blocks, 16-bit ones on fp32
+    copies) and any ``T``, 0 included.
+
+    ``log_gamma <= 0``; ``-inf`` wipes the state before the token, which is how
+    packed sequences are kept apart. A decay below ``2^-128`` counts as a wipe
+    and its ``log_gamma`` gets no gradient. The products run on the tensor
+    cores over chunks of 128 tokens, so a non-finite value spreads to earlier
+    tokens of its own chunk (and to all later ones, as the recurrence has it).
+    """
+    if Q.ndim != 4 or K.ndim != 4 or V.ndim != 4:
+        raise ValueError(
+            f"{_OP}: need 4-D Q, K (B, n_heads, T, d_k) and V (B, n_heads, T, d_v); got ranks "
+            f"Q={Q.ndim}, K={K.ndim}, V={V.ndim}"
+        )
+    B, H, T, dk = Q.shape
+    dv = V.shape[3]
+    if K.shape != Q.shape or V.shape[:3] != Q.shape[:3] or dk < 1 or dv < 1:
+        raise ValueError(
+            f"{_OP}: shapes disagree: from Q={tuple(Q.shape)} expected K={tuple(Q.shape)} and "
+            f"V={(B, H, T, 'd_v')}, d_k, d_v >= 1; got K={tuple(K.shape)}, V={tuple(V.shape)}"
+        )
+    if H0 is not None and tuple(H0.shape) != (B, H, dk, dv):
+        raise ValueError(f"{_OP}: H0 must have shape {(B, H, dk, dv)} (got {tuple(H0.shape)})")
+    try:
+        lg = torch.broadcast_to(log_gamma, (B, H, T))
+    except RuntimeError:
+        raise ValueError(f"{_OP}: log_gamma must broadcast to {(B, H, T)} (got "
+                         f"{tuple(log_gamma.shape)})") from None
+    _require_cuda(_OP, Q, K, V, lg, *(() if H0 is None else (H0,)))
+    if K.dtype != Q.dtype or V.dtype != Q.dtype:
+        raise ValueError(f"{_OP}: Q, K and V must share a dtype")
+    _dtype_code(_OP, Q)
+    if not lg.is_floating_point() or not (H0 is None or H0.is_floating_point()):
+        raise ValueError(f"{_OP}: log_gamma and H0 must be floating point")
+    return _run(Q, K, V, lg.float(), None if H0 is None else H0.float())
