@@ -432,6 +432,40 @@ int mgs_linear_attn_bwd(const void* Q, const void* K, const void* V, const float
                         int H, int64_t T, int dk, int dv, int dtype, void* workspace,
                         size_t workspace_bytes, void* stream);
 
+/* One token of linear attention for every (b, head): S = exp(log_gamma) S_prev
+ * + k v^T, y = S^T q. q, k (B, H, dk), v, y (B, H, dv) op dtype and S, S_prev
+ * (B, H, dk, dv) fp32, C-contiguous; log_gamma fp32 with the given batch and
+ * head strides. S may be S_prev. */
+int mgs_linear_attn_step(const void* q, const void* k, const void* v, const float* log_gamma,
+                         int64_t lg_stride_b, int64_t lg_stride_h, const float* S_prev, void* y, float* S,
+                         int64_t B, int heads, int dk, int dv, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* The norms around a block (no counterpart in the reference, which runs torch's
+ * LayerNorm and adds). Per row of D channels in `groups` groups of n = D / groups:
+ *   h = residual + scale * x      (h = x without a residual; scale may be NULL: 1)
+ *   z = (h - mean) / sqrt(var + eps) per group   (rms != 0: h / sqrt(mean(h^2) + eps))
+ *   y = (z * weight + bias) * silu(gate)         (bias, gate may be NULL)
+ * x, residual, gate, y, h in `dtype`; weight, bias, scale (D) in `weight_dtype`
+ * (the same or fp32); fp32 arithmetic. row_strides (host memory, in elements):
+ * x, residual, gate, and for the backward dy, dh; outputs are dense. h is
+ * written only with a residual; stats (rows * groups * 3 floats) is what the
+ * backward reads, or NULL. Envelope: n <= 16384. */
+size_t mgs_block_norm_workspace_size(int64_t rows, int64_t D, int groups, int dtype); /* backward */
+int mgs_block_norm_fwd(const void* x, const void* residual, const void* gate, const void* weight,
+                       const void* bias, const void* scale, void* y, void* h, float* stats,
+                       const int64_t* row_strides, int64_t rows, int64_t D, int groups, int rms,
+                       float eps, int dtype, int weight_dtype, void* stream);
+/* Backward of sum(y * dy) + sum(h * dh); dh may be NULL. dresidual and dscale are
+ * written only with a scale (without one dresidual is dx), dgate only with a
+ * gate, dbias only with a bias. */
+int mgs_block_norm_bwd(const void* x, const void* residual, const void* gate, const void* weight,
+                       const void* bias, const void* scale, const float* stats, const void* dy,
+                       const void* dh, void* dx, void* dresidual, void* dgate, void* dweight, void* dbias,
+                       void* dscale, const int64_t* row_strides, int64_t rows, int64_t D, int groups,
+                       int rms, int dtype, int weight_dtype, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif

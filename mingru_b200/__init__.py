@@ -19,6 +19,7 @@ from .modules import (
     g,
     log_g,
 )
+from .norm_ops import block_norm
 from .scan_ops import (
     delta_gated_scan_impl,
     delta_scan_impl,
@@ -55,4 +56,5 @@ __all__ = [
     "raise_device_error",
     "take_device_error",
     "linear_attention",
+    "block_norm",
 ]

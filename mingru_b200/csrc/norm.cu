@@ -1,0 +1,518 @@
+// norm.cu -- the norms around a block: residual add with a scale for the branch
+// before a LayerNorm / RMS norm, and a norm per group of channels with a gate
+// after a mixer, one kernel forward and two backward.
+//
+// Per row, with groups of n = D / G channels (fp32 throughout, tensors rounded
+// once on the way out):
+//   h = residual + scale * x            (h = x without a residual)
+//   z = (h - mean) * r,  r = 1 / sqrt(mean((h - mean)^2) + eps)   (mean 0 for RMS)
+//   y = (z * weight + bias) * silu(gate)
+// Backward, da = dy * silu(gate), dz = da * weight, gh the gradient of h itself:
+//   dh = r (dz - mean(dz) - z mean(dz z)) + gh    (without mean(dz) for RMS)
+//   dx = scale * dh, dresidual = dh, dgate = dy * (z * weight + bias) * silu'(gate)
+//   dweight = sum da z, dbias = sum da, dscale = sum dh x     (over rows)
+//
+// Memory bound: the forward reads each input once and writes each output once,
+// a group's values staying in its threads' registers between the two
+// reductions; the backward reads the inputs again instead of z (and h is taken
+// in fp32 from x and residual, not from its rounded copy), with mean and r from
+// the forward. Sums over rows stay in the threads' registers while a CTA walks
+// its rows, then go through shared memory to one partial row per CTA and, in
+// order, to the result: the same bits on every run.
+#include "common.cuh"
+
+namespace mgs {
+namespace norm {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxGroup = 16384;  // 1024 threads of 16 values
+
+struct Args {
+  const void *x, *res, *gate, *w, *b, *s, *dy, *dh;
+  void *y, *h, *dx, *dres, *dgate;
+  float* stats;  // (rows * G, 3): mean, what it leaves, r
+  float* part;   // (3, grid, D): sums over a CTA's rows of dweight, dbias, dscale
+  long long ldx, ldres, ldgate, lddy, lddh;  // row strides of the inputs; outputs are dense
+  long long rows;
+  int D, G, n, tpg, gpc, rpc;  // threads to a group, groups and rows to a CTA
+  int rms;
+  float eps;
+};
+
+// VEC consecutive elements.
+template <typename T, int VEC>
+__device__ __forceinline__ void ldv(const void* p, long long i, float* v) {
+  const T* q = static_cast<const T*>(p) + i;
+  if constexpr (VEC == 1) {
+    v[0] = to_f32<T>(*q);
+  } else {
+    constexpr int kN = 16 / (int)sizeof(T) < VEC ? 16 / (int)sizeof(T) : VEC;
+#pragma unroll
+    for (int k = 0; k < VEC; k += kN) {
+      const uint4 u = __ldg(reinterpret_cast<const uint4*>(q + k));
+      const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+      for (int j = 0; j < kN; ++j) v[k + j] = to_f32<T>(e[j]);
+    }
+  }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void stv(void* p, long long i, const float* v) {
+  T* q = static_cast<T*>(p) + i;
+  if constexpr (VEC == 1) {
+    *q = from_f32<T>(v[0]);
+  } else {
+    uint4 u;
+    T* e = reinterpret_cast<T*>(&u);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) e[j] = from_f32<T>(v[j]);
+    *reinterpret_cast<uint4*>(q) = u;
+  }
+}
+
+// Sums over the tpg threads of a group: a segment of a warp, or whole warps
+// that meet at a named barrier of the group's own. `buf` alternates, so that
+// one barrier is enough for each sum.
+struct Reduce {
+  float2 (*red)[32];
+  int tpg, slot, buf;
+  __device__ __forceinline__ float2 operator()(float a, float b) {
+    const int lane = threadIdx.x & 31;
+    const int width = tpg < 32 ? tpg : 32;
+    const unsigned mask = width == 32 ? 0xffffffffu : ((1u << width) - 1) << (lane & ~(width - 1));
+    for (int o = width / 2; o > 0; o >>= 1) {
+      a += __shfl_xor_sync(mask, a, o);
+      b += __shfl_xor_sync(mask, b, o);
+    }
+    if (tpg > 32) {
+      const int nw = tpg / 32, w0 = slot * nw;
+      if (lane == 0) red[buf][threadIdx.x >> 5] = make_float2(a, b);
+      named_bar(1 + slot, tpg);
+      a = b = 0.f;
+      for (int w = 0; w < nw; ++w) {
+        const float2 f = red[buf][w0 + w];
+        a += f.x;
+        b += f.y;
+      }
+      buf ^= 1;
+    }
+    return make_float2(a, b);
+  }
+};
+
+__device__ __forceinline__ float sigm(float x) { return 1.f / (1.f + __expf(-x)); }
+
+// Where a thread stands: its group (of the row), row slot and first column.
+struct Place {
+  int slot, rs, g, t;
+  bool on;
+  __device__ explicit Place(const Args& p) {
+    slot = (int)threadIdx.x / p.tpg;
+    t = (int)threadIdx.x % p.tpg;
+    rs = slot / p.gpc;
+    g = blockIdx.y * p.gpc + slot % p.gpc;
+    on = rs < p.rpc && g < p.G;
+  }
+};
+
+template <typename E, typename W, int VEC, int K, int MAXT>
+__global__ void __launch_bounds__(MAXT) fwd_kernel(const Args p) {
+  __shared__ float2 red[2][32];
+  const Place at(p);
+  if (!at.on) return;
+  Reduce sum{red, p.tpg, at.slot, 0};
+  const float inv_n = 1.f / (float)p.n;
+  for (long long row = (long long)blockIdx.x * p.rpc + at.rs; row < p.rows;
+       row += (long long)gridDim.x * p.rpc) {
+    float h[K * VEC];
+    float acc = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * p.tpg + at.t) * VEC, col = at.g * p.n + c;
+      float* v = h + k * VEC;
+      if (c < p.n) {
+        ldv<E, VEC>(p.x, row * p.ldx + col, v);
+        if (p.res) {
+          float r[VEC];
+          ldv<E, VEC>(p.res, row * p.ldres + col, r);
+          if (p.s) {
+            float s[VEC];
+            ldv<W, VEC>(p.s, col, s);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v[i] = fmaf(s[i], v[i], r[i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v[i] += r[i];
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) acc += v[i];
+    }
+    // The fp32 mean is off by up to half a unit of its last place: what it leaves in the
+    // differences, `rest`, is their own mean, and comes with the sum of their squares.
+    const float mean = p.rms ? 0.f : sum(acc, 0.f).x * inv_n;
+    float sq = 0.f, rs = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const bool in = (k * p.tpg + at.t) * VEC < p.n;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float d = in ? h[k * VEC + i] - mean : 0.f;
+        sq = fmaf(d, d, sq);
+        rs += d;
+      }
+    }
+    const float2 m = sum(sq, rs);
+    const float rest = p.rms ? 0.f : m.y * inv_n;
+    const float r = rsqrtf(fmaxf(fmaf(-rest, rest, m.x * inv_n), 0.f) + p.eps);
+    if (p.stats && at.t == 0) {
+      float* st = p.stats + (row * p.G + at.g) * 3;
+      st[0] = mean, st[1] = rest, st[2] = r;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * p.tpg + at.t) * VEC, col = at.g * p.n + c;
+      if (c >= p.n) continue;
+      const long long o = row * p.D + col;
+      if (p.h) stv<E, VEC>(p.h, o, h + k * VEC);
+      float y[VEC], w[VEC];
+      ldv<W, VEC>(p.w, col, w);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) y[i] = ((h[k * VEC + i] - mean) - rest) * r * w[i];
+      if (p.b) {
+        ldv<W, VEC>(p.b, col, w);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) y[i] += w[i];
+      }
+      if (p.gate) {
+        ldv<E, VEC>(p.gate, row * p.ldgate + col, w);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) y[i] *= w[i] * sigm(w[i]);
+      }
+      stv<E, VEC>(p.y, o, y);
+    }
+  }
+}
+
+template <typename E, typename W, int VEC, int K, int MAXT>
+__global__ void __launch_bounds__(MAXT) bwd_kernel(const Args p) {
+  __shared__ float2 red[2][32];
+  extern __shared__ float cols[];
+  const Place at(p);
+  Reduce sum{red, p.tpg, at.slot, 0};
+  const float inv_n = 1.f / (float)p.n;
+  float gw[K * VEC], gb[K * VEC], gs[K * VEC];
+#pragma unroll
+  for (int i = 0; i < K * VEC; ++i) gw[i] = gb[i] = gs[i] = 0.f;
+  if (at.on) {
+    for (long long row = (long long)blockIdx.x * p.rpc + at.rs; row < p.rows;
+         row += (long long)gridDim.x * p.rpc) {
+      const float* st = p.stats + (row * p.G + at.g) * 3;
+      const float mean = st[0], rest = st[1], r = st[2];
+      float z[K * VEC], dz[K * VEC], x[K * VEC];
+      float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int c = (k * p.tpg + at.t) * VEC, col = at.g * p.n + c;
+        const int e = k * VEC;
+        if (c >= p.n) continue;
+        float a[VEC], w[VEC];
+        ldv<E, VEC>(p.x, row * p.ldx + col, x + e);
+        ldv<E, VEC>(p.dy, row * p.lddy + col, dz + e);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) z[e + i] = x[e + i];
+        if (p.res) {
+          ldv<E, VEC>(p.res, row * p.ldres + col, a);
+          if (p.s) {
+            ldv<W, VEC>(p.s, col, w);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) z[e + i] = fmaf(w[i], z[e + i], a[i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) z[e + i] += a[i];
+          }
+        }
+        ldv<W, VEC>(p.w, col, w);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) z[e + i] = ((z[e + i] - mean) - rest) * r;
+        if (p.gate) {
+          float gt[VEC], b[VEC];
+          ldv<E, VEC>(p.gate, row * p.ldgate + col, gt);
+          if (p.b) ldv<W, VEC>(p.b, col, b);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            const float sg = sigm(gt[i]), o = fmaf(z[e + i], w[i], p.b ? b[i] : 0.f), d = dz[e + i];
+            a[i] = d * o * sg * fmaf(gt[i], 1.f - sg, 1.f);
+            dz[e + i] = d * gt[i] * sg;
+          }
+          stv<E, VEC>(p.dgate, row * p.D + col, a);
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          gw[e + i] = fmaf(dz[e + i], z[e + i], gw[e + i]);
+          gb[e + i] += dz[e + i];
+          dz[e + i] *= w[i];
+          s1 += dz[e + i];
+          s2 = fmaf(dz[e + i], z[e + i], s2);
+        }
+      }
+      const float2 m = sum(s1, s2);
+      const float m1 = p.rms ? 0.f : m.x * inv_n, m2 = m.y * inv_n;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int c = (k * p.tpg + at.t) * VEC, col = at.g * p.n + c;
+        const int e = k * VEC;
+        if (c >= p.n) continue;
+        float d[VEC], a[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) d[i] = r * (dz[e + i] - m1 - z[e + i] * m2);
+        if (p.dh) {
+          ldv<E, VEC>(p.dh, row * p.lddh + col, a);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) d[i] += a[i];
+        }
+        if (p.s) {
+          stv<E, VEC>(p.dres, row * p.D + col, d);
+          ldv<W, VEC>(p.s, col, a);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            gs[e + i] = fmaf(d[i], x[e + i], gs[e + i]);
+            d[i] *= a[i];
+          }
+        }
+        stv<E, VEC>(p.dx, row * p.D + col, d);
+      }
+    }
+  }
+  // the CTA's rows: one partial row of each sum
+  const int width = p.gpc * p.n;  // columns of this CTA
+  for (int q = 0; q < 3; ++q) {
+    if ((q == 1 && !p.b) || (q == 2 && !p.s)) continue;
+    __syncthreads();
+    if (at.on) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int c = (k * p.tpg + at.t) * VEC;
+        if (c >= p.n) continue;
+        float* o = cols + (long long)at.rs * width + (at.slot % p.gpc) * p.n + c;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) o[i] = q == 0 ? gw[k * VEC + i] : q == 1 ? gb[k * VEC + i] : gs[k * VEC + i];
+      }
+    }
+    __syncthreads();
+    const int first = blockIdx.y * width;
+    for (int c = threadIdx.x; c < width && first + c < p.D; c += blockDim.x) {
+      float a = 0.f;
+      for (int i = 0; i < p.rpc; ++i) a += cols[i * width + c];
+      p.part[((long long)q * gridDim.x + blockIdx.x) * p.D + first + c] = a;
+    }
+  }
+}
+
+// Partial rows -> dweight, dbias, dscale (blockIdx.y), 32 columns to a CTA.
+template <typename W>
+__global__ void __launch_bounds__(1024) sum_kernel(const float* part, W* dw, W* db, W* ds, int n, int D) {
+  __shared__ float s[32][33];
+  W* out = blockIdx.y == 0 ? dw : blockIdx.y == 1 ? db : ds;
+  if (!out) return;
+  const int c = blockIdx.x * 32 + threadIdx.x;
+  const float* q = part + (long long)blockIdx.y * n * D;
+  float a = 0.f;
+  if (c < D)
+    for (int i = threadIdx.y; i < n; i += 32) a += q[(long long)i * D + c];
+  s[threadIdx.y][threadIdx.x] = a;
+  __syncthreads();
+  a = s[threadIdx.x][threadIdx.y];  // column threadIdx.y, partial threadIdx.x
+  for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+  const int col = blockIdx.x * 32 + threadIdx.y;
+  if (threadIdx.x == 0 && col < D) out[col] = from_f32<W>(a);
+}
+
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) {
+    (void)cudaGetLastError();
+    n = 148;  // no device here: the sizes of a B200
+  }
+  return n;
+}
+
+struct Plan {
+  int vec, k, tpg, gpc, rpc, threads;
+  unsigned gx, gy;
+};
+
+// Threads to a group: as few as hold it at up to 16 values each, so that sums
+// need few steps; groups side by side in a CTA as they lie in a row.
+bool make_plan(Plan& pl, long long rows, int D, int G, int size, bool vec) {
+  const int n = D / G;
+  if (n > kMaxGroup) return false;
+  pl.vec = vec ? 16 / size : 1;
+  const int need = (n + pl.vec - 1) / pl.vec, most = 16 / pl.vec;
+  pl.tpg = 8;
+  while (pl.tpg * most < need) pl.tpg *= 2;
+  const int k = (need + pl.tpg - 1) / pl.tpg;
+  pl.k = 1;
+  while (pl.k < k) pl.k *= 2;
+  pl.threads = pl.tpg > kThreads ? pl.tpg : kThreads;
+  pl.gpc = pl.threads / pl.tpg < G ? pl.threads / pl.tpg : G;
+  pl.rpc = pl.threads / (pl.tpg * pl.gpc);
+  pl.gy = (unsigned)((G + pl.gpc - 1) / pl.gpc);
+  // a few CTAs to an SM, each walking rows
+  const long long most_x = ((long long)sm_count() * (1024 / pl.threads) + pl.gy - 1) / pl.gy;
+  const long long want = (rows + pl.rpc - 1) / pl.rpc;
+  pl.gx = (unsigned)(want < most_x ? (want < 1 ? 1 : want) : most_x);
+  return true;
+}
+
+template <typename E, typename W, class F>
+int by_plan(const Plan& pl, F&& f) {
+  constexpr int V = 16 / (int)sizeof(E);
+#define MGS_NORM_CASE(v, kk)                                                                \
+  if (pl.vec == v && pl.k == kk)                                                            \
+    return pl.threads <= 512 ? f(fwd_kernel<E, W, v, kk, 512>, bwd_kernel<E, W, v, kk, 512>) \
+                             : f(fwd_kernel<E, W, v, kk, 1024>, bwd_kernel<E, W, v, kk, 1024>);
+  MGS_NORM_CASE(V, 1)
+  MGS_NORM_CASE(V, 2)
+  if constexpr (V == 4) {
+    MGS_NORM_CASE(V, 4)
+  }
+  MGS_NORM_CASE(1, 1)
+  MGS_NORM_CASE(1, 2)
+  MGS_NORM_CASE(1, 4)
+  MGS_NORM_CASE(1, 8)
+  MGS_NORM_CASE(1, 16)
+#undef MGS_NORM_CASE
+  return MGS_UNSUPPORTED;
+}
+
+template <class F>
+int by_dtypes(int dtype, int wdtype, F&& f) {
+  const bool same = dtype == wdtype;
+  if (!same && wdtype != MGS_F32) return MGS_BAD_DTYPE;
+  switch (dtype) {
+    case MGS_F32: return f(float{}, float{});
+    case MGS_BF16: return same ? f(__nv_bfloat16{}, __nv_bfloat16{}) : f(__nv_bfloat16{}, float{});
+    case MGS_F16: return same ? f(__half{}, __half{}) : f(__half{}, float{});
+    default: return MGS_BAD_DTYPE;
+  }
+}
+
+bool shape_ok(int64_t rows, int64_t D, int groups) {
+  return rows >= 0 && D >= 1 && D <= 0x3fffffff && groups >= 1 && D % groups == 0;
+}
+
+// Whole 16-byte vectors everywhere: addresses, row strides, group starts.
+bool vec_ok(const Args& a, int size, int wsize) {
+  const int v = 16 / size;
+  bool ok = a.n % v == 0 && (long long)a.n * wsize % 16 == 0;
+  for (const void* q : {a.x, a.res, a.gate, a.w, a.b, a.s, a.dy, a.dh, (const void*)a.y, (const void*)a.h,
+                        (const void*)a.dx, (const void*)a.dres, (const void*)a.dgate})
+    ok = ok && aligned(q, 16);
+  for (long long s : {a.ldx, a.ldres, a.ldgate, a.lddy, a.lddh}) ok = ok && s % v == 0;
+  return ok;
+}
+
+void set_plan(Args& a, const Plan& pl) { a.tpg = pl.tpg, a.gpc = pl.gpc, a.rpc = pl.rpc; }
+
+int launched() { return cudaGetLastError() == cudaSuccess ? MGS_OK : MGS_LAUNCH_FAILED; }
+
+}  // namespace
+}  // namespace norm
+}  // namespace mgs
+
+extern "C" {
+
+size_t mgs_block_norm_workspace_size(int64_t rows, int64_t D, int groups, int dtype) {
+  using namespace mgs::norm;
+  const int size = mgs::dtype_size(dtype);
+  if (!shape_ok(rows, D, groups) || size == 0) return 0;
+  size_t most = 0;
+  for (bool vec : {false, true}) {
+    Plan pl;
+    if (!make_plan(pl, rows, (int)D, groups, size, vec)) return 0;
+    const size_t n = 3 * (size_t)pl.gx * (size_t)D * sizeof(float);
+    most = n > most ? n : most;
+  }
+  return most;
+}
+
+int mgs_block_norm_fwd(const void* x, const void* residual, const void* gate, const void* weight,
+                       const void* bias, const void* scale, void* y, void* h, float* stats,
+                       const int64_t* row_strides, int64_t rows, int64_t D, int groups, int rms,
+                       float eps, int dtype, int weight_dtype, void* stream) {
+  using namespace mgs::norm;
+  if (!shape_ok(rows, D, groups) || (scale && !residual) || (residual && !h)) return MGS_BAD_SHAPE;
+  return by_dtypes(dtype, weight_dtype, [&](auto e, auto wt) -> int {
+    using E = decltype(e);
+    using W = decltype(wt);
+    if (rows == 0) return MGS_OK;
+    Args a{};
+    a.x = x, a.res = residual, a.gate = gate, a.w = weight, a.b = bias, a.s = scale, a.y = y;
+    a.h = residual ? h : nullptr, a.stats = stats;
+    a.ldx = row_strides[0], a.ldres = row_strides[1], a.ldgate = row_strides[2];
+    a.rows = rows, a.D = (int)D, a.G = groups, a.n = (int)D / groups, a.rms = rms, a.eps = eps;
+    Plan pl;
+    if (!make_plan(pl, rows, (int)D, groups, sizeof(E), vec_ok(a, sizeof(E), sizeof(W)))) return MGS_UNSUPPORTED;
+    if (pl.gy > 65535) return MGS_UNSUPPORTED;
+    set_plan(a, pl);
+    return by_plan<E, W>(pl, [&](auto fwd, auto) -> int {
+      fwd<<<dim3(pl.gx, pl.gy), pl.threads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+      return launched();
+    });
+  });
+}
+
+int mgs_block_norm_bwd(const void* x, const void* residual, const void* gate, const void* weight,
+                       const void* bias, const void* scale, const float* stats, const void* dy,
+                       const void* dh, void* dx, void* dresidual, void* dgate, void* dweight, void* dbias,
+                       void* dscale, const int64_t* row_strides, int64_t rows, int64_t D, int groups,
+                       int rms, int dtype, int weight_dtype, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  using namespace mgs::norm;
+  if (!shape_ok(rows, D, groups) || (scale && (!residual || !dresidual || !dscale)) || (gate && !dgate) ||
+      (bias && !dbias))
+    return MGS_BAD_SHAPE;
+  return by_dtypes(dtype, weight_dtype, [&](auto e, auto wt) -> int {
+    using E = decltype(e);
+    using W = decltype(wt);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (rows == 0) {
+      for (void* q : {dweight, bias ? dbias : nullptr, scale ? dscale : nullptr})
+        if (q) MGS_CUDA_OK(cudaMemsetAsync(q, 0, (size_t)D * sizeof(W), st));
+      return MGS_OK;
+    }
+    Args a{};
+    a.x = x, a.res = residual, a.gate = gate, a.w = weight, a.b = bias, a.s = scale;
+    a.dy = dy, a.dh = dh, a.dx = dx, a.dres = dresidual, a.dgate = dgate;
+    a.stats = const_cast<float*>(stats), a.part = static_cast<float*>(workspace);
+    a.ldx = row_strides[0], a.ldres = row_strides[1], a.ldgate = row_strides[2], a.lddy = row_strides[3],
+    a.lddh = row_strides[4];
+    a.rows = rows, a.D = (int)D, a.G = groups, a.n = (int)D / groups, a.rms = rms;
+    Plan pl;
+    if (!make_plan(pl, rows, (int)D, groups, sizeof(E), vec_ok(a, sizeof(E), sizeof(W)))) return MGS_UNSUPPORTED;
+    if (pl.gy > 65535) return MGS_UNSUPPORTED;
+    if (workspace_bytes < 3 * (size_t)pl.gx * (size_t)D * sizeof(float)) return MGS_WORKSPACE_TOO_SMALL;
+    set_plan(a, pl);
+    int r = by_plan<E, W>(pl, [&](auto, auto bwd) -> int {
+      const size_t smem = (size_t)pl.rpc * pl.gpc * a.n * sizeof(float);
+      if (smem > 48 * 1024)
+        MGS_CUDA_OK(cudaFuncSetAttribute(bwd, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+      bwd<<<dim3(pl.gx, pl.gy), pl.threads, smem, st>>>(a);
+      return launched();
+    });
+    if (r) return r;
+    sum_kernel<W><<<dim3((unsigned)((D + 31) / 32), 3), dim3(32, 32), 0, st>>>(
+        a.part, static_cast<W*>(dweight), bias ? static_cast<W*>(dbias) : nullptr,
+        scale ? static_cast<W*>(dscale) : nullptr, (int)pl.gx, (int)D);
+    return launched();
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,185 @@
+"""The norms around a block, each one kernel (:func:`block_norm`).
+
+Before a mixer or an MLP: the residual add, with a scale for the branch, and
+the LayerNorm or RMS norm of the sum. After a mixer: the norm of each head's
+channels and the gate. No counterpart in the reference, whose blocks run
+torch's LayerNorm and adds (``min_gru.py:3698-3922``).
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .scan_ops import _dense, _dtype_code, _ptr, _require_cuda, _stream, _workspace
+
+__all__ = ["block_norm"]
+
+_OP = "block_norm"
+
+
+def _rows(t: torch.Tensor | None, D: int):
+    """``t`` as rows of D: (tensor that owns them, row stride)."""
+    if t is None:
+        return None, 0
+    if t.stride(-1) == 1 or D == 1:
+        if t.dim() == 1:
+            return t, D
+        if t.is_contiguous():
+            return t, D
+        # one stride from row to row over all the leading dimensions
+        s, ok = t.stride(-2), True
+        for i in range(t.dim() - 2):
+            ok = ok and (t.shape[i] == 1 or t.stride(i) == t.stride(i + 1) * t.shape[i + 1])
+        if ok and all(n > 0 for n in t.shape):
+            return t, s
+    return t.contiguous(), D
+
+
+def _codes(x, weight):
+    return _dtype_code(_OP, x), _dtype_code(_OP, weight)
+
+
+def _forward(x, weight, bias, residual, scale, gate, groups, eps, rms, save):
+    with torch.cuda.device(x.device):  # sizes are queried on the launch device
+        D = x.shape[-1]
+        rows = x.numel() // D
+        (x, lx), (residual, lr), (gate, lg) = _rows(x, D), _rows(residual, D), _rows(gate, D)
+        weight, bias, scale = (None if t is None else _dense(t) for t in (weight, bias, scale))
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        h = torch.empty_like(y) if residual is not None else y.new_empty(0)
+        stats = torch.empty(rows * groups * 3 if save else 0, dtype=torch.float32, device=x.device)
+        code, wcode = _codes(x, weight)
+        st = _lib.load().mgs_block_norm_fwd(
+            _ptr(x), _ptr(residual), _ptr(gate), _ptr(weight), _ptr(bias), _ptr(scale), _ptr(y),
+            _ptr(h) if residual is not None else None, _ptr(stats) if save else None,
+            (ctypes.c_int64 * 3)(lx, lr, lg), rows, D, groups, int(rms), eps, code, wcode, _stream(x),
+        )
+        _lib.check(st, f"{_OP} forward")
+        return y, h, stats
+
+
+@torch.library.custom_op("mingru_b200::block_norm_fwd", mutates_args=())
+def _block_norm_fwd(
+    x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, residual: torch.Tensor | None,
+    scale: torch.Tensor | None, gate: torch.Tensor | None, groups: int, eps: float, rms: bool,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _forward(x, weight, bias, residual, scale, gate, groups, eps, rms, True)
+
+
+@_block_norm_fwd.register_fake
+def _(x, weight, bias, residual, scale, gate, groups, eps, rms):
+    y = x.new_empty(x.shape)
+    h = x.new_empty(x.shape) if residual is not None else x.new_empty((0,))
+    return y, h, x.new_empty((x.numel() // x.shape[-1] * groups * 3,), dtype=torch.float32)
+
+
+@torch.library.custom_op("mingru_b200::block_norm_bwd", mutates_args=())
+def _block_norm_bwd(
+    x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, residual: torch.Tensor | None,
+    scale: torch.Tensor | None, gate: torch.Tensor | None, stats: torch.Tensor, dy: torch.Tensor,
+    dh: torch.Tensor | None, groups: int, rms: bool,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    lib = _lib.load()
+    with torch.cuda.device(x.device):  # sizes are queried on the launch device
+        D = x.shape[-1]
+        rows = x.numel() // D
+        dy = dy.to(x.dtype)
+        dh = None if dh is None else dh.to(x.dtype)
+        (x, lx), (residual, lr), (gate, lg) = _rows(x, D), _rows(residual, D), _rows(gate, D)
+        (dy, ly), (dh, lh) = _rows(dy, D), _rows(dh, D)
+        weight, bias, scale = (None if t is None else _dense(t) for t in (weight, bias, scale))
+        like = lambda on, t: torch.empty(t.shape if on else (0,), dtype=t.dtype, device=t.device)  # noqa: E731
+        dx, dres, dgate = like(True, x), like(scale is not None, x), like(gate is not None, x)
+        dw, db, ds = like(True, weight), like(bias is not None, weight), like(scale is not None, weight)
+        code, wcode = _codes(x, weight)
+        ws = _workspace(lib.mgs_block_norm_workspace_size(rows, D, groups, code), x.device)
+        st = lib.mgs_block_norm_bwd(
+            _ptr(x), _ptr(residual), _ptr(gate), _ptr(weight), _ptr(bias), _ptr(scale), _ptr(stats),
+            _ptr(dy), _ptr(dh), _ptr(dx), _ptr(dres), _ptr(dgate), _ptr(dw), _ptr(db), _ptr(ds),
+            (ctypes.c_int64 * 5)(lx, lr, lg, ly, lh), rows, D, groups, int(rms), code, wcode, _ptr(ws),
+            ws.numel(), _stream(x),
+        )
+        _lib.check(st, f"{_OP} backward")
+        return dx, dw, db, dres, ds, dgate
+
+
+@_block_norm_bwd.register_fake
+def _(x, weight, bias, residual, scale, gate, stats, dy, dh, groups, rms):
+    e = lambda on, t: t.new_empty(t.shape if on else (0,))  # noqa: E731
+    return (e(True, x), e(True, weight), e(bias is not None, weight), e(scale is not None, x),
+            e(scale is not None, weight), e(gate is not None, x))
+
+
+def _setup(ctx, inputs, output):
+    x, weight, bias, residual, scale, gate, groups, _eps, rms = inputs
+    ctx.save_for_backward(x, weight, bias, residual, scale, gate, output[2])
+    ctx.groups, ctx.rms = groups, rms
+    ctx.mark_non_differentiable(output[2], *(() if residual is not None else (output[1],)))
+    ctx.set_materialize_grads(False)
+
+
+def _backward(ctx, dy, dh, _gstats):
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{_OP} does not support second-order autograd (create_graph=True)")
+    x, weight, bias, residual, scale, gate, stats = ctx.saved_tensors
+    if dy is None and dh is None:
+        return (None,) * 9
+    if dy is None:
+        dy = torch.zeros_like(x)
+    dx, dw, db, dres, ds, dgate = _block_norm_bwd(x, weight, bias, residual, scale, gate, stats, dy,
+                                                  dh if residual is not None else None, ctx.groups, ctx.rms)
+    return (dx, dw, db if bias is not None else None,
+            None if residual is None else dx if scale is None else dres,
+            ds if scale is not None else None, dgate if gate is not None else None, None, None, None)
+
+
+torch.library.register_autograd("mingru_b200::block_norm_fwd", _backward, setup_context=_setup)
+
+
+def block_norm(
+    x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
+    residual: torch.Tensor | None = None, scale: torch.Tensor | None = None,
+    gate: torch.Tensor | None = None, groups: int = 1, eps: float = 1e-5, rms: bool = False,
+):
+    """Residual add, norm and gate over the last dimension, in one kernel.
+
+    ``h = residual + scale * x`` (``h = x`` without a ``residual``; ``scale``
+    ``(D,)`` only with one), the LayerNorm (``rms``: the RMS norm) of each of
+    ``groups`` equal groups of channels, ``* weight + bias``, and ``*
+    silu(gate)`` where there is a ``gate``. Returns ``y``, or ``(y, h)`` with a
+    ``residual``: ``h`` is the residual stream that goes on.
+
+    ``x``, ``residual`` and ``gate`` ``(..., D)`` share a shape and a dtype
+    (fp32, bf16, fp16); ``weight``, ``bias`` and ``scale`` ``(D,)`` are in that
+    dtype or in fp32. Arithmetic is fp32, the norm is taken of the unrounded
+    sum, and outputs are rounded once. Rows may lie at any one stride. Groups
+    of up to 16384 channels. Differentiable w.r.t. all tensors.
+    """
+    D = x.shape[-1] if x.ndim else 0
+    if D < 1:
+        raise ValueError(f"{_OP}: need x (..., D) with D >= 1 (got {tuple(x.shape)})")
+    if groups < 1 or D % groups:
+        raise ValueError(f"{_OP}: D={D} does not split into groups={groups}")
+    if scale is not None and residual is None:
+        raise ValueError(f"{_OP}: scale needs a residual")
+    for name, t in (("residual", residual), ("gate", gate)):
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
+            raise ValueError(f"{_OP}: {name} must have x's shape {tuple(x.shape)} and dtype {x.dtype} "
+                             f"(got {tuple(t.shape)}, {t.dtype})")
+    for name, t in (("weight", weight), ("bias", bias), ("scale", scale)):
+        if t is not None and (tuple(t.shape) != (D,) or t.dtype != weight.dtype):
+            raise ValueError(f"{_OP}: {name} must have shape {(D,)} and weight's dtype (got "
+                             f"{tuple(t.shape)}, {t.dtype})")
+    _dtype_code(_OP, x)
+    if weight.dtype not in (x.dtype, torch.float32):
+        raise ValueError(f"{_OP}: weight must be {x.dtype} or float32 (got {weight.dtype})")
+    given = [t for t in (x, weight, bias, residual, scale, gate) if t is not None]
+    _require_cuda(_OP, *given)
+    if torch.compiler.is_compiling() or (torch.is_grad_enabled() and any(t.requires_grad for t in given)):
+        y, h, _ = _block_norm_fwd(x, weight, bias, residual, scale, gate, groups, float(eps), bool(rms))
+    else:  # nothing to differentiate: no dispatcher
+        y, h, _ = _forward(x, weight, bias, residual, scale, gate, groups, float(eps), bool(rms), False)
+    return y if residual is None else (y, h)

@@ -17,7 +17,8 @@ import torch
 from . import _lib
 from .scan_ops import _dtype_code, _require_cuda
 
-__all__ = ["mingru_step", "signed_step", "rotation_step", "givens_step", "delta_step"]
+__all__ = ["mingru_step", "signed_step", "rotation_step", "givens_step", "delta_step",
+           "linear_attention_step"]
 
 
 def _prep(op, *ts, like):
@@ -102,3 +103,40 @@ def delta_step(q, k, v, beta, H_prev, gamma=None):
     _run(op, _lib.load().mgs_delta_step, q.device, _p(q), _p(k), _p(v), _p(beta), _p(gamma),
          _p(H_prev), _p(y), _p(H), B, nH, nh, dk, dv, _dtype_code(op, q))
     return y, H
+
+
+def linear_attention_step(q, k, v, log_gamma, H_prev, out=None):
+    """One token of :func:`mingru_b200.linear_attention` per head:
+    ``H = exp(log_gamma) H_prev + k v^T``; readout ``y = H^T q``. ``q``, ``k``
+    ``(B, H, dk)``, ``v`` ``(B, H, dv)``, ``log_gamma`` ``(B, H)`` or
+    broadcastable to it, ``H_prev`` ``(B, H, dk, dv)`` fp32 -- the state stays
+    in fp32 whatever the inputs' dtype. The new state is written to ``out``
+    where it is given (``H_prev`` itself for an update in place). Returns
+    ``(y (B, H, dv), H)``."""
+    op = "linear_attention_step"
+    q, k, v = _prep(op, q, k, v, like=q)
+    if q.ndim != 3 or k.shape != q.shape or v.ndim != 3 or v.shape[:2] != q.shape[:2]:
+        raise ValueError(f"{op}: need q, k (B, n_heads, d_k) and v (B, n_heads, d_v); got "
+                         f"q={tuple(q.shape)}, k={tuple(k.shape)}, v={tuple(v.shape)}")
+    B, nH, dk = q.shape
+    dv = v.shape[2]
+    shape = (B, nH, dk, dv)
+    for name, t in (("H_prev", H_prev), ("out", out)):
+        if t is not None and (tuple(t.shape) != shape or t.dtype != torch.float32):
+            raise ValueError(f"{op}: {name} must be a float32 tensor of shape {shape} (got "
+                             f"{t.dtype}, {tuple(t.shape)})")
+    if out is None:
+        out = torch.empty(shape, dtype=torch.float32, device=q.device)
+    elif not out.is_contiguous():
+        raise ValueError(f"{op}: out must be contiguous")
+    _require_cuda(op, q, log_gamma, H_prev, out)
+    try:
+        lg = torch.broadcast_to(log_gamma, (B, nH)).float()
+    except RuntimeError:
+        raise ValueError(f"{op}: log_gamma must broadcast to {(B, nH)} (got "
+                         f"{tuple(log_gamma.shape)})") from None
+    H_prev = H_prev.contiguous()
+    y = torch.empty_like(v)
+    _run(op, _lib.load().mgs_linear_attn_step, q.device, _p(q), _p(k), _p(v), _p(lg), lg.stride(0),
+         lg.stride(1), _p(H_prev), _p(y), _p(out), B, nH, dk, dv, _dtype_code(op, q))
+    return y, out
