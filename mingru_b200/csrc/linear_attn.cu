@@ -284,32 +284,44 @@ __device__ __forceinline__ void mma_ta(uint32_t d, uint32_t a, uint64_t b, uint3
       : "memory");
 }
 
-// D (M x N) (+)= A B over K = 16 ks, level pairs i + j <= 2. One thread.
+// The products below take the level pairs (i, j) with i + j <= 2, the small
+// ones first: the accumulators round towards zero at each step of 16, by what
+// the sum has reached, so only the steps of the leading pair count.
+constexpr int kMaxPair = 2;
+
+// D (M x N) (+)= A B over K = 16 ks. One thread.
 template <int NA, int NB, int M, int N>
 __device__ __forceinline__ void product(uint32_t d, const Op& a, const Op& b, int ks, bool acc = false) {
   const uint32_t id = um::idesc64(a.mn, b.mn, M == 128, N);
-#pragma unroll 1
-  for (int k = 0; k < ks; ++k)
 #pragma unroll
-    for (int i = 0; i < NA; ++i)
+  for (int o = kMaxPair; o >= 0; --o)
 #pragma unroll
-      for (int j = 0; j < NB; ++j)
-        if (i + j <= 2)
-          um::mma(d, a.d + k * a.step + i * a.level, b.d + k * b.step + j * b.level, id,
-                  acc || k + i + j > 0);
+    for (int i = 0; i < NA; ++i) {
+      const int j = o - i;
+      if (j < 0 || j >= NB) continue;
+#pragma unroll 4
+      for (int k = 0; k < ks; ++k) {
+        um::mma(d, a.d + k * a.step + i * a.level, b.d + k * b.step + j * b.level, id, acc);
+        acc = true;
+      }
+    }
 }
 // The same with A (128 rows, 128 deep) in TMEM: NA levels of 64 columns each.
 template <int NA, int NB, int N>
 __device__ __forceinline__ void product_ta(uint32_t d, uint32_t a, const Op& b, bool acc) {
   const uint32_t id = um::idesc64(false, b.mn, true, N);
-#pragma unroll 1
-  for (int k = 0; k < kC / 16; ++k)
 #pragma unroll
-    for (int i = 0; i < NA; ++i)
+  for (int o = kMaxPair; o >= 0; --o)
 #pragma unroll
-      for (int j = 0; j < NB; ++j)
-        if (i + j <= 2)
-          mma_ta(d, a + k * 8 + i * 64, b.d + k * b.step + j * b.level, id, acc || k + i + j > 0);
+    for (int i = 0; i < NA; ++i) {
+      const int j = o - i;
+      if (j < 0 || j >= NB) continue;
+#pragma unroll 4
+      for (int k = 0; k < kC / 16; ++k) {
+        mma_ta(d, a + k * 8 + i * 64, b.d + k * b.step + j * b.level, id, acc);
+        acc = true;
+      }
+    }
 }
 
 __device__ __forceinline__ void st16(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -449,14 +461,18 @@ __device__ __forceinline__ void product_rows(uint32_t d, bf16* const (&a)[3], co
   const uint32_t id = um::idesc64(true, true, D == 128, D);
   const Op o = op_mn(b, D, kC * D);
   const uint64_t da[3] = {op_mn(a[0], D, 0).d, op_mn(a[1], D, 0).d, op_mn(a[2], D, 0).d};
-#pragma unroll 1
-  for (int k = 0; k < kC / 16; ++k)
 #pragma unroll
-    for (int i = 0; i < 3; ++i)
+  for (int r = kMaxPair; r >= 0; --r)
 #pragma unroll
-      for (int j = 0; j < NL; ++j)
-        if (i + j <= 2)
-          um::mma(d, da[i] + k * o.step, o.d + k * o.step + j * o.level, id, acc || k + i + j > 0);
+    for (int i = 0; i < 3; ++i) {
+      const int j = r - i;
+      if (j < 0 || j >= NL) continue;
+#pragma unroll 4
+      for (int k = 0; k < kC / 16; ++k) {
+        um::mma(d, da[i] + k * o.step, o.d + k * o.step + j * o.level, id, acc);
+        acc = true;
+      }
+    }
 }
 
 struct Small {  // the tables of a CTA
@@ -472,7 +488,7 @@ static_assert(sizeof(Small) <= kSmallBytes, "");
 
 // What segment s adds to the state: forward sum_j e^{c_end - c_j} k_j v_j^T,
 // backward (kBwd) sum_i e^{c_i} q_i dy_i^T with c from the segment's start.
-// Every factor is <= 1, so the chunks of a segment add up in one accumulator.
+// Every factor is <= 1, so the chunks of a segment just add up.
 template <typename E, int D, bool kBwd>
 __global__ void __launch_bounds__(kThreads) state_kernel(const Args<E> p) {
   constexpr int NL = kLevels<E>, kTileE = kC * D;
@@ -503,6 +519,8 @@ __global__ void __launch_bounds__(kThreads) state_kernel(const Args<E> p) {
     um::fence_after();
   };
   const int c0 = s * p.m, c1 = min(c0 + p.m, p.nchunks);
+  State<D> st;
+  st.zero();
   double run = 0.0;  // log2 decay of the chunks already summed
   unsigned phase = 0;
   for (int i = 0; i < c1 - c0; ++i) {
@@ -522,17 +540,15 @@ __global__ void __launch_bounds__(kThreads) state_kernel(const Args<E> p) {
     run += total;
     sync();
     if (ok && tid == 0) {
-      product_rows<NL, D>(sm.tbase, lv, Bt, i > 0);
+      product_rows<NL, D>(sm.tbase, lv, Bt, false);
       um::commit(&sm.bar);
     }
     if (ok) ok = mbar_wait(&sm.bar, phase & 1, &g_sticky_err);
     ++phase;
     um::fence_after();
+    st.update(1.f, sm.tbase, 0);  // in registers: round to nearest
   }
   // forward: the state that enters segment s + 1; backward: the gradient that leaves s - 1
-  State<D> st;
-  st.zero();
-  st.update(0.f, sm.tbase, 0);
   if (ok) {
     st.store_own(p.seg + (bh * p.nseg + s + (kBwd ? -1 : 1)) * (D * D));
     if (tid == 0) p.segl[bh * p.nseg + s] = (float)run;
