@@ -51,6 +51,8 @@ namespace um = umma;
 constexpr int kC = 128;        // tokens of a chunk: the rows of an M = 128 accumulator
 constexpr int kThreads = 256;  // two warps for each quarter of the TMEM lanes
 constexpr float kMinLog2 = -128.f;
+// Polls of an mbarrier before a wait gives up (each suspends for some 10 us: over a second).
+constexpr long long kPolls = 1ll << 17;
 
 template <typename E>
 constexpr int kLevels = 1;
@@ -60,16 +62,19 @@ template <>
 constexpr int kLevels<float> = 3;
 
 // A (B, H, T, d) tensor: base and strides in elements (the last dimension is
-// dense); vec: every row starts on 16 bytes and holds whole groups of 8.
+// dense); vec: every row starts on 16 bytes and holds whole groups of 8, wide:
+// on 32 bytes and whole groups of 32 bytes.
 template <typename P>
 struct Ten {
   P* p;
   long long sb, sh, st;
-  int vec;
+  int vec, wide;
 };
 
 template <typename E>
 struct Args {
+  CUtensorMap mQ, mK, mV, mdy, my, mdQ, mdK, mdV;  // bf16 with tma set
+  int tma;                                         // every tensor has a map
   Ten<const E> Q, K, V, dy;
   Ten<E> y, dQ, dK, dV;
   const float* lg;
@@ -80,23 +85,15 @@ struct Args {
   float* dH0;        // (B, H, dk, dv) or null: not wanted
   float* dlg;        // (B, H, T)
   float* saved;      // (BH, nchunks, D * D) chunk-start states, or null (forward without a backward)
-  float* seg;        // (BH, nseg, D * D) segment states (workspace)
-  float* segl;       // (BH, nseg) log2 of each segment's total decay (workspace)
+  float* seg;        // (BH, nsub, D * D) states at the parts' starts (backward: ends) (workspace)
+  float* segl;       // (BH, nsub) log2 of each part's total decay (workspace)
   long long T;
   int H, dk, dv, nchunks, m, nseg;  // m chunks to a segment
+  int ms, r, nsub;                  // segments in r parts of ms chunks for the state sums, nsub in all
   long long BH;
 };
 
 // ------------------------------------------------------------- tile loads --
-
-__device__ __forceinline__ void cp_async16(void* dst, const void* src, int src_bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem_u32(dst)), "l"(src),
-               "r"(src_bytes)
-               : "memory");
-}
-__device__ __forceinline__ void cp_async_wait_all() {
-  asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;\n" ::: "memory");
-}
 
 // x[0..7] -> NL bf16 levels at element offset o of tiles `stride` elements apart.
 template <int NL>
@@ -137,44 +134,40 @@ __device__ __forceinline__ void load_levels8(const bf16* t, long long stride, in
   }
 }
 
-// Row and first column of item `idx` (8 elements) of a blocked 128 x D tile;
-// the item's element offset is 8 * idx. A warp's items are 8 rows x 4 groups:
-// whole 32-byte sectors of global memory, and a conflict-free 512-byte run of
-// shared memory.
-template <int D>
-__device__ __forceinline__ void item_rc(int idx, int& r, int& c) {
-  r = (idx / D) * 8 + (idx & 7);
-  c = ((idx >> 3) & (D / 8 - 1)) * 8;
+// Tiles are what the tensor maps' 128-byte swizzle makes of 64 columns: rows of
+// 128 bytes, the 16-byte group g of row r at group g ^ (r % 8); wider tiles are
+// such halves one after the other. Reading or writing a row with a lane for each
+// row, or whole rows with eight lanes to a row, is free of bank conflicts.
+template <int R>
+__device__ __forceinline__ int sw(int r, int c) {
+  return (c >> 6) * (R * 64) + r * 64 + ((((c >> 3) & 7) ^ (r & 7)) << 3) + (c & 7);
 }
 
-// Rows [t0, t0 + n) of one head as NL bf16 levels in blocked tiles; rows from
-// n and columns from d are zeros. bf16 rows that allow it go by cp.async (the
-// caller waits), others through registers.
-template <typename E, int D>
-__device__ __forceinline__ void load_tile(bf16* tile, const Ten<const E>& x, const E* head, long long t0,
-                                          int n, int d) {
-  constexpr int NL = kLevels<E>, kItems = kC * D / 8 / kThreads;
-  const E* base = head + t0 * x.st;
-  if constexpr (NL == 1) {
-    if (x.vec) {
-#pragma unroll
-      for (int it = 0; it < kItems; ++it) {
-        const int idx = it * kThreads + (int)threadIdx.x;
-        int r, c;
-        item_rc<D>(idx, r, c);
-        const bool in = r < n && c < d;
-        cp_async16(tile + 8 * idx, in ? base + r * x.st + c : head, in ? 16 : 0);
-      }
-      return;
-    }
+// A 128 x D tile in items of 16 bytes in memory order: thread t has items t,
+// t + 256, ..., which are the same columns of rows 32 apart in each half.
+template <int D>
+struct Items {
+  static constexpr int kN = kC * D / 8 / kThreads;
+  __device__ static int row(int i) { return (i & 3) * 32 + (threadIdx.x >> 3); }
+  __device__ static int col(int i) {
+    return (i >> 2) * 64 + (((threadIdx.x & 7) ^ ((threadIdx.x >> 3) & 7)) << 3);
   }
+  __device__ static int offset(int i) { return 8 * (i * kThreads + (int)threadIdx.x); }
+};
+
+// Rows [t0, t0 + n) of a head as bf16 levels in a tile, through registers; rows
+// from n on and columns from d are zeros.
+template <typename E, int D>
+__device__ __forceinline__ void load_tile(bf16* tile, const Ten<const E>& x, long long b, long long h,
+                                          long long t0, int n, int d) {
+  using I = Items<D>;
+  constexpr int NL = kLevels<E>;
+  const E* head = x.p + b * x.sb + h * x.sh + t0 * x.st;
 #pragma unroll
-  for (int it = 0; it < kItems; ++it) {
-    const int idx = it * kThreads + (int)threadIdx.x;
-    int r, c;
-    item_rc<D>(idx, r, c);
+  for (int i = 0; i < I::kN; ++i) {
+    const int r = I::row(i), c = I::col(i);
+    const E* s = head + r * x.st + c;
     float v[8];
-    const E* s = base + r * x.st + c;
     if (x.vec) {
       if (r < n && c < d) {
         constexpr int kN = 16 / (int)sizeof(E);
@@ -183,34 +176,101 @@ __device__ __forceinline__ void load_tile(bf16* tile, const Ten<const E>& x, con
           const uint4 u = __ldg(reinterpret_cast<const uint4*>(s + k));
           const E* e = reinterpret_cast<const E*>(&u);
 #pragma unroll
-          for (int i = 0; i < kN; ++i) v[k + i] = to_f32<E>(e[i]);
+          for (int j = 0; j < kN; ++j) v[k + j] = to_f32<E>(e[j]);
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.f;
+        for (int j = 0; j < 8; ++j) v[j] = 0.f;
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = r < n && c + i < d ? to_f32<E>(s[i]) : 0.f;
+      for (int j = 0; j < 8; ++j) v[j] = r < n && c + j < d ? to_f32<E>(s[j]) : 0.f;
     }
-    store_levels8<NL>(tile, kC * D, 8 * idx, v);
+    store_levels8<NL>(tile, kC * D, I::offset(i), v);
   }
 }
 
-// 16 values of one row (columns c0..) to global memory.
+// The same rows into L2, ahead of their load.
 template <typename E>
-__device__ __forceinline__ void store_row16(E* row, int c0, int d, bool vec, const float (&v)[16]) {
-  if (vec) {
-    constexpr int kN = 16 / (int)sizeof(E);
+__device__ __forceinline__ void prefetch_rows(const Ten<const E>& x, long long b, long long h, long long t0,
+                                              int n, int d) {
+  const E* head = x.p + b * x.sb + h * x.sh + t0 * x.st;
+  const int bytes = d * (int)sizeof(E), lines = (bytes + 127) / 128;
+  for (int i = threadIdx.x; i < n * lines; i += kThreads) {
+    const char* a = reinterpret_cast<const char*>(head + (i / lines) * x.st) + (i % lines) * 128;
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(a));
+  }
+}
+
+// bf16 tensors that a tensor map can describe (columns, time, head, batch) come
+// and go by TMA, one thread issuing: rows and columns outside read as zeros and
+// are not written.
+template <int D>
+__device__ __forceinline__ void tma_load(bf16* tile, const CUtensorMap* m, long long t0, int h, int b,
+                                         uint64_t* bar) {
 #pragma unroll
-    for (int k = 0; k < 16; k += kN)
-      if (c0 + k < d) {
-        uint4 u;
-        E* e = reinterpret_cast<E*>(&u);
+  for (int x = 0; x < D; x += 64)
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(tile + x * kC)),
+        "l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"((int)t0), "r"(h), "r"(b), "r"(smem_u32(bar))
+        : "memory");
+}
+template <int D>
+__device__ __forceinline__ void tma_store(const CUtensorMap* m, long long t0, int h, int b, int d,
+                                          const bf16* tile) {
 #pragma unroll
-        for (int i = 0; i < kN; ++i) e[i] = from_f32<E>(v[k + i]);
-        *reinterpret_cast<uint4*>(row + c0 + k) = u;
+  for (int x = 0; x < D; x += 64) {
+    if (x >= d) break;
+    asm volatile(
+        "cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(
+            reinterpret_cast<uint64_t>(m)),
+        "r"(x), "r"((int)t0), "r"(h), "r"(b), "r"(smem_u32(tile + x * kC))
+        : "memory");
+  }
+  bulk_commit();
+}
+template <int D>
+__device__ __forceinline__ void tma_prefetch(const CUtensorMap* m, long long t0, int h, int b, int d) {
+#pragma unroll
+  for (int x = 0; x < D; x += 64)
+    if (x < d)
+    asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(
+                     reinterpret_cast<uint64_t>(m)),
+                 "r"(x), "r"((int)t0), "r"(h), "r"(b)
+                 : "memory");
+}
+constexpr int tile_bytes(int D) { return kC * D * 2; }
+
+// 16 values of one row (columns c0.., c0 % 16 == 0) into a bf16 tile.
+__device__ __forceinline__ void row16_to_tile(bf16* tile, int r, int c0, const float (&v)[16]) {
+  store_levels8<1>(tile, 0, sw<kC>(r, c0), v);
+  store_levels8<1>(tile, 0, sw<kC>(r, c0 + 8), v + 8);
+}
+
+// 16 values of one row (columns c0..) to global memory, in whole 32-byte sectors
+// where the rows allow it.
+template <typename E>
+__device__ __forceinline__ void store_row16(E* row, int c0, int d, const Ten<E>& x, const float (&v)[16]) {
+  if (x.vec) {
+    constexpr int kN = 32 / (int)sizeof(E);
+#pragma unroll
+    for (int k = 0; k < 16; k += kN) {
+      uint32_t w[8];
+      E* e = reinterpret_cast<E*>(w);
+#pragma unroll
+      for (int i = 0; i < kN; ++i) e[i] = from_f32<E>(v[k + i]);
+      E* o = row + c0 + k;
+      if (x.wide) {
+        if (c0 + k < d)
+          asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(o), "r"(w[0]), "r"(w[1]),
+                       "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                       : "memory");
+      } else {
+        if (c0 + k < d) *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
+        if (c0 + k + kN / 2 < d) *reinterpret_cast<uint4*>(o + kN / 2) = make_uint4(w[4], w[5], w[6], w[7]);
       }
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 16; ++i)
@@ -226,55 +286,91 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// Inclusive sums of a chunk's log2 decays as ch + cl, by one warp (four tokens
-// to a lane, fp64). Tokens from n on add nothing.
-__device__ __forceinline__ void decay_table(const float* lg, long long st, int n, float* ch, float* cl) {
-  const int lane = threadIdx.x & 31;
-  double s[4];
-  double run = 0.0;
+// A chunk's decays: inclusive sums of the log2 decays as ch + cl, and cf, a
+// token's factor to the edge of its block of 16: 2^(c_last - c_t) (kStart:
+// 2^(c_t - c_first)). For a whole block on one side of token i the factor
+// between i and any t of it is one of i's to the block's edge times cf[t], both
+// <= 1, so nothing is lost that the product would keep.
+struct Decays {
+  float ch[kC], cl[kC], cf[kC];
+  __device__ __forceinline__ float to(float h, float l, int t) const { return ex2((h - ch[t]) + (l - cl[t])); }
+  __device__ __forceinline__ float from(float h, float l, int t) const { return ex2((ch[t] - h) + (cl[t] - l)); }
+};
+
+// By one warp, four tokens to a lane, in fp64. Tokens from n on add nothing.
+struct DecayWarp {
+  float lg[4];
+  __device__ __forceinline__ void load(const float* p, long long st, int n) {
+    const int t0 = 4 * (threadIdx.x & 31);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int t = 4 * lane + i;
-    double v = 0.0;
-    if (t < n) {
-      v = (double)lg[t * st] * 1.4426950408889634;
+    for (int i = 0; i < 4; ++i) lg[i] = t0 + i < n ? p[(t0 + i) * st] : 0.f;
+  }
+  template <bool kStart>
+  __device__ __forceinline__ void table(Decays& o) const {
+    const int lane = threadIdx.x & 31;
+    double s[4];
+    double run = 0.0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      double v = (double)lg[i] * 1.4426950408889634;
       if (v < (double)kMinLog2) v = (double)kMinLog2;
+      run += v;
+      s[i] = run;
     }
-    run += v;
-    s[i] = run;
-  }
-  double inc = run;
+    double inc = run;
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const double o = __shfl_up_sync(0xffffffffu, inc, d);
-    if (lane >= d) inc += o;
-  }
-  const double before = inc - run;
+    for (int d = 1; d < 32; d <<= 1) {
+      const double x = __shfl_up_sync(0xffffffffu, inc, d);
+      if (lane >= d) inc += x;
+    }
+    const double before = inc - run;
+    float h[4], l[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const double c = before + s[i];
-    const float h = rintf((float)c * 512.f) * (1.f / 512.f);
-    ch[4 * lane + i] = h;
-    cl[4 * lane + i] = (float)(c - (double)h);
+    for (int i = 0; i < 4; ++i) {
+      const double c = before + s[i];
+      h[i] = rintf((float)c * 512.f) * (1.f / 512.f);
+      l[i] = (float)(c - (double)h[i]);
+    }
+    const int edge = kStart ? lane & ~3 : lane | 3;
+    const float eh = __shfl_sync(0xffffffffu, kStart ? h[0] : h[3], edge);
+    const float el = __shfl_sync(0xffffffffu, kStart ? l[0] : l[3], edge);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      o.ch[4 * lane + i] = h[i];
+      o.cl[4 * lane + i] = l[i];
+      o.cf[4 * lane + i] = kStart ? ex2((h[i] - eh) + (l[i] - el)) : ex2((eh - h[i]) + (el - l[i]));
+    }
   }
-}
+};
 
 // ------------------------------------------------------------ MMA issuing --
 
-// Descriptor of a blocked tile of `cols` columns: contraction over its columns
-// (K-major) or over its rows (MN-major), and the step of 16 along it.
+// A tile of R rows as an operand: contraction over its columns (K-major) or
+// over its rows (MN-major), as descriptors of the 128-byte swizzle (groups of
+// eight rows 1024 bytes apart, halves of 64 columns R rows apart).
+template <int R>
 struct Op {
   uint64_t d;
-  uint32_t step, level;  // in 16-byte units
+  uint32_t level;  // from one level to the next, in 16-byte units
   bool mn;
+  // k-th step of 16 along the contraction, in 16-byte units
+  __device__ __forceinline__ uint32_t at(int k) const {
+    return mn ? k * 128 : (k & 3) * 2 + (k >> 2) * (R * 8);
+  }
 };
-__device__ __forceinline__ Op op_k(const bf16* t, int cols, int level_elems) {
-  return {um::desc(um::saddr(t), 128, cols * 16), 256 / 16, (uint32_t)(level_elems * 2 / 16), false};
+template <int R>
+__device__ __forceinline__ Op<R> operand(const bf16* t, bool mn, int level_elems) {
+  return {um::desc(um::saddr(t), mn ? R * 128 : 16, 1024) | ((uint64_t)2 << 61),
+          (uint32_t)(level_elems * 2 / 16), mn};
 }
-__device__ __forceinline__ Op op_mn(const bf16* t, int cols, int level_elems) {
-  return {um::desc(um::saddr(t), cols * 16, 128), (uint32_t)(2 * cols * 16 / 16),
-          (uint32_t)(level_elems * 2 / 16), true};
-}
+template <int D>
+__device__ __forceinline__ Op<kC> op_k(const bf16* t) { return operand<kC>(t, false, kC * D); }
+template <int D>
+__device__ __forceinline__ Op<kC> op_mn(const bf16* t) { return operand<kC>(t, true, kC * D); }
+template <int D>
+__device__ __forceinline__ Op<D> state_k(const bf16* t) { return operand<D>(t, false, D * D); }
+template <int D>
+__device__ __forceinline__ Op<D> state_mn(const bf16* t) { return operand<D>(t, true, D * D); }
 
 __device__ __forceinline__ void mma_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
   asm volatile(
@@ -290,8 +386,8 @@ __device__ __forceinline__ void mma_ta(uint32_t d, uint32_t a, uint64_t b, uint3
 constexpr int kMaxPair = 2;
 
 // D (M x N) (+)= A B over K = 16 ks. One thread.
-template <int NA, int NB, int M, int N>
-__device__ __forceinline__ void product(uint32_t d, const Op& a, const Op& b, int ks, bool acc = false) {
+template <int NA, int NB, int M, int N, int RA, int RB>
+__device__ __forceinline__ void product(uint32_t d, const Op<RA>& a, const Op<RB>& b, int ks, bool acc = false) {
   const uint32_t id = um::idesc64(a.mn, b.mn, M == 128, N);
 #pragma unroll
   for (int o = kMaxPair; o >= 0; --o)
@@ -301,14 +397,14 @@ __device__ __forceinline__ void product(uint32_t d, const Op& a, const Op& b, in
       if (j < 0 || j >= NB) continue;
 #pragma unroll 4
       for (int k = 0; k < ks; ++k) {
-        um::mma(d, a.d + k * a.step + i * a.level, b.d + k * b.step + j * b.level, id, acc);
+        um::mma(d, a.d + a.at(k) + i * a.level, b.d + b.at(k) + j * b.level, id, acc);
         acc = true;
       }
     }
 }
 // The same with A (128 rows, 128 deep) in TMEM: NA levels of 64 columns each.
 template <int NA, int NB, int N>
-__device__ __forceinline__ void product_ta(uint32_t d, uint32_t a, const Op& b, bool acc) {
+__device__ __forceinline__ void product_ta(uint32_t d, uint32_t a, const Op<kC>& b, bool acc) {
   const uint32_t id = um::idesc64(false, b.mn, true, N);
 #pragma unroll
   for (int o = kMaxPair; o >= 0; --o)
@@ -318,7 +414,7 @@ __device__ __forceinline__ void product_ta(uint32_t d, uint32_t a, const Op& b, 
       if (j < 0 || j >= NB) continue;
 #pragma unroll 4
       for (int k = 0; k < kC / 16; ++k) {
-        mma_ta(d, a + k * 8 + i * 64, b.d + k * b.step + j * b.level, id, acc);
+        mma_ta(d, a + k * 8 + i * 64, b.d + b.at(k) + j * b.level, id, acc);
         acc = true;
       }
     }
@@ -412,14 +508,14 @@ struct State {
       *reinterpret_cast<float4*>(p + (((col0() + i) / 4) * D + row()) * 4) =
           make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
   }
-  // levels into blocked D x D tiles
+  // levels into D x D tiles
   template <int NL>
   __device__ __forceinline__ void to_smem(bf16* t) const {
     if (!valid()) return;
     const int r = row();
 #pragma unroll
     for (int i = 0; i < kCols; i += 8)
-      store_levels8<NL>(t, D * D, um::boff_n(r, col0() + i, D), v + i);
+      store_levels8<NL>(t, D * D, sw<D>(r, col0() + i), v + i);
   }
   // v = g v + accumulator at TMEM column `col` (every lane of the warp takes part)
   __device__ __forceinline__ void update(float g, uint32_t tb, int col) {
@@ -437,20 +533,20 @@ struct State {
 // Rows of a tile (NL levels) times w(row), as three levels in dst[0..2].
 template <int NL, int D, typename W>
 __device__ __forceinline__ void scale_rows(const bf16* src, bf16* const (&dst)[3], W w) {
+  using I = Items<D>;
 #pragma unroll
-  for (int it = 0; it < kC * D / 8 / kThreads; ++it) {
-    const int idx = it * kThreads + (int)threadIdx.x;
-    int r, c;
-    item_rc<D>(idx, r, c);
-    float x[8], f = w(r);
-    load_levels8<NL>(src, kC * D, 8 * idx, x);
+  for (int it = 0; it < I::kN; ++it) {
+    const int o = I::offset(it);
+    const float f = w(I::row(it));
+    float x[8];
+    load_levels8<NL>(src, kC * D, o, x);
     uint32_t lv[3][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       um::split3_pack(x[2 * i] * f, x[2 * i + 1] * f, lv[0][i], lv[1][i], lv[2][i]);
 #pragma unroll
     for (int l = 0; l < 3; ++l)
-      *reinterpret_cast<uint4*>(dst[l] + 8 * idx) = make_uint4(lv[l][0], lv[l][1], lv[l][2], lv[l][3]);
+      *reinterpret_cast<uint4*>(dst[l] + o) = make_uint4(lv[l][0], lv[l][1], lv[l][2], lv[l][3]);
   }
 }
 
@@ -459,8 +555,8 @@ __device__ __forceinline__ void scale_rows(const bf16* src, bf16* const (&dst)[3
 template <int NL, int D>
 __device__ __forceinline__ void product_rows(uint32_t d, bf16* const (&a)[3], const bf16* b, bool acc) {
   const uint32_t id = um::idesc64(true, true, D == 128, D);
-  const Op o = op_mn(b, D, kC * D);
-  const uint64_t da[3] = {op_mn(a[0], D, 0).d, op_mn(a[1], D, 0).d, op_mn(a[2], D, 0).d};
+  const Op<kC> o = op_mn<D>(b);
+  const uint64_t da[3] = {op_mn<D>(a[0]).d, op_mn<D>(a[1]).d, op_mn<D>(a[2]).d};
 #pragma unroll
   for (int r = kMaxPair; r >= 0; --r)
 #pragma unroll
@@ -469,28 +565,40 @@ __device__ __forceinline__ void product_rows(uint32_t d, bf16* const (&a)[3], co
       if (j < 0 || j >= NL) continue;
 #pragma unroll 4
       for (int k = 0; k < kC / 16; ++k) {
-        um::mma(d, da[i] + k * o.step, o.d + k * o.step + j * o.level, id, acc);
+        um::mma(d, da[i] + o.at(k), o.d + o.at(k) + j * o.level, id, acc);
         acc = true;
       }
     }
 }
 
-struct Small {  // the tables of a CTA
-  uint64_t bar;
+struct Small {  // a CTA's barriers, TMEM address and decays
+  uint64_t bar, full[3];
   uint32_t tbase;
-  uint32_t pad;
-  float ch[kC], cl[kC];
+  uint32_t pad[3];
+  Decays dec;
 };
 constexpr int kSmallBytes = 2048;
 static_assert(sizeof(Small) <= kSmallBytes, "");
+constexpr int kDecayWarp = 4;  // builds the next chunk's table, during the products that no longer need this one's
+
+// An mbarrier's phases are waited for by every thread; two of them in a row need
+// a __syncthreads between the first wait and the second phase's arrival, or a
+// thread that is late for the first never sees it.
 
 // ----------------------------------------------------------- state kernel --
 
-// What segment s adds to the state: forward sum_j e^{c_end - c_j} k_j v_j^T,
-// backward (kBwd) sum_i e^{c_i} q_i dy_i^T with c from the segment's start.
-// Every factor is <= 1, so the chunks of a segment just add up.
+template <typename E, int D>
+struct Sums {
+  static constexpr int NL = kLevels<E>, kTileE = kC * D;
+  static constexpr size_t kSmem = kSmallBytes + 2 * (3 + NL) * (size_t)kTileE;
+  static constexpr int kPerSm = (int)(228 * 1024 / (kSmem + 1024)) < 3 ? (int)(228 * 1024 / (kSmem + 1024)) : 3;
+};
+
+// What part s of a sequence (ms chunks) adds to the state: forward
+// sum_j e^{c_end - c_j} k_j v_j^T, backward (kBwd) sum_i e^{c_i} q_i dy_i^T with
+// c from the part's start. Every factor is <= 1, so the chunks just add up.
 template <typename E, int D, bool kBwd>
-__global__ void __launch_bounds__(kThreads) state_kernel(const Args<E> p) {
+__global__ void __launch_bounds__(kThreads, Sums<E, D>::kPerSm) state_kernel(const __grid_constant__ Args<E> p) {
   constexpr int NL = kLevels<E>, kTileE = kC * D;
   extern __shared__ __align__(1024) unsigned char smem[];
   Small& sm = *reinterpret_cast<Small*>(smem);
@@ -498,18 +606,26 @@ __global__ void __launch_bounds__(kThreads) state_kernel(const Args<E> p) {
   bf16* Bt = A + 3 * kTileE;
   const int tid = threadIdx.x, warp = tid >> 5;
   const long long bh = blockIdx.x % p.BH;
-  const int s = (int)(blockIdx.x / p.BH) + (kBwd ? 1 : 0);
-  const long long b = bh / p.H, h = bh % p.H;
-  const Ten<const E>&ta = kBwd ? p.Q : p.K, &tv = kBwd ? p.dy : p.V;
-  const E* ha = ta.p + b * ta.sb + h * ta.sh;
-  const E* hv = tv.p + b * tv.sb + h * tv.sh;
+  const int s = (int)(blockIdx.x / p.BH) + (kBwd ? p.r : 0);
+  const int b = (int)(bh / p.H), h = (int)(bh % p.H);
   const float* lg = p.lg + b * p.lsb + h * p.lsh;
   bf16* const lv[3] = {A, A + kTileE, A + 2 * kTileE};
+  const int c0 = s * p.ms, c1 = min(c0 + p.ms, p.nchunks), count = c1 - c0;
+  const int first = kBwd ? c0 : c1 - 1, step = kBwd ? 1 : -1;
+  auto rows = [&](int c) { return (int)min((long long)kC, p.T - (long long)c * kC); };
+  const bool tma = NL == 1 && p.tma;
+  auto load = [&](int c) {  // by one thread
+    mbar_arrive_expect_tx(&sm.full[0], 2 * tile_bytes(D));
+    tma_load<D>(A, kBwd ? &p.mQ : &p.mK, (long long)c * kC, h, b, &sm.full[0]);
+    tma_load<D>(Bt, kBwd ? &p.mdy : &p.mV, (long long)c * kC, h, b, &sm.full[0]);
+  };
 
   if (warp == 0) um::alloc(&sm.tbase, D);
   if (tid == 0) {
     mbar_init(&sm.bar, 1);
+    mbar_init(&sm.full[0], 1);
     mbar_fence_init();
+    if (tma && count > 0) load(first);
   }
   bool ok = true;
   auto sync = [&]() {
@@ -518,52 +634,59 @@ __global__ void __launch_bounds__(kThreads) state_kernel(const Args<E> p) {
     ok = !__syncthreads_or(!ok);
     um::fence_after();
   };
-  const int c0 = s * p.m, c1 = min(c0 + p.m, p.nchunks);
   State<D> st;
   st.zero();
+  DecayWarp dw;
+  if (warp == kDecayWarp && count > 0) {
+    dw.load(lg + (long long)first * kC * p.lst, p.lst, rows(first));
+    dw.table<false>(sm.dec);
+  }
+  sync();
   double run = 0.0;  // log2 decay of the chunks already summed
-  unsigned phase = 0;
-  for (int i = 0; i < c1 - c0; ++i) {
-    const int c = kBwd ? c0 + i : c1 - 1 - i;
-    const long long t0 = (long long)c * kC;
-    const int n = (int)min((long long)kC, p.T - t0);
-    load_tile<E, D>(A, ta, ha, t0, n, p.dk);
-    load_tile<E, D>(Bt, tv, hv, t0, n, p.dv);
-    if (warp == 0) decay_table(lg + t0 * p.lst, p.lst, n, sm.ch, sm.cl);
-    cp_async_wait_all();
-    sync();
-    const double total = (double)sm.ch[kC - 1] + (double)sm.cl[kC - 1];
-    const float rh = (float)run, th = sm.ch[kC - 1], tl = sm.cl[kC - 1];
-    scale_rows<NL, D>(A, lv, [&](int r) {
-      return kBwd ? ex2((sm.ch[r] + rh) + sm.cl[r]) : ex2(((th - sm.ch[r]) + rh) + (tl - sm.cl[r]));
+  for (int i = 0, c = first; i < count; ++i, c += step) {
+    const bool more = i + 1 < count;
+    if (tma) {
+      if (ok) ok = mbar_wait(&sm.full[0], i & 1, &g_sticky_err, kPolls);
+    } else {
+      load_tile<E, D>(A, kBwd ? p.Q : p.K, b, h, (long long)c * kC, rows(c), p.dk);
+      load_tile<E, D>(Bt, kBwd ? p.dy : p.V, b, h, (long long)c * kC, rows(c), p.dv);
+    }
+    if (warp == kDecayWarp && more) dw.load(lg + (long long)(c + step) * kC * p.lst, p.lst, rows(c + step));
+    const float rh = (float)run, th = sm.dec.ch[kC - 1], tl = sm.dec.cl[kC - 1];
+    scale_rows<NL, D>(A, lv, [&](int r) {  // a thread's own items, in place
+      const Decays& d = sm.dec;
+      return kBwd ? ex2((d.ch[r] + rh) + d.cl[r]) : ex2(((th - d.ch[r]) + rh) + (tl - d.cl[r]));
     });
-    run += total;
+    run += (double)th + (double)tl;
     sync();
     if (ok && tid == 0) {
       product_rows<NL, D>(sm.tbase, lv, Bt, false);
       um::commit(&sm.bar);
     }
-    if (ok) ok = mbar_wait(&sm.bar, phase & 1, &g_sticky_err);
-    ++phase;
+    if (warp == kDecayWarp && more) dw.table<false>(sm.dec);
+    if (ok) ok = mbar_wait(&sm.bar, i & 1, &g_sticky_err, kPolls);
     um::fence_after();
+    if (tma && ok && tid == 0 && more) load(c + step);
     st.update(1.f, sm.tbase, 0);  // in registers: round to nearest
+    sync();                       // the next table; the sum has been read
   }
-  // forward: the state that enters segment s + 1; backward: the gradient that leaves s - 1
+  // forward: the state that enters part s + 1; backward: the gradient that leaves s - 1
   if (ok) {
-    st.store_own(p.seg + (bh * p.nseg + s + (kBwd ? -1 : 1)) * (D * D));
-    if (tid == 0) p.segl[bh * p.nseg + s] = (float)run;
+    st.store_own(p.seg + (bh * p.nsub + s + (kBwd ? -1 : 1)) * (D * D));
+    if (tid == 0) p.segl[bh * p.nsub + s] = (float)run;
   }
   um::fence_before();
   __syncthreads();
   if (warp == 0) um::dealloc(sm.tbase, D);
 }
 
-// Joins the segments along the sequence: slot s + 1 = e^{L_s} slot s + what s
+// Joins the parts along the sequence: slot s + 1 = e^{L_s} slot s + what s
 // added, from H0 (backward: slot s - 1 from slot s, from dH_T). One thread to
-// four elements of one (batch, head).
+// four elements of one (batch, head). Parts before the first segment's end
+// (backward: after the last one's start) have nobody to add for.
 template <int D, bool kBwd>
 __global__ void __launch_bounds__(256) scan_kernel(float* seg, const float* segl, const float* init,
-                                                   long long BH, int nseg, int dk, int dv) {
+                                                   long long BH, int nsub, int steps, int dk, int dv) {
   const long long g = (long long)blockIdx.x * 256 + threadIdx.x;
   const long long bh = g / (D * D / 4);
   if (bh >= BH) return;
@@ -572,11 +695,11 @@ __global__ void __launch_bounds__(256) scan_kernel(float* seg, const float* segl
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     x[i] = init && row < dk && col + i < dv ? init[(bh * dk + row) * dv + col + i] : 0.f;
-  float4* sp = reinterpret_cast<float4*>(seg + bh * nseg * (long long)(D * D)) + e;
-  const float* lp = segl + bh * nseg;
+  float4* sp = reinterpret_cast<float4*>(seg + bh * nsub * (long long)(D * D)) + e;
+  const float* lp = segl + bh * nsub;
 #pragma unroll 4
-  for (int i = 0; i < nseg - 1; ++i) {
-    const int s = kBwd ? nseg - 1 - i : i, to = kBwd ? s - 1 : s + 1;
+  for (int i = 0; i < steps; ++i) {
+    const int s = kBwd ? nsub - 1 - i : i, to = kBwd ? s - 1 : s + 1;
     const float f = ex2(lp[s]);
     float4 u = sp[(long long)to * (D * D / 4)];
     x[0] = fmaf(f, x[0], u.x), x[1] = fmaf(f, x[1], u.y);
@@ -593,47 +716,65 @@ template <typename E, int D>
 struct Fwd {
   static constexpr int NL = kLevels<E>, kTileE = kC * D;
   static constexpr int kY = 128, kP = 128 + D, kCols = kP + 64 * NL <= 256 ? 256 : 512;
+  // bf16: two buffers for Q and K, the next chunk's on their way during this one
+  static constexpr int kBufs = NL == 1 ? 2 : 1;
   static constexpr int kExtra = NL == 1 ? 1 : 0;  // third level of the scaled K rows
-  static constexpr size_t kSmem = kSmallBytes + 2 * ((3 * NL + kExtra) * (size_t)kTileE + NL * (size_t)D * D);
+  static constexpr size_t kSmem =
+      kSmallBytes + 2 * (((2 * kBufs + 1) * NL + kExtra) * (size_t)kTileE + NL * (size_t)D * D);
   static constexpr int kPerSm = 2 * (kSmem + 1024) <= 228 * 1024 && kCols <= 256 ? 2 : 1;
+  static_assert(kSmem <= 227 * 1024, "");
 };
 
 template <typename E, int D>
-__global__ void __launch_bounds__(kThreads, Fwd<E, D>::kPerSm) fwd_kernel(const Args<E> p) {
+__global__ void __launch_bounds__(kThreads, Fwd<E, D>::kPerSm) fwd_kernel(const __grid_constant__ Args<E> p) {
   using F = Fwd<E, D>;
   constexpr int NL = F::NL, kTileE = F::kTileE;
   extern __shared__ __align__(1024) unsigned char smem[];
   Small& sm = *reinterpret_cast<Small*>(smem);
-  bf16* Q = reinterpret_cast<bf16*>(smem + kSmallBytes);
-  bf16 *K = Q + NL * kTileE, *V = K + NL * kTileE, *X = V + (NL + F::kExtra) * kTileE;
-  // the scaled K rows go over K and, below three levels, over Q (read by then) and the extra tile
-  bf16* const lv[3] = {K, NL == 1 ? Q : K + kTileE, NL == 1 ? V + kTileE : NL == 2 ? Q : K + 2 * kTileE};
+  bf16* const Q0 = reinterpret_cast<bf16*>(smem + kSmallBytes);
+  bf16 *const K0 = Q0 + F::kBufs * NL * kTileE, *const V = K0 + F::kBufs * NL * kTileE,
+              *const X = V + (NL + F::kExtra) * kTileE;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q = warp & 3, wg = warp >> 2;
   const long long bh = blockIdx.x % p.BH;
   const int s = (int)(blockIdx.x / p.BH);
-  const long long b = bh / p.H, h = bh % p.H;
-  const E* hq = p.Q.p + b * p.Q.sb + h * p.Q.sh;
-  const E* hk = p.K.p + b * p.K.sb + h * p.K.sh;
-  const E* hv = p.V.p + b * p.V.sb + h * p.V.sh;
-  E* hy = p.y.p + b * p.y.sb + h * p.y.sh;
+  const int b = (int)(bh / p.H), h = (int)(bh % p.H);
   const float* lg = p.lg + b * p.lsb + h * p.lsh;
   const long long dkv = (long long)p.dk * p.dv;
+  const int c0 = s * p.m, c1 = min(c0 + p.m, p.nchunks);
+  auto rows = [&](int c) { return (int)min((long long)kC, p.T - (long long)c * kC); };
+  const bool tma = NL == 1 && p.tma;
+  auto load_v = [&](int c) {  // by one thread
+    mbar_arrive_expect_tx(&sm.full[2], tile_bytes(D));
+    tma_load<D>(V, &p.mV, (long long)c * kC, h, b, &sm.full[2]);
+  };
 
   if (warp == 0) um::alloc(&sm.tbase, F::kCols);
   if (tid == 0) {
     mbar_init(&sm.bar, 1);
+    for (int i = 0; i < 3; ++i) mbar_init(&sm.full[i], 1);
     mbar_fence_init();
+    if (tma) {
+      mbar_arrive_expect_tx(&sm.full[0], 2 * tile_bytes(D));
+      tma_load<D>(Q0, &p.mQ, (long long)c0 * kC, h, b, &sm.full[0]);
+      tma_load<D>(K0, &p.mK, (long long)c0 * kC, h, b, &sm.full[0]);
+      load_v(c0);
+    }
+  }
+  DecayWarp dw;
+  if (warp == kDecayWarp) {
+    dw.load(lg + (long long)c0 * kC * p.lst, p.lst, rows(c0));
+    dw.table<false>(sm.dec);
   }
   State<D> S;
   if (s > 0)
-    S.load_own(p.seg + (bh * p.nseg + s) * (D * D));
+    S.load_own(p.seg + (bh * p.nsub + s * p.r) * (D * D));
   else if (p.H0)
     S.load(p.H0 + bh * dkv, p.dk, p.dv);
   else
     S.zero();
   S.template to_smem<NL>(X);
   // After a wait that runs out (recorded in the sticky word) the CTA issues no
-  // MMA, waits on nothing and writes no output; sync makes the flag common.
+  // MMA or copy, waits on nothing and writes no output; sync makes the flag common.
   bool ok = true;
   auto sync = [&]() {
     fence_proxy_async_smem();
@@ -643,44 +784,68 @@ __global__ void __launch_bounds__(kThreads, Fwd<E, D>::kPerSm) fwd_kernel(const 
   };
   unsigned phase = 0;
   auto wait = [&]() {
-    if (ok) ok = mbar_wait(&sm.bar, phase & 1, &g_sticky_err);
+    if (ok) ok = mbar_wait(&sm.bar, phase & 1, &g_sticky_err, kPolls);
     ++phase;
     um::fence_after();
   };
+  if (tma) sync();  // the barriers
   const int row = 32 * q + lane;
-  const int c0 = s * p.m, c1 = min(c0 + p.m, p.nchunks);
   for (int c = c0; c < c1; ++c) {
+    const int n = rows(c), i_ = c - c0, buf = tma ? i_ & 1 : 0;
     const long long t0 = (long long)c * kC;
-    const int n = (int)min((long long)kC, p.T - t0);
-    load_tile<E, D>(Q, p.Q, hq, t0, n, p.dk);
-    load_tile<E, D>(K, p.K, hk, t0, n, p.dk);
-    load_tile<E, D>(V, p.V, hv, t0, n, p.dv);
-    if (warp == 0) decay_table(lg + t0 * p.lst, p.lst, n, sm.ch, sm.cl);
-    if (p.saved) S.store_own(p.saved + (bh * p.nchunks + c) * (D * D));
-    cp_async_wait_all();
+    const bool more = c + 1 < c1;
+    Decays& dec = sm.dec;
+    bf16 *const Q = Q0 + buf * NL * kTileE, *const K = K0 + buf * NL * kTileE;
+    bf16 *const Qn = Q0 + (buf ^ 1) * NL * kTileE, *const Kn = K0 + (buf ^ 1) * NL * kTileE;
+    // the scaled K rows go over K and, below three levels, over Q (read by then) and the extra tile
+    bf16* const lv[3] = {K, NL == 1 ? Q : K + kTileE, NL == 1 ? V + kTileE : NL == 2 ? Q : K + 2 * kTileE};
+    if (tma) {
+      if (ok) ok = mbar_wait(&sm.full[buf], (i_ >> 1) & 1, &g_sticky_err, kPolls);
+    } else {
+      load_tile<E, D>(Q, p.Q, b, h, t0, n, p.dk);
+      load_tile<E, D>(K, p.K, b, h, t0, n, p.dk);
+      load_tile<E, D>(V, p.V, b, h, t0, n, p.dv);
+    }
     sync();
     const uint32_t tb = sm.tbase;
     if (ok && tid == 0) {
-      product<NL, NL, 128, 128>(tb, op_k(Q, D, kTileE), op_k(K, D, kTileE), D / 16);
-      product<NL, NL, 128, D>(tb + F::kY, op_k(Q, D, kTileE), op_mn(X, D, D * D), D / 16);
+      product<NL, NL, 128, 128>(tb, op_k<D>(Q), op_k<D>(K), D / 16);
+      product<NL, NL, 128, D>(tb + F::kY, op_k<D>(Q), state_mn<D>(X), D / 16);
       um::commit(&sm.bar);
+      if (tma) {
+        if (c > c0) tma_store<D>(&p.my, t0 - kC, h, b, p.dv, Qn);  // the last chunk's y
+        if (more) {
+          mbar_arrive_expect_tx(&sm.full[buf ^ 1], 2 * tile_bytes(D));
+          tma_load<D>(Kn, &p.mK, t0 + kC, h, b, &sm.full[buf ^ 1]);
+        }
+      }
     }
+    if (warp == kDecayWarp && more) dw.load(lg + (t0 + kC) * p.lst, p.lst, rows(c + 1));
+    if (p.saved) S.store_own(p.saved + (bh * p.nchunks + c) * (D * D));
     wait();
     const uint32_t lb = tb + ((uint32_t)(32 * q) << 16);
-    const float rh = sm.ch[row], rl = sm.cl[row];
+    const float rh = dec.ch[row], rl = dec.cl[row];
+    // P = D * Q K^T, every other block of 16 columns to a warp
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {  // P = D * Q K^T, 64 columns to a warp
-      const int j0 = 64 * wg + 16 * k;
+    for (int k = 0; k < 4; ++k) {
+      const int j0 = 32 * k + 16 * wg;
       float v[16];
-      if (j0 > 32 * q + 31) {
+      if (j0 > 32 * q + 31) {  // after every row of the warp
+        if (c > c0) continue;  // zeros from the first chunk on
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = 0.f;
       } else {
         um::ld16(lb + j0, v);
+        if (j0 < 32 * q) {  // before every row
+          const float f = dec.to(rh, rl, j0 + 15);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float f = ex2((rh - sm.ch[j0 + i]) + (rl - sm.cl[j0 + i]));
-          v[i] = j0 + i <= row ? v[i] * f : 0.f;
+          for (int i = 0; i < 16; ++i) v[i] *= f * dec.cf[j0 + i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float f = dec.to(rh, rl, j0 + i);
+            v[i] = j0 + i <= row ? v[i] * f : 0.f;
+          }
         }
       }
       st_levels16<NL>(lb + F::kP + j0 / 2, v);
@@ -698,32 +863,48 @@ __global__ void __launch_bounds__(kThreads, Fwd<E, D>::kPerSm) fwd_kernel(const 
         st16(a, w);
       }
     }
+    if (tma && ok && tid == 0 && more) {
+      bulk_wait_read();  // y has left
+      tma_load<D>(Qn, &p.mQ, t0 + kC, h, b, &sm.full[buf ^ 1]);
+    }
+    const float th = dec.ch[kC - 1], tl = dec.cl[kC - 1];
+    const bool add = more || s + 1 == p.nseg;  // a later chunk of this CTA, or H_T, needs S'
+    if (add) scale_rows<NL, D>(K, lv, [&](int r) { return dec.to(th, tl, r); });
     st_wait();
-    const float th = sm.ch[kC - 1], tl = sm.cl[kC - 1];
-    const bool add = c + 1 < c1 || s + 1 == p.nseg;  // a later chunk of this CTA, or H_T, needs S'
-    if (add)
-      scale_rows<NL, D>(K, lv, [&](int r) { return ex2((th - sm.ch[r]) + (tl - sm.cl[r])); });
     sync();
     if (ok && tid == 0) {
-      product_ta<NL, NL, D>(tb + F::kY, tb + F::kP, op_mn(V, D, kTileE), true);
-      if (add) product_rows<NL, D>(tb, lv, V, false);
-      um::commit(&sm.bar);
-    }
-    wait();
-    if (ok) {
-#pragma unroll
-      for (int k = 0; k < D / 32; ++k) {
-        const int j0 = wg * (D / 2) + 16 * k;
-        float v[16];
-        um::ld16(lb + F::kY + j0, v);
-        if (row < n) store_row16<E>(hy + (t0 + row) * p.y.st, j0, p.dv, p.y.vec, v);
+      if (tma) ok = mbar_wait(&sm.full[2], i_ & 1, &g_sticky_err, kPolls);
+      if (ok) {
+        product_ta<NL, NL, D>(tb + F::kY, tb + F::kP, op_mn<D>(V), true);
+        if (add) product_rows<NL, D>(tb, lv, V, false);
+        um::commit(&sm.bar);
       }
+    }
+    if (warp == kDecayWarp && more) dw.table<false>(dec);
+    wait();
+    if (tma && ok && tid == 0 && more) load_v(c + 1);
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) {
+      const int j0 = wg * (D / 2) + 16 * k;
+      float v[16];
+      um::ld16(lb + F::kY + j0, v);
+      if (tma)
+        row16_to_tile(Q, row, j0, v);
+      else if (ok && row < n)
+        store_row16<E>(p.y.p + b * p.y.sb + h * p.y.sh + (t0 + row) * p.y.st, j0, p.dv, p.y, v);
     }
     if (add) {
       S.update(ex2(th + tl), tb, 0);
       S.template to_smem<NL>(X);
     }
+    if (!tma) sync();  // the tiles are loaded over at once
+  }
+  if (tma) {
     sync();
+    if (ok && tid == 0) {
+      tma_store<D>(&p.my, (long long)(c1 - 1) * kC, h, b, p.dv, Q0 + ((c1 - 1 - c0) & 1) * NL * kTileE);
+      bulk_wait_read();
+    }
   }
   if (ok && s + 1 == p.nseg) S.store(p.HT + bh * dkv, p.dk, p.dv);
   um::fence_before();
@@ -734,14 +915,13 @@ __global__ void __launch_bounds__(kThreads, Fwd<E, D>::kPerSm) fwd_kernel(const 
 // --------------------------------------------------------------- backward --
 
 struct SmallB {
-  uint64_t bar;
+  uint64_t bar, bar2, full;
   uint32_t tbase;
   float dot;
-  float ch[kC], cl[kC];  // decay table; at the end of a chunk what a token adds to later ones
-  float a[2][kC];        // per half: what token i adds to dlog_gamma_t for t <= i
+  float a[2][kC];  // per half: what token i adds to dlog_gamma_t for t <= i
+  Decays dec[1];   // two where there is room; ch and cl end as what a token adds to later ones
 };
-constexpr int kSmallB = 3072;
-static_assert(sizeof(SmallB) <= kSmallB, "");
+static_assert(sizeof(SmallB) <= 3072, "");
 
 // NL = 1: 64 masked products of a lane's row, rounded and packed while both
 // accumulators are still being read; NL > 1: as they are.
@@ -761,13 +941,13 @@ struct Held {
       }
     }
   }
-  __device__ __forceinline__ void store(uint32_t taddr) const {
+  __device__ __forceinline__ void store(uint32_t taddr, int wg) const {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < 4; ++k) {  // block 2 k + wg: eight packed columns each
       if constexpr (NL == 1)
-        st8(taddr + 8 * k, v + 8 * k);
+        st8(taddr + 16 * k + 8 * wg, v + 8 * k);
       else
-        st_levels16<NL>(taddr + 8 * k, v + 16 * k);
+        st_levels16<NL>(taddr + 16 * k + 8 * wg, v + 16 * k);
     }
   }
 };
@@ -785,48 +965,93 @@ struct Bwd {
   static constexpr int kDq = 64 * NL, kIq = kDq + D;
   static constexpr int kCols = kDk + D <= 256 ? 256 : 512;
   static_assert(kDk + D <= 512 && kIk + D <= 512 && kIq + D <= kCols, "");
-  // dS rests in shared memory between its uses where two CTAs share an SM's registers
-  static constexpr bool kPark = NL == 1 && D == 64;
+  // Two CTAs to an SM: dS is spread over all threads (16 entries each), and a
+  // tile of its own stages the gradients on their way out.
+  static constexpr bool kEven = NL == 1 && D == 64;
+  static constexpr int kTabs = D == 64 ? 2 : 1;
+  static constexpr size_t kSmallB = kTabs == 2 ? 5120 : 3072;
   static constexpr size_t kSmem =
-      kSmallB + 2 * (4 * NL * (size_t)kTileE + 3 * (size_t)D * D) + (kPark ? 4 * D * D : 0);
+      kSmallB + 2 * ((4 * NL + (kEven ? 1 : 0)) * (size_t)kTileE + 3 * (size_t)D * D);
+  static_assert(sizeof(SmallB) + (kTabs - 1) * sizeof(Decays) <= kSmallB && kSmem <= 227 * 1024, "");
   static constexpr int kPerSm = 2 * (kSmem + 1024) <= 228 * 1024 && kCols <= 256 ? 2 : 1;
 };
 template <typename E, int D>
-__global__ void __launch_bounds__(kThreads, Bwd<E, D>::kPerSm) bwd_kernel(const Args<E> p) {
+__global__ void __launch_bounds__(kThreads, Bwd<E, D>::kPerSm) bwd_kernel(const __grid_constant__ Args<E> p) {
   using F = Bwd<E, D>;
   constexpr int NL = F::NL, kTileE = F::kTileE;
   extern __shared__ __align__(1024) unsigned char smem[];
   SmallB& sm = *reinterpret_cast<SmallB*>(smem);
-  bf16* Q = reinterpret_cast<bf16*>(smem + kSmallB);
+  bf16* Q = reinterpret_cast<bf16*>(smem + F::kSmallB);
   bf16 *K = Q + NL * kTileE, *V = K + NL * kTileE, *G = V + NL * kTileE, *X = G + NL * kTileE;
+  bf16* stage = X + 3 * D * D;
   // the scaled Q rows go over Q and, below three levels, over K and V (read by then)
   bf16* const lv[3] = {Q, NL == 1 ? K : Q + kTileE, NL == 1 ? V : NL == 2 ? K : Q + 2 * kTileE};
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q = warp & 3, wg = warp >> 2;
   const long long bh = blockIdx.x % p.BH;
   const int s = p.nseg - 1 - (int)(blockIdx.x / p.BH);
-  const long long b = bh / p.H, h = bh % p.H;
-  const E* hq = p.Q.p + b * p.Q.sb + h * p.Q.sh;
-  const E* hk = p.K.p + b * p.K.sb + h * p.K.sh;
-  const E* hv = p.V.p + b * p.V.sb + h * p.V.sh;
-  const E* hg = p.dy.p + b * p.dy.sb + h * p.dy.sh;
+  const int b = (int)(bh / p.H), h = (int)(bh % p.H);
   const float* lg = p.lg + b * p.lsb + h * p.lsh;
   const long long dkv = (long long)p.dk * p.dv;
+  const int c0 = s * p.m, c1 = min(c0 + p.m, p.nchunks);
+  auto rows = [&](int c) { return (int)min((long long)kC, p.T - (long long)c * kC); };
+  const bool tma = NL == 1 && p.tma, staged = F::kEven && p.tma;
+  auto load = [&](int c) {  // by one thread
+    mbar_arrive_expect_tx(&sm.full, 4 * tile_bytes(D));
+    tma_load<D>(K, &p.mK, (long long)c * kC, h, b, &sm.full);
+    tma_load<D>(Q, &p.mQ, (long long)c * kC, h, b, &sm.full);
+    tma_load<D>(V, &p.mV, (long long)c * kC, h, b, &sm.full);
+    tma_load<D>(G, &p.mdy, (long long)c * kC, h, b, &sm.full);
+  };
 
   if (warp == 0) um::alloc(&sm.tbase, F::kCols);
   if (tid == 0) {
     mbar_init(&sm.bar, 1);
+    mbar_init(&sm.bar2, 1);
+    mbar_init(&sm.full, 1);
     mbar_fence_init();
+    if (tma) load(c1 - 1);
   }
-  float* park = reinterpret_cast<float*>(X + 3 * D * D);
+  DecayWarp dw;
+  if (F::kTabs == 2 && warp == kDecayWarp) {
+    dw.load(lg + (long long)(c1 - 1) * kC * p.lst, p.lst, rows(c1 - 1));
+    dw.table<true>(sm.dec[(c1 - 1) & 1]);
+  }
+  // dS: kEven, 16 entries of one row to a thread; otherwise as accumulators are read
+  const int erow = tid & 63, ecol = (tid >> 6) * 16;
+  auto even_own = [&](const float* src, float (&v)[16]) {  // from a state in its own order
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const float4 f = *reinterpret_cast<const float4*>(src + (((ecol + i) / 4) * D + erow) * 4);
+      v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
+    }
+  };
+  auto even_to_smem = [&](const float (&v)[16]) {
+    store_levels8<3>(X, D * D, sw<D>(erow, ecol), v);
+    store_levels8<3>(X, D * D, sw<D>(erow, ecol + 8), v + 8);
+  };
+  float dSe[16];
   State<D> dS;
-  if (s + 1 < p.nseg)
-    dS.load_own(p.seg + (bh * p.nseg + s) * (D * D));
-  else if (p.dHT)
-    dS.load(p.dHT + bh * dkv, p.dk, p.dv);
-  else
-    dS.zero();
-  dS.template to_smem<3>(X);
-  if (F::kPark) dS.store_own(park);
+  {
+    const float* end = s + 1 < p.nseg ? p.seg + (bh * p.nsub + (s + 1) * p.r - 1) * (D * D) : nullptr;
+    if constexpr (F::kEven) {
+      if (end) {
+        even_own(end, dSe);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          dSe[i] = p.dHT && erow < p.dk && ecol + i < p.dv ? p.dHT[bh * dkv + erow * p.dv + ecol + i] : 0.f;
+      }
+      even_to_smem(dSe);
+    } else {
+      if (end)
+        dS.load_own(end);
+      else if (p.dHT)
+        dS.load(p.dHT + bh * dkv, p.dk, p.dv);
+      else
+        dS.zero();
+      dS.template to_smem<3>(X);
+    }
+  }
   bool ok = true;
   auto sync = [&]() {
     fence_proxy_async_smem();
@@ -836,33 +1061,57 @@ __global__ void __launch_bounds__(kThreads, Bwd<E, D>::kPerSm) bwd_kernel(const 
   };
   unsigned phase = 0;
   auto wait = [&]() {
-    if (ok) ok = mbar_wait(&sm.bar, phase & 1, &g_sticky_err);
+    if (ok) ok = mbar_wait(&sm.bar, phase & 1, &g_sticky_err, kPolls);
     ++phase;
     um::fence_after();
   };
+  if (tma) sync();  // the barriers
   const int row = 32 * q + lane;
-  const int c0 = s * p.m, c1 = min(c0 + p.m, p.nchunks);
   for (int c = c1 - 1; c >= c0; --c) {
     const long long t0 = (long long)c * kC;
-    const int n = (int)min((long long)kC, p.T - t0);
-    load_tile<E, D>(Q, p.Q, hq, t0, n, p.dk);
-    load_tile<E, D>(K, p.K, hk, t0, n, p.dk);
-    load_tile<E, D>(V, p.V, hv, t0, n, p.dv);
-    load_tile<E, D>(G, p.dy, hg, t0, n, p.dv);
-    if (warp == 0) decay_table(lg + t0 * p.lst, p.lst, n, sm.ch, sm.cl);
-    cp_async_wait_all();
+    const int n = rows(c), turn = (c1 - 1 - c) & 1;
+    const bool more = c > c0;
+    Decays& dec = sm.dec[F::kTabs == 2 ? c & 1 : 0];
+    if (F::kTabs == 1 && warp == 0) {
+      dw.load(lg + t0 * p.lst, p.lst, n);
+      dw.table<true>(dec);
+    }
+    if (tma) {
+      if (ok) ok = mbar_wait(&sm.full, turn, &g_sticky_err, kPolls);
+    } else {
+      load_tile<E, D>(K, p.K, b, h, t0, n, p.dk);
+      load_tile<E, D>(Q, p.Q, b, h, t0, n, p.dk);
+      load_tile<E, D>(V, p.V, b, h, t0, n, p.dv);
+      load_tile<E, D>(G, p.dy, b, h, t0, n, p.dv);
+    }
     sync();
     const uint32_t tb = sm.tbase, lb = tb + ((uint32_t)(32 * q) << 16);
-    const Op kQ = op_k(Q, D, kTileE), kK = op_k(K, D, kTileE), kV = op_k(V, D, kTileE),
-             kG = op_k(G, D, kTileE);
     if (ok && tid == 0) {
-      product<NL, NL, 128, 128>(tb, kK, kQ, D / 16);
-      product<NL, NL, 128, 128>(tb + 128, kV, kG, D / 16);
+      product<NL, NL, 128, 128>(tb, op_k<D>(K), op_k<D>(Q), D / 16);
+      product<NL, NL, 128, 128>(tb + 128, op_k<D>(V), op_k<D>(G), D / 16);
       um::commit(&sm.bar);
+      if (tma && more) {  // the next chunk's rows and state on their way into L2
+        tma_prefetch<D>(&p.mK, t0 - kC, h, b, p.dk);
+        tma_prefetch<D>(&p.mQ, t0 - kC, h, b, p.dk);
+        tma_prefetch<D>(&p.mV, t0 - kC, h, b, p.dv);
+        tma_prefetch<D>(&p.mdy, t0 - kC, h, b, p.dv);
+      }
+    }
+    if (!tma && more) {
+      prefetch_rows(p.Q, b, h, t0 - kC, kC, p.dk);
+      prefetch_rows(p.K, b, h, t0 - kC, kC, p.dk);
+      prefetch_rows(p.V, b, h, t0 - kC, kC, p.dv);
+      prefetch_rows(p.dy, b, h, t0 - kC, kC, p.dv);
+    }
+    if (tid < D * D / 32)  // the state that entered this chunk: 128 bytes to a thread
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(p.saved + (bh * p.nchunks + c) * (D * D) + tid * 32));
+    if (F::kTabs == 2 && warp == kDecayWarp && more) {
+      dw.load(lg + (t0 - kC) * p.lst, p.lst, kC);
+      dw.table<true>(sm.dec[(c - 1) & 1]);
     }
     wait();
-    const float rh = sm.ch[row], rl = sm.cl[row], th = sm.ch[kC - 1], tl = sm.cl[kC - 1];
-    const float to_end = ex2((th - rh) + (tl - rl)), from_start = ex2(rh + rl);
+    const float rh = dec.ch[row], rl = dec.cl[row], th = dec.ch[kC - 1], tl = dec.cl[kC - 1];
+    const float to_end = dec.to(th, tl, row), from_start = ex2(rh + rl);
     float tok = 0.f;  // this half's part of what token `row` adds for t <= row
     float bk = 0.f;   // what it adds for t > row
     {
@@ -870,9 +1119,9 @@ __global__ void __launch_bounds__(kThreads, Bwd<E, D>::kPerSm) bwd_kernel(const 
       Held<NL> a1, a2;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int i0 = 64 * wg + 16 * k;
+        const int i0 = 32 * k + 16 * wg;
         float x[16], z[16];
-        if (i0 + 15 < 32 * q) {
+        if (i0 + 15 < 32 * q) {  // before every row of the warp
 #pragma unroll
           for (int i = 0; i < 16; ++i) x[i] = z[i] = 0.f;
         } else {
@@ -882,38 +1131,49 @@ __global__ void __launch_bounds__(kThreads, Bwd<E, D>::kPerSm) bwd_kernel(const 
           um::ld_wait();
           um::ld_bind(r1, x);
           um::ld_bind(r2, z);
+          if (i0 > 32 * q + 31) {  // after every row
+            const float f0 = dec.from(rh, rl, i0);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float f = ex2((sm.ch[i0 + i] - rh) + (sm.cl[i0 + i] - rl));
-            const float pf = x[i] * f;
-            tok -= i0 + i > row ? pf * z[i] : 0.f;
-            x[i] = i0 + i >= row ? pf : 0.f;
-            z[i] = i0 + i >= row ? z[i] * f : 0.f;
+            for (int i = 0; i < 16; ++i) {
+              const float f = f0 * dec.cf[i0 + i];
+              x[i] *= f;
+              tok = fmaf(-x[i], z[i], tok);
+              z[i] *= f;
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float f = dec.from(rh, rl, i0 + i);
+              const float pf = x[i] * f;
+              tok -= i0 + i > row ? pf * z[i] : 0.f;
+              x[i] = i0 + i >= row ? pf : 0.f;
+              z[i] = i0 + i >= row ? z[i] * f : 0.f;
+            }
           }
         }
         a2.set(k, x);
         a1.set(k, z);
       }
       sync();  // both products have been read
-      a2.store(lb + 32 * wg);
-      a1.store(lb + 64 * NL + 32 * wg);
+      a2.store(lb, wg);
+      a1.store(lb + 64 * NL, wg);
       st_wait();
     }
     sync();
     if (ok && tid == 0) {
-      product_ta<NL, NL, D>(tb + F::kDv, tb, op_mn(G, D, kTileE), false);
-      product_ta<NL, NL, D>(tb + F::kDk, tb + 64 * NL, op_mn(Q, D, kTileE), false);
+      product_ta<NL, NL, D>(tb + F::kDv, tb, op_mn<D>(G), false);
+      product_ta<NL, NL, D>(tb + F::kDk, tb + 64 * NL, op_mn<D>(Q), false);
       um::commit(&sm.bar);
     }
     wait();
     if (ok && tid == 0) {
-      product<NL, 3, 128, D>(tb + F::kIv, kK, op_mn(X, D, D * D), D / 16);
-      product<NL, 3, 128, D>(tb + F::kIk, kV, op_k(X, D, D * D), D / 16);
-      um::commit(&sm.bar);
+      product<NL, 3, 128, D>(tb + F::kIv, op_k<D>(K), state_mn<D>(X), D / 16);
+      product<NL, 3, 128, D>(tb + F::kIk, op_k<D>(V), state_k<D>(X), D / 16);
+      um::commit(&sm.bar2);
     }
-    wait();
-    E* gv = p.dV.p + b * p.dV.sb + h * p.dV.sh + (t0 + row) * p.dV.st;
-    E* gk = p.dK.p + b * p.dK.sb + h * p.dK.sh + (t0 + row) * p.dK.st;
+    if (ok) ok = mbar_wait(&sm.bar2, turn, &g_sticky_err, kPolls);
+    um::fence_after();
+    uint32_t dkp[F::kEven ? 16 : 1];  // dK, packed, until the stage is free
 #pragma unroll
     for (int k = 0; k < D / 32; ++k) {
       const int j0 = wg * (D / 2) + 16 * k;
@@ -926,41 +1186,65 @@ __global__ void __launch_bounds__(kThreads, Bwd<E, D>::kPerSm) bwd_kernel(const 
       um::ld_bind(r2, z);
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] = fmaf(to_end, z[i], x[i]);
-      if (ok && row < n) store_row16<E>(gv, j0, p.dv, p.dV.vec, x);
+      if (staged)
+        row16_to_tile(stage, row, j0, x);
+      else if (ok && row < n)
+        store_row16<E>(p.dV.p + b * p.dV.sb + h * p.dV.sh + (t0 + row) * p.dV.st, j0, p.dv, p.dV, x);
       um::ld16_async(lb + F::kDk + j0, r1);
       um::ld16_async(lb + F::kIk + j0, r2);
       um::ld_wait();
       um::ld_bind(r1, x);
       um::ld_bind(r2, z);
       float kr[16];
-      load_levels8<NL>(K, kTileE, um::boff_n(row, j0, D), kr);
-      load_levels8<NL>(K, kTileE, um::boff_n(row, j0 + 8, D), kr + 8);
+      load_levels8<NL>(K, kTileE, sw<kC>(row, j0), kr);
+      load_levels8<NL>(K, kTileE, sw<kC>(row, j0 + 8), kr + 8);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         bk = fmaf(kr[i], z[i], bk);
         x[i] = fmaf(to_end, z[i], x[i]);
       }
-      if (ok && row < n) store_row16<E>(gk, j0, p.dk, p.dK.vec, x);
+      if (staged) {
+        if constexpr (F::kEven) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const __nv_bfloat162 u = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+            dkp[8 * k + i] = *reinterpret_cast<const uint32_t*>(&u);
+          }
+        }
+      } else if (ok && row < n) {
+        store_row16<E>(p.dK.p + b * p.dK.sb + h * p.dK.sh + (t0 + row) * p.dK.st, j0, p.dk, p.dK, x);
+      }
     }
     bk *= to_end;
     {  // S, the state that entered the chunk, takes dS's place in shared memory
-      State<D> S;
-      S.load_own(p.saved + (bh * p.nchunks + c) * (D * D));
-      if (F::kPark) dS.load_own(park);
+      const float* src = p.saved + (bh * p.nchunks + c) * (D * D);
       float d = 0.f;
+      if constexpr (F::kEven) {
+        float v[16];
+        even_own(src, v);
+        even_to_smem(v);
 #pragma unroll
-      for (int i = 0; i < State<D>::kCols; ++i) d = fmaf(S.v[i], dS.v[i], d);
-      if (!State<D>::valid()) d = 0.f;  // lanes without a row hold what their TMEM lanes held
-      S.template to_smem<3>(X);
+        for (int i = 0; i < 16; ++i) d = fmaf(v[i], dSe[i], d);
+      } else {
+        State<D> S;
+        S.load_own(src);
+#pragma unroll
+        for (int i = 0; i < State<D>::kCols; ++i) d = fmaf(S.v[i], dS.v[i], d);
+        if (!State<D>::valid()) d = 0.f;  // lanes without a row hold what their TMEM lanes held
+        S.template to_smem<3>(X);
+      }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
       if (lane == 0) sm.a[0][warp] = d;  // joined below, in order
     }
+    // from here on a token's factor is to its block's end
+    if (tid < kC) dec.cf[tid] = dec.to(dec.ch[tid | 15], dec.cl[tid | 15], tid);
     sync();
     if (ok && tid == 0) {
-      product<NL, NL, 128, 128>(tb, kG, kV, D / 16);
-      product<NL, NL, 128, 128>(tb + 128, kQ, kK, D / 16);
+      product<NL, NL, 128, 128>(tb, op_k<D>(G), op_k<D>(V), D / 16);
+      product<NL, NL, 128, 128>(tb + 128, op_k<D>(Q), op_k<D>(K), D / 16);
       um::commit(&sm.bar);
+      if (staged) tma_store<D>(&p.mdV, t0, h, b, p.dv, stage);
     }
     if (tid == 32) {
       float d = 0.f;
@@ -973,9 +1257,9 @@ __global__ void __launch_bounds__(kThreads, Bwd<E, D>::kPerSm) bwd_kernel(const 
       Held<NL> a1;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int j0 = 64 * wg + 16 * k;
+        const int j0 = 32 * k + 16 * wg;
         float x[16], z[16];
-        if (j0 > 32 * q + 31) {
+        if (j0 > 32 * q + 31) {  // after every row of the warp
 #pragma unroll
           for (int i = 0; i < 16; ++i) z[i] = 0.f;
         } else {
@@ -985,29 +1269,48 @@ __global__ void __launch_bounds__(kThreads, Bwd<E, D>::kPerSm) bwd_kernel(const 
           um::ld_wait();
           um::ld_bind(r1, z);
           um::ld_bind(r2, x);
+          if (j0 < 32 * q) {  // before every row
+            const float f0 = dec.to(rh, rl, j0 + 15);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float f = ex2((rh - sm.ch[j0 + i]) + (rl - sm.cl[j0 + i]));
-            const float zf = z[i] * f;
-            tok += j0 + i < row ? zf * x[i] : 0.f;
-            z[i] = j0 + i <= row ? zf : 0.f;
+            for (int i = 0; i < 16; ++i) {
+              z[i] *= f0 * dec.cf[j0 + i];
+              tok = fmaf(z[i], x[i], tok);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float f = dec.to(rh, rl, j0 + i);
+              const float zf = z[i] * f;
+              tok += j0 + i < row ? zf * x[i] : 0.f;
+              z[i] = j0 + i <= row ? zf : 0.f;
+            }
           }
         }
         a1.set(k, z);
       }
+      if (staged && tid == 0) bulk_wait_read();  // dV has left the stage
       sync();
-      a1.store(lb + 32 * wg);
+      a1.store(lb, wg);
+      if constexpr (F::kEven) {
+        if (staged) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint4*>(stage + sw<kC>(row, wg * (D / 2) + 8 * i)) =
+                make_uint4(dkp[4 * i], dkp[4 * i + 1], dkp[4 * i + 2], dkp[4 * i + 3]);
+        }
+      }
       st_wait();
     }
     sync();
     if (ok && tid == 0) {
-      product_ta<NL, NL, D>(tb + F::kDq, tb, op_mn(K, D, kTileE), false);
-      product<NL, 3, 128, D>(tb + F::kIq, kG, op_k(X, D, D * D), D / 16);
+      product_ta<NL, NL, D>(tb + F::kDq, tb, op_mn<D>(K), false);
+      product<NL, 3, 128, D>(tb + F::kIq, op_k<D>(G), state_k<D>(X), D / 16);
       um::commit(&sm.bar);
+      if (staged) tma_store<D>(&p.mdK, t0, h, b, p.dk, stage);
     }
     wait();
-    E* gq = p.dQ.p + b * p.dQ.sb + h * p.dQ.sh + (t0 + row) * p.dQ.st;
     float aq = 0.f;
+    uint32_t dqp[F::kEven ? 16 : 1];
 #pragma unroll
     for (int k = 0; k < D / 32; ++k) {
       const int j0 = wg * (D / 2) + 16 * k;
@@ -1018,31 +1321,67 @@ __global__ void __launch_bounds__(kThreads, Bwd<E, D>::kPerSm) bwd_kernel(const 
       um::ld_wait();
       um::ld_bind(r1, x);
       um::ld_bind(r2, z);
-      load_levels8<NL>(Q, kTileE, um::boff_n(row, j0, D), qr);
-      load_levels8<NL>(Q, kTileE, um::boff_n(row, j0 + 8, D), qr + 8);
+      load_levels8<NL>(Q, kTileE, sw<kC>(row, j0), qr);
+      load_levels8<NL>(Q, kTileE, sw<kC>(row, j0 + 8), qr + 8);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         aq = fmaf(qr[i], z[i], aq);
         x[i] = fmaf(from_start, z[i], x[i]);
       }
-      if (ok && row < n) store_row16<E>(gq, j0, p.dk, p.dQ.vec, x);
+      if (staged) {
+        if constexpr (F::kEven) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const __nv_bfloat162 u = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+            dqp[8 * k + i] = *reinterpret_cast<const uint32_t*>(&u);
+          }
+        }
+      } else if (ok && row < n) {
+        store_row16<E>(p.dQ.p + b * p.dQ.sb + h * p.dQ.sh + (t0 + row) * p.dQ.st, j0, p.dk, p.dQ, x);
+      }
     }
     sm.a[wg][row] = fmaf(from_start, aq, tok);
+    if (staged && tid == 0) bulk_wait_read();  // dK has left the stage
     sync();
-    scale_rows<NL, D>(Q, lv, [&](int r) { return ex2(sm.ch[r] + sm.cl[r]); });
+    if constexpr (F::kEven) {
+      if (staged) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<uint4*>(stage + sw<kC>(row, wg * (D / 2) + 8 * i)) =
+              make_uint4(dqp[4 * i], dqp[4 * i + 1], dqp[4 * i + 2], dqp[4 * i + 3]);
+      }
+    }
+    scale_rows<NL, D>(Q, lv, [&](int r) { return ex2(dec.ch[r] + dec.cl[r]); });
     sync();
     if (ok && tid == 0) {
       product_rows<NL, D>(tb, lv, G, false);
       um::commit(&sm.bar);
+      if (staged) tma_store<D>(&p.mdQ, t0, h, b, p.dk, stage);
     }
-    (wg == 0 ? sm.ch : sm.cl)[row] = bk;  // the decay table has been used
+    (wg == 0 ? dec.ch : dec.cl)[row] = bk;  // the decay table has been used
     wait();
+    if (tma && ok && tid == 0) {
+      if (staged) bulk_wait_read();  // dQ has left the stage
+      if (more) load(c - 1);
+    }
     const float g = ex2(th + tl);
-    if (F::kPark) dS.load_own(park);
-    dS.update(g, tb, 0);
-    dS.template to_smem<3>(X);
-    if (F::kPark) dS.store_own(park);
-    sync();
+    if constexpr (F::kEven) {  // the sum goes over X in its own order, then to all threads
+      State<D> u;
+      u.zero();
+      u.update(0.f, tb, 0);
+      u.store_own(reinterpret_cast<float*>(X));
+      sync();
+      float v[16];
+      even_own(reinterpret_cast<const float*>(X), v);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) dSe[i] = fmaf(g, dSe[i], v[i]);
+      sync();
+      even_to_smem(dSe);
+    } else {
+      dS.update(g, tb, 0);
+      dS.template to_smem<3>(X);
+      sync();
+    }
     if (warp == 0 && ok) {
       // Token i adds a to dlog_gamma_t for t <= i and bk for t > i: four tokens to a lane,
       // a summed from the end and bk from the start.
@@ -1053,7 +1392,7 @@ __global__ void __launch_bounds__(kThreads, Bwd<E, D>::kPerSm) bwd_kernel(const 
         ra += (double)sm.a[0][e] + (double)sm.a[1][e];
         va[3 - i] = ra;
         vb[i] = rb;
-        rb += (double)sm.ch[f] + (double)sm.cl[f];
+        rb += (double)dec.ch[f] + (double)dec.cl[f];
       }
       double ia = ra, ib = rb;
 #pragma unroll
@@ -1074,7 +1413,15 @@ __global__ void __launch_bounds__(kThreads, Bwd<E, D>::kPerSm) bwd_kernel(const 
     }
     __syncwarp();
   }
-  if (ok && s == 0 && p.dH0) dS.store(p.dH0 + bh * dkv, p.dk, p.dv);
+  if (ok && s == 0 && p.dH0) {
+    if constexpr (F::kEven) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (erow < p.dk && ecol + i < p.dv) p.dH0[bh * dkv + erow * p.dv + ecol + i] = dSe[i];
+    } else {
+      dS.store(p.dH0 + bh * dkv, p.dk, p.dv);
+    }
+  }
   um::fence_before();
   __syncthreads();
   if (warp == 0) um::dealloc(sm.tbase, F::kCols);
@@ -1083,7 +1430,7 @@ __global__ void __launch_bounds__(kThreads, Bwd<E, D>::kPerSm) bwd_kernel(const 
 // ------------------------------------------------------------------- host --
 
 struct Plan {
-  int D, nchunks, m, nseg;
+  int D, nchunks, m, nseg, ms, r, nsub;
 };
 
 int sm_count() {
@@ -1096,16 +1443,25 @@ int sm_count() {
   return n;
 }
 
-// Segments: as many as there are places for CTAs, whole chunks to each.
-Plan plan_for(long long BH, long long T, int D, int per_sm) {
-  Plan pl;
+// Segments: as many as there are places for CTAs of the main kernel, whole
+// chunks to each. For the state sums, whose CTAs are smaller, segments split
+// again while the parts have places.
+Plan plan_for(long long BH, long long T, int D, int per_sm, int sums_per_sm) {
+  Plan pl{};
   pl.D = D;
   pl.nchunks = (int)((T + kC - 1) / kC);
-  const long long places = (long long)sm_count() * per_sm;
-  long long want = BH > 0 ? places / BH : 1;
+  if (BH <= 0 || pl.nchunks <= 0) return pl;
+  long long want = (long long)sm_count() * per_sm / BH;
   want = want < 1 ? 1 : want > pl.nchunks ? pl.nchunks : want;
-  pl.m = want > 0 ? (int)((pl.nchunks + want - 1) / want) : 1;
-  pl.nseg = pl.m > 0 ? (pl.nchunks + pl.m - 1) / pl.m : 0;
+  pl.m = (int)((pl.nchunks + want - 1) / want);
+  pl.nseg = (pl.nchunks + pl.m - 1) / pl.m;
+  pl.ms = pl.m, pl.r = 1, pl.nsub = pl.nseg;
+  if (pl.nseg > 1) {
+    long long r = (long long)sm_count() * sums_per_sm / (BH * (pl.nseg - 1));
+    r = r < 1 ? 1 : r > pl.m ? pl.m : r;
+    while (pl.m % r) --r;  // equal parts, so that segments begin where parts do
+    pl.r = (int)r, pl.ms = pl.m / pl.r, pl.nsub = pl.nseg * pl.r;
+  }
   return pl;
 }
 
@@ -1123,7 +1479,12 @@ int by_shape(int dtype, int dk, int dv, F&& f) {
 }
 
 size_t seg_bytes(const Plan& pl, long long BH) {
-  return pl.nseg > 1 ? (size_t)BH * pl.nseg * ((size_t)pl.D * pl.D + 1) * sizeof(float) : 0;
+  return pl.nseg > 1 ? (size_t)BH * pl.nsub * ((size_t)pl.D * pl.D + 1) * sizeof(float) : 0;
+}
+
+template <typename E, int D>
+Plan plan_of(bool fwd, long long BH, long long T) {
+  return plan_for(BH, T, D, fwd ? Fwd<E, D>::kPerSm : Bwd<E, D>::kPerSm, Sums<E, D>::kPerSm);
 }
 
 bool shape_ok(int64_t B, int H, int64_t T, int dk, int dv) {
@@ -1131,12 +1492,39 @@ bool shape_ok(int64_t B, int H, int64_t T, int dk, int dv) {
          (B == 0 || H == 0 || B <= 0x7fffffffLL / H);
 }
 
+// Whether every row starts on `bytes` and holds whole groups of them (of 8
+// elements at least).
+template <typename P>
+bool whole(P* p, const int64_t* s, int d, int bytes) {
+  const long long e = bytes / (int)sizeof(P);
+  return reinterpret_cast<uintptr_t>(p) % bytes == 0 && d % (e > 8 ? e : 8) == 0 && s[0] % e == 0 &&
+         s[1] % e == 0 && s[2] % e == 0;
+}
 template <typename P>
 Ten<P> ten(P* p, const int64_t* s, int d) {
-  const long long e = 16 / sizeof(P);
-  const bool vec = reinterpret_cast<uintptr_t>(p) % 16 == 0 && d % 8 == 0 && s[0] % e == 0 &&
-                   s[1] % e == 0 && s[2] % e == 0;
-  return {p, (long long)s[0], (long long)s[1], (long long)s[2], vec ? 1 : 0};
+  const bool vec = whole(p, s, d, 16);
+  return {p, (long long)s[0], (long long)s[1], (long long)s[2], vec, vec && whole(p, s, d, 32)};
+}
+
+// Tensor map over (columns, time, head, batch) with boxes of 64 columns x 128
+// tokens; false where the tensor does not lie as a map can say: addresses and
+// strides in whole 16 bytes, no stride of zero, extents of 32 bits.
+template <typename P>
+bool map_of(CUtensorMap* m, const Ten<P>& x, int d, long long T, long long H, long long B) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  const long long s[3] = {x.st, x.sh, x.sb}, n[3] = {T, H, B};
+  cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)T, (cuuint64_t)H, (cuuint64_t)B}, strides[3];
+  bool ok = fn != nullptr && reinterpret_cast<uintptr_t>(x.p) % 16 == 0 && T < (1ll << 31);
+  for (int i = 0; i < 3; ++i) {
+    const long long bytes = s[i] * (long long)sizeof(P);
+    ok = ok && (n[i] == 1 || (bytes > 0 && bytes % 16 == 0 && bytes < (1ll << 40)));
+    strides[i] = n[i] == 1 ? 16 * (cuuint64_t)((d * sizeof(P) + 15) / 16) : (cuuint64_t)bytes;
+  }
+  if (!ok) return false;
+  const cuuint32_t box[4] = {64u, (cuuint32_t)kC, 1u, 1u}, step[4] = {1u, 1u, 1u, 1u};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(static_cast<const void*>(x.p)), dims,
+            strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename K>
@@ -1151,14 +1539,14 @@ int launched() { return cudaGetLastError() == cudaSuccess ? MGS_OK : MGS_LAUNCH_
 template <typename E, int D, bool kBwd>
 int run_segments(const Args<E>& a, cudaStream_t st) {
   if (a.nseg <= 1) return MGS_OK;
-  constexpr size_t smem = kSmallBytes + 2 * (3 + kLevels<E>)*(size_t)(kC * D);
+  constexpr size_t smem = Sums<E, D>::kSmem;
   auto k1 = state_kernel<E, D, kBwd>;
   if (int r = set_smem(k1, smem)) return r;
-  k1<<<(unsigned)(a.BH * (a.nseg - 1)), kThreads, smem, st>>>(a);
+  k1<<<(unsigned)(a.BH * (a.nseg - 1) * a.r), kThreads, smem, st>>>(a);
   if (int r = launched()) return r;
   const long long n = a.BH * (D * D / 4);
   scan_kernel<D, kBwd><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(
-      a.seg, a.segl, kBwd ? a.dHT : a.H0, a.BH, a.nseg, a.dk, a.dv);
+      a.seg, a.segl, kBwd ? a.dHT : a.H0, a.BH, a.nsub, (a.nseg - 1) * a.r, a.dk, a.dv);
   return launched();
 }
 
@@ -1176,13 +1564,23 @@ template <typename E, int D>
 int fill(Args<E>& a, bool fwd, const float* lg, const int64_t* ls, int64_t B, int H, int64_t T, int dk,
          int dv, void* ws, size_t ws_bytes) {
   const long long BH = B * (long long)H;
-  const Plan pl = plan_for(BH, T, D, fwd ? Fwd<E, D>::kPerSm : Bwd<E, D>::kPerSm);
+  const Plan pl = plan_of<E, D>(fwd, BH, T);
   if (seg_bytes(pl, BH) > ws_bytes) return MGS_WORKSPACE_TOO_SMALL;
   if (seg_bytes(pl, BH) && (!ws || reinterpret_cast<uintptr_t>(ws) % 16)) return MGS_BAD_ALIGNMENT;
   a.lg = lg, a.lsb = ls[0], a.lsh = ls[1], a.lst = ls[2];
   a.seg = static_cast<float*>(ws);
-  a.segl = a.seg + (size_t)BH * pl.nseg * D * D;
+  a.segl = a.seg + (size_t)BH * pl.nsub * D * D;
   a.T = T, a.H = H, a.dk = dk, a.dv = dv, a.nchunks = pl.nchunks, a.m = pl.m, a.nseg = pl.nseg, a.BH = BH;
+  a.ms = pl.ms, a.r = pl.r, a.nsub = pl.nsub;
+  if constexpr (std::is_same_v<E, bf16>) {
+    bool ok = map_of(&a.mQ, a.Q, dk, T, H, B) && map_of(&a.mK, a.K, dk, T, H, B) && map_of(&a.mV, a.V, dv, T, H, B);
+    if (fwd)
+      ok = ok && map_of(&a.my, a.y, dv, T, H, B);
+    else
+      ok = ok && map_of(&a.mdy, a.dy, dv, T, H, B) && map_of(&a.mdQ, a.dQ, dk, T, H, B) &&
+           map_of(&a.mdK, a.dK, dk, T, H, B) && map_of(&a.mdV, a.dV, dv, T, H, B);
+    a.tma = ok;
+  }
   return MGS_OK;
 }
 
@@ -1202,8 +1600,8 @@ size_t mgs_linear_attn_workspace_size(int64_t B, int H, int64_t T, int dk, int d
   (void)by_shape(dtype, dk, dv, [&](auto e, auto d) -> int {
     using E = decltype(e);
     constexpr int D = decltype(d)::value;
-    const size_t f = seg_bytes(plan_for(B * H, T, D, Fwd<E, D>::kPerSm), B * H);
-    const size_t b = seg_bytes(plan_for(B * H, T, D, Bwd<E, D>::kPerSm), B * H);
+    const size_t f = seg_bytes(plan_of<E, D>(true, B * H, T), B * H);
+    const size_t b = seg_bytes(plan_of<E, D>(false, B * H, T), B * H);
     n = f > b ? f : b;
     return MGS_OK;
   });
