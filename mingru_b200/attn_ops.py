@@ -19,11 +19,12 @@ second-order autograd.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
 from . import _lib
-from .scan_ops import _dense, _dtype_code, _ptr, _require_cuda, _stream, _workspace
+from .scan_ops import _dense, _dtype_code, _ptr, _require_cuda, _workspace, on_device, raw_stream
 
 __all__ = ["linear_attention"]
 
@@ -41,34 +42,38 @@ def _strides(*ts: torch.Tensor):
     return (ctypes.c_int64 * len(flat))(*flat)
 
 
-def _saved_floats(Q: torch.Tensor, V: torch.Tensor) -> int:
-    B, H, T, dk = Q.shape
-    return _lib.load().mgs_linear_attn_saved_size(B, H, T, dk, V.shape[3], _dtype_code(_OP, Q)) // 4
+@functools.lru_cache(maxsize=1024)
+def _sizes(device: int, B: int, H: int, T: int, dk: int, dv: int, code: int) -> tuple[int, int]:
+    """(workspace bytes, saved floats) on a device, which must be current."""
+    lib = _lib.load()
+    return (lib.mgs_linear_attn_workspace_size(B, H, T, dk, dv, code),
+            lib.mgs_linear_attn_saved_size(B, H, T, dk, dv, code) // 4)
 
 
 def _forward(Q, K, V, lg, H0, save):
-    lib = _lib.load()
-    with torch.cuda.device(Q.device):  # sizes are queried on the launch device
+    dev = Q.device
+    with on_device(dev):  # sizes are queried on the launch device
         Q, K, V = _rows(Q), _rows(K), _rows(V)
         B, H, T, dk = Q.shape
         dv = V.shape[3]
         code = _dtype_code(_OP, Q)
+        n, nsaved = _sizes(dev.index, B, H, T, dk, dv, code)
         y = torch.empty_like(V)
-        HT = torch.empty(B, H, dk, dv, dtype=torch.float32, device=Q.device)
-        saved = torch.empty(_saved_floats(Q, V) if save else 0, dtype=torch.float32, device=Q.device)
+        HT = torch.empty((B, H, dk, dv), dtype=torch.float32, device=dev)
+        saved = torch.empty(nsaved, dtype=torch.float32, device=dev) if save else HT.new_empty(0)
         if T == 0:  # no token: the state passes through
             HT.zero_() if H0 is None else HT.copy_(H0)
             return y, HT, saved
         if H0 is not None:
             H0 = _dense(H0)
-        n = lib.mgs_linear_attn_workspace_size(B, H, T, dk, dv, code)
-        ws = _workspace(n, Q.device) if n else None
-        st = lib.mgs_linear_attn_fwd(
-            _ptr(Q), _ptr(K), _ptr(V), _ptr(lg), _ptr(H0), _ptr(y), _ptr(HT),
-            _ptr(saved) if save else None, _strides(Q, K, V, lg, y), B, H, T, dk, dv, code, _ptr(ws), n,
-            _stream(Q),
+        ws = _workspace(n, dev) if n else None
+        st = _lib.load().mgs_linear_attn_fwd(
+            Q.data_ptr(), K.data_ptr(), V.data_ptr(), lg.data_ptr(), _ptr(H0), y.data_ptr(), HT.data_ptr(),
+            saved.data_ptr() if save else None, _strides(Q, K, V, lg, y), B, H, T, dk, dv, code, _ptr(ws), n,
+            raw_stream(dev),
         )
-        _lib.check(st, f"{_OP} forward")
+        if st:
+            _lib.check(st, f"{_OP} forward")
         return y, HT, saved
 
 
@@ -84,7 +89,37 @@ def _linear_attn_fwd(
 def _(Q, K, V, lg, H0, save):
     B, H, T, dk = Q.shape
     return (torch.empty_like(V), Q.new_empty((B, H, dk, V.shape[3]), dtype=torch.float32),
-            Q.new_empty((_saved_floats(Q, V) if save else 0,), dtype=torch.float32))
+            Q.new_empty((_sizes(Q.device.index, B, H, T, dk, V.shape[3], _dtype_code(_OP, Q))[1] if save else 0,),
+                        dtype=torch.float32))
+
+
+def _gradients(Q, K, V, lg, saved, dy, dHT, want_dH0):
+    dev = Q.device
+    with on_device(dev):  # sizes are queried on the launch device
+        Q, K, V, dy = _rows(Q), _rows(K), _rows(V), _rows(dy.to(Q.dtype))
+        B, H, T, dk = Q.shape
+        dv = V.shape[3]
+        code = _dtype_code(_OP, Q)
+        dQ, dK, dV = torch.empty_like(Q), torch.empty_like(K), torch.empty_like(V)
+        dlg = torch.empty((B, H, T), dtype=torch.float32, device=dev)
+        dH0 = torch.empty((B, H, dk, dv) if want_dH0 else (0,), dtype=torch.float32, device=dev)
+        if dHT is not None:
+            dHT = _dense(dHT.float())
+        if T == 0:
+            if want_dH0:
+                dH0.zero_() if dHT is None else dH0.copy_(dHT)
+            return dQ, dK, dV, dlg, dH0
+        n, _ = _sizes(dev.index, B, H, T, dk, dv, code)
+        ws = _workspace(n, dev) if n else None
+        st = _lib.load().mgs_linear_attn_bwd(
+            Q.data_ptr(), K.data_ptr(), V.data_ptr(), lg.data_ptr(), saved.data_ptr(), dy.data_ptr(),
+            _ptr(dHT), dQ.data_ptr(), dK.data_ptr(), dV.data_ptr(), dlg.data_ptr(),
+            dH0.data_ptr() if want_dH0 else None, _strides(Q, K, V, lg, dy, dQ, dK, dV), B, H, T, dk, dv,
+            code, _ptr(ws), n, raw_stream(dev),
+        )
+        if st:
+            _lib.check(st, f"{_OP} backward")
+        return dQ, dK, dV, dlg, dH0
 
 
 @torch.library.custom_op("mingru_b200::linear_attn_bwd", mutates_args=())
@@ -92,30 +127,7 @@ def _linear_attn_bwd(
     Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, lg: torch.Tensor, saved: torch.Tensor,
     dy: torch.Tensor, dHT: torch.Tensor | None, want_dH0: bool,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    lib = _lib.load()
-    with torch.cuda.device(Q.device):  # sizes are queried on the launch device
-        Q, K, V, dy = (_rows(x) for x in (Q, K, V, dy.to(Q.dtype)))
-        B, H, T, dk = Q.shape
-        dv = V.shape[3]
-        code = _dtype_code(_OP, Q)
-        dQ, dK, dV = (torch.empty_like(x) for x in (Q, K, V))
-        dlg = torch.empty(B, H, T, dtype=torch.float32, device=Q.device)
-        dH0 = torch.empty((B, H, dk, dv) if want_dH0 else (0,), dtype=torch.float32, device=Q.device)
-        if dHT is not None:
-            dHT = _dense(dHT.float())
-        if T == 0:
-            if want_dH0:
-                dH0.zero_() if dHT is None else dH0.copy_(dHT)
-            return dQ, dK, dV, dlg, dH0
-        n = lib.mgs_linear_attn_workspace_size(B, H, T, dk, dv, code)
-        ws = _workspace(n, Q.device) if n else None
-        st = lib.mgs_linear_attn_bwd(
-            _ptr(Q), _ptr(K), _ptr(V), _ptr(lg), _ptr(saved), _ptr(dy), _ptr(dHT), _ptr(dQ), _ptr(dK),
-            _ptr(dV), _ptr(dlg), _ptr(dH0) if want_dH0 else None,
-            _strides(Q, K, V, lg, dy, dQ, dK, dV), B, H, T, dk, dv, code, _ptr(ws), n, _stream(Q),
-        )
-        _lib.check(st, f"{_OP} backward")
-        return dQ, dK, dV, dlg, dH0
+    return _gradients(Q, K, V, lg, saved, dy, dHT, want_dH0)
 
 
 @_linear_attn_bwd.register_fake
@@ -134,20 +146,38 @@ def _setup(ctx, inputs, output):
     ctx.set_materialize_grads(False)
 
 
-def _backward(ctx, dy, dHT, _gsaved):
+def _backward(ctx, dy, dHT, _gsaved=None, run=_linear_attn_bwd):
     if torch.is_grad_enabled():
         raise RuntimeError(f"{_OP} does not support second-order autograd (create_graph=True)")
-    Q, K, V, lg, saved = ctx.saved_tensors
     if dy is None and dHT is None:
         return (None,) * 6
+    Q, K, V, lg, saved = ctx.saved_tensors
     if dy is None:
         dy = torch.zeros_like(V)
     want = ctx.has_h0 and ctx.needs_input_grad[4]
-    dQ, dK, dV, dlg, dH0 = _linear_attn_bwd(Q, K, V, lg, saved, dy, dHT, want)
+    dQ, dK, dV, dlg, dH0 = run(Q, K, V, lg, saved, dy, dHT, want)
     return dQ, dK, dV, dlg, dH0 if want else None, None
 
 
 torch.library.register_autograd("mingru_b200::linear_attn_fwd", _backward, setup_context=_setup)
+
+
+class _Eager(torch.autograd.Function):
+    """The custom op's forward and backward without the dispatcher, whose
+    Python layers cost more than the kernels of a small call (a training step
+    of an 8 x 8 x 1024 x 64 call: 390 us of host time with it)."""
+
+    @staticmethod
+    def forward(ctx, Q, K, V, lg, H0):
+        y, HT, saved = _forward(Q, K, V, lg, H0, True)
+        ctx.save_for_backward(Q, K, V, lg, saved)
+        ctx.has_h0 = H0 is not None
+        ctx.set_materialize_grads(False)
+        return y, HT
+
+    @staticmethod
+    def backward(ctx, dy, dHT):
+        return _backward(ctx, dy, dHT, run=_gradients)[:5]
 
 
 def _blocks(d: int, width: int):
@@ -158,11 +188,12 @@ def _run(Q, K, V, lg, H0):
     dk, dv = Q.shape[3], V.shape[3]
     wide = _MAX_D[Q.dtype]
     if max(dk, dv) <= wide:
-        if torch.compiler.is_compiling() or (
-                torch.is_grad_enabled()
-                and any(t is not None and t.requires_grad for t in (Q, K, V, lg, H0))):
+        if torch.compiler.is_compiling():
             return _linear_attn_fwd(Q, K, V, lg, H0, True)[:2]
-        return _forward(Q, K, V, lg, H0, False)[:2]  # nothing to differentiate: no dispatcher
+        if torch.is_grad_enabled() and (Q.requires_grad or K.requires_grad or V.requires_grad
+                                        or lg.requires_grad or (H0 is not None and H0.requires_grad)):
+            return _Eager.apply(Q, K, V, lg, H0)
+        return _forward(Q, K, V, lg, H0, False)[:2]
     if Q.dtype != torch.float32:
         # Blocks of 16-bit inputs run on fp32 copies, so that their partial
         # outputs and gradients are added before the one rounding.
@@ -218,11 +249,13 @@ def linear_attention(
         )
     if H0 is not None and tuple(H0.shape) != (B, H, dk, dv):
         raise ValueError(f"{_OP}: H0 must have shape {(B, H, dk, dv)} (got {tuple(H0.shape)})")
-    try:
-        lg = torch.broadcast_to(log_gamma, (B, H, T))
-    except RuntimeError:
-        raise ValueError(f"{_OP}: log_gamma must broadcast to {(B, H, T)} (got "
-                         f"{tuple(log_gamma.shape)})") from None
+    lg = log_gamma
+    if lg.shape != Q.shape[:3]:
+        try:
+            lg = torch.broadcast_to(lg, (B, H, T))
+        except RuntimeError:
+            raise ValueError(f"{_OP}: log_gamma must broadcast to {(B, H, T)} (got "
+                             f"{tuple(lg.shape)})") from None
     _require_cuda(_OP, Q, K, V, lg, *(() if H0 is None else (H0,)))
     if K.dtype != Q.dtype or V.dtype != Q.dtype:
         raise ValueError(f"{_OP}: Q, K and V must share a dtype")

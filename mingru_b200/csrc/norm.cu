@@ -40,34 +40,49 @@ struct Args {
   float eps;
 };
 
-// VEC consecutive elements.
-template <typename T, int VEC>
-__device__ __forceinline__ void ldv(const void* p, long long i, float* v) {
-  const T* q = static_cast<const T*>(p) + i;
-  if constexpr (VEC == 1) {
-    v[0] = to_f32<T>(*q);
-  } else {
-    constexpr int kN = 16 / (int)sizeof(T) < VEC ? 16 / (int)sizeof(T) : VEC;
+// A thread's K vectors of VEC elements, tpg vectors apart, as fp32; zeros from
+// column n on. One loop of loads and nothing else, so that they are all under
+// way before the first is used.
+template <typename T, int VEC, int K>
+__device__ __forceinline__ void ldrow(const void* p, long long i, int t, int tpg, int n, float (&v)[K * VEC]) {
+  const T* q = static_cast<const T*>(p) + i + t * VEC;
+  constexpr int kBytes = VEC * (int)sizeof(T);
+  using U = std::conditional_t<VEC == 1, T, uint4>;
+  constexpr int kN = VEC == 1 ? 1 : kBytes / 16;
+  U raw[K][kN];
 #pragma unroll
-    for (int k = 0; k < VEC; k += kN) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(q + k));
-      const T* e = reinterpret_cast<const T*>(&u);
+  for (int k = 0; k < K; ++k) {
+    const bool in = (k * tpg + t) * VEC < n;
 #pragma unroll
-      for (int j = 0; j < kN; ++j) v[k + j] = to_f32<T>(e[j]);
+    for (int j = 0; j < kN; ++j) {
+      if constexpr (VEC == 1)
+        raw[k][j] = in ? q[k * tpg] : from_f32<T>(0.f);
+      else
+        raw[k][j] = in ? __ldg(reinterpret_cast<const uint4*>(q + k * tpg * VEC) + j) : make_uint4(0, 0, 0, 0);
     }
   }
-}
-template <typename T, int VEC>
-__device__ __forceinline__ void stv(void* p, long long i, const float* v) {
-  T* q = static_cast<T*>(p) + i;
-  if constexpr (VEC == 1) {
-    *q = from_f32<T>(v[0]);
-  } else {
-    uint4 u;
-    T* e = reinterpret_cast<T*>(&u);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) e[j] = from_f32<T>(v[j]);
-    *reinterpret_cast<uint4*>(q) = u;
+  for (int k = 0; k < K; ++k) {
+    const T* e = reinterpret_cast<const T*>(raw[k]);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[k * VEC + j] = to_f32<T>(e[j]);
+  }
+}
+template <typename T, int VEC, int K>
+__device__ __forceinline__ void strow(void* p, long long i, int t, int tpg, int n, const float (&v)[K * VEC]) {
+  T* q = static_cast<T*>(p) + i + t * VEC;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if ((k * tpg + t) * VEC >= n) break;
+    if constexpr (VEC == 1) {
+      q[k * tpg] = from_f32<T>(v[k]);
+    } else {
+      uint4 u;
+      T* e = reinterpret_cast<T*>(&u);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) e[j] = from_f32<T>(v[k * VEC + j]);
+      *reinterpret_cast<uint4*>(q + k * tpg * VEC) = u;
+    }
   }
 }
 
@@ -77,31 +92,47 @@ __device__ __forceinline__ void stv(void* p, long long i, const float* v) {
 struct Reduce {
   float2 (*red)[32];
   int tpg, slot, buf;
-  __device__ __forceinline__ float2 operator()(float a, float b) {
-    const int lane = threadIdx.x & 31;
-    const int width = tpg < 32 ? tpg : 32;
-    const unsigned mask = width == 32 ? 0xffffffffu : ((1u << width) - 1) << (lane & ~(width - 1));
-    for (int o = width / 2; o > 0; o >>= 1) {
+  template <int W>
+  __device__ __forceinline__ static void lanes(unsigned mask, float& a, float& b) {
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) {
       a += __shfl_xor_sync(mask, a, o);
       b += __shfl_xor_sync(mask, b, o);
     }
-    if (tpg > 32) {
-      const int nw = tpg / 32, w0 = slot * nw;
-      if (lane == 0) red[buf][threadIdx.x >> 5] = make_float2(a, b);
-      named_bar(1 + slot, tpg);
-      a = b = 0.f;
-      for (int w = 0; w < nw; ++w) {
-        const float2 f = red[buf][w0 + w];
-        a += f.x;
-        b += f.y;
+  }
+  __device__ __forceinline__ float2 operator()(float a, float b) {
+    const int lane = threadIdx.x & 31;
+    if (tpg == 8) {
+      lanes<8>(0xffu << (lane & 24), a, b);
+    } else if (tpg == 16) {
+      lanes<16>(0xffffu << (lane & 16), a, b);
+    } else {
+      lanes<32>(0xffffffffu, a, b);
+      if (tpg > 32) {
+        const int nw = tpg / 32, w0 = slot * nw;
+        if (lane == 0) red[buf][threadIdx.x >> 5] = make_float2(a, b);
+        named_bar(1 + slot, tpg);
+        a = b = 0.f;
+        for (int w = 0; w < nw; ++w) {
+          const float2 f = red[buf][w0 + w];
+          a += f.x;
+          b += f.y;
+        }
+        buf ^= 1;
       }
-      buf ^= 1;
     }
     return make_float2(a, b);
   }
 };
 
-__device__ __forceinline__ float sigm(float x) { return 1.f / (1.f + __expf(-x)); }
+__device__ __forceinline__ float sigm(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+
+// 1 / sqrt(v) to the last place, by a step of Newton's on the hardware's: the
+// gradient takes differences of z * z and 1.
+__device__ __forceinline__ float inv_sqrt(float v) {
+  const float r = rsqrtf(v);
+  return fmaf(0.5f * r, fmaf(-v * r, r, 1.f), r);
+}
 
 // Where a thread stands: its group (of the row), row slot and first column.
 struct Place {
@@ -116,183 +147,168 @@ struct Place {
   }
 };
 
+// CTAs to an SM that the registers are held to: latency is hidden by rows under
+// way, 1024 threads' worth forward and 768 backward.
+constexpr int fwd_ctas(int threads) { return 1024 / threads; }
+constexpr int bwd_ctas(int threads) { return threads == 256 ? 3 : 1; }
+
 template <typename E, typename W, int VEC, int K, int MAXT>
-__global__ void __launch_bounds__(MAXT) fwd_kernel(const Args p) {
+__global__ void __launch_bounds__(MAXT, fwd_ctas(MAXT)) fwd_kernel(const Args p) {
+  constexpr int N = K * VEC;
   __shared__ float2 red[2][32];
   const Place at(p);
   if (!at.on) return;
   Reduce sum{red, p.tpg, at.slot, 0};
   const float inv_n = 1.f / (float)p.n;
+  const int col = at.g * p.n;
+  auto in = [&](int i) { return ((i / VEC) * p.tpg + at.t) * VEC < p.n; };
   for (long long row = (long long)blockIdx.x * p.rpc + at.rs; row < p.rows;
        row += (long long)gridDim.x * p.rpc) {
-    float h[K * VEC];
-    float acc = 0.f;
+    float h[N], a[N], w[N];
+    ldrow<E, VEC, K>(p.x, row * p.ldx + col, at.t, p.tpg, p.n, h);
+    if (p.res) {
+      ldrow<E, VEC, K>(p.res, row * p.ldres + col, at.t, p.tpg, p.n, a);
+      if (p.s) {
+        ldrow<W, VEC, K>(p.s, col, at.t, p.tpg, p.n, w);
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int c = (k * p.tpg + at.t) * VEC, col = at.g * p.n + c;
-      float* v = h + k * VEC;
-      if (c < p.n) {
-        ldv<E, VEC>(p.x, row * p.ldx + col, v);
-        if (p.res) {
-          float r[VEC];
-          ldv<E, VEC>(p.res, row * p.ldres + col, r);
-          if (p.s) {
-            float s[VEC];
-            ldv<W, VEC>(p.s, col, s);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) v[i] = fmaf(s[i], v[i], r[i]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) v[i] += r[i];
-          }
-        }
+        for (int i = 0; i < N; ++i) h[i] = fmaf(w[i], h[i], a[i]);
       } else {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[i] = 0.f;
+        for (int i = 0; i < N; ++i) h[i] += a[i];
       }
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) acc += v[i];
     }
+    if (p.gate) ldrow<E, VEC, K>(p.gate, row * p.ldgate + col, at.t, p.tpg, p.n, a);
+    ldrow<W, VEC, K>(p.w, col, at.t, p.tpg, p.n, w);
+    float acc = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc += h[i];
     // The fp32 mean is off by up to half a unit of its last place: what it leaves in the
     // differences, `rest`, is their own mean, and comes with the sum of their squares.
     const float mean = p.rms ? 0.f : sum(acc, 0.f).x * inv_n;
     float sq = 0.f, rs = 0.f;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const bool in = (k * p.tpg + at.t) * VEC < p.n;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float d = in ? h[k * VEC + i] - mean : 0.f;
-        sq = fmaf(d, d, sq);
-        rs += d;
-      }
+    for (int i = 0; i < N; ++i) {
+      const float d = in(i) ? h[i] - mean : 0.f;
+      sq = fmaf(d, d, sq);
+      rs += d;
     }
     const float2 m = sum(sq, rs);
     const float rest = p.rms ? 0.f : m.y * inv_n;
-    const float r = rsqrtf(fmaxf(fmaf(-rest, rest, m.x * inv_n), 0.f) + p.eps);
+    const float r = inv_sqrt(fmaxf(fmaf(-rest, rest, m.x * inv_n), 0.f) + p.eps);
     if (p.stats && at.t == 0) {
       float* st = p.stats + (row * p.G + at.g) * 3;
       st[0] = mean, st[1] = rest, st[2] = r;
     }
+    const long long o = row * p.D + col;
+    if (p.h) strow<E, VEC, K>(p.h, o, at.t, p.tpg, p.n, h);
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int c = (k * p.tpg + at.t) * VEC, col = at.g * p.n + c;
-      if (c >= p.n) continue;
-      const long long o = row * p.D + col;
-      if (p.h) stv<E, VEC>(p.h, o, h + k * VEC);
-      float y[VEC], w[VEC];
-      ldv<W, VEC>(p.w, col, w);
+    for (int i = 0; i < N; ++i) h[i] = ((h[i] - mean) - rest) * r * w[i];
+    if (p.b) {
+      ldrow<W, VEC, K>(p.b, col, at.t, p.tpg, p.n, w);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) y[i] = ((h[k * VEC + i] - mean) - rest) * r * w[i];
-      if (p.b) {
-        ldv<W, VEC>(p.b, col, w);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) y[i] += w[i];
-      }
-      if (p.gate) {
-        ldv<E, VEC>(p.gate, row * p.ldgate + col, w);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) y[i] *= w[i] * sigm(w[i]);
-      }
-      stv<E, VEC>(p.y, o, y);
+      for (int i = 0; i < N; ++i) h[i] += w[i];
     }
+    if (p.gate) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) h[i] *= a[i] * sigm(a[i]);
+    }
+    strow<E, VEC, K>(p.y, o, at.t, p.tpg, p.n, h);
   }
 }
 
-template <typename E, typename W, int VEC, int K, int MAXT>
-__global__ void __launch_bounds__(MAXT) bwd_kernel(const Args p) {
+// GATE and SCALE: whether they are there, so that a call without them keeps no registers for them.
+template <typename E, typename W, int VEC, int K, int MAXT, bool GATE, bool SCALE>
+__global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT)) bwd_kernel(const Args p) {
+  constexpr int N = K * VEC;
   __shared__ float2 red[2][32];
   extern __shared__ float cols[];
   const Place at(p);
   Reduce sum{red, p.tpg, at.slot, 0};
   const float inv_n = 1.f / (float)p.n;
-  float gw[K * VEC], gb[K * VEC], gs[K * VEC];
+  const int col = at.g * p.n;
+  float gw[N], gb[N], gs[SCALE ? N : 1];
 #pragma unroll
-  for (int i = 0; i < K * VEC; ++i) gw[i] = gb[i] = gs[i] = 0.f;
+  for (int i = 0; i < N; ++i) {
+    gw[i] = gb[i] = 0.f;
+    if constexpr (SCALE) gs[i] = 0.f;
+  }
   if (at.on) {
     for (long long row = (long long)blockIdx.x * p.rpc + at.rs; row < p.rows;
          row += (long long)gridDim.x * p.rpc) {
       const float* st = p.stats + (row * p.G + at.g) * 3;
+      const long long o = row * p.D + col;
+      float x[N], d[N], z[N], w[N];
+      ldrow<E, VEC, K>(p.x, row * p.ldx + col, at.t, p.tpg, p.n, x);
+      ldrow<E, VEC, K>(p.dy, row * p.lddy + col, at.t, p.tpg, p.n, d);
       const float mean = st[0], rest = st[1], r = st[2];
-      float z[K * VEC], dz[K * VEC], x[K * VEC];
-      float s1 = 0.f, s2 = 0.f;
+      if (SCALE || p.res) {
+        ldrow<E, VEC, K>(p.res, row * p.ldres + col, at.t, p.tpg, p.n, z);
+        if constexpr (SCALE) {
+          ldrow<W, VEC, K>(p.s, col, at.t, p.tpg, p.n, w);
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const int c = (k * p.tpg + at.t) * VEC, col = at.g * p.n + c;
-        const int e = k * VEC;
-        if (c >= p.n) continue;
-        float a[VEC], w[VEC];
-        ldv<E, VEC>(p.x, row * p.ldx + col, x + e);
-        ldv<E, VEC>(p.dy, row * p.lddy + col, dz + e);
+          for (int i = 0; i < N; ++i) z[i] = fmaf(w[i], x[i], z[i]);
+        } else {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) z[e + i] = x[e + i];
-        if (p.res) {
-          ldv<E, VEC>(p.res, row * p.ldres + col, a);
-          if (p.s) {
-            ldv<W, VEC>(p.s, col, w);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) z[e + i] = fmaf(w[i], z[e + i], a[i]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) z[e + i] += a[i];
-          }
+          for (int i = 0; i < N; ++i) z[i] += x[i];
         }
-        ldv<W, VEC>(p.w, col, w);
+      } else {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) z[e + i] = ((z[e + i] - mean) - rest) * r;
-        if (p.gate) {
-          float gt[VEC], b[VEC];
-          ldv<E, VEC>(p.gate, row * p.ldgate + col, gt);
-          if (p.b) ldv<W, VEC>(p.b, col, b);
+        for (int i = 0; i < N; ++i) z[i] = x[i];
+      }
+      ldrow<W, VEC, K>(p.w, col, at.t, p.tpg, p.n, w);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            const float sg = sigm(gt[i]), o = fmaf(z[e + i], w[i], p.b ? b[i] : 0.f), d = dz[e + i];
-            a[i] = d * o * sg * fmaf(gt[i], 1.f - sg, 1.f);
-            dz[e + i] = d * gt[i] * sg;
-          }
-          stv<E, VEC>(p.dgate, row * p.D + col, a);
+      for (int i = 0; i < N; ++i) z[i] = ((z[i] - mean) - rest) * r;
+      if constexpr (GATE) {
+        float g[N], b[N];
+        ldrow<E, VEC, K>(p.gate, row * p.ldgate + col, at.t, p.tpg, p.n, g);
+        if (p.b) {
+          ldrow<W, VEC, K>(p.b, col, at.t, p.tpg, p.n, b);
+        } else {
+#pragma unroll
+          for (int i = 0; i < N; ++i) b[i] = 0.f;
         }
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          gw[e + i] = fmaf(dz[e + i], z[e + i], gw[e + i]);
-          gb[e + i] += dz[e + i];
-          dz[e + i] *= w[i];
-          s1 += dz[e + i];
-          s2 = fmaf(dz[e + i], z[e + i], s2);
+        for (int i = 0; i < N; ++i) {
+          const float sg = sigm(g[i]), a = fmaf(z[i], w[i], b[i]);
+          b[i] = d[i] * a * sg * fmaf(g[i], 1.f - sg, 1.f);
+          d[i] *= g[i] * sg;
         }
+        strow<E, VEC, K>(p.dgate, o, at.t, p.tpg, p.n, b);
+      }
+      float s1 = 0.f, s2 = 0.f;  // columns past n have d = w = 0
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        gw[i] = fmaf(d[i], z[i], gw[i]);
+        gb[i] += d[i];
+        d[i] *= w[i];
+        s1 += d[i];
+        s2 = fmaf(d[i], z[i], s2);
       }
       const float2 m = sum(s1, s2);
       const float m1 = p.rms ? 0.f : m.x * inv_n, m2 = m.y * inv_n;
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const int c = (k * p.tpg + at.t) * VEC, col = at.g * p.n + c;
-        const int e = k * VEC;
-        if (c >= p.n) continue;
-        float d[VEC], a[VEC];
+      for (int i = 0; i < N; ++i) d[i] = r * (d[i] - m1 - z[i] * m2);
+      if (p.dh) {
+        ldrow<E, VEC, K>(p.dh, row * p.lddh + col, at.t, p.tpg, p.n, w);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) d[i] = r * (dz[e + i] - m1 - z[e + i] * m2);
-        if (p.dh) {
-          ldv<E, VEC>(p.dh, row * p.lddh + col, a);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) d[i] += a[i];
-        }
-        if (p.s) {
-          stv<E, VEC>(p.dres, row * p.D + col, d);
-          ldv<W, VEC>(p.s, col, a);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            gs[e + i] = fmaf(d[i], x[e + i], gs[e + i]);
-            d[i] *= a[i];
-          }
-        }
-        stv<E, VEC>(p.dx, row * p.D + col, d);
+        for (int i = 0; i < N; ++i) d[i] += w[i];
       }
+      if constexpr (SCALE) {
+        strow<E, VEC, K>(p.dres, o, at.t, p.tpg, p.n, d);
+        ldrow<W, VEC, K>(p.s, col, at.t, p.tpg, p.n, w);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          gs[i] = fmaf(d[i], x[i], gs[i]);
+          d[i] *= w[i];
+        }
+      }
+      strow<E, VEC, K>(p.dx, o, at.t, p.tpg, p.n, d);
     }
   }
   // the CTA's rows: one partial row of each sum
   const int width = p.gpc * p.n;  // columns of this CTA
-  for (int q = 0; q < 3; ++q) {
-    if ((q == 1 && !p.b) || (q == 2 && !p.s)) continue;
+  for (int q = 0; q < 2 + SCALE; ++q) {
+    if (q == 1 && !p.b) continue;
     __syncthreads();
     if (at.on) {
 #pragma unroll
@@ -301,7 +317,12 @@ __global__ void __launch_bounds__(MAXT) bwd_kernel(const Args p) {
         if (c >= p.n) continue;
         float* o = cols + (long long)at.rs * width + (at.slot % p.gpc) * p.n + c;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) o[i] = q == 0 ? gw[k * VEC + i] : q == 1 ? gb[k * VEC + i] : gs[k * VEC + i];
+        for (int i = 0; i < VEC; ++i) {
+          float v = q == 0 ? gw[k * VEC + i] : gb[k * VEC + i];
+          if constexpr (SCALE)
+            if (q == 2) v = gs[k * VEC + i];
+          o[i] = v;
+        }
       }
     }
     __syncthreads();
@@ -348,49 +369,73 @@ struct Plan {
   unsigned gx, gy;
 };
 
-// Threads to a group: as few as hold it at up to 16 values each, so that sums
-// need few steps; groups side by side in a CTA as they lie in a row.
-bool make_plan(Plan& pl, long long rows, int D, int G, int size, bool vec) {
+// Threads to a group: as few as hold it at `values` each (a row's sums then need
+// few steps, and more rows are under way), a part of a warp or whole warps;
+// groups side by side in a CTA as they lie in a row. 16 values forward; 8
+// backward, which keeps seven arrays of them in registers, while a CTA of 1024
+// threads holds the group at that.
+bool make_plan(Plan& pl, long long rows, int D, int G, int size, bool vec, bool fwd) {
   const int n = D / G;
   if (n > kMaxGroup) return false;
+  const int values = fwd || n > kMaxGroup / 2 ? 16 : 8;
   pl.vec = vec ? 16 / size : 1;
-  const int need = (n + pl.vec - 1) / pl.vec, most = 16 / pl.vec;
-  pl.tpg = 8;
-  while (pl.tpg * most < need) pl.tpg *= 2;
-  const int k = (need + pl.tpg - 1) / pl.tpg;
+  const int need = (n + pl.vec - 1) / pl.vec, most = values / pl.vec;
   pl.k = 1;
-  while (pl.k < k) pl.k *= 2;
+  while (pl.k < most && pl.k * 8 < need) pl.k *= 2;
+  if (!vec && pl.k < 4) pl.k = 4;
+  const int t = (need + pl.k - 1) / pl.k;
+  pl.tpg = t <= 8 ? 8 : t <= 16 ? 16 : (t + 31) / 32 * 32;
   pl.threads = pl.tpg > kThreads ? pl.tpg : kThreads;
   pl.gpc = pl.threads / pl.tpg < G ? pl.threads / pl.tpg : G;
   pl.rpc = pl.threads / (pl.tpg * pl.gpc);
   pl.gy = (unsigned)((G + pl.gpc - 1) / pl.gpc);
   // a few CTAs to an SM, each walking rows
-  const long long most_x = ((long long)sm_count() * (1024 / pl.threads) + pl.gy - 1) / pl.gy;
+  const int per_sm = fwd ? 1024 / pl.threads : pl.threads > 512 ? 1 : pl.threads > 256 ? 2 : 3;
+  const long long most_x = ((long long)sm_count() * per_sm + pl.gy - 1) / pl.gy;
   const long long want = (rows + pl.rpc - 1) / pl.rpc;
   pl.gx = (unsigned)(want < most_x ? (want < 1 ? 1 : want) : most_x);
   return true;
 }
 
+// The kernels that make_plan's rules reach: the most values to a thread with any
+// number of threads, fewer with the smallest groups only.
+#define MGS_NORM_CASE(v, kk, maxt) \
+  if (pl.vec == v && pl.k == kk && pl.threads <= maxt) return MGS_NORM_KERNEL(v, kk, maxt);
+#define MGS_NORM_SIZES(v, kk) MGS_NORM_CASE(v, kk, 256) MGS_NORM_CASE(v, kk, 512) MGS_NORM_CASE(v, kk, 1024)
+
 template <typename E, typename W, class F>
-int by_plan(const Plan& pl, F&& f) {
+int by_plan_fwd(const Plan& pl, F&& f) {
   constexpr int V = 16 / (int)sizeof(E);
-#define MGS_NORM_CASE(v, kk)                                                                \
-  if (pl.vec == v && pl.k == kk)                                                            \
-    return pl.threads <= 512 ? f(fwd_kernel<E, W, v, kk, 512>, bwd_kernel<E, W, v, kk, 512>) \
-                             : f(fwd_kernel<E, W, v, kk, 1024>, bwd_kernel<E, W, v, kk, 1024>);
-  MGS_NORM_CASE(V, 1)
-  MGS_NORM_CASE(V, 2)
+#define MGS_NORM_KERNEL(v, kk, maxt) f(fwd_kernel<E, W, v, kk, maxt>)
+  MGS_NORM_CASE(V, 1, 256)
   if constexpr (V == 4) {
-    MGS_NORM_CASE(V, 4)
+    MGS_NORM_CASE(V, 2, 256)
   }
-  MGS_NORM_CASE(1, 1)
-  MGS_NORM_CASE(1, 2)
-  MGS_NORM_CASE(1, 4)
-  MGS_NORM_CASE(1, 8)
-  MGS_NORM_CASE(1, 16)
-#undef MGS_NORM_CASE
+  MGS_NORM_SIZES(V, 16 / V)
+  MGS_NORM_CASE(1, 4, 256)
+  MGS_NORM_CASE(1, 8, 256)
+  MGS_NORM_SIZES(1, 16)
+#undef MGS_NORM_KERNEL
   return MGS_UNSUPPORTED;
 }
+
+template <typename E, typename W, bool GATE, bool SCALE, class F>
+int by_plan_bwd(const Plan& pl, F&& f) {
+  constexpr int V = 16 / (int)sizeof(E);
+#define MGS_NORM_KERNEL(v, kk, maxt) f(bwd_kernel<E, W, v, kk, maxt, GATE, SCALE>)
+  if constexpr (V == 4) {
+    MGS_NORM_CASE(V, 1, 256)
+  }
+  MGS_NORM_SIZES(V, 8 / V)
+  MGS_NORM_CASE(V, 16 / V, 1024)
+  MGS_NORM_CASE(1, 4, 256)
+  MGS_NORM_SIZES(1, 8)
+  MGS_NORM_CASE(1, 16, 1024)
+#undef MGS_NORM_KERNEL
+  return MGS_UNSUPPORTED;
+}
+#undef MGS_NORM_SIZES
+#undef MGS_NORM_CASE
 
 template <class F>
 int by_dtypes(int dtype, int wdtype, F&& f) {
@@ -436,7 +481,7 @@ size_t mgs_block_norm_workspace_size(int64_t rows, int64_t D, int groups, int dt
   size_t most = 0;
   for (bool vec : {false, true}) {
     Plan pl;
-    if (!make_plan(pl, rows, (int)D, groups, size, vec)) return 0;
+    if (!make_plan(pl, rows, (int)D, groups, size, vec, false)) return 0;
     const size_t n = 3 * (size_t)pl.gx * (size_t)D * sizeof(float);
     most = n > most ? n : most;
   }
@@ -459,10 +504,10 @@ int mgs_block_norm_fwd(const void* x, const void* residual, const void* gate, co
     a.ldx = row_strides[0], a.ldres = row_strides[1], a.ldgate = row_strides[2];
     a.rows = rows, a.D = (int)D, a.G = groups, a.n = (int)D / groups, a.rms = rms, a.eps = eps;
     Plan pl;
-    if (!make_plan(pl, rows, (int)D, groups, sizeof(E), vec_ok(a, sizeof(E), sizeof(W)))) return MGS_UNSUPPORTED;
+    if (!make_plan(pl, rows, (int)D, groups, sizeof(E), vec_ok(a, sizeof(E), sizeof(W)), true)) return MGS_UNSUPPORTED;
     if (pl.gy > 65535) return MGS_UNSUPPORTED;
     set_plan(a, pl);
-    return by_plan<E, W>(pl, [&](auto fwd, auto) -> int {
+    return by_plan_fwd<E, W>(pl, [&](auto fwd) -> int {
       fwd<<<dim3(pl.gx, pl.gy), pl.threads, 0, static_cast<cudaStream_t>(stream)>>>(a);
       return launched();
     });
@@ -496,17 +541,19 @@ int mgs_block_norm_bwd(const void* x, const void* residual, const void* gate, co
     a.lddh = row_strides[4];
     a.rows = rows, a.D = (int)D, a.G = groups, a.n = (int)D / groups, a.rms = rms;
     Plan pl;
-    if (!make_plan(pl, rows, (int)D, groups, sizeof(E), vec_ok(a, sizeof(E), sizeof(W)))) return MGS_UNSUPPORTED;
+    if (!make_plan(pl, rows, (int)D, groups, sizeof(E), vec_ok(a, sizeof(E), sizeof(W)), false)) return MGS_UNSUPPORTED;
     if (pl.gy > 65535) return MGS_UNSUPPORTED;
     if (workspace_bytes < 3 * (size_t)pl.gx * (size_t)D * sizeof(float)) return MGS_WORKSPACE_TOO_SMALL;
     set_plan(a, pl);
-    int r = by_plan<E, W>(pl, [&](auto, auto bwd) -> int {
+    auto launch = [&](auto bwd) -> int {
       const size_t smem = (size_t)pl.rpc * pl.gpc * a.n * sizeof(float);
       if (smem > 48 * 1024)
         MGS_CUDA_OK(cudaFuncSetAttribute(bwd, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
       bwd<<<dim3(pl.gx, pl.gy), pl.threads, smem, st>>>(a);
       return launched();
-    });
+    };
+    const int r = gate ? (scale ? by_plan_bwd<E, W, true, true>(pl, launch) : by_plan_bwd<E, W, true, false>(pl, launch))
+                       : (scale ? by_plan_bwd<E, W, false, true>(pl, launch) : by_plan_bwd<E, W, false, false>(pl, launch));
     if (r) return r;
     sum_kernel<W><<<dim3((unsigned)((D + 31) / 32), 3), dim3(32, 32), 0, st>>>(
         a.part, static_cast<W*>(dweight), bias ? static_cast<W*>(dbias) : nullptr,

@@ -9,11 +9,12 @@ torch's LayerNorm and adds (``min_gru.py:3698-3922``).
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
 from . import _lib
-from .scan_ops import _dense, _dtype_code, _ptr, _require_cuda, _stream, _workspace
+from .scan_ops import _dense, _dtype_code, _ptr, _require_cuda, _workspace, on_device, raw_stream
 
 __all__ = ["block_norm"]
 
@@ -38,24 +39,30 @@ def _rows(t: torch.Tensor | None, D: int):
     return t.contiguous(), D
 
 
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(device: int, rows: int, D: int, groups: int, code: int) -> int:
+    """On a device, which must be current."""
+    return _lib.load().mgs_block_norm_workspace_size(rows, D, groups, code)
+
+
 def _codes(x, weight):
     return _dtype_code(_OP, x), _dtype_code(_OP, weight)
 
 
 def _forward(x, weight, bias, residual, scale, gate, groups, eps, rms, save):
-    with torch.cuda.device(x.device):  # sizes are queried on the launch device
+    with on_device(x.device):  # sizes are queried on the launch device
         D = x.shape[-1]
         rows = x.numel() // D
         (x, lx), (residual, lr), (gate, lg) = _rows(x, D), _rows(residual, D), _rows(gate, D)
         weight, bias, scale = (None if t is None else _dense(t) for t in (weight, bias, scale))
         y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        h = torch.empty_like(y) if residual is not None else y.new_empty(0)
-        stats = torch.empty(rows * groups * 3 if save else 0, dtype=torch.float32, device=x.device)
+        h = torch.empty_like(y) if residual is not None else None
+        stats = torch.empty(rows * groups * 3, dtype=torch.float32, device=x.device) if save else None
         code, wcode = _codes(x, weight)
         st = _lib.load().mgs_block_norm_fwd(
             _ptr(x), _ptr(residual), _ptr(gate), _ptr(weight), _ptr(bias), _ptr(scale), _ptr(y),
-            _ptr(h) if residual is not None else None, _ptr(stats) if save else None,
-            (ctypes.c_int64 * 3)(lx, lr, lg), rows, D, groups, int(rms), eps, code, wcode, _stream(x),
+            _ptr(h), _ptr(stats),
+            (ctypes.c_int64 * 3)(lx, lr, lg), rows, D, groups, int(rms), eps, code, wcode, raw_stream(x.device),
         )
         _lib.check(st, f"{_OP} forward")
         return y, h, stats
@@ -66,7 +73,8 @@ def _block_norm_fwd(
     x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, residual: torch.Tensor | None,
     scale: torch.Tensor | None, gate: torch.Tensor | None, groups: int, eps: float, rms: bool,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return _forward(x, weight, bias, residual, scale, gate, groups, eps, rms, True)
+    y, h, stats = _forward(x, weight, bias, residual, scale, gate, groups, eps, rms, True)
+    return y, x.new_empty(0) if h is None else h, stats
 
 
 @_block_norm_fwd.register_fake
@@ -76,14 +84,9 @@ def _(x, weight, bias, residual, scale, gate, groups, eps, rms):
     return y, h, x.new_empty((x.numel() // x.shape[-1] * groups * 3,), dtype=torch.float32)
 
 
-@torch.library.custom_op("mingru_b200::block_norm_bwd", mutates_args=())
-def _block_norm_bwd(
-    x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, residual: torch.Tensor | None,
-    scale: torch.Tensor | None, gate: torch.Tensor | None, stats: torch.Tensor, dy: torch.Tensor,
-    dh: torch.Tensor | None, groups: int, rms: bool,
-) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+def _gradients(x, weight, bias, residual, scale, gate, stats, dy, dh, groups, rms):
     lib = _lib.load()
-    with torch.cuda.device(x.device):  # sizes are queried on the launch device
+    with on_device(x.device):  # sizes are queried on the launch device
         D = x.shape[-1]
         rows = x.numel() // D
         dy = dy.to(x.dtype)
@@ -91,19 +94,31 @@ def _block_norm_bwd(
         (x, lx), (residual, lr), (gate, lg) = _rows(x, D), _rows(residual, D), _rows(gate, D)
         (dy, ly), (dh, lh) = _rows(dy, D), _rows(dh, D)
         weight, bias, scale = (None if t is None else _dense(t) for t in (weight, bias, scale))
-        like = lambda on, t: torch.empty(t.shape if on else (0,), dtype=t.dtype, device=t.device)  # noqa: E731
-        dx, dres, dgate = like(True, x), like(scale is not None, x), like(gate is not None, x)
-        dw, db, ds = like(True, weight), like(bias is not None, weight), like(scale is not None, weight)
+        dense = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
+        dx, dw = dense(x), dense(weight)
+        dres, ds = (None, None) if scale is None else (dense(x), dense(weight))
+        db = None if bias is None else dense(weight)
+        dgate = None if gate is None else dense(x)
         code, wcode = _codes(x, weight)
-        ws = _workspace(lib.mgs_block_norm_workspace_size(rows, D, groups, code), x.device)
+        ws = _workspace(_workspace_bytes(x.device.index, rows, D, groups, code), x.device)
         st = lib.mgs_block_norm_bwd(
             _ptr(x), _ptr(residual), _ptr(gate), _ptr(weight), _ptr(bias), _ptr(scale), _ptr(stats),
             _ptr(dy), _ptr(dh), _ptr(dx), _ptr(dres), _ptr(dgate), _ptr(dw), _ptr(db), _ptr(ds),
             (ctypes.c_int64 * 5)(lx, lr, lg, ly, lh), rows, D, groups, int(rms), code, wcode, _ptr(ws),
-            ws.numel(), _stream(x),
+            ws.numel(), raw_stream(x.device),
         )
         _lib.check(st, f"{_OP} backward")
         return dx, dw, db, dres, ds, dgate
+
+
+@torch.library.custom_op("mingru_b200::block_norm_bwd", mutates_args=())
+def _block_norm_bwd(
+    x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, residual: torch.Tensor | None,
+    scale: torch.Tensor | None, gate: torch.Tensor | None, stats: torch.Tensor, dy: torch.Tensor,
+    dh: torch.Tensor | None, groups: int, rms: bool,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    got = _gradients(x, weight, bias, residual, scale, gate, stats, dy, dh, groups, rms)
+    return tuple(x.new_empty(0) if t is None else t for t in got)
 
 
 @_block_norm_bwd.register_fake
@@ -121,7 +136,7 @@ def _setup(ctx, inputs, output):
     ctx.set_materialize_grads(False)
 
 
-def _backward(ctx, dy, dh, _gstats):
+def _backward(ctx, dy, dh, _gstats=None, run=_block_norm_bwd):
     if torch.is_grad_enabled():
         raise RuntimeError(f"{_OP} does not support second-order autograd (create_graph=True)")
     x, weight, bias, residual, scale, gate, stats = ctx.saved_tensors
@@ -129,14 +144,30 @@ def _backward(ctx, dy, dh, _gstats):
         return (None,) * 9
     if dy is None:
         dy = torch.zeros_like(x)
-    dx, dw, db, dres, ds, dgate = _block_norm_bwd(x, weight, bias, residual, scale, gate, stats, dy,
-                                                  dh if residual is not None else None, ctx.groups, ctx.rms)
+    dx, dw, db, dres, ds, dgate = run(x, weight, bias, residual, scale, gate, stats, dy,
+                                      dh if residual is not None else None, ctx.groups, ctx.rms)
     return (dx, dw, db if bias is not None else None,
             None if residual is None else dx if scale is None else dres,
             ds if scale is not None else None, dgate if gate is not None else None, None, None, None)
 
 
 torch.library.register_autograd("mingru_b200::block_norm_fwd", _backward, setup_context=_setup)
+
+
+class _Eager(torch.autograd.Function):
+    """The custom op's forward and backward without the dispatcher's Python layers."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, scale, gate, groups, eps, rms):
+        y, h, stats = _forward(x, weight, bias, residual, scale, gate, groups, eps, rms, True)
+        ctx.save_for_backward(x, weight, bias, residual, scale, gate, stats)
+        ctx.groups, ctx.rms = groups, rms
+        ctx.set_materialize_grads(False)
+        return y if residual is None else (y, h)
+
+    @staticmethod
+    def backward(ctx, dy, dh=None):
+        return _backward(ctx, dy, dh, run=_gradients)
 
 
 def block_norm(
@@ -178,8 +209,11 @@ def block_norm(
         raise ValueError(f"{_OP}: weight must be {x.dtype} or float32 (got {weight.dtype})")
     given = [t for t in (x, weight, bias, residual, scale, gate) if t is not None]
     _require_cuda(_OP, *given)
-    if torch.compiler.is_compiling() or (torch.is_grad_enabled() and any(t.requires_grad for t in given)):
-        y, h, _ = _block_norm_fwd(x, weight, bias, residual, scale, gate, groups, float(eps), bool(rms))
-    else:  # nothing to differentiate: no dispatcher
-        y, h, _ = _forward(x, weight, bias, residual, scale, gate, groups, float(eps), bool(rms), False)
+    args = (x, weight, bias, residual, scale, gate, groups, float(eps), bool(rms))
+    if torch.compiler.is_compiling():
+        y, h, _ = _block_norm_fwd(*args)
+    elif torch.is_grad_enabled() and any(t.requires_grad for t in given):
+        return _Eager.apply(*args)
+    else:
+        y, h, _ = _forward(*args, False)
     return y if residual is None else (y, h)

@@ -21,6 +21,8 @@ autograd is not supported and raises, as in the reference
 
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from . import _lib
@@ -59,6 +61,19 @@ def _dense(t: torch.Tensor) -> torch.Tensor:
 
 def _stream(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def on_device(device: torch.device):
+    """``device`` made current, at no cost where it is."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def raw_stream(device: torch.device) -> int:
+    """The current stream's handle, without a ``torch.cuda.Stream`` around it."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _ptr(t: torch.Tensor | None):

@@ -15,7 +15,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .scan_ops import _dtype_code, _require_cuda
+from .scan_ops import _dtype_code, _require_cuda, on_device, raw_stream
 
 __all__ = ["mingru_step", "signed_step", "rotation_step", "givens_step", "delta_step",
            "linear_attention_step"]
@@ -35,8 +35,8 @@ def _p(t):
 
 
 def _run(op, fn, dev, *args):
-    with torch.cuda.device(dev):
-        st = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    with on_device(dev):
+        st = fn(*args, raw_stream(dev))
     _lib.check(st, op)
 
 
@@ -130,11 +130,13 @@ def linear_attention_step(q, k, v, log_gamma, H_prev, out=None):
     elif not out.is_contiguous():
         raise ValueError(f"{op}: out must be contiguous")
     _require_cuda(op, q, log_gamma, H_prev, out)
-    try:
-        lg = torch.broadcast_to(log_gamma, (B, nH)).float()
-    except RuntimeError:
-        raise ValueError(f"{op}: log_gamma must broadcast to {(B, nH)} (got "
-                         f"{tuple(log_gamma.shape)})") from None
+    lg = log_gamma.float()
+    if tuple(lg.shape) != shape[:2]:
+        try:
+            lg = torch.broadcast_to(lg, shape[:2])
+        except RuntimeError:
+            raise ValueError(f"{op}: log_gamma must broadcast to {shape[:2]} (got "
+                             f"{tuple(lg.shape)})") from None
     H_prev = H_prev.contiguous()
     y = torch.empty_like(v)
     _run(op, _lib.load().mgs_linear_attn_step, q.device, _p(q), _p(k), _p(v), _p(lg), lg.stride(0),
