@@ -411,10 +411,9 @@ int mgs_delta_step(const void* q, const void* k, const void* v, const void* beta
  * to a tensor: forward Q, K, V, log_gamma, y; backward Q, K, V, log_gamma, dy,
  * dQ, dK, dV. Rows that start on 16 bytes and hold a multiple of 8 elements are
  * read and written in vectors, others element by element.
- * Envelope: dk, dv <= 128 for bf16, <= 64 for fp32 and fp16 (both dimensions
- * are linear: a wider head is a sum over blocks of dk and a concatenation over
- * blocks of dv). The size queries return 0 outside it, the entry points
- * MGS_UNSUPPORTED.
+ * Envelope: dk, dv <= 128 for bf16, any for fp32 and fp16 (beyond 64 in blocks
+ * of 64: the recurrence is linear in q and k and separate in the columns of v).
+ * The size queries return 0 outside it, the entry points MGS_UNSUPPORTED.
  * `saved` (mgs_linear_attn_saved_size bytes, 16-byte aligned) takes the states
  * at the chunks' starts for the backward; NULL: no backward follows.        */
 size_t mgs_linear_attn_workspace_size(int64_t B, int H, int64_t T, int dk, int dv, int dtype);

@@ -29,7 +29,7 @@ from .scan_ops import _dense, _dtype_code, _ptr, _require_cuda, _workspace, on_d
 __all__ = ["linear_attention"]
 
 _OP = "linear_attention"
-_MAX_D = {torch.bfloat16: 128, torch.float32: 64, torch.float16: 64}  # d_k, d_v of one kernel call
+_MAX_BF16 = 128  # d_k, d_v of a bf16 kernel call
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -180,34 +180,17 @@ class _Eager(torch.autograd.Function):
         return _backward(ctx, dy, dHT, run=_gradients)[:5]
 
 
-def _blocks(d: int, width: int):
-    return [slice(i, min(d, i + width)) for i in range(0, d, width)]
-
-
 def _run(Q, K, V, lg, H0):
-    dk, dv = Q.shape[3], V.shape[3]
-    wide = _MAX_D[Q.dtype]
-    if max(dk, dv) <= wide:
-        if torch.compiler.is_compiling():
-            return _linear_attn_fwd(Q, K, V, lg, H0, True)[:2]
-        if torch.is_grad_enabled() and (Q.requires_grad or K.requires_grad or V.requires_grad
-                                        or lg.requires_grad or (H0 is not None and H0.requires_grad)):
-            return _Eager.apply(Q, K, V, lg, H0)
-        return _forward(Q, K, V, lg, H0, False)[:2]
-    if Q.dtype != torch.float32:
-        # Blocks of 16-bit inputs run on fp32 copies, so that their partial
-        # outputs and gradients are added before the one rounding.
+    if Q.dtype == torch.bfloat16 and max(Q.shape[3], V.shape[3]) > _MAX_BF16:
+        # the fp32 kernels take blocks of any number, added before the one rounding
         y, HT = _run(Q.float(), K.float(), V.float(), lg, H0)
         return y.to(Q.dtype), HT
-    # The recurrence is linear in k and q and separate in the columns of v: y
-    # adds up over blocks of d_k, and value columns are independent.
-    ys, hts = [], []
-    for j in _blocks(dv, wide):
-        parts = [_run(Q[..., i], K[..., i], V[..., j], lg, None if H0 is None else H0[:, :, i, j])
-                 for i in _blocks(dk, wide)]
-        ys.append(sum((y for y, _ in parts[1:]), parts[0][0]))
-        hts.append(torch.cat([h for _, h in parts], 2))
-    return torch.cat(ys, -1), torch.cat(hts, -1)
+    if torch.compiler.is_compiling():
+        return _linear_attn_fwd(Q, K, V, lg, H0, True)[:2]
+    if torch.is_grad_enabled() and (Q.requires_grad or K.requires_grad or V.requires_grad
+                                    or lg.requires_grad or (H0 is not None and H0.requires_grad)):
+        return _Eager.apply(Q, K, V, lg, H0)
+    return _forward(Q, K, V, lg, H0, False)[:2]
 
 
 def linear_attention(
@@ -225,9 +208,9 @@ def linear_attention(
 
     Batch, head and time strides are free: views such as ``(B, T, n_heads,
     d).transpose(1, 2)`` or slices of one projection are read in place, and
-    gradients come in the same order. Any ``d_k``, ``d_v`` (heads wider than
-    128 in bf16, or 64 in fp32 and fp16, run as blocks, 16-bit ones on fp32
-    copies) and any ``T``, 0 included.
+    gradients come in the same order. Any ``d_k``, ``d_v`` (fp32 and fp16 heads
+    wider than 64 run as blocks of 64 whose sums are fp32; bf16 heads wider
+    than 128 run that way on fp32 copies) and any ``T``, 0 included.
 
     ``log_gamma <= 0``; ``-inf`` wipes the state before the token, which is how
     packed sequences are kept apart. A decay below ``2^-128`` counts as a wipe

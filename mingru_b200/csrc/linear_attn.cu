@@ -38,6 +38,8 @@
 // (batch, head) pairs than CTAs fit the GPU: state_kernel sums what a segment
 // adds to the state, scan_kernel joins these along the sequence, and the main
 // kernels then run all segments at once, chunk by chunk inside each.
+#include <type_traits>
+
 #include "common.cuh"
 #include "umma.cuh"
 
@@ -69,7 +71,11 @@ struct Ten {
   P* p;
   long long sb, sh, st;
   int vec, wide;
+  // outputs that are sums over blocks of the heads: fp32 rows of 64 (BH, T, 64)
+  float* part;
+  int mode;
 };
+constexpr int kAdd = 1, kKeep = 2;  // part holds earlier blocks' share; more blocks follow
 
 template <typename E>
 struct Args {
@@ -91,6 +97,9 @@ struct Args {
   int H, dk, dv, nchunks, m, nseg;  // m chunks to a segment
   int ms, r, nsub;                  // segments in r parts of ms chunks for the state sums, nsub in all
   long long BH;
+  long long sbh;  // H0, H_T and their gradients: from one (batch, head) to the next,
+  int sld;        // and from one row to the next
+  int dlg_add;    // dlog_gamma holds earlier blocks' share
 };
 
 // ------------------------------------------------------------- tile loads --
@@ -248,10 +257,24 @@ __device__ __forceinline__ void row16_to_tile(bf16* tile, int r, int c0, const f
   store_levels8<1>(tile, 0, sw<kC>(r, c0 + 8), v + 8);
 }
 
-// 16 values of one row (columns c0..) to global memory, in whole 32-byte sectors
+// 16 values of row t (columns c0..) of a head's output, in whole 32-byte sectors
 // where the rows allow it.
 template <typename E>
-__device__ __forceinline__ void store_row16(E* row, int c0, int d, const Ten<E>& x, const float (&v)[16]) {
+__device__ __forceinline__ void store_row16(const Ten<E>& x, int b, int h, int H, long long t, long long T, int c0,
+                                            int d, float (&v)[16]) {
+  if (x.mode) {
+    float4* o = reinterpret_cast<float4*>(x.part + (((long long)b * H + h) * T + t) * 64 + c0);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (x.mode & kAdd) {
+        const float4 f = o[k];
+        v[4 * k] += f.x, v[4 * k + 1] += f.y, v[4 * k + 2] += f.z, v[4 * k + 3] += f.w;
+      }
+      if (x.mode & kKeep) o[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+    }
+    if (x.mode & kKeep) return;
+  }
+  E* row = x.p + b * x.sb + h * x.sh + t * x.st;
   if (x.vec) {
     constexpr int kN = 32 / (int)sizeof(E);
 #pragma unroll
@@ -478,19 +501,19 @@ struct State {
 #pragma unroll
     for (int i = 0; i < kCols; ++i) v[i] = 0.f;
   }
-  // (dk, dv) row-major
-  __device__ __forceinline__ void load(const float* p, int dk, int dv) {
+  // dk x dv entries of rows ld apart
+  __device__ __forceinline__ void load(const float* p, int dk, int dv, int ld) {
     const int r = row(), c = col0();
 #pragma unroll
     for (int i = 0; i < kCols; ++i)
-      v[i] = valid() && r < dk && c + i < dv ? p[(long long)r * dv + c + i] : 0.f;
+      v[i] = valid() && r < dk && c + i < dv ? p[(long long)r * ld + c + i] : 0.f;
   }
-  __device__ __forceinline__ void store(float* p, int dk, int dv) const {
+  __device__ __forceinline__ void store(float* p, int dk, int dv, int ld) const {
     const int r = row(), c = col0();
     if (!valid() || r >= dk) return;
 #pragma unroll
     for (int i = 0; i < kCols; ++i)
-      if (c + i < dv) p[(long long)r * dv + c + i] = v[i];
+      if (c + i < dv) p[(long long)r * ld + c + i] = v[i];
   }
   // D x D in the order [column / 4][row][4]: whole lines to a warp's access
   __device__ __forceinline__ void load_own(const float* p) {
@@ -686,7 +709,8 @@ __global__ void __launch_bounds__(kThreads, Sums<E, D>::kPerSm) state_kernel(con
 // (backward: after the last one's start) have nobody to add for.
 template <int D, bool kBwd>
 __global__ void __launch_bounds__(256) scan_kernel(float* seg, const float* segl, const float* init,
-                                                   long long BH, int nsub, int steps, int dk, int dv) {
+                                                   long long BH, int nsub, int steps, int dk, int dv,
+                                                   long long sbh, int sld) {
   const long long g = (long long)blockIdx.x * 256 + threadIdx.x;
   const long long bh = g / (D * D / 4);
   if (bh >= BH) return;
@@ -694,7 +718,7 @@ __global__ void __launch_bounds__(256) scan_kernel(float* seg, const float* segl
   float x[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    x[i] = init && row < dk && col + i < dv ? init[(bh * dk + row) * dv + col + i] : 0.f;
+    x[i] = init && row < dk && col + i < dv ? init[bh * sbh + row * sld + col + i] : 0.f;
   float4* sp = reinterpret_cast<float4*>(seg + bh * nsub * (long long)(D * D)) + e;
   const float* lp = segl + bh * nsub;
 #pragma unroll 4
@@ -739,7 +763,6 @@ __global__ void __launch_bounds__(kThreads, Fwd<E, D>::kPerSm) fwd_kernel(const 
   const int s = (int)(blockIdx.x / p.BH);
   const int b = (int)(bh / p.H), h = (int)(bh % p.H);
   const float* lg = p.lg + b * p.lsb + h * p.lsh;
-  const long long dkv = (long long)p.dk * p.dv;
   const int c0 = s * p.m, c1 = min(c0 + p.m, p.nchunks);
   auto rows = [&](int c) { return (int)min((long long)kC, p.T - (long long)c * kC); };
   const bool tma = NL == 1 && p.tma;
@@ -769,7 +792,7 @@ __global__ void __launch_bounds__(kThreads, Fwd<E, D>::kPerSm) fwd_kernel(const 
   if (s > 0)
     S.load_own(p.seg + (bh * p.nsub + s * p.r) * (D * D));
   else if (p.H0)
-    S.load(p.H0 + bh * dkv, p.dk, p.dv);
+    S.load(p.H0 + bh * p.sbh, p.dk, p.dv, p.sld);
   else
     S.zero();
   S.template to_smem<NL>(X);
@@ -891,7 +914,7 @@ __global__ void __launch_bounds__(kThreads, Fwd<E, D>::kPerSm) fwd_kernel(const 
       if (tma)
         row16_to_tile(Q, row, j0, v);
       else if (ok && row < n)
-        store_row16<E>(p.y.p + b * p.y.sb + h * p.y.sh + (t0 + row) * p.y.st, j0, p.dv, p.y, v);
+        store_row16<E>(p.y, b, h, p.H, t0 + row, p.T, j0, p.dv, v);
     }
     if (add) {
       S.update(ex2(th + tl), tb, 0);
@@ -906,7 +929,7 @@ __global__ void __launch_bounds__(kThreads, Fwd<E, D>::kPerSm) fwd_kernel(const 
       bulk_wait_read();
     }
   }
-  if (ok && s + 1 == p.nseg) S.store(p.HT + bh * dkv, p.dk, p.dv);
+  if (ok && s + 1 == p.nseg) S.store(p.HT + bh * p.sbh, p.dk, p.dv, p.sld);
   um::fence_before();
   __syncthreads();
   if (warp == 0) um::dealloc(sm.tbase, F::kCols);
@@ -991,7 +1014,6 @@ __global__ void __launch_bounds__(kThreads, Bwd<E, D>::kPerSm) bwd_kernel(const 
   const int s = p.nseg - 1 - (int)(blockIdx.x / p.BH);
   const int b = (int)(bh / p.H), h = (int)(bh % p.H);
   const float* lg = p.lg + b * p.lsb + h * p.lsh;
-  const long long dkv = (long long)p.dk * p.dv;
   const int c0 = s * p.m, c1 = min(c0 + p.m, p.nchunks);
   auto rows = [&](int c) { return (int)min((long long)kC, p.T - (long long)c * kC); };
   const bool tma = NL == 1 && p.tma, staged = F::kEven && p.tma;
@@ -1039,14 +1061,14 @@ __global__ void __launch_bounds__(kThreads, Bwd<E, D>::kPerSm) bwd_kernel(const 
       } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          dSe[i] = p.dHT && erow < p.dk && ecol + i < p.dv ? p.dHT[bh * dkv + erow * p.dv + ecol + i] : 0.f;
+          dSe[i] = p.dHT && erow < p.dk && ecol + i < p.dv ? p.dHT[bh * p.sbh + erow * p.sld + ecol + i] : 0.f;
       }
       even_to_smem(dSe);
     } else {
       if (end)
         dS.load_own(end);
       else if (p.dHT)
-        dS.load(p.dHT + bh * dkv, p.dk, p.dv);
+        dS.load(p.dHT + bh * p.sbh, p.dk, p.dv, p.sld);
       else
         dS.zero();
       dS.template to_smem<3>(X);
@@ -1189,7 +1211,7 @@ __global__ void __launch_bounds__(kThreads, Bwd<E, D>::kPerSm) bwd_kernel(const 
       if (staged)
         row16_to_tile(stage, row, j0, x);
       else if (ok && row < n)
-        store_row16<E>(p.dV.p + b * p.dV.sb + h * p.dV.sh + (t0 + row) * p.dV.st, j0, p.dv, p.dV, x);
+        store_row16<E>(p.dV, b, h, p.H, t0 + row, p.T, j0, p.dv, x);
       um::ld16_async(lb + F::kDk + j0, r1);
       um::ld16_async(lb + F::kIk + j0, r2);
       um::ld_wait();
@@ -1212,7 +1234,7 @@ __global__ void __launch_bounds__(kThreads, Bwd<E, D>::kPerSm) bwd_kernel(const 
           }
         }
       } else if (ok && row < n) {
-        store_row16<E>(p.dK.p + b * p.dK.sb + h * p.dK.sh + (t0 + row) * p.dK.st, j0, p.dk, p.dK, x);
+        store_row16<E>(p.dK, b, h, p.H, t0 + row, p.T, j0, p.dk, x);
       }
     }
     bk *= to_end;
@@ -1337,7 +1359,7 @@ __global__ void __launch_bounds__(kThreads, Bwd<E, D>::kPerSm) bwd_kernel(const 
           }
         }
       } else if (ok && row < n) {
-        store_row16<E>(p.dQ.p + b * p.dQ.sb + h * p.dQ.sh + (t0 + row) * p.dQ.st, j0, p.dk, p.dQ, x);
+        store_row16<E>(p.dQ, b, h, p.H, t0 + row, p.T, j0, p.dk, x);
       }
     }
     sm.a[wg][row] = fmaf(from_start, aq, tok);
@@ -1407,7 +1429,9 @@ __global__ void __launch_bounds__(kThreads, Bwd<E, D>::kPerSm) bwd_kernel(const 
         const int t = 4 * lane + i;
         if (t < n) {
           const float l = lg[(t0 + t) * p.lst] * 1.4426950408889634f;
-          p.dlg[bh * p.T + t0 + t] = l <= kMinLog2 ? 0.f : (float)(va[i] + vb[i] + rest);
+          float* o = p.dlg + bh * p.T + t0 + t;
+          const double all = va[i] + vb[i] + rest + (p.dlg_add ? (double)*o : 0.0);
+          *o = l <= kMinLog2 ? 0.f : (float)all;
         }
       }
     }
@@ -1417,9 +1441,9 @@ __global__ void __launch_bounds__(kThreads, Bwd<E, D>::kPerSm) bwd_kernel(const 
     if constexpr (F::kEven) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        if (erow < p.dk && ecol + i < p.dv) p.dH0[bh * dkv + erow * p.dv + ecol + i] = dSe[i];
+        if (erow < p.dk && ecol + i < p.dv) p.dH0[bh * p.sbh + erow * p.sld + ecol + i] = dSe[i];
     } else {
-      dS.store(p.dH0 + bh * dkv, p.dk, p.dv);
+      dS.store(p.dH0 + bh * p.sbh, p.dk, p.dv, p.sld);
     }
   }
   um::fence_before();
@@ -1465,17 +1489,22 @@ Plan plan_for(long long BH, long long T, int D, int per_sm, int sums_per_sm) {
   return pl;
 }
 
+// Element type and the width that kernels run at. bf16 heads up to 128 run
+// whole; fp32 and fp16, whose operands take two or three times the room, in
+// blocks of 64: the recurrence is linear in q and k (a sum over blocks of dk)
+// and separate in the columns of v.
 template <class F>
 int by_shape(int dtype, int dk, int dv, F&& f) {
   const int d = dk > dv ? dk : dv;
-  if (dtype == MGS_BF16)
-    return d <= 64    ? f(bf16{}, std::integral_constant<int, 64>{})
-           : d <= 128 ? f(bf16{}, std::integral_constant<int, 128>{})
-                      : (int)MGS_UNSUPPORTED;
-  if (dtype != MGS_F32 && dtype != MGS_F16) return MGS_BAD_DTYPE;
-  if (d > 64) return MGS_UNSUPPORTED;
-  return dtype == MGS_F32 ? f(float{}, std::integral_constant<int, 64>{})
-                          : f(__half{}, std::integral_constant<int, 64>{});
+  switch (dtype) {
+    case MGS_BF16:
+      return d <= 64    ? f(bf16{}, std::integral_constant<int, 64>{})
+             : d <= 128 ? f(bf16{}, std::integral_constant<int, 128>{})
+                        : (int)MGS_UNSUPPORTED;
+    case MGS_F32: return f(float{}, std::integral_constant<int, 64>{});
+    case MGS_F16: return f(__half{}, std::integral_constant<int, 64>{});
+    default: return MGS_BAD_DTYPE;
+  }
 }
 
 size_t seg_bytes(const Plan& pl, long long BH) {
@@ -1503,7 +1532,7 @@ bool whole(P* p, const int64_t* s, int d, int bytes) {
 template <typename P>
 Ten<P> ten(P* p, const int64_t* s, int d) {
   const bool vec = whole(p, s, d, 16);
-  return {p, (long long)s[0], (long long)s[1], (long long)s[2], vec, vec && whole(p, s, d, 32)};
+  return {p, (long long)s[0], (long long)s[1], (long long)s[2], vec, vec && whole(p, s, d, 32), nullptr, 0};
 }
 
 // Tensor map over (columns, time, head, batch) with boxes of 64 columns x 128
@@ -1546,7 +1575,8 @@ int run_segments(const Args<E>& a, cudaStream_t st) {
   if (int r = launched()) return r;
   const long long n = a.BH * (D * D / 4);
   scan_kernel<D, kBwd><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(
-      a.seg, a.segl, kBwd ? a.dHT : a.H0, a.BH, a.nsub, (a.nseg - 1) * a.r, a.dk, a.dv);
+      a.seg, a.segl, kBwd ? a.dHT : a.H0, a.BH, a.nsub, (a.nseg - 1) * a.r, a.dk, a.dv, a.sbh,
+      a.sld);
   return launched();
 }
 
@@ -1560,27 +1590,83 @@ int run_main(bool fwd, const Args<E>& a, cudaStream_t st) {
   return launched();
 }
 
+struct Blocks {  // of a head, in both dimensions
+  int nk, nv;
+  Blocks(int dk, int dv, int D) : nk((dk + D - 1) / D), nv((dv + D - 1) / D) {}
+};
+
+// fp32 rows for sums over blocks: dV's of one block of dv, dQ's and dK's of all.
+size_t part_floats(const Blocks& n, bool fwd) {
+  return fwd ? (n.nk > 1 ? 1 : 0) : (n.nk > 1 ? 1 : 0) + (n.nv > 1 ? 2 * (size_t)n.nk : 0);
+}
+
 template <typename E, int D>
-int fill(Args<E>& a, bool fwd, const float* lg, const int64_t* ls, int64_t B, int H, int64_t T, int dk,
-         int dv, void* ws, size_t ws_bytes) {
+size_t workspace_bytes_of(bool fwd, int64_t B, int H, int64_t T, int dk, int dv) {
+  const long long BH = B * (long long)H;
+  return (seg_bytes(plan_of<E, D>(fwd, BH, T), BH) + 255) / 256 * 256 +
+         part_floats(Blocks(dk, dv, D), fwd) * (size_t)BH * T * 64 * sizeof(float);
+}
+
+// One call, over a head's blocks. What all blocks share is set in `a`.
+template <typename E, int D>
+int run_blocks(Args<E>& a, bool fwd, const float* lg, const int64_t* s, int64_t B, int H, int64_t T, int dk,
+               int dv, void* ws, size_t ws_bytes, cudaStream_t st) {
   const long long BH = B * (long long)H;
   const Plan pl = plan_of<E, D>(fwd, BH, T);
-  if (seg_bytes(pl, BH) > ws_bytes) return MGS_WORKSPACE_TOO_SMALL;
-  if (seg_bytes(pl, BH) && (!ws || reinterpret_cast<uintptr_t>(ws) % 16)) return MGS_BAD_ALIGNMENT;
-  a.lg = lg, a.lsb = ls[0], a.lsh = ls[1], a.lst = ls[2];
+  const size_t need = workspace_bytes_of<E, D>(fwd, B, H, T, dk, dv);
+  if (need > ws_bytes) return MGS_WORKSPACE_TOO_SMALL;
+  if ((need && !aligned(ws, 16)) || !aligned(a.saved, 16)) return MGS_BAD_ALIGNMENT;
+  a.lg = lg, a.lsb = s[9], a.lsh = s[10], a.lst = s[11];
   a.seg = static_cast<float*>(ws);
   a.segl = a.seg + (size_t)BH * pl.nsub * D * D;
-  a.T = T, a.H = H, a.dk = dk, a.dv = dv, a.nchunks = pl.nchunks, a.m = pl.m, a.nseg = pl.nseg, a.BH = BH;
+  a.T = T, a.H = H, a.nchunks = pl.nchunks, a.m = pl.m, a.nseg = pl.nseg, a.BH = BH;
   a.ms = pl.ms, a.r = pl.r, a.nsub = pl.nsub;
-  if constexpr (std::is_same_v<E, bf16>) {
-    bool ok = map_of(&a.mQ, a.Q, dk, T, H, B) && map_of(&a.mK, a.K, dk, T, H, B) && map_of(&a.mV, a.V, dv, T, H, B);
-    if (fwd)
-      ok = ok && map_of(&a.my, a.y, dv, T, H, B);
-    else
-      ok = ok && map_of(&a.mdy, a.dy, dv, T, H, B) && map_of(&a.mdQ, a.dQ, dk, T, H, B) &&
-           map_of(&a.mdK, a.dK, dk, T, H, B) && map_of(&a.mdV, a.dV, dv, T, H, B);
-    a.tma = ok;
-  }
+  a.sbh = (long long)dk * dv, a.sld = dv;
+  const Blocks n(dk, dv, D);
+  const size_t rows = (size_t)BH * T * 64;
+  float* part = reinterpret_cast<float*>(static_cast<char*>(ws) + (seg_bytes(pl, BH) + 255) / 256 * 256);
+  float *part_v = part, *part_q = part + (n.nk > 1 ? rows : 0), *part_k = part_q + n.nk * rows;
+  const Args<E> whole = a;
+  auto sum = [](auto& x, float* rows_, int i, int last) {  // x: a sum over blocks 0..last
+    if (last == 0) return;
+    x.part = rows_, x.mode = (i > 0 ? kAdd : 0) | (i < last ? kKeep : 0);
+  };
+  for (int j = 0; j < n.nv; ++j)
+    for (int i = 0; i < n.nk; ++i) {
+      const int k0 = i * D, v0 = j * D, bk = dk - k0 < D ? dk - k0 : D, bv = dv - v0 < D ? dv - v0 : D;
+      const long long s0 = (long long)k0 * dv + v0;
+      a = whole;
+      a.dk = bk, a.dv = bv;
+      a.Q = ten(whole.Q.p + k0, s, bk), a.K = ten(whole.K.p + k0, s + 3, bk), a.V = ten(whole.V.p + v0, s + 6, bv);
+      if (fwd) {
+        a.y = ten(whole.y.p + v0, s + 12, bv);
+        sum(a.y, part_v, i, n.nk - 1);
+        a.HT = whole.HT + s0;
+        if (whole.H0) a.H0 = whole.H0 + s0;
+      } else {
+        a.dy = ten(whole.dy.p + v0, s + 12, bv);
+        a.dQ = ten(whole.dQ.p + k0, s + 15, bk), a.dK = ten(whole.dK.p + k0, s + 18, bk);
+        a.dV = ten(whole.dV.p + v0, s + 21, bv);
+        sum(a.dV, part_v, i, n.nk - 1);
+        sum(a.dQ, part_q + i * rows, j, n.nv - 1);
+        sum(a.dK, part_k + i * rows, j, n.nv - 1);
+        if (whole.dHT) a.dHT = whole.dHT + s0;
+        if (whole.dH0) a.dH0 = whole.dH0 + s0;
+        a.dlg_add = i + j > 0;
+      }
+      if (whole.saved) a.saved = whole.saved + (size_t)(j * n.nk + i) * BH * pl.nchunks * D * D;
+      if constexpr (std::is_same_v<E, bf16>) {
+        bool ok = map_of(&a.mQ, a.Q, dk, T, H, B) && map_of(&a.mK, a.K, dk, T, H, B) &&
+                  map_of(&a.mV, a.V, dv, T, H, B);
+        if (fwd)
+          ok = ok && map_of(&a.my, a.y, dv, T, H, B);
+        else
+          ok = ok && map_of(&a.mdy, a.dy, dv, T, H, B) && map_of(&a.mdQ, a.dQ, dk, T, H, B) &&
+               map_of(&a.mdK, a.dK, dk, T, H, B) && map_of(&a.mdV, a.dV, dv, T, H, B);
+        a.tma = ok;
+      }
+      if (int r = run_main<E, D>(fwd, a, st)) return r;
+    }
   return MGS_OK;
 }
 
@@ -1600,8 +1686,8 @@ size_t mgs_linear_attn_workspace_size(int64_t B, int H, int64_t T, int dk, int d
   (void)by_shape(dtype, dk, dv, [&](auto e, auto d) -> int {
     using E = decltype(e);
     constexpr int D = decltype(d)::value;
-    const size_t f = seg_bytes(plan_of<E, D>(true, B * H, T), B * H);
-    const size_t b = seg_bytes(plan_of<E, D>(false, B * H, T), B * H);
+    const size_t f = workspace_bytes_of<E, D>(true, B, H, T, dk, dv);
+    const size_t b = workspace_bytes_of<E, D>(false, B, H, T, dk, dv);
     n = f > b ? f : b;
     return MGS_OK;
   });
@@ -1614,7 +1700,8 @@ size_t mgs_linear_attn_saved_size(int64_t B, int H, int64_t T, int dk, int dv, i
   size_t n = 0;
   (void)by_shape(dtype, dk, dv, [&](auto, auto d) -> int {
     constexpr int D = decltype(d)::value;
-    n = (size_t)(B * H) * (size_t)((T + kC - 1) / kC) * D * D * sizeof(float);
+    const Blocks blocks(dk, dv, D);
+    n = (size_t)blocks.nk * blocks.nv * (size_t)(B * H) * (size_t)((T + kC - 1) / kC) * D * D * sizeof(float);
     return MGS_OK;
   });
   return n;
@@ -1628,18 +1715,12 @@ int mgs_linear_attn_fwd(const void* Q, const void* K, const void* V, const float
   if (!shape_ok(B, H, T, dk, dv)) return MGS_BAD_SHAPE;
   return by_shape(dtype, dk, dv, [&](auto e, auto d) -> int {
     using E = decltype(e);
-    constexpr int D = decltype(d)::value;
     if (B == 0 || H == 0 || T == 0) return MGS_OK;
-    if (reinterpret_cast<uintptr_t>(saved) % 16) return MGS_BAD_ALIGNMENT;
     Args<E> a{};
-    a.Q = ten(static_cast<const E*>(Q), strides, dk);
-    a.K = ten(static_cast<const E*>(K), strides + 3, dk);
-    a.V = ten(static_cast<const E*>(V), strides + 6, dv);
-    a.y = ten(static_cast<E*>(y), strides + 12, dv);
-    a.H0 = H0, a.HT = H_T, a.saved = saved;
-    if (int r = fill<E, D>(a, true, log_gamma, strides + 9, B, H, T, dk, dv, workspace, workspace_bytes))
-      return r;
-    return run_main<E, D>(true, a, static_cast<cudaStream_t>(stream));
+    a.Q.p = static_cast<const E*>(Q), a.K.p = static_cast<const E*>(K), a.V.p = static_cast<const E*>(V);
+    a.y.p = static_cast<E*>(y), a.H0 = H0, a.HT = H_T, a.saved = saved;
+    return run_blocks<E, decltype(d)::value>(a, true, log_gamma, strides, B, H, T, dk, dv, workspace,
+                                             workspace_bytes, static_cast<cudaStream_t>(stream));
   });
 }
 
@@ -1652,21 +1733,14 @@ int mgs_linear_attn_bwd(const void* Q, const void* K, const void* V, const float
   if (!shape_ok(B, H, T, dk, dv)) return MGS_BAD_SHAPE;
   return by_shape(dtype, dk, dv, [&](auto e, auto d) -> int {
     using E = decltype(e);
-    constexpr int D = decltype(d)::value;
     if (B == 0 || H == 0 || T == 0) return MGS_OK;
-    if (reinterpret_cast<uintptr_t>(saved) % 16) return MGS_BAD_ALIGNMENT;
     Args<E> a{};
-    a.Q = ten(static_cast<const E*>(Q), strides, dk);
-    a.K = ten(static_cast<const E*>(K), strides + 3, dk);
-    a.V = ten(static_cast<const E*>(V), strides + 6, dv);
-    a.dy = ten(static_cast<const E*>(dy), strides + 12, dv);
-    a.dQ = ten(static_cast<E*>(dQ), strides + 15, dk);
-    a.dK = ten(static_cast<E*>(dK), strides + 18, dk);
-    a.dV = ten(static_cast<E*>(dV), strides + 21, dv);
+    a.Q.p = static_cast<const E*>(Q), a.K.p = static_cast<const E*>(K), a.V.p = static_cast<const E*>(V);
+    a.dy.p = static_cast<const E*>(dy);
+    a.dQ.p = static_cast<E*>(dQ), a.dK.p = static_cast<E*>(dK), a.dV.p = static_cast<E*>(dV);
     a.saved = const_cast<float*>(saved), a.dHT = dH_T, a.dH0 = dH0, a.dlg = dlog_gamma;
-    if (int r = fill<E, D>(a, false, log_gamma, strides + 9, B, H, T, dk, dv, workspace, workspace_bytes))
-      return r;
-    return run_main<E, D>(false, a, static_cast<cudaStream_t>(stream));
+    return run_blocks<E, decltype(d)::value>(a, false, log_gamma, strides, B, H, T, dk, dv, workspace,
+                                             workspace_bytes, static_cast<cudaStream_t>(stream));
   });
 }
 

@@ -25,10 +25,10 @@ def _rows(t: torch.Tensor | None, D: int):
     """``t`` as rows of D: (tensor that owns them, row stride)."""
     if t is None:
         return None, 0
+    if t.is_contiguous():
+        return t, D
     if t.stride(-1) == 1 or D == 1:
         if t.dim() == 1:
-            return t, D
-        if t.is_contiguous():
             return t, D
         # one stride from row to row over all the leading dimensions
         s, ok = t.stride(-2), True
@@ -45,6 +45,10 @@ def _workspace_bytes(device: int, rows: int, D: int, groups: int, code: int) -> 
     return _lib.load().mgs_block_norm_workspace_size(rows, D, groups, code)
 
 
+def _dense_like(x):
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
 def _codes(x, weight):
     return _dtype_code(_OP, x), _dtype_code(_OP, weight)
 
@@ -55,7 +59,7 @@ def _forward(x, weight, bias, residual, scale, gate, groups, eps, rms, save):
         rows = x.numel() // D
         (x, lx), (residual, lr), (gate, lg) = _rows(x, D), _rows(residual, D), _rows(gate, D)
         weight, bias, scale = (None if t is None else _dense(t) for t in (weight, bias, scale))
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        y = _dense_like(x)
         h = torch.empty_like(y) if residual is not None else None
         stats = torch.empty(rows * groups * 3, dtype=torch.float32, device=x.device) if save else None
         code, wcode = _codes(x, weight)
@@ -94,11 +98,10 @@ def _gradients(x, weight, bias, residual, scale, gate, stats, dy, dh, groups, rm
         (x, lx), (residual, lr), (gate, lg) = _rows(x, D), _rows(residual, D), _rows(gate, D)
         (dy, ly), (dh, lh) = _rows(dy, D), _rows(dh, D)
         weight, bias, scale = (None if t is None else _dense(t) for t in (weight, bias, scale))
-        dense = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
-        dx, dw = dense(x), dense(weight)
-        dres, ds = (None, None) if scale is None else (dense(x), dense(weight))
-        db = None if bias is None else dense(weight)
-        dgate = None if gate is None else dense(x)
+        dx, dw = _dense_like(x), torch.empty_like(weight)
+        dres, ds = (None, None) if scale is None else (torch.empty_like(dx), torch.empty_like(weight))
+        db = None if bias is None else torch.empty_like(weight)
+        dgate = None if gate is None else torch.empty_like(dx)
         code, wcode = _codes(x, weight)
         ws = _workspace(_workspace_bytes(x.device.index, rows, D, groups, code), x.device)
         st = lib.mgs_block_norm_bwd(

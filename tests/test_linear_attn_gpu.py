@@ -322,7 +322,8 @@ def test_c_entry_refuses(cuda):
     assert name(call(-1, 1, 1, 8, 8, 0)) == "MGS_BAD_SHAPE"
     assert name(call(1, 1, 1, 0, 8, 0)) == "MGS_BAD_SHAPE"
     assert name(call(1, 1, 1, 8, 8, 7)) == "MGS_BAD_DTYPE"
-    assert name(call(1, 1, 1, 8, 65, 0)) == "MGS_UNSUPPORTED"
+    assert name(call(1, 1, 1, 8, 129, 1)) == "MGS_UNSUPPORTED"
+    assert name(call(1, 1, 1, 130, 8, 0)) == "MGS_WORKSPACE_TOO_SMALL"
     assert name(call(1, 1, 1, 129, 8, 1)) == "MGS_UNSUPPORTED"
     assert name(call(1, 1, 1000, 8, 8, 0)) == "MGS_WORKSPACE_TOO_SMALL"
     assert name(call(1, 1, 1, 8, 8, 0, saved=p + 4)) == "MGS_BAD_ALIGNMENT"
