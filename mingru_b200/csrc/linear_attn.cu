@@ -90,9 +90,11 @@ struct Args {
   const float* dHT;  // (B, H, dk, dv) or null: zeros
   float* dH0;        // (B, H, dk, dv) or null: not wanted
   float* dlg;        // (B, H, T)
-  float* saved;      // (BH, nchunks, D * D) chunk-start states, or null (forward without a backward)
+  float* saved;      // (BH, nchunks + 1, D * D) states at the chunks' starts and the end, or null: no backward
   float* seg;        // (BH, nsub, D * D) states at the parts' starts (backward: ends) (workspace)
   float* segl;       // (BH, nsub) log2 of each part's total decay (workspace)
+  float* tq;         // (BH, T) a token's row sums and q . its gradient's state part (workspace)
+  float* aq;         // (BH, nchunks) sums of the latter over a chunk (workspace)
   long long T;
   int H, dk, dv, nchunks, m, nseg;  // m chunks to a segment
   int ms, r, nsub;                  // segments in r parts of ms chunks for the state sums, nsub in all
@@ -844,7 +846,7 @@ __global__ void __launch_bounds__(kThreads, Fwd<E, D>::kPerSm) fwd_kernel(const 
       }
     }
     if (warp == kDecayWarp && more) dw.load(lg + (t0 + kC) * p.lst, p.lst, rows(c + 1));
-    if (p.saved) S.store_own(p.saved + (bh * p.nchunks + c) * (D * D));
+    if (p.saved) S.store_own(p.saved + (bh * (p.nchunks + 1) + c) * (D * D));
     wait();
     const uint32_t lb = tb + ((uint32_t)(32 * q) << 16);
     const float rh = dec.ch[row], rl = dec.cl[row];
@@ -929,22 +931,40 @@ __global__ void __launch_bounds__(kThreads, Fwd<E, D>::kPerSm) fwd_kernel(const 
       bulk_wait_read();
     }
   }
-  if (ok && s + 1 == p.nseg) S.store(p.HT + bh * p.sbh, p.dk, p.dv, p.sld);
+  if (ok && s + 1 == p.nseg) {
+    S.store(p.HT + bh * p.sbh, p.dk, p.dv, p.sld);
+    if (p.saved) S.store_own(p.saved + (bh * (p.nchunks + 1) + c1) * (D * D));
+  }
   um::fence_before();
   __syncthreads();
   if (warp == 0) um::dealloc(sm.tbase, F::kCols);
 }
 
 // --------------------------------------------------------------- backward --
+//
+// Two kernels. dQ and what it needs come from single chunks, with the states
+// that the forward saved: dq_kernel takes chunks in any order. dK, dV and the
+// states' gradient go through a segment's chunks from its end: dkv_kernel. Both
+// form the masked products anew, each as its own rows want them.
+//
+// dlog_gamma. Token i's row of R and its state part add to every t <= i, token
+// j's column of R takes the pairs with i, j >= t out again, and its state part
+// bk_j = k_j . dK'_j adds to every t > j. The part that passes through a chunk
+// whole, e^{c_C} <S, dS'>, follows from chunk to chunk: with F = <S, dS> at a
+// chunk's end it is F - sum_j bk_j, and F at its start that plus sum_i q_i .
+// dQ'_i. So with tq_i = sum_j R_ij + q_i . dQ'_i, from dq_kernel,
+//   dlog_gamma_t = sum_{i >= t} (tq_i - sum_{i' > i} R_i'i - bk_i) + F.
 
 struct SmallB {
   uint64_t bar, bar2, full;
-  uint32_t tbase;
-  float dot;
-  float a[2][kC];  // per half: what token i adds to dlog_gamma_t for t <= i
-  Decays dec[1];   // two where there is room; ch and cl end as what a token adds to later ones
+  uint32_t tbase, pad;
+  float red[8], red2[8];  // by warp
+  float a[2][kC];         // per half of the columns: a token's share of the sums above
+  Decays dec;
 };
-static_assert(sizeof(SmallB) <= 3072, "");
+constexpr int kSmallB = 3072;
+static_assert(sizeof(SmallB) <= kSmallB, "");
+constexpr int kSumWarp = 5;  // puts dlog_gamma together, during the next chunk's first products
 
 // NL = 1: 64 masked products of a lane's row, rounded and packed while both
 // accumulators are still being read; NL > 1: as they are.
@@ -975,104 +995,101 @@ struct Held {
   }
 };
 
-// TMEM columns, first half of a chunk: (K Q^T) 0..127 and (V dy^T) 128..255;
-// once read, their masked forms A2 at 0, A1 at 64 NL (NL levels of 64), dV at
-// 128 NL, dK after it; once these are done, the state parts at kIv and kIk.
-// Second half: (dy V^T) 0..127 and (Q K^T) 128..255; once read, A1 at 0, dQ at
-// 64 NL, its state part after it, and at last the state's sum at 0.
-template <typename E, int D>
-struct Bwd {
-  static constexpr int NL = kLevels<E>, kTileE = kC * D;
-  static constexpr int kDv = 128 * NL, kDk = kDv + D;
-  static constexpr int kIv = 0, kIk = 2 * D <= kDv ? D : kDk + D;
-  static constexpr int kDq = 64 * NL, kIq = kDq + D;
-  static constexpr int kCols = kDk + D <= 256 ? 256 : 512;
-  static_assert(kDk + D <= 512 && kIk + D <= 512 && kIq + D <= kCols, "");
-  // Two CTAs to an SM: dS is spread over all threads (16 entries each), and a
-  // tile of its own stages the gradients on their way out.
-  static constexpr bool kEven = NL == 1 && D == 64;
-  static constexpr int kTabs = D == 64 ? 2 : 1;
-  static constexpr size_t kSmallB = kTabs == 2 ? 5120 : 3072;
-  static constexpr size_t kSmem =
-      kSmallB + 2 * ((4 * NL + (kEven ? 1 : 0)) * (size_t)kTileE + 3 * (size_t)D * D);
-  static_assert(sizeof(SmallB) + (kTabs - 1) * sizeof(Decays) <= kSmallB && kSmem <= 227 * 1024, "");
-  static constexpr int kPerSm = 2 * (kSmem + 1024) <= 228 * 1024 && kCols <= 256 ? 2 : 1;
+// D = 64: 16 entries of one row of a state to each thread, all lanes busy.
+struct Even {
+  static constexpr int D = 64;
+  __device__ static int row() { return threadIdx.x & 63; }
+  __device__ static int col() { return (threadIdx.x >> 6) * 16; }
+  __device__ static void load_own(const float* src, float (&v)[16]) {  // State's own order
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const float4 f = *reinterpret_cast<const float4*>(src + (((col() + i) / 4) * D + row()) * 4);
+      v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
+    }
+  }
+  __device__ static void to_smem(bf16* t, const float (&v)[16]) {
+    store_levels8<3>(t, D * D, sw<D>(row(), col()), v);
+    store_levels8<3>(t, D * D, sw<D>(row(), col() + 8), v + 8);
+  }
 };
+
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
+// 16 values, rounded to bf16 and packed, and back into a tile's row.
+__device__ __forceinline__ void pack16(const float (&x)[16], uint32_t* w) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const __nv_bfloat162 u = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&u);
+  }
+}
+__device__ __forceinline__ void packed16_to_tile(bf16* tile, int r, int c0, const uint32_t* w) {
+  *reinterpret_cast<uint4*>(tile + sw<kC>(r, c0)) = make_uint4(w[0], w[1], w[2], w[3]);
+  *reinterpret_cast<uint4*>(tile + sw<kC>(r, c0 + 8)) = make_uint4(w[4], w[5], w[6], w[7]);
+}
+
+// TMEM columns: (dy V^T) 0..127 and (Q K^T) 128..255; once both are read, the
+// masked A1 at 0 (NL levels of 64), dQ at 64 NL and its state part after it.
 template <typename E, int D>
-__global__ void __launch_bounds__(kThreads, Bwd<E, D>::kPerSm) bwd_kernel(const __grid_constant__ Args<E> p) {
-  using F = Bwd<E, D>;
+struct Dq {
+  static constexpr int NL = kLevels<E>, kTileE = kC * D;
+  static constexpr int kDq = 64 * NL, kIq = kDq + D, kCols = kIq + D <= 256 ? 256 : 512;
+  static constexpr size_t kSmem = kSmallB + 2 * (4 * NL * (size_t)kTileE + 3 * (size_t)D * D);
+  static constexpr int kPerSm = 2 * (kSmem + 1024) <= 228 * 1024 && kCols <= 256 ? 2 : 1;
+  static_assert(kSmem <= 227 * 1024, "");
+};
+
+template <typename E, int D>
+__global__ void __launch_bounds__(kThreads, Dq<E, D>::kPerSm) dq_kernel(const __grid_constant__ Args<E> p) {
+  using F = Dq<E, D>;
   constexpr int NL = F::NL, kTileE = F::kTileE;
   extern __shared__ __align__(1024) unsigned char smem[];
   SmallB& sm = *reinterpret_cast<SmallB*>(smem);
-  bf16* Q = reinterpret_cast<bf16*>(smem + F::kSmallB);
+  bf16* Q = reinterpret_cast<bf16*>(smem + kSmallB);
   bf16 *K = Q + NL * kTileE, *V = K + NL * kTileE, *G = V + NL * kTileE, *X = G + NL * kTileE;
-  bf16* stage = X + 3 * D * D;
-  // the scaled Q rows go over Q and, below three levels, over K and V (read by then)
-  bf16* const lv[3] = {Q, NL == 1 ? K : Q + kTileE, NL == 1 ? V : NL == 2 ? K : Q + 2 * kTileE};
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q = warp & 3, wg = warp >> 2;
-  const long long bh = blockIdx.x % p.BH;
-  const int s = p.nseg - 1 - (int)(blockIdx.x / p.BH);
-  const int b = (int)(bh / p.H), h = (int)(bh % p.H);
-  const float* lg = p.lg + b * p.lsb + h * p.lsh;
-  const int c0 = s * p.m, c1 = min(c0 + p.m, p.nchunks);
-  auto rows = [&](int c) { return (int)min((long long)kC, p.T - (long long)c * kC); };
-  const bool tma = NL == 1 && p.tma, staged = F::kEven && p.tma;
-  auto load = [&](int c) {  // by one thread
-    mbar_arrive_expect_tx(&sm.full, 4 * tile_bytes(D));
-    tma_load<D>(K, &p.mK, (long long)c * kC, h, b, &sm.full);
-    tma_load<D>(Q, &p.mQ, (long long)c * kC, h, b, &sm.full);
-    tma_load<D>(V, &p.mV, (long long)c * kC, h, b, &sm.full);
-    tma_load<D>(G, &p.mdy, (long long)c * kC, h, b, &sm.full);
+  const int row = 32 * q + lane;
+  const long long total = p.BH * p.nchunks;
+  struct At {  // a chunk's place
+    long long bh, t0;
+    int b, h, c, n;
+  };
+  auto at = [&](long long id) {
+    At a;
+    a.bh = id % p.BH, a.c = (int)(id / p.BH);
+    a.b = (int)(a.bh / p.H), a.h = (int)(a.bh % p.H);
+    a.t0 = (long long)a.c * kC;
+    a.n = (int)min((long long)kC, p.T - a.t0);
+    return a;
+  };
+  const bool tma = NL == 1 && p.tma;
+  Decays& dec = sm.dec;
+  DecayWarp dw;
+  auto load_decay = [&](const At& a) {
+    dw.load(p.lg + a.b * p.lsb + a.h * p.lsh + a.t0 * p.lst, p.lst, a.n);
   };
 
   if (warp == 0) um::alloc(&sm.tbase, F::kCols);
+  At a = at(blockIdx.x);
   if (tid == 0) {
     mbar_init(&sm.bar, 1);
-    mbar_init(&sm.bar2, 1);
     mbar_init(&sm.full, 1);
     mbar_fence_init();
-    if (tma) load(c1 - 1);
-  }
-  DecayWarp dw;
-  if (F::kTabs == 2 && warp == kDecayWarp) {
-    dw.load(lg + (long long)(c1 - 1) * kC * p.lst, p.lst, rows(c1 - 1));
-    dw.table<true>(sm.dec[(c1 - 1) & 1]);
-  }
-  // dS: kEven, 16 entries of one row to a thread; otherwise as accumulators are read
-  const int erow = tid & 63, ecol = (tid >> 6) * 16;
-  auto even_own = [&](const float* src, float (&v)[16]) {  // from a state in its own order
-#pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      const float4 f = *reinterpret_cast<const float4*>(src + (((ecol + i) / 4) * D + erow) * 4);
-      v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
+    if (tma) {
+      mbar_arrive_expect_tx(&sm.full, 4 * tile_bytes(D));
+      tma_load<D>(G, &p.mdy, a.t0, a.h, a.b, &sm.full);
+      tma_load<D>(V, &p.mV, a.t0, a.h, a.b, &sm.full);
+      tma_load<D>(Q, &p.mQ, a.t0, a.h, a.b, &sm.full);
+      tma_load<D>(K, &p.mK, a.t0, a.h, a.b, &sm.full);
     }
-  };
-  auto even_to_smem = [&](const float (&v)[16]) {
-    store_levels8<3>(X, D * D, sw<D>(erow, ecol), v);
-    store_levels8<3>(X, D * D, sw<D>(erow, ecol + 8), v + 8);
-  };
-  float dSe[16];
-  State<D> dS;
-  {
-    const float* end = s + 1 < p.nseg ? p.seg + (bh * p.nsub + (s + 1) * p.r - 1) * (D * D) : nullptr;
-    if constexpr (F::kEven) {
-      if (end) {
-        even_own(end, dSe);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          dSe[i] = p.dHT && erow < p.dk && ecol + i < p.dv ? p.dHT[bh * p.sbh + erow * p.sld + ecol + i] : 0.f;
-      }
-      even_to_smem(dSe);
-    } else {
-      if (end)
-        dS.load_own(end);
-      else if (p.dHT)
-        dS.load(p.dHT + bh * p.sbh, p.dk, p.dv, p.sld);
-      else
-        dS.zero();
-      dS.template to_smem<3>(X);
-    }
+  }
+  if (warp == kDecayWarp) {
+    load_decay(a);
+    dw.table<false>(dec);
   }
   bool ok = true;
   auto sync = [&]() {
@@ -1088,16 +1105,313 @@ __global__ void __launch_bounds__(kThreads, Bwd<E, D>::kPerSm) bwd_kernel(const 
     um::fence_after();
   };
   if (tma) sync();  // the barriers
+  unsigned turn = 0;
+  for (long long id = blockIdx.x; id < total; id += gridDim.x, turn ^= 1) {
+    const bool more = id + gridDim.x < total;
+    const At next = at(more ? id + gridDim.x : id);
+    {  // the state that entered the chunk
+      const float* src = p.saved + (a.bh * (p.nchunks + 1) + a.c) * (D * D);
+      if constexpr (D == 64) {
+        float v[16];
+        Even::load_own(src, v);
+        Even::to_smem(X, v);
+      } else {
+        State<D> S;
+        S.load_own(src);
+        S.template to_smem<3>(X);
+      }
+    }
+    if (tma) {
+      if (ok) ok = mbar_wait(&sm.full, turn, &g_sticky_err, kPolls);
+    } else {
+      load_tile<E, D>(Q, p.Q, a.b, a.h, a.t0, a.n, p.dk);
+      load_tile<E, D>(K, p.K, a.b, a.h, a.t0, a.n, p.dk);
+      load_tile<E, D>(V, p.V, a.b, a.h, a.t0, a.n, p.dv);
+      load_tile<E, D>(G, p.dy, a.b, a.h, a.t0, a.n, p.dv);
+    }
+    sync();
+    const uint32_t tb = sm.tbase, lb = tb + ((uint32_t)(32 * q) << 16);
+    if (ok && tid == 0) {
+      product<NL, NL, 128, 128>(tb, op_k<D>(G), op_k<D>(V), D / 16);
+      product<NL, NL, 128, 128>(tb + 128, op_k<D>(Q), op_k<D>(K), D / 16);
+      um::commit(&sm.bar);
+      if (tma && more) {
+        tma_prefetch<D>(&p.mdy, next.t0, next.h, next.b, p.dv);
+        tma_prefetch<D>(&p.mV, next.t0, next.h, next.b, p.dv);
+        tma_prefetch<D>(&p.mQ, next.t0, next.h, next.b, p.dk);
+        tma_prefetch<D>(&p.mK, next.t0, next.h, next.b, p.dk);
+      }
+    }
+    if (tid < D * D / 32)  // the next state's lines
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(
+          p.saved + (next.bh * (p.nchunks + 1) + next.c) * (D * D) + tid * 32));
+    if (warp == kDecayWarp && more) load_decay(next);
+    wait();
+    const float rh = dec.ch[row], rl = dec.cl[row], from_start = ex2(rh + rl);
+    float tok = 0.f;
+    Held<NL> a1;
+    // Lane: token i = row; columns: tokens j <= i. A1 = D * (dy V^T).
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int j0 = 32 * k + 16 * wg;
+      float x[16], z[16];
+      if (j0 > 32 * q + 31) {  // after every row of the warp
+#pragma unroll
+        for (int i = 0; i < 16; ++i) z[i] = 0.f;
+      } else {
+        uint32_t r1[16], r2[16];
+        um::ld16_async(lb + j0, r1);
+        um::ld16_async(lb + 128 + j0, r2);
+        um::ld_wait();
+        um::ld_bind(r1, z);
+        um::ld_bind(r2, x);
+        if (j0 < 32 * q) {  // before every row
+          const float f0 = dec.to(rh, rl, j0 + 15);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            z[i] *= f0 * dec.cf[j0 + i];
+            tok = fmaf(z[i], x[i], tok);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float f = dec.to(rh, rl, j0 + i);
+            const float zf = z[i] * f;
+            tok += j0 + i < row ? zf * x[i] : 0.f;
+            z[i] = j0 + i <= row ? zf : 0.f;
+          }
+        }
+      }
+      a1.set(k, z);
+    }
+    sync();  // both products have been read, and the table
+    a1.store(lb, wg);
+    if (warp == kDecayWarp && more) dw.table<false>(dec);
+    st_wait();
+    sync();
+    if (ok && tid == 0) {
+      product_ta<NL, NL, D>(tb + F::kDq, tb, op_mn<D>(K), false);
+      product<NL, 3, 128, D>(tb + F::kIq, op_k<D>(G), state_k<D>(X), D / 16);
+      um::commit(&sm.bar);
+    }
+    wait();
+    float aq = 0.f;
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) {
+      const int j0 = wg * (D / 2) + 16 * k;
+      uint32_t r1[16], r2[16];
+      float x[16], z[16], qr[16];
+      um::ld16_async(lb + F::kDq + j0, r1);
+      um::ld16_async(lb + F::kIq + j0, r2);
+      load_levels8<NL>(Q, kTileE, sw<kC>(row, j0), qr);
+      load_levels8<NL>(Q, kTileE, sw<kC>(row, j0 + 8), qr + 8);
+      um::ld_wait();
+      um::ld_bind(r1, x);
+      um::ld_bind(r2, z);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        aq = fmaf(qr[i], z[i], aq);
+        x[i] = fmaf(from_start, z[i], x[i]);
+      }
+      if (tma)
+        row16_to_tile(V, row, j0, x);  // V has been used
+      else if (ok && row < a.n)
+        store_row16<E>(p.dQ, a.b, a.h, p.H, a.t0 + row, p.T, j0, p.dk, x);
+    }
+    aq *= from_start;
+    sm.a[wg][row] = aq + tok;
+    const float ws = warp_sum(aq);
+    if (lane == 0) sm.red[warp] = ws;
+    sync();
+    if (ok && tid < a.n) p.tq[a.bh * p.T + a.t0 + tid] = sm.a[0][tid] + sm.a[1][tid];
+    if (ok && tid == kC) {
+      float s = 0.f;
+      for (int i = 0; i < 8; ++i) s += sm.red[i];
+      p.aq[a.bh * p.nchunks + a.c] = s;
+    }
+    if (tma && ok && tid == 0) {
+      tma_store<D>(&p.mdQ, a.t0, a.h, a.b, p.dk, V);
+      if (more) {
+        mbar_arrive_expect_tx(&sm.full, 4 * tile_bytes(D));
+        tma_load<D>(G, &p.mdy, next.t0, next.h, next.b, &sm.full);
+        tma_load<D>(Q, &p.mQ, next.t0, next.h, next.b, &sm.full);
+        tma_load<D>(K, &p.mK, next.t0, next.h, next.b, &sm.full);
+        bulk_wait_read();
+        tma_load<D>(V, &p.mV, next.t0, next.h, next.b, &sm.full);
+      }
+    }
+    a = next;
+  }
+  if (tma && tid == 0) bulk_wait_read();
+  um::fence_before();
+  __syncthreads();
+  if (warp == 0) um::dealloc(sm.tbase, F::kCols);
+}
+
+// TMEM columns: (K Q^T) 0..127 and (V dy^T) 128..255; once read, their masked
+// forms A2 at 0 and A1 at 64 NL (NL levels of 64), dV at 128 NL, dK after it; once
+// these are done, the state parts of dV at 0 and of dK at kIk, and the states'
+// sum at kU.
+template <typename E, int D>
+struct Dkv {
+  static constexpr int NL = kLevels<E>, kTileE = kC * D;
+  // Two CTAs to an SM: dS is spread over all threads, and one tile more holds the
+  // decayed K rows, so that dV's state part adds up in dV's own accumulator.
+  static constexpr bool kE = NL == 1 && D == 64;
+  static constexpr int kDv = 128 * NL, kDk = kDv + D;
+  static constexpr int kIk = kE ? 0 : 2 * D <= kDv ? D : kDk + D, kU = kE ? D : 0;
+  static constexpr int kCols = kDk + D <= 256 ? 256 : 512;
+  static_assert(kDk + D <= 512 && kIk + D <= 512, "");
+  static constexpr size_t kSmem =
+      kSmallB + 2 * ((4 * NL + (kE ? 1 : 0)) * (size_t)kTileE + 3 * (size_t)D * D);
+  static constexpr int kPerSm = 2 * (kSmem + 1024) <= 228 * 1024 && kCols <= 256 ? 2 : 1;
+  static_assert(kSmem <= 227 * 1024, "");
+};
+
+template <typename E, int D>
+__global__ void __launch_bounds__(kThreads, Dkv<E, D>::kPerSm) dkv_kernel(const __grid_constant__ Args<E> p) {
+  using F = Dkv<E, D>;
+  constexpr int NL = F::NL, kTileE = F::kTileE;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  SmallB& sm = *reinterpret_cast<SmallB*>(smem);
+  bf16* Q = reinterpret_cast<bf16*>(smem + kSmallB);
+  bf16 *K = Q + NL * kTileE, *V = K + NL * kTileE, *G = V + NL * kTileE, *X = G + NL * kTileE;
+  bf16* Ex = X + 3 * D * D;
+  // the scaled Q rows go over Q and, below three levels, over what has been read by then
+  bf16* const lv[3] = {Q, F::kE ? V : NL == 1 ? K : Q + kTileE,
+                       F::kE ? Ex : NL == 1 ? V : NL == 2 ? K : Q + 2 * kTileE};
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q = warp & 3, wg = warp >> 2;
+  const long long bh = blockIdx.x % p.BH;
+  const int s = p.nseg - 1 - (int)(blockIdx.x / p.BH);
+  const int b = (int)(bh / p.H), h = (int)(bh % p.H);
+  const float* lg = p.lg + b * p.lsb + h * p.lsh;
+  const int c0 = s * p.m, c1 = min(c0 + p.m, p.nchunks);
+  auto rows = [&](int c) { return (int)min((long long)kC, p.T - (long long)c * kC); };
+  const bool tma = NL == 1 && p.tma;
+  Decays& dec = sm.dec;
+
+  if (warp == 0) um::alloc(&sm.tbase, F::kCols);
+  if (tid == 0) {
+    mbar_init(&sm.bar, 1);
+    mbar_init(&sm.bar2, 1);
+    mbar_init(&sm.full, 1);
+    mbar_fence_init();
+    if (tma) {
+      const long long t0 = (long long)(c1 - 1) * kC;
+      mbar_arrive_expect_tx(&sm.full, 4 * tile_bytes(D));
+      tma_load<D>(K, &p.mK, t0, h, b, &sm.full);
+      tma_load<D>(Q, &p.mQ, t0, h, b, &sm.full);
+      tma_load<D>(V, &p.mV, t0, h, b, &sm.full);
+      tma_load<D>(G, &p.mdy, t0, h, b, &sm.full);
+    }
+  }
+  DecayWarp dw;
+  if (warp == kDecayWarp) {
+    dw.load(lg + (long long)(c1 - 1) * kC * p.lst, p.lst, rows(c1 - 1));
+    dw.table<true>(dec);
+  }
+  float dSe[16];  // kE
+  State<D> dS;    // otherwise
+  {
+    const float* end = s + 1 < p.nseg ? p.seg + (bh * p.nsub + (s + 1) * p.r - 1) * (D * D) : nullptr;
+    const float* S_end = p.saved + (bh * (p.nchunks + 1) + c1) * (D * D);
+    float d = 0.f;  // <S, dS> at the segment's end
+    if constexpr (F::kE) {
+      const int er = Even::row(), ec = Even::col();
+      if (end) {
+        Even::load_own(end, dSe);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          dSe[i] = p.dHT && er < p.dk && ec + i < p.dv ? p.dHT[bh * p.sbh + er * p.sld + ec + i] : 0.f;
+      }
+      float v[16];
+      Even::load_own(S_end, v);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) d = fmaf(v[i], dSe[i], d);
+      Even::to_smem(X, dSe);
+    } else {
+      if (end)
+        dS.load_own(end);
+      else if (p.dHT)
+        dS.load(p.dHT + bh * p.sbh, p.dk, p.dv, p.sld);
+      else
+        dS.zero();
+      State<D> S;
+      S.load_own(S_end);
+#pragma unroll
+      for (int i = 0; i < State<D>::kCols; ++i) d = fmaf(S.v[i], dS.v[i], d);
+      dS.template to_smem<3>(X);
+    }
+    d = warp_sum(d);
+    if (lane == 0) sm.red[warp] = d;
+  }
+  bool ok = true;
+  auto sync = [&]() {
+    fence_proxy_async_smem();
+    um::fence_before();
+    ok = !__syncthreads_or(!ok);
+    um::fence_after();
+  };
+  unsigned phase = 0;
+  auto wait = [&]() {
+    if (ok) ok = mbar_wait(&sm.bar, phase & 1, &g_sticky_err, kPolls);
+    ++phase;
+    um::fence_after();
+  };
+  sync();
+  double Fend = 0.0;  // kSumWarp: <S, dS> at the end of the chunk being summed
+  float tq[4], lgs[4], aqs = 0.f;
+  if (warp == kSumWarp)
+    for (int i = 0; i < 8; ++i) Fend += (double)sm.red[i];
+  // What chunk c's dlog_gamma needs from memory, and its sums once sm.a is complete:
+  // four tokens to a lane, from the end, in fp64.
+  auto sums_load = [&](int c) {
+    const long long t0 = (long long)c * kC;
+    const int n = rows(c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = 4 * lane + i;
+      tq[i] = t < n ? p.tq[bh * p.T + t0 + t] : 0.f;
+      lgs[i] = t < n ? lg[(t0 + t) * p.lst] : 0.f;
+    }
+    aqs = p.aq[bh * p.nchunks + c];
+  };
+  auto sums = [&](int c) {
+    const long long t0 = (long long)c * kC;
+    const int n = rows(c);
+    double v[4], run = 0.0;
+#pragma unroll
+    for (int i = 3; i >= 0; --i) {
+      const int t = 4 * lane + i;
+      run += (double)tq[i] + (double)sm.a[0][t] + (double)sm.a[1][t];
+      v[i] = run;
+    }
+    double inc = run;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double x = __shfl_down_sync(0xffffffffu, inc, o);
+      if (lane + o < 32) inc += x;
+    }
+    const double rest = inc - run + Fend;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = 4 * lane + i;
+      if (t < n && ok) {
+        float* o = p.dlg + bh * p.T + t0 + t;
+        const double all = v[i] + rest + (p.dlg_add ? (double)*o : 0.0);
+        *o = lgs[i] * 1.4426950408889634f <= kMinLog2 ? 0.f : (float)all;
+      }
+    }
+    double bk = 0.0;
+    for (int i = 0; i < 8; ++i) bk += (double)sm.red2[i];
+    Fend += (double)aqs - bk;
+  };
   const int row = 32 * q + lane;
   for (int c = c1 - 1; c >= c0; --c) {
     const long long t0 = (long long)c * kC;
     const int n = rows(c), turn = (c1 - 1 - c) & 1;
     const bool more = c > c0;
-    Decays& dec = sm.dec[F::kTabs == 2 ? c & 1 : 0];
-    if (F::kTabs == 1 && warp == 0) {
-      dw.load(lg + t0 * p.lst, p.lst, n);
-      dw.table<true>(dec);
-    }
     if (tma) {
       if (ok) ok = mbar_wait(&sm.full, turn, &g_sticky_err, kPolls);
     } else {
@@ -1112,7 +1426,7 @@ __global__ void __launch_bounds__(kThreads, Bwd<E, D>::kPerSm) bwd_kernel(const 
       product<NL, NL, 128, 128>(tb, op_k<D>(K), op_k<D>(Q), D / 16);
       product<NL, NL, 128, 128>(tb + 128, op_k<D>(V), op_k<D>(G), D / 16);
       um::commit(&sm.bar);
-      if (tma && more) {  // the next chunk's rows and state on their way into L2
+      if (tma && more) {  // the next chunk's rows on their way into L2
         tma_prefetch<D>(&p.mK, t0 - kC, h, b, p.dk);
         tma_prefetch<D>(&p.mQ, t0 - kC, h, b, p.dk);
         tma_prefetch<D>(&p.mV, t0 - kC, h, b, p.dv);
@@ -1125,17 +1439,15 @@ __global__ void __launch_bounds__(kThreads, Bwd<E, D>::kPerSm) bwd_kernel(const 
       prefetch_rows(p.V, b, h, t0 - kC, kC, p.dv);
       prefetch_rows(p.dy, b, h, t0 - kC, kC, p.dv);
     }
-    if (tid < D * D / 32)  // the state that entered this chunk: 128 bytes to a thread
-      asm volatile("prefetch.global.L2 [%0];" ::"l"(p.saved + (bh * p.nchunks + c) * (D * D) + tid * 32));
-    if (F::kTabs == 2 && warp == kDecayWarp && more) {
-      dw.load(lg + (t0 - kC) * p.lst, p.lst, kC);
-      dw.table<true>(sm.dec[(c - 1) & 1]);
+    if (warp == kDecayWarp && more) dw.load(lg + (t0 - kC) * p.lst, p.lst, kC);
+    if (warp == kSumWarp) {
+      if (c + 1 < c1) sums(c + 1);
+      sums_load(c);
     }
     wait();
     const float rh = dec.ch[row], rl = dec.cl[row], th = dec.ch[kC - 1], tl = dec.cl[kC - 1];
-    const float to_end = dec.to(th, tl, row), from_start = ex2(rh + rl);
-    float tok = 0.f;  // this half's part of what token `row` adds for t <= row
-    float bk = 0.f;   // what it adds for t > row
+    const float to_end = dec.to(th, tl, row);
+    float tok = 0.f;  // this half's part of what token `row` takes from t <= row
     {
       // Lane: token j = row; columns: tokens i >= j. A2 = D * (K Q^T), A1 = D * (V dy^T).
       Held<NL> a1, a2;
@@ -1176,6 +1488,18 @@ __global__ void __launch_bounds__(kThreads, Bwd<E, D>::kPerSm) bwd_kernel(const 
         a2.set(k, x);
         a1.set(k, z);
       }
+      if constexpr (F::kE) {  // decayed K rows, one level: they end in dV alone
+        using I = Items<D>;
+#pragma unroll
+        for (int i = 0; i < I::kN; ++i) {
+          float x[8];
+          const float f = dec.to(th, tl, I::row(i));
+          load_levels8<1>(K, 0, I::offset(i), x);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] *= f;
+          store_levels8<1>(Ex, 0, I::offset(i), x);
+        }
+      }
       sync();  // both products have been read
       a2.store(lb, wg);
       a1.store(lb + 64 * NL, wg);
@@ -1184,264 +1508,131 @@ __global__ void __launch_bounds__(kThreads, Bwd<E, D>::kPerSm) bwd_kernel(const 
     sync();
     if (ok && tid == 0) {
       product_ta<NL, NL, D>(tb + F::kDv, tb, op_mn<D>(G), false);
+      if (F::kE) product<1, 2, 128, D>(tb + F::kDv, op_k<D>(Ex), state_mn<D>(X), D / 16, true);
       product_ta<NL, NL, D>(tb + F::kDk, tb + 64 * NL, op_mn<D>(Q), false);
       um::commit(&sm.bar);
     }
     wait();
     if (ok && tid == 0) {
-      product<NL, 3, 128, D>(tb + F::kIv, op_k<D>(K), state_mn<D>(X), D / 16);
+      if (!F::kE) product<NL, 3, 128, D>(tb, op_k<D>(K), state_mn<D>(X), D / 16);
       product<NL, 3, 128, D>(tb + F::kIk, op_k<D>(V), state_k<D>(X), D / 16);
       um::commit(&sm.bar2);
     }
+    auto scale = [&]() { scale_rows<NL, D>(Q, lv, [&](int r) { return ex2(dec.ch[r] + dec.cl[r]); }); };
+    auto sum_states = [&]() {
+      if (ok && tid == 0) {
+        product_rows<NL, D>(tb + F::kU, lv, G, false);
+        um::commit(&sm.bar);
+      }
+      if (warp == kDecayWarp && more) dw.table<true>(dec);  // the table has been used
+    };
     if (ok) ok = mbar_wait(&sm.bar2, turn, &g_sticky_err, kPolls);
     um::fence_after();
-    uint32_t dkp[F::kEven ? 16 : 1];  // dK, packed, until the stage is free
+    if (F::kE) {  // over Q, V and the extra tile; the gradients are read meanwhile
+      scale();
+      sync();
+      sum_states();
+    }
+    float bk = 0.f;  // k . its gradient's state part
+    uint32_t dvp[F::kE ? 16 : 1];
 #pragma unroll
     for (int k = 0; k < D / 32; ++k) {
       const int j0 = wg * (D / 2) + 16 * k;
       uint32_t r1[16], r2[16];
       float x[16], z[16];
       um::ld16_async(lb + F::kDv + j0, r1);
-      um::ld16_async(lb + F::kIv + j0, r2);
+      if (!F::kE) um::ld16_async(lb + j0, r2);
       um::ld_wait();
       um::ld_bind(r1, x);
-      um::ld_bind(r2, z);
+      if (!F::kE) {
+        um::ld_bind(r2, z);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = fmaf(to_end, z[i], x[i]);
-      if (staged)
-        row16_to_tile(stage, row, j0, x);
+        for (int i = 0; i < 16; ++i) x[i] = fmaf(to_end, z[i], x[i]);
+      }
+      if (F::kE && tma)
+        pack16(x, dvp + (F::kE ? 8 * k : 0));
       else if (ok && row < n)
         store_row16<E>(p.dV, b, h, p.H, t0 + row, p.T, j0, p.dv, x);
       um::ld16_async(lb + F::kDk + j0, r1);
       um::ld16_async(lb + F::kIk + j0, r2);
-      um::ld_wait();
-      um::ld_bind(r1, x);
-      um::ld_bind(r2, z);
       float kr[16];
       load_levels8<NL>(K, kTileE, sw<kC>(row, j0), kr);
       load_levels8<NL>(K, kTileE, sw<kC>(row, j0 + 8), kr + 8);
+      um::ld_wait();
+      um::ld_bind(r1, x);
+      um::ld_bind(r2, z);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         bk = fmaf(kr[i], z[i], bk);
         x[i] = fmaf(to_end, z[i], x[i]);
       }
-      if (staged) {
-        if constexpr (F::kEven) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const __nv_bfloat162 u = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-            dkp[8 * k + i] = *reinterpret_cast<const uint32_t*>(&u);
-          }
-        }
-      } else if (ok && row < n) {
+      if (F::kE && tma)
+        row16_to_tile(K, row, j0, x);  // over the row that this thread has read
+      else if (ok && row < n)
         store_row16<E>(p.dK, b, h, p.H, t0 + row, p.T, j0, p.dk, x);
-      }
     }
     bk *= to_end;
-    {  // S, the state that entered the chunk, takes dS's place in shared memory
-      const float* src = p.saved + (bh * p.nchunks + c) * (D * D);
-      float d = 0.f;
-      if constexpr (F::kEven) {
-        float v[16];
-        even_own(src, v);
-        even_to_smem(v);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) d = fmaf(v[i], dSe[i], d);
-      } else {
-        State<D> S;
-        S.load_own(src);
-#pragma unroll
-        for (int i = 0; i < State<D>::kCols; ++i) d = fmaf(S.v[i], dS.v[i], d);
-        if (!State<D>::valid()) d = 0.f;  // lanes without a row hold what their TMEM lanes held
-        S.template to_smem<3>(X);
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-      if (lane == 0) sm.a[0][warp] = d;  // joined below, in order
-    }
-    // from here on a token's factor is to its block's end
-    if (tid < kC) dec.cf[tid] = dec.to(dec.ch[tid | 15], dec.cl[tid | 15], tid);
-    sync();
-    if (ok && tid == 0) {
-      product<NL, NL, 128, 128>(tb, op_k<D>(G), op_k<D>(V), D / 16);
-      product<NL, NL, 128, 128>(tb + 128, op_k<D>(Q), op_k<D>(K), D / 16);
-      um::commit(&sm.bar);
-      if (staged) tma_store<D>(&p.mdV, t0, h, b, p.dv, stage);
-    }
-    if (tid == 32) {
-      float d = 0.f;
-      for (int i = 0; i < 8; ++i) d += sm.a[0][i];
-      sm.dot = d;
-    }
-    wait();
-    {
-      // Lane: token i = row; columns: tokens j <= i. A1 = D * (dy V^T).
-      Held<NL> a1;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int j0 = 32 * k + 16 * wg;
-        float x[16], z[16];
-        if (j0 > 32 * q + 31) {  // after every row of the warp
-#pragma unroll
-          for (int i = 0; i < 16; ++i) z[i] = 0.f;
-        } else {
-          uint32_t r1[16], r2[16];
-          um::ld16_async(lb + j0, r1);
-          um::ld16_async(lb + 128 + j0, r2);
-          um::ld_wait();
-          um::ld_bind(r1, z);
-          um::ld_bind(r2, x);
-          if (j0 < 32 * q) {  // before every row
-            const float f0 = dec.to(rh, rl, j0 + 15);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              z[i] *= f0 * dec.cf[j0 + i];
-              tok = fmaf(z[i], x[i], tok);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float f = dec.to(rh, rl, j0 + i);
-              const float zf = z[i] * f;
-              tok += j0 + i < row ? zf * x[i] : 0.f;
-              z[i] = j0 + i <= row ? zf : 0.f;
-            }
-          }
-        }
-        a1.set(k, z);
-      }
-      if (staged && tid == 0) bulk_wait_read();  // dV has left the stage
+    sm.a[wg][row] = tok - bk;
+    bk = warp_sum(bk);
+    if (lane == 0) sm.red2[warp] = bk;
+    if (!F::kE) {  // over Q and what else has been read
       sync();
-      a1.store(lb, wg);
-      if constexpr (F::kEven) {
-        if (staged) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<uint4*>(stage + sw<kC>(row, wg * (D / 2) + 8 * i)) =
-                make_uint4(dkp[4 * i], dkp[4 * i + 1], dkp[4 * i + 2], dkp[4 * i + 3]);
-        }
-      }
-      st_wait();
-    }
-    sync();
-    if (ok && tid == 0) {
-      product_ta<NL, NL, D>(tb + F::kDq, tb, op_mn<D>(K), false);
-      product<NL, 3, 128, D>(tb + F::kIq, op_k<D>(G), state_k<D>(X), D / 16);
-      um::commit(&sm.bar);
-      if (staged) tma_store<D>(&p.mdK, t0, h, b, p.dk, stage);
+      scale();
+      sync();
+      sum_states();
     }
     wait();
-    float aq = 0.f;
-    uint32_t dqp[F::kEven ? 16 : 1];
-#pragma unroll
-    for (int k = 0; k < D / 32; ++k) {
-      const int j0 = wg * (D / 2) + 16 * k;
-      uint32_t r1[16], r2[16];
-      float x[16], z[16], qr[16];
-      um::ld16_async(lb + F::kDq + j0, r1);
-      um::ld16_async(lb + F::kIq + j0, r2);
-      um::ld_wait();
-      um::ld_bind(r1, x);
-      um::ld_bind(r2, z);
-      load_levels8<NL>(Q, kTileE, sw<kC>(row, j0), qr);
-      load_levels8<NL>(Q, kTileE, sw<kC>(row, j0 + 8), qr + 8);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        aq = fmaf(qr[i], z[i], aq);
-        x[i] = fmaf(from_start, z[i], x[i]);
-      }
-      if (staged) {
-        if constexpr (F::kEven) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const __nv_bfloat162 u = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-            dqp[8 * k + i] = *reinterpret_cast<const uint32_t*>(&u);
-          }
-        }
-      } else if (ok && row < n) {
-        store_row16<E>(p.dQ, b, h, p.H, t0 + row, p.T, j0, p.dk, x);
-      }
-    }
-    sm.a[wg][row] = fmaf(from_start, aq, tok);
-    if (staged && tid == 0) bulk_wait_read();  // dK has left the stage
-    sync();
-    if constexpr (F::kEven) {
-      if (staged) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<uint4*>(stage + sw<kC>(row, wg * (D / 2) + 8 * i)) =
-              make_uint4(dqp[4 * i], dqp[4 * i + 1], dqp[4 * i + 2], dqp[4 * i + 3]);
-      }
-    }
-    scale_rows<NL, D>(Q, lv, [&](int r) { return ex2(dec.ch[r] + dec.cl[r]); });
-    sync();
-    if (ok && tid == 0) {
-      product_rows<NL, D>(tb, lv, G, false);
-      um::commit(&sm.bar);
-      if (staged) tma_store<D>(&p.mdQ, t0, h, b, p.dk, stage);
-    }
-    (wg == 0 ? dec.ch : dec.cl)[row] = bk;  // the decay table has been used
-    wait();
-    if (tma && ok && tid == 0) {
-      if (staged) bulk_wait_read();  // dQ has left the stage
-      if (more) load(c - 1);
-    }
     const float g = ex2(th + tl);
-    if constexpr (F::kEven) {  // the sum goes over X in its own order, then to all threads
+    if constexpr (F::kE) {
+      // the sum goes over the extra tile in its own order, then to all threads
+      if (tma) {
+        packed16_to_tile(V, row, wg * 32, dvp);
+        packed16_to_tile(V, row, wg * 32 + 16, dvp + 8);
+      }
       State<D> u;
       u.zero();
-      u.update(0.f, tb, 0);
-      u.store_own(reinterpret_cast<float*>(X));
+      u.update(0.f, tb, F::kU);
+      u.store_own(reinterpret_cast<float*>(Ex));
       sync();
+      if (tma && ok && tid == 0) {
+        tma_store<D>(&p.mdV, t0, h, b, p.dv, V);
+        tma_store<D>(&p.mdK, t0, h, b, p.dk, K);
+        if (more) {
+          mbar_arrive_expect_tx(&sm.full, 4 * tile_bytes(D));
+          tma_load<D>(Q, &p.mQ, t0 - kC, h, b, &sm.full);
+          tma_load<D>(G, &p.mdy, t0 - kC, h, b, &sm.full);
+          bulk_wait_read();
+          tma_load<D>(K, &p.mK, t0 - kC, h, b, &sm.full);
+          tma_load<D>(V, &p.mV, t0 - kC, h, b, &sm.full);
+        }
+      }
       float v[16];
-      even_own(reinterpret_cast<const float*>(X), v);
+      Even::load_own(reinterpret_cast<const float*>(Ex), v);
 #pragma unroll
       for (int i = 0; i < 16; ++i) dSe[i] = fmaf(g, dSe[i], v[i]);
-      sync();
-      even_to_smem(dSe);
+      Even::to_smem(X, dSe);
     } else {
-      dS.update(g, tb, 0);
+      if (tma && ok && tid == 0 && more) {
+        mbar_arrive_expect_tx(&sm.full, 4 * tile_bytes(D));
+        tma_load<D>(K, &p.mK, t0 - kC, h, b, &sm.full);
+        tma_load<D>(Q, &p.mQ, t0 - kC, h, b, &sm.full);
+        tma_load<D>(V, &p.mV, t0 - kC, h, b, &sm.full);
+        tma_load<D>(G, &p.mdy, t0 - kC, h, b, &sm.full);
+      }
+      dS.update(g, tb, F::kU);
       dS.template to_smem<3>(X);
       sync();
     }
-    if (warp == 0 && ok) {
-      // Token i adds a to dlog_gamma_t for t <= i and bk for t > i: four tokens to a lane,
-      // a summed from the end and bk from the start.
-      double va[4], vb[4], ra = 0.0, rb = 0.0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int e = 4 * lane + 3 - i, f = 4 * lane + i;
-        ra += (double)sm.a[0][e] + (double)sm.a[1][e];
-        va[3 - i] = ra;
-        vb[i] = rb;
-        rb += (double)dec.ch[f] + (double)dec.cl[f];
-      }
-      double ia = ra, ib = rb;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double x = __shfl_down_sync(0xffffffffu, ia, o), y = __shfl_up_sync(0xffffffffu, ib, o);
-        if (lane + o < 32) ia += x;
-        if (lane >= o) ib += y;
-      }
-      const double rest = (ia - ra) + (ib - rb) + (double)(sm.dot * g);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = 4 * lane + i;
-        if (t < n) {
-          const float l = lg[(t0 + t) * p.lst] * 1.4426950408889634f;
-          float* o = p.dlg + bh * p.T + t0 + t;
-          const double all = va[i] + vb[i] + rest + (p.dlg_add ? (double)*o : 0.0);
-          *o = l <= kMinLog2 ? 0.f : (float)all;
-        }
-      }
-    }
-    __syncwarp();
   }
+  sync();
+  if (warp == kSumWarp) sums(c0);
+  if (tma && tid == 0) bulk_wait_read();
   if (ok && s == 0 && p.dH0) {
-    if constexpr (F::kEven) {
+    if constexpr (F::kE) {
+      const int er = Even::row(), ec = Even::col();
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        if (erow < p.dk && ecol + i < p.dv) p.dH0[bh * p.sbh + erow * p.sld + ecol + i] = dSe[i];
+        if (er < p.dk && ec + i < p.dv) p.dH0[bh * p.sbh + er * p.sld + ec + i] = dSe[i];
     } else {
       dS.store(p.dH0 + bh * p.sbh, p.dk, p.dv, p.sld);
     }
@@ -1513,7 +1704,7 @@ size_t seg_bytes(const Plan& pl, long long BH) {
 
 template <typename E, int D>
 Plan plan_of(bool fwd, long long BH, long long T) {
-  return plan_for(BH, T, D, fwd ? Fwd<E, D>::kPerSm : Bwd<E, D>::kPerSm, Sums<E, D>::kPerSm);
+  return plan_for(BH, T, D, fwd ? Fwd<E, D>::kPerSm : Dkv<E, D>::kPerSm, Sums<E, D>::kPerSm);
 }
 
 bool shape_ok(int64_t B, int H, int64_t T, int dk, int dv) {
@@ -1583,8 +1774,15 @@ int run_segments(const Args<E>& a, cudaStream_t st) {
 template <typename E, int D>
 int run_main(bool fwd, const Args<E>& a, cudaStream_t st) {
   if (int r = fwd ? run_segments<E, D, false>(a, st) : run_segments<E, D, true>(a, st)) return r;
-  auto k = fwd ? fwd_kernel<E, D> : bwd_kernel<E, D>;
-  const size_t smem = fwd ? Fwd<E, D>::kSmem : Bwd<E, D>::kSmem;
+  if (!fwd) {  // any order of chunks: a CTA takes every so many
+    using F = Dq<E, D>;
+    if (int r = set_smem(dq_kernel<E, D>, F::kSmem)) return r;
+    const long long n = a.BH * a.nchunks, places = (long long)sm_count() * F::kPerSm;
+    dq_kernel<E, D><<<(unsigned)(n < places ? n : places), kThreads, F::kSmem, st>>>(a);
+    if (int r = launched()) return r;
+  }
+  auto k = fwd ? fwd_kernel<E, D> : dkv_kernel<E, D>;
+  const size_t smem = fwd ? Fwd<E, D>::kSmem : Dkv<E, D>::kSmem;
   if (int r = set_smem(k, smem)) return r;
   k<<<(unsigned)(a.BH * a.nseg), kThreads, smem, st>>>(a);
   return launched();
@@ -1600,10 +1798,14 @@ size_t part_floats(const Blocks& n, bool fwd) {
   return fwd ? (n.nk > 1 ? 1 : 0) : (n.nk > 1 ? 1 : 0) + (n.nv > 1 ? 2 * (size_t)n.nk : 0);
 }
 
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+size_t sums_floats(const Plan& pl, long long BH, long long T) { return (size_t)BH * (T + pl.nchunks); }
+
 template <typename E, int D>
 size_t workspace_bytes_of(bool fwd, int64_t B, int H, int64_t T, int dk, int dv) {
   const long long BH = B * (long long)H;
-  return (seg_bytes(plan_of<E, D>(fwd, BH, T), BH) + 255) / 256 * 256 +
+  const Plan pl = plan_of<E, D>(fwd, BH, T);
+  return up256(seg_bytes(pl, BH)) + (fwd ? 0 : up256(sums_floats(pl, BH, T) * sizeof(float))) +
          part_floats(Blocks(dk, dv, D), fwd) * (size_t)BH * T * 64 * sizeof(float);
 }
 
@@ -1624,7 +1826,12 @@ int run_blocks(Args<E>& a, bool fwd, const float* lg, const int64_t* s, int64_t 
   a.sbh = (long long)dk * dv, a.sld = dv;
   const Blocks n(dk, dv, D);
   const size_t rows = (size_t)BH * T * 64;
-  float* part = reinterpret_cast<float*>(static_cast<char*>(ws) + (seg_bytes(pl, BH) + 255) / 256 * 256);
+  char* rest = static_cast<char*>(ws) + up256(seg_bytes(pl, BH));
+  if (!fwd) {
+    a.tq = reinterpret_cast<float*>(rest), a.aq = a.tq + (size_t)BH * T;
+    rest += up256(sums_floats(pl, BH, T) * sizeof(float));
+  }
+  float* part = reinterpret_cast<float*>(rest);
   float *part_v = part, *part_q = part + (n.nk > 1 ? rows : 0), *part_k = part_q + n.nk * rows;
   const Args<E> whole = a;
   auto sum = [](auto& x, float* rows_, int i, int last) {  // x: a sum over blocks 0..last
@@ -1654,7 +1861,7 @@ int run_blocks(Args<E>& a, bool fwd, const float* lg, const int64_t* s, int64_t 
         if (whole.dH0) a.dH0 = whole.dH0 + s0;
         a.dlg_add = i + j > 0;
       }
-      if (whole.saved) a.saved = whole.saved + (size_t)(j * n.nk + i) * BH * pl.nchunks * D * D;
+      if (whole.saved) a.saved = whole.saved + (size_t)(j * n.nk + i) * BH * (pl.nchunks + 1) * D * D;
       if constexpr (std::is_same_v<E, bf16>) {
         bool ok = map_of(&a.mQ, a.Q, dk, T, H, B) && map_of(&a.mK, a.K, dk, T, H, B) &&
                   map_of(&a.mV, a.V, dv, T, H, B);
@@ -1701,7 +1908,8 @@ size_t mgs_linear_attn_saved_size(int64_t B, int H, int64_t T, int dk, int dv, i
   (void)by_shape(dtype, dk, dv, [&](auto, auto d) -> int {
     constexpr int D = decltype(d)::value;
     const Blocks blocks(dk, dv, D);
-    n = (size_t)blocks.nk * blocks.nv * (size_t)(B * H) * (size_t)((T + kC - 1) / kC) * D * D * sizeof(float);
+    n = (size_t)blocks.nk * blocks.nv * (size_t)(B * H) * (size_t)((T + kC - 1) / kC + 1) * D * D *
+        sizeof(float);
     return MGS_OK;
   });
   return n;
