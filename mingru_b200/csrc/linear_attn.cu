@@ -427,7 +427,15 @@ __device__ __forceinline__ void product(uint32_t d, const Op<RA>& a, const Op<RB
       }
     }
 }
-// The same with A (128 rows, 128 deep) in TMEM: NA levels of 64 columns each.
+// A masked product in TMEM, 128 deep, as an operand. One level lies packed at the
+// two ends of the accumulator it was made from, columns 0..31 and 96..127, so that
+// each warp packs what it alone has read, with no word to the others, and the 64
+// columns between are free; more levels lie one after the other, 64 columns each.
+template <int NL>
+__device__ __forceinline__ int packed_at(int col) {  // of product column `col`, a multiple of 16
+  return col / 2 + (NL == 1 && col >= 64 ? 64 : 0);
+}
+// The same with A (128 rows, 128 deep) in TMEM, NA levels.
 template <int NA, int NB, int N>
 __device__ __forceinline__ void product_ta(uint32_t d, uint32_t a, const Op<kC>& b, bool acc) {
   const uint32_t id = um::idesc64(false, b.mn, true, N);
@@ -439,7 +447,7 @@ __device__ __forceinline__ void product_ta(uint32_t d, uint32_t a, const Op<kC>&
       if (j < 0 || j >= NB) continue;
 #pragma unroll 4
       for (int k = 0; k < kC / 16; ++k) {
-        mma_ta(d, a + k * 8 + i * 64, b.d + b.at(k) + j * b.level, id, acc);
+        mma_ta(d, a + packed_at<NA>(16 * k) + i * 64, b.d + b.at(k) + j * b.level, id, acc);
         acc = true;
       }
     }
@@ -480,6 +488,21 @@ __device__ __forceinline__ void st_levels16(uint32_t taddr, const float* x) {
       a[2 * i + 1] -= f.y;
     }
     st8(taddr + 64 * l, w);
+  }
+}
+
+// The four blocks of 16 columns of a 128-wide product that are half wg's, in an
+// order in which a block packed in place (packed_at) lands on columns that the
+// warp has read: from the outer end inwards. One level: a loop, for the sake of
+// the instruction cache, which a chunk's straight code would fill by itself.
+template <int NL, class F>
+__device__ __forceinline__ void masked_blocks(int wg, F&& f) {
+  if constexpr (NL == 1) {
+#pragma unroll 1
+    for (int k = 0; k < 4; ++k) f(wg == 0 ? 16 * k : 112 - 16 * k);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f(64 * wg + 16 * k);
   }
 }
 
@@ -597,9 +620,9 @@ __device__ __forceinline__ void product_rows(uint32_t d, bf16* const (&a)[3], co
 }
 
 struct Small {  // a CTA's barriers, TMEM address and decays
-  uint64_t bar, full[3];
+  uint64_t bar, bar2, full[3];
   uint32_t tbase;
-  uint32_t pad[3];
+  uint32_t pad;
   Decays dec;
 };
 constexpr int kSmallBytes = 2048;
@@ -736,12 +759,13 @@ __global__ void __launch_bounds__(256) scan_kernel(float* seg, const float* segl
 
 // ---------------------------------------------------------------- forward --
 
-// TMEM columns: masked product 0..127, y 128.., P (NL levels of 64) after it;
-// the state's sum takes 0.. once the product has been read.
+// TMEM columns: Q K^T 0..127 (one level: P packed in its place), y 128.., the
+// states' sum after it, P's levels after that.
 template <typename E, int D>
 struct Fwd {
   static constexpr int NL = kLevels<E>, kTileE = kC * D;
-  static constexpr int kY = 128, kP = 128 + D, kCols = kP + 64 * NL <= 256 ? 256 : 512;
+  static constexpr int kY = 128, kU = 128 + D, kP = NL == 1 ? 0 : kU + D;
+  static constexpr int kCols = (NL == 1 ? kU + D : kP + 64 * NL) <= 256 ? 256 : 512;
   // bf16: two buffers for Q and K, the next chunk's on their way during this one
   static constexpr int kBufs = NL == 1 ? 2 : 1;
   static constexpr int kExtra = NL == 1 ? 1 : 0;  // third level of the scaled K rows
@@ -776,6 +800,7 @@ __global__ void __launch_bounds__(kThreads, Fwd<E, D>::kPerSm) fwd_kernel(const 
   if (warp == 0) um::alloc(&sm.tbase, F::kCols);
   if (tid == 0) {
     mbar_init(&sm.bar, 1);
+    mbar_init(&sm.bar2, 1);
     for (int i = 0; i < 3; ++i) mbar_init(&sm.full[i], 1);
     mbar_fence_init();
     if (tma) {
@@ -849,31 +874,20 @@ __global__ void __launch_bounds__(kThreads, Fwd<E, D>::kPerSm) fwd_kernel(const 
     if (p.saved) S.store_own(p.saved + (bh * (p.nchunks + 1) + c) * (D * D));
     wait();
     const uint32_t lb = tb + ((uint32_t)(32 * q) << 16);
-    const float rh = dec.ch[row], rl = dec.cl[row];
-    // P = D * Q K^T, every other block of 16 columns to a warp
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int j0 = 32 * k + 16 * wg;
-      float v[16];
-      if (j0 > 32 * q + 31) {  // after every row of the warp
-        if (c > c0) continue;  // zeros from the first chunk on
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = 0.f;
-      } else {
-        um::ld16(lb + j0, v);
-        if (j0 < 32 * q) {  // before every row
-          const float f = dec.to(rh, rl, j0 + 15);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] *= f * dec.cf[j0 + i];
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float f = dec.to(rh, rl, j0 + i);
-            v[i] = j0 + i <= row ? v[i] * f : 0.f;
-          }
+    const float rh = dec.ch[row], rl = dec.cl[row], th = dec.ch[kC - 1], tl = dec.cl[kC - 1];
+    const bool add = more || s + 1 == p.nseg;  // a later chunk of this CTA, or H_T, needs S'
+    if (add) {  // its products run while the masked product is read
+      scale_rows<NL, D>(K, lv, [&](int r) { return dec.to(th, tl, r); });
+      sync();
+      if (ok && tid == 0) {
+        if (tma) ok = mbar_wait(&sm.full[2], i_ & 1, &g_sticky_err, kPolls);
+        if (ok) {
+          product_rows<NL, D>(tb + F::kU, lv, V, false);
+          um::commit(&sm.bar2);
         }
       }
-      st_levels16<NL>(lb + F::kP + j0 / 2, v);
+    } else if (tma && ok && tid == 0) {
+      ok = mbar_wait(&sm.full[2], i_ & 1, &g_sticky_err, kPolls);
     }
     {  // the state's part of y: diag(e^c) Q S
       const float f = ex2(rh + rl);
@@ -888,24 +902,45 @@ __global__ void __launch_bounds__(kThreads, Fwd<E, D>::kPerSm) fwd_kernel(const 
         st16(a, w);
       }
     }
+    // P = D * Q K^T, a half of the columns to a warp
+    masked_blocks<NL>(wg, [&](int j0) {
+      float v[16];
+      if (j0 > 32 * q + 31) {  // after every row of the warp
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = 0.f;
+      } else {
+        um::ld16(lb + j0, v);
+        if (j0 + 15 < 32 * q) {  // before every row
+          const float f = dec.to(rh, rl, j0 + 15);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] *= f * dec.cf[j0 + i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float f = dec.to(rh, rl, j0 + i);
+            v[i] = j0 + i <= row ? v[i] * f : 0.f;
+          }
+        }
+      }
+      st_levels16<NL>(lb + F::kP + packed_at<NL>(j0), v);
+    });
     if (tma && ok && tid == 0 && more) {
       bulk_wait_read();  // y has left
       tma_load<D>(Qn, &p.mQ, t0 + kC, h, b, &sm.full[buf ^ 1]);
     }
-    const float th = dec.ch[kC - 1], tl = dec.cl[kC - 1];
-    const bool add = more || s + 1 == p.nseg;  // a later chunk of this CTA, or H_T, needs S'
-    if (add) scale_rows<NL, D>(K, lv, [&](int r) { return dec.to(th, tl, r); });
     st_wait();
     sync();
     if (ok && tid == 0) {
-      if (tma) ok = mbar_wait(&sm.full[2], i_ & 1, &g_sticky_err, kPolls);
-      if (ok) {
-        product_ta<NL, NL, D>(tb + F::kY, tb + F::kP, op_mn<D>(V), true);
-        if (add) product_rows<NL, D>(tb, lv, V, false);
-        um::commit(&sm.bar);
-      }
+      product_ta<NL, NL, D>(tb + F::kY, tb + F::kP, op_mn<D>(V), true);
+      um::commit(&sm.bar);
     }
     if (warp == kDecayWarp && more) dw.table<false>(dec);
+    if (add) {
+      if (ok) ok = mbar_wait(&sm.bar2, i_ & 1, &g_sticky_err, kPolls);
+      um::fence_after();
+      S.update(ex2(th + tl), tb, F::kU);
+      S.template to_smem<NL>(X);
+    }
     wait();
     if (tma && ok && tid == 0 && more) load_v(c + 1);
 #pragma unroll
@@ -917,10 +952,6 @@ __global__ void __launch_bounds__(kThreads, Fwd<E, D>::kPerSm) fwd_kernel(const 
         row16_to_tile(Q, row, j0, v);
       else if (ok && row < n)
         store_row16<E>(p.y, b, h, p.H, t0 + row, p.T, j0, p.dv, v);
-    }
-    if (add) {
-      S.update(ex2(th + tl), tb, 0);
-      S.template to_smem<NL>(X);
     }
     if (!tma) sync();  // the tiles are loaded over at once
   }
@@ -966,32 +997,24 @@ constexpr int kSmallB = 3072;
 static_assert(sizeof(SmallB) <= kSmallB, "");
 constexpr int kSumWarp = 5;  // puts dlog_gamma together, during the next chunk's first products
 
-// NL = 1: 64 masked products of a lane's row, rounded and packed while both
-// accumulators are still being read; NL > 1: as they are.
+// The masked blocks of a lane's row. One level goes straight to its place; more
+// levels are held until both accumulators have been read.
 template <int NL>
 struct Held {
-  std::conditional_t<NL == 1, uint32_t, float> v[NL == 1 ? 32 : 64];
-  __device__ __forceinline__ void set(int k, const float (&x)[16]) {
+  float v[64];
+  __device__ __forceinline__ void put(int c0, uint32_t, const float (&x)[16]) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      if constexpr (NL == 1) {
-        if (i % 2 == 0) {
-          const __nv_bfloat162 h = __floats2bfloat162_rn(x[i], x[i + 1]);
-          v[8 * k + i / 2] = *reinterpret_cast<const uint32_t*>(&h);
-        }
-      } else {
-        v[16 * k + i] = x[i];
-      }
-    }
+    for (int i = 0; i < 16; ++i) v[(c0 & 63) + i] = x[i];
   }
   __device__ __forceinline__ void store(uint32_t taddr, int wg) const {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {  // block 2 k + wg: eight packed columns each
-      if constexpr (NL == 1)
-        st8(taddr + 16 * k + 8 * wg, v + 8 * k);
-      else
-        st_levels16<NL>(taddr + 16 * k + 8 * wg, v + 16 * k);
-    }
+    for (int k = 0; k < 4; ++k) st_levels16<NL>(taddr + 32 * wg + 8 * k, v + 16 * k);
+  }
+};
+template <>
+struct Held<1> {
+  __device__ __forceinline__ void put(int c0, uint32_t taddr, const float (&x)[16]) const {
+    st_levels16<1>(taddr + packed_at<1>(c0), x);
   }
 };
 
@@ -1032,12 +1055,13 @@ __device__ __forceinline__ void packed16_to_tile(bf16* tile, int r, int c0, cons
   *reinterpret_cast<uint4*>(tile + sw<kC>(r, c0 + 8)) = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
-// TMEM columns: (dy V^T) 0..127 and (Q K^T) 128..255; once both are read, the
-// masked A1 at 0 (NL levels of 64), dQ at 64 NL and its state part after it.
+// TMEM columns: (dy V^T) 0..127 and (Q K^T) 128..255. One level: the masked A1 in
+// the former's place, and once both are read dQ and its state part in the latter's;
+// more levels: A1 at 0, the others after it.
 template <typename E, int D>
 struct Dq {
   static constexpr int NL = kLevels<E>, kTileE = kC * D;
-  static constexpr int kDq = 64 * NL, kIq = kDq + D, kCols = kIq + D <= 256 ? 256 : 512;
+  static constexpr int kDq = NL == 1 ? 128 : 64 * NL, kIq = kDq + D, kCols = kIq + D <= 256 ? 256 : 512;
   static constexpr size_t kSmem = kSmallB + 2 * (4 * NL * (size_t)kTileE + 3 * (size_t)D * D);
   static constexpr int kPerSm = 2 * (kSmem + 1024) <= 228 * 1024 && kCols <= 256 ? 2 : 1;
   static_assert(kSmem <= 227 * 1024, "");
@@ -1151,9 +1175,7 @@ __global__ void __launch_bounds__(kThreads, Dq<E, D>::kPerSm) dq_kernel(const __
     float tok = 0.f;
     Held<NL> a1;
     // Lane: token i = row; columns: tokens j <= i. A1 = D * (dy V^T).
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int j0 = 32 * k + 16 * wg;
+    masked_blocks<NL>(wg, [&](int j0) {
       float x[16], z[16];
       if (j0 > 32 * q + 31) {  // after every row of the warp
 #pragma unroll
@@ -1165,7 +1187,7 @@ __global__ void __launch_bounds__(kThreads, Dq<E, D>::kPerSm) dq_kernel(const __
         um::ld_wait();
         um::ld_bind(r1, z);
         um::ld_bind(r2, x);
-        if (j0 < 32 * q) {  // before every row
+        if (j0 + 15 < 32 * q) {  // before every row
           const float f0 = dec.to(rh, rl, j0 + 15);
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
@@ -1182,13 +1204,15 @@ __global__ void __launch_bounds__(kThreads, Dq<E, D>::kPerSm) dq_kernel(const __
           }
         }
       }
-      a1.set(k, z);
+      a1.put(j0, lb, z);
+    });
+    if constexpr (NL > 1) {
+      sync();  // both products have been read
+      a1.store(lb, wg);
     }
-    sync();  // both products have been read, and the table
-    a1.store(lb, wg);
-    if (warp == kDecayWarp && more) dw.table<false>(dec);
     st_wait();
     sync();
+    if (warp == kDecayWarp && more) dw.table<false>(dec);
     if (ok && tid == 0) {
       product_ta<NL, NL, D>(tb + F::kDq, tb, op_mn<D>(K), false);
       product<NL, 3, 128, D>(tb + F::kIq, op_k<D>(G), state_k<D>(X), D / 16);
@@ -1248,20 +1272,22 @@ __global__ void __launch_bounds__(kThreads, Dq<E, D>::kPerSm) dq_kernel(const __
   if (warp == 0) um::dealloc(sm.tbase, F::kCols);
 }
 
-// TMEM columns: (K Q^T) 0..127 and (V dy^T) 128..255; once read, their masked
-// forms A2 at 0 and A1 at 64 NL (NL levels of 64), dV at 128 NL, dK after it; once
-// these are done, the state parts of dV at 0 and of dK at kIk, and the states'
-// sum at kU.
+// TMEM columns: (K Q^T) 0..127 and (V dy^T) 128..255. One level: their masked forms
+// A2 and A1 in their places, dV and dK (D = 64) in the columns these leave free
+// (D = 128: from 256 on); more levels: A2 at 0 and A1 at 64 NL once both are read, dV
+// and dK after them. The state parts and the states' sum take the masked forms'
+// places: for one level and D = 64 dK's state part the ends, 0..31 and 224..255.
 template <typename E, int D>
 struct Dkv {
   static constexpr int NL = kLevels<E>, kTileE = kC * D;
   // Two CTAs to an SM: dS is spread over all threads, and one tile more holds the
   // decayed K rows, so that dV's state part adds up in dV's own accumulator.
   static constexpr bool kE = NL == 1 && D == 64;
-  static constexpr int kDv = 128 * NL, kDk = kDv + D;
-  static constexpr int kIk = kE ? 0 : 2 * D <= kDv ? D : kDk + D, kU = kE ? D : 0;
-  static constexpr int kCols = kDk + D <= 256 ? 256 : 512;
-  static_assert(kDk + D <= 512 && kIk + D <= 512, "");
+  static constexpr int kA1 = NL == 1 ? 128 : 64 * NL;
+  static constexpr int kDv = kE ? 32 : NL == 1 ? 256 : 128 * NL, kDk = kE ? 160 : kDv + D;
+  static constexpr int kIk = D, kU = kE ? 96 : 0;
+  static constexpr int kCols = kE ? 256 : 512;
+  static_assert(kDk + D <= kCols && (kE || 2 * D <= kDv), "");
   static constexpr size_t kSmem =
       kSmallB + 2 * ((4 * NL + (kE ? 1 : 0)) * (size_t)kTileE + 3 * (size_t)D * D);
   static constexpr int kPerSm = 2 * (kSmem + 1024) <= 228 * 1024 && kCols <= 256 ? 2 : 1;
@@ -1451,9 +1477,7 @@ __global__ void __launch_bounds__(kThreads, Dkv<E, D>::kPerSm) dkv_kernel(const 
     {
       // Lane: token j = row; columns: tokens i >= j. A2 = D * (K Q^T), A1 = D * (V dy^T).
       Held<NL> a1, a2;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int i0 = 32 * k + 16 * wg;
+      masked_blocks<NL>(wg, [&](int i0) {
         float x[16], z[16];
         if (i0 + 15 < 32 * q) {  // before every row of the warp
 #pragma unroll
@@ -1485,9 +1509,9 @@ __global__ void __launch_bounds__(kThreads, Dkv<E, D>::kPerSm) dkv_kernel(const 
             }
           }
         }
-        a2.set(k, x);
-        a1.set(k, z);
-      }
+        a2.put(i0, lb, x);
+        a1.put(i0, lb + F::kA1, z);
+      });
       if constexpr (F::kE) {  // decayed K rows, one level: they end in dV alone
         using I = Items<D>;
 #pragma unroll
@@ -1500,22 +1524,29 @@ __global__ void __launch_bounds__(kThreads, Dkv<E, D>::kPerSm) dkv_kernel(const 
           store_levels8<1>(Ex, 0, I::offset(i), x);
         }
       }
-      sync();  // both products have been read
-      a2.store(lb, wg);
-      a1.store(lb + 64 * NL, wg);
+      if constexpr (NL > 1) {
+        sync();  // both products have been read
+        a2.store(lb, wg);
+        a1.store(lb + F::kA1, wg);
+      }
       st_wait();
     }
     sync();
     if (ok && tid == 0) {
       product_ta<NL, NL, D>(tb + F::kDv, tb, op_mn<D>(G), false);
       if (F::kE) product<1, 2, 128, D>(tb + F::kDv, op_k<D>(Ex), state_mn<D>(X), D / 16, true);
-      product_ta<NL, NL, D>(tb + F::kDk, tb + 64 * NL, op_mn<D>(Q), false);
+      product_ta<NL, NL, D>(tb + F::kDk, tb + F::kA1, op_mn<D>(Q), false);
       um::commit(&sm.bar);
     }
     wait();
     if (ok && tid == 0) {
-      if (!F::kE) product<NL, 3, 128, D>(tb, op_k<D>(K), state_mn<D>(X), D / 16);
-      product<NL, 3, 128, D>(tb + F::kIk, op_k<D>(V), state_k<D>(X), D / 16);
+      if constexpr (F::kE) {  // in two halves of its columns: rows of dS
+        product<NL, 3, 128, 32>(tb, op_k<D>(V), state_k<D>(X), D / 16);
+        product<NL, 3, 128, 32>(tb + 224, op_k<D>(V), state_k<D>(X + 32 * 64), D / 16);
+      } else {
+        product<NL, 3, 128, D>(tb, op_k<D>(K), state_mn<D>(X), D / 16);
+        product<NL, 3, 128, D>(tb + F::kIk, op_k<D>(V), state_k<D>(X), D / 16);
+      }
       um::commit(&sm.bar2);
     }
     auto scale = [&]() { scale_rows<NL, D>(Q, lv, [&](int r) { return ex2(dec.ch[r] + dec.cl[r]); }); };
@@ -1554,7 +1585,7 @@ __global__ void __launch_bounds__(kThreads, Dkv<E, D>::kPerSm) dkv_kernel(const 
       else if (ok && row < n)
         store_row16<E>(p.dV, b, h, p.H, t0 + row, p.T, j0, p.dv, x);
       um::ld16_async(lb + F::kDk + j0, r1);
-      um::ld16_async(lb + F::kIk + j0, r2);
+      um::ld16_async(lb + (F::kE ? (wg == 0 ? 0 : 192) : F::kIk) + j0, r2);
       float kr[16];
       load_levels8<NL>(K, kTileE, sw<kC>(row, j0), kr);
       load_levels8<NL>(K, kTileE, sw<kC>(row, j0 + 8), kr + 8);
