@@ -51,7 +51,9 @@ using bf16 = __nv_bfloat16;
 namespace um = umma;
 
 constexpr int kC = 128;        // tokens of a chunk: the rows of an M = 128 accumulator
-constexpr int kThreads = 256;  // two warps for each quarter of the TMEM lanes
+// A CTA has two or four warps for each quarter of the TMEM lanes: 256 threads where
+// two or three CTAs share an SM, 512 where one has it. "Part" is a warp's share of
+// an accumulator's columns, warp / 4.
 constexpr float kMinLog2 = -128.f;
 // Polls of an mbarrier before a wait gives up (each suspends for some 10 us: over a second).
 constexpr long long kPolls = 1ll << 17;
@@ -154,24 +156,24 @@ __device__ __forceinline__ int sw(int r, int c) {
   return (c >> 6) * (R * 64) + r * 64 + ((((c >> 3) & 7) ^ (r & 7)) << 3) + (c & 7);
 }
 
-// A 128 x D tile in items of 16 bytes in memory order: thread t has items t,
-// t + 256, ..., which are the same columns of rows 32 apart in each half.
-template <int D>
+// A 128 x D tile in items of 16 bytes in memory order: thread t of NT has items t,
+// t + NT, ..., which are the same columns of rows NT / 8 apart in each half.
+template <int D, int NT>
 struct Items {
-  static constexpr int kN = kC * D / 8 / kThreads;
-  __device__ static int row(int i) { return (i & 3) * 32 + (threadIdx.x >> 3); }
+  static constexpr int kN = kC * D / 8 / NT, kHalf = 1024 / NT;
+  __device__ static int row(int i) { return (i % kHalf) * (NT / 8) + (threadIdx.x >> 3); }
   __device__ static int col(int i) {
-    return (i >> 2) * 64 + (((threadIdx.x & 7) ^ ((threadIdx.x >> 3) & 7)) << 3);
+    return (i / kHalf) * 64 + (((threadIdx.x & 7) ^ ((threadIdx.x >> 3) & 7)) << 3);
   }
-  __device__ static int offset(int i) { return 8 * (i * kThreads + (int)threadIdx.x); }
+  __device__ static int offset(int i) { return 8 * (i * NT + (int)threadIdx.x); }
 };
 
 // Rows [t0, t0 + n) of a head as bf16 levels in a tile, through registers; rows
 // from n on and columns from d are zeros.
-template <typename E, int D>
+template <typename E, int D, int NT>
 __device__ __forceinline__ void load_tile(bf16* tile, const Ten<const E>& x, long long b, long long h,
                                           long long t0, int n, int d) {
-  using I = Items<D>;
+  using I = Items<D, NT>;
   constexpr int NL = kLevels<E>;
   const E* head = x.p + b * x.sb + h * x.sh + t0 * x.st;
 #pragma unroll
@@ -207,7 +209,7 @@ __device__ __forceinline__ void prefetch_rows(const Ten<const E>& x, long long b
                                               int n, int d) {
   const E* head = x.p + b * x.sb + h * x.sh + t0 * x.st;
   const int bytes = d * (int)sizeof(E), lines = (bytes + 127) / 128;
-  for (int i = threadIdx.x; i < n * lines; i += kThreads) {
+  for (int i = threadIdx.x; i < n * lines; i += (int)blockDim.x) {
     const char* a = reinterpret_cast<const char*>(head + (i / lines) * x.st) + (i % lines) * 128;
     asm volatile("prefetch.global.L2 [%0];" ::"l"(a));
   }
@@ -491,29 +493,76 @@ __device__ __forceinline__ void st_levels16(uint32_t taddr, const float* x) {
   }
 }
 
-// The four blocks of 16 columns of a 128-wide product that are half wg's, in an
-// order in which a block packed in place (packed_at) lands on columns that the
-// warp has read: from the outer end inwards. One level: a loop, for the sake of
-// the instruction cache, which a chunk's straight code would fill by itself.
-template <int NL, class F>
-__device__ __forceinline__ void masked_blocks(int wg, F&& f) {
-  if constexpr (NL == 1) {
+// The blocks of 16 columns of a 128-wide product that fall to a part, W parts in all.
+// One level, two parts: a half each, in an order in which a block packed in place
+// (packed_at) lands on columns that the warp has read, from the outer end inwards;
+// a loop, for the sake of the instruction cache, which a chunk's straight code
+// would fill by itself. Otherwise blocks are held until they have been read.
+template <int NL, int W>
+__device__ __forceinline__ int block_of(int part, int k) {
+  if (W == 4) return 64 * (part >> 1) + 32 * k + 16 * (part & 1);
+  return NL == 1 && part == 1 ? 112 - 16 * k : 64 * part + 16 * k;
+}
+template <int NL, int W, class F>
+__device__ __forceinline__ void masked_blocks(int part, F&& f) {
+  if constexpr (NL == 1 && W == 2) {
 #pragma unroll 1
-    for (int k = 0; k < 4; ++k) f(wg == 0 ? 16 * k : 112 - 16 * k);
+    for (int k = 0; k < 4; ++k) f(k, block_of<NL, W>(part, k));
   } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) f(64 * wg + 16 * k);
+    for (int k = 0; k < 8 / W; ++k) f(k, block_of<NL, W>(part, k));
   }
+}
+
+// The masked blocks of a lane's row, on their way to an operand's place.
+template <int NL, int W>
+struct Held {
+  static constexpr bool kDirect = NL == 1 && W == 2;
+  std::conditional_t<NL == 1, uint32_t, float> v[kDirect ? 1 : (NL == 1 ? 8 : 16) * (8 / W)];
+  __device__ __forceinline__ void put(int k, int c0, uint32_t taddr, const float (&x)[16]) {
+    if constexpr (kDirect) {
+      st_levels16<1>(taddr + packed_at<1>(c0), x);
+    } else if constexpr (NL == 1) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+        v[8 * k + i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[16 * k + i] = x[i];
+    }
+  }
+  __device__ __forceinline__ void store(uint32_t taddr, int part) const {
+    if constexpr (!kDirect) {
+#pragma unroll
+      for (int k = 0; k < 8 / W; ++k) {
+        const uint32_t at = taddr + packed_at<NL>(block_of<NL, W>(part, k));
+        if constexpr (NL == 1)
+          st8(at, v + 8 * k);
+        else
+          st_levels16<NL>(at, v + 16 * k);
+      }
+    }
+  }
+};
+
+// Four parts, one level: the two warps that share a lane quarter and a half of the
+// columns have both read it (barriers 1..8).
+__device__ __forceinline__ void half_read(int q, int part) {
+  um::fence_before();
+  named_bar(1 + q + 4 * (part >> 1), 64);
+  um::fence_after();
 }
 
 // ------------------------------------------------------------------ state --
 
 // The D x D fp32 state in registers, as the accumulator of a D-row product is
 // read: M = 64 keeps row 16 q + lane in lanes 0-15 of quarter q, M = 128 row
-// 32 q + lane; warps 0-3 hold the left half of the columns, 4-7 the right.
-template <int D>
+// 32 q + lane; a part holds its share of the columns.
+template <int D, int NT>
 struct State {
-  static constexpr int kCols = D / 2;
+  static constexpr int kCols = D * 128 / NT;
   float v[kCols];
   __device__ static int row() {
     const int q = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
@@ -579,9 +628,9 @@ struct State {
 };
 
 // Rows of a tile (NL levels) times w(row), as three levels in dst[0..2].
-template <int NL, int D, typename W>
+template <int NL, int D, int NT, typename W>
 __device__ __forceinline__ void scale_rows(const bf16* src, bf16* const (&dst)[3], W w) {
-  using I = Items<D>;
+  using I = Items<D, NT>;
 #pragma unroll
   for (int it = 0; it < I::kN; ++it) {
     const int o = I::offset(it);
@@ -640,14 +689,15 @@ struct Sums {
   static constexpr int NL = kLevels<E>, kTileE = kC * D;
   static constexpr size_t kSmem = kSmallBytes + 2 * (3 + NL) * (size_t)kTileE;
   static constexpr int kPerSm = (int)(228 * 1024 / (kSmem + 1024)) < 3 ? (int)(228 * 1024 / (kSmem + 1024)) : 3;
+  static constexpr int kThreads = kPerSm == 1 ? 512 : 256;
 };
 
 // What part s of a sequence (ms chunks) adds to the state: forward
 // sum_j e^{c_end - c_j} k_j v_j^T, backward (kBwd) sum_i e^{c_i} q_i dy_i^T with
 // c from the part's start. Every factor is <= 1, so the chunks just add up.
 template <typename E, int D, bool kBwd>
-__global__ void __launch_bounds__(kThreads, Sums<E, D>::kPerSm) state_kernel(const __grid_constant__ Args<E> p) {
-  constexpr int NL = kLevels<E>, kTileE = kC * D;
+__global__ void __launch_bounds__(Sums<E, D>::kThreads, Sums<E, D>::kPerSm) state_kernel(const __grid_constant__ Args<E> p) {
+  constexpr int NL = kLevels<E>, kTileE = kC * D, NT = Sums<E, D>::kThreads;
   extern __shared__ __align__(1024) unsigned char smem[];
   Small& sm = *reinterpret_cast<Small*>(smem);
   bf16* A = reinterpret_cast<bf16*>(smem + kSmallBytes);  // three levels (NL on arrival)
@@ -682,7 +732,7 @@ __global__ void __launch_bounds__(kThreads, Sums<E, D>::kPerSm) state_kernel(con
     ok = !__syncthreads_or(!ok);
     um::fence_after();
   };
-  State<D> st;
+  State<D, NT> st;
   st.zero();
   DecayWarp dw;
   if (warp == kDecayWarp && count > 0) {
@@ -696,12 +746,12 @@ __global__ void __launch_bounds__(kThreads, Sums<E, D>::kPerSm) state_kernel(con
     if (tma) {
       if (ok) ok = mbar_wait(&sm.full[0], i & 1, &g_sticky_err, kPolls);
     } else {
-      load_tile<E, D>(A, kBwd ? p.Q : p.K, b, h, (long long)c * kC, rows(c), p.dk);
-      load_tile<E, D>(Bt, kBwd ? p.dy : p.V, b, h, (long long)c * kC, rows(c), p.dv);
+      load_tile<E, D, NT>(A, kBwd ? p.Q : p.K, b, h, (long long)c * kC, rows(c), p.dk);
+      load_tile<E, D, NT>(Bt, kBwd ? p.dy : p.V, b, h, (long long)c * kC, rows(c), p.dv);
     }
     if (warp == kDecayWarp && more) dw.load(lg + (long long)(c + step) * kC * p.lst, p.lst, rows(c + step));
     const float rh = (float)run, th = sm.dec.ch[kC - 1], tl = sm.dec.cl[kC - 1];
-    scale_rows<NL, D>(A, lv, [&](int r) {  // a thread's own items, in place
+    scale_rows<NL, D, NT>(A, lv, [&](int r) {  // a thread's own items, in place
       const Decays& d = sm.dec;
       return kBwd ? ex2((d.ch[r] + rh) + d.cl[r]) : ex2(((th - d.ch[r]) + rh) + (tl - d.cl[r]));
     });
@@ -772,13 +822,14 @@ struct Fwd {
   static constexpr size_t kSmem =
       kSmallBytes + 2 * (((2 * kBufs + 1) * NL + kExtra) * (size_t)kTileE + NL * (size_t)D * D);
   static constexpr int kPerSm = 2 * (kSmem + 1024) <= 228 * 1024 && kCols <= 256 ? 2 : 1;
+  static constexpr int kThreads = kPerSm == 1 ? 512 : 256;
   static_assert(kSmem <= 227 * 1024, "");
 };
 
 template <typename E, int D>
-__global__ void __launch_bounds__(kThreads, Fwd<E, D>::kPerSm) fwd_kernel(const __grid_constant__ Args<E> p) {
+__global__ void __launch_bounds__(Fwd<E, D>::kThreads, Fwd<E, D>::kPerSm) fwd_kernel(const __grid_constant__ Args<E> p) {
   using F = Fwd<E, D>;
-  constexpr int NL = F::NL, kTileE = F::kTileE;
+  constexpr int NL = F::NL, kTileE = F::kTileE, NT = F::kThreads, W = NT / 128;
   extern __shared__ __align__(1024) unsigned char smem[];
   Small& sm = *reinterpret_cast<Small*>(smem);
   bf16* const Q0 = reinterpret_cast<bf16*>(smem + kSmallBytes);
@@ -815,7 +866,7 @@ __global__ void __launch_bounds__(kThreads, Fwd<E, D>::kPerSm) fwd_kernel(const 
     dw.load(lg + (long long)c0 * kC * p.lst, p.lst, rows(c0));
     dw.table<false>(sm.dec);
   }
-  State<D> S;
+  State<D, NT> S;
   if (s > 0)
     S.load_own(p.seg + (bh * p.nsub + s * p.r) * (D * D));
   else if (p.H0)
@@ -852,9 +903,9 @@ __global__ void __launch_bounds__(kThreads, Fwd<E, D>::kPerSm) fwd_kernel(const 
     if (tma) {
       if (ok) ok = mbar_wait(&sm.full[buf], (i_ >> 1) & 1, &g_sticky_err, kPolls);
     } else {
-      load_tile<E, D>(Q, p.Q, b, h, t0, n, p.dk);
-      load_tile<E, D>(K, p.K, b, h, t0, n, p.dk);
-      load_tile<E, D>(V, p.V, b, h, t0, n, p.dv);
+      load_tile<E, D, NT>(Q, p.Q, b, h, t0, n, p.dk);
+      load_tile<E, D, NT>(K, p.K, b, h, t0, n, p.dk);
+      load_tile<E, D, NT>(V, p.V, b, h, t0, n, p.dv);
     }
     sync();
     const uint32_t tb = sm.tbase;
@@ -877,7 +928,7 @@ __global__ void __launch_bounds__(kThreads, Fwd<E, D>::kPerSm) fwd_kernel(const 
     const float rh = dec.ch[row], rl = dec.cl[row], th = dec.ch[kC - 1], tl = dec.cl[kC - 1];
     const bool add = more || s + 1 == p.nseg;  // a later chunk of this CTA, or H_T, needs S'
     if (add) {  // its products run while the masked product is read
-      scale_rows<NL, D>(K, lv, [&](int r) { return dec.to(th, tl, r); });
+      scale_rows<NL, D, NT>(K, lv, [&](int r) { return dec.to(th, tl, r); });
       sync();
       if (ok && tid == 0) {
         if (tma) ok = mbar_wait(&sm.full[2], i_ & 1, &g_sticky_err, kPolls);
@@ -892,8 +943,8 @@ __global__ void __launch_bounds__(kThreads, Fwd<E, D>::kPerSm) fwd_kernel(const 
     {  // the state's part of y: diag(e^c) Q S
       const float f = ex2(rh + rl);
 #pragma unroll
-      for (int k = 0; k < D / 32; ++k) {
-        const uint32_t a = lb + F::kY + wg * (D / 2) + 16 * k;
+      for (int k = 0; k < D / (16 * W); ++k) {
+        const uint32_t a = lb + F::kY + wg * (D / W) + 16 * k;
         float v[16];
         uint32_t w[16];
         um::ld16(a, v);
@@ -903,7 +954,8 @@ __global__ void __launch_bounds__(kThreads, Fwd<E, D>::kPerSm) fwd_kernel(const 
       }
     }
     // P = D * Q K^T, a half of the columns to a warp
-    masked_blocks<NL>(wg, [&](int j0) {
+    Held<1, W> held;
+    masked_blocks<NL, W>(wg, [&](int bk_, int j0) {
       float v[16];
       if (j0 > 32 * q + 31) {  // after every row of the warp
 #pragma unroll
@@ -922,8 +974,15 @@ __global__ void __launch_bounds__(kThreads, Fwd<E, D>::kPerSm) fwd_kernel(const 
           }
         }
       }
-      st_levels16<NL>(lb + F::kP + packed_at<NL>(j0), v);
+      if constexpr (NL == 1)
+        held.put(bk_, j0, lb, v);
+      else  // in columns of their own
+        st_levels16<NL>(lb + F::kP + packed_at<NL>(j0), v);
     });
+    if constexpr (NL == 1) {
+      if constexpr (W == 4) half_read(q, wg);
+      held.store(lb, wg);
+    }
     if (tma && ok && tid == 0 && more) {
       bulk_wait_read();  // y has left
       tma_load<D>(Qn, &p.mQ, t0 + kC, h, b, &sm.full[buf ^ 1]);
@@ -944,8 +1003,8 @@ __global__ void __launch_bounds__(kThreads, Fwd<E, D>::kPerSm) fwd_kernel(const 
     wait();
     if (tma && ok && tid == 0 && more) load_v(c + 1);
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k) {
-      const int j0 = wg * (D / 2) + 16 * k;
+    for (int k = 0; k < D / (16 * W); ++k) {
+      const int j0 = wg * (D / W) + 16 * k;
       float v[16];
       um::ld16(lb + F::kY + j0, v);
       if (tma)
@@ -989,50 +1048,30 @@ __global__ void __launch_bounds__(kThreads, Fwd<E, D>::kPerSm) fwd_kernel(const 
 struct SmallB {
   uint64_t bar, bar2, full;
   uint32_t tbase, pad;
-  float red[8], red2[8];  // by warp
-  float a[2][kC];         // per half of the columns: a token's share of the sums above
+  float red[16], red2[16];  // by warp
+  float a[2][kC];           // a token's share of the sums above, in two parts
   Decays dec;
 };
 constexpr int kSmallB = 3072;
 static_assert(sizeof(SmallB) <= kSmallB, "");
 constexpr int kSumWarp = 5;  // puts dlog_gamma together, during the next chunk's first products
 
-// The masked blocks of a lane's row. One level goes straight to its place; more
-// levels are held until both accumulators have been read.
-template <int NL>
-struct Held {
-  float v[64];
-  __device__ __forceinline__ void put(int c0, uint32_t, const float (&x)[16]) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[(c0 & 63) + i] = x[i];
-  }
-  __device__ __forceinline__ void store(uint32_t taddr, int wg) const {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) st_levels16<NL>(taddr + 32 * wg + 8 * k, v + 16 * k);
-  }
-};
-template <>
-struct Held<1> {
-  __device__ __forceinline__ void put(int c0, uint32_t taddr, const float (&x)[16]) const {
-    st_levels16<1>(taddr + packed_at<1>(c0), x);
-  }
-};
-
-// D = 64: 16 entries of one row of a state to each thread, all lanes busy.
+// D = 64: 16 or 8 entries of one row of a state to each thread, all lanes busy.
+template <int NT>
 struct Even {
-  static constexpr int D = 64;
+  static constexpr int D = 64, kN = D * D / NT;
   __device__ static int row() { return threadIdx.x & 63; }
-  __device__ static int col() { return (threadIdx.x >> 6) * 16; }
-  __device__ static void load_own(const float* src, float (&v)[16]) {  // State's own order
+  __device__ static int col() { return (threadIdx.x >> 6) * kN; }
+  __device__ static void load_own(const float* src, float (&v)[kN]) {  // State's own order
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) {
+    for (int i = 0; i < kN; i += 4) {
       const float4 f = *reinterpret_cast<const float4*>(src + (((col() + i) / 4) * D + row()) * 4);
       v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
     }
   }
-  __device__ static void to_smem(bf16* t, const float (&v)[16]) {
-    store_levels8<3>(t, D * D, sw<D>(row(), col()), v);
-    store_levels8<3>(t, D * D, sw<D>(row(), col() + 8), v + 8);
+  __device__ static void to_smem(bf16* t, const float (&v)[kN]) {
+#pragma unroll
+    for (int i = 0; i < kN; i += 8) store_levels8<3>(t, D * D, sw<D>(row(), col() + i), v + i);
   }
 };
 
@@ -1040,6 +1079,18 @@ __device__ __forceinline__ float warp_sum(float x) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
   return x;
+}
+
+// a[0][row] + a[1][row], after the next barrier: the sum of all parts' shares.
+template <int W>
+__device__ __forceinline__ void token_share(float (&a)[2][kC], int q, int part, int row, float x) {
+  if constexpr (W == 4) {
+    if (part >= 2) a[part - 2][row] = x;
+    named_bar(9 + q, 128);
+    if (part >= 2) return;
+    x += a[part][row];
+  }
+  a[part][row] = x;
 }
 
 // 16 values, rounded to bf16 and packed, and back into a tile's row.
@@ -1064,14 +1115,16 @@ struct Dq {
   static constexpr int kDq = NL == 1 ? 128 : 64 * NL, kIq = kDq + D, kCols = kIq + D <= 256 ? 256 : 512;
   static constexpr size_t kSmem = kSmallB + 2 * (4 * NL * (size_t)kTileE + 3 * (size_t)D * D);
   static constexpr int kPerSm = 2 * (kSmem + 1024) <= 228 * 1024 && kCols <= 256 ? 2 : 1;
+  static constexpr int kThreads = kPerSm == 1 ? 512 : 256;
   static_assert(kSmem <= 227 * 1024, "");
 };
 
 template <typename E, int D>
-__global__ void __launch_bounds__(kThreads, Dq<E, D>::kPerSm) dq_kernel(const __grid_constant__ Args<E> p) {
+__global__ void __launch_bounds__(Dq<E, D>::kThreads, Dq<E, D>::kPerSm) dq_kernel(const __grid_constant__ Args<E> p) {
   using F = Dq<E, D>;
-  constexpr int NL = F::NL, kTileE = F::kTileE;
+  constexpr int NL = F::NL, kTileE = F::kTileE, NT = F::kThreads, W = NT / 128;
   extern __shared__ __align__(1024) unsigned char smem[];
+  using Ev = Even<NT>;
   SmallB& sm = *reinterpret_cast<SmallB*>(smem);
   bf16* Q = reinterpret_cast<bf16*>(smem + kSmallB);
   bf16 *K = Q + NL * kTileE, *V = K + NL * kTileE, *G = V + NL * kTileE, *X = G + NL * kTileE;
@@ -1136,11 +1189,11 @@ __global__ void __launch_bounds__(kThreads, Dq<E, D>::kPerSm) dq_kernel(const __
     {  // the state that entered the chunk
       const float* src = p.saved + (a.bh * (p.nchunks + 1) + a.c) * (D * D);
       if constexpr (D == 64) {
-        float v[16];
-        Even::load_own(src, v);
-        Even::to_smem(X, v);
+        float v[Ev::kN];
+        Ev::load_own(src, v);
+        Ev::to_smem(X, v);
       } else {
-        State<D> S;
+        State<D, NT> S;
         S.load_own(src);
         S.template to_smem<3>(X);
       }
@@ -1148,10 +1201,10 @@ __global__ void __launch_bounds__(kThreads, Dq<E, D>::kPerSm) dq_kernel(const __
     if (tma) {
       if (ok) ok = mbar_wait(&sm.full, turn, &g_sticky_err, kPolls);
     } else {
-      load_tile<E, D>(Q, p.Q, a.b, a.h, a.t0, a.n, p.dk);
-      load_tile<E, D>(K, p.K, a.b, a.h, a.t0, a.n, p.dk);
-      load_tile<E, D>(V, p.V, a.b, a.h, a.t0, a.n, p.dv);
-      load_tile<E, D>(G, p.dy, a.b, a.h, a.t0, a.n, p.dv);
+      load_tile<E, D, NT>(Q, p.Q, a.b, a.h, a.t0, a.n, p.dk);
+      load_tile<E, D, NT>(K, p.K, a.b, a.h, a.t0, a.n, p.dk);
+      load_tile<E, D, NT>(V, p.V, a.b, a.h, a.t0, a.n, p.dv);
+      load_tile<E, D, NT>(G, p.dy, a.b, a.h, a.t0, a.n, p.dv);
     }
     sync();
     const uint32_t tb = sm.tbase, lb = tb + ((uint32_t)(32 * q) << 16);
@@ -1173,9 +1226,9 @@ __global__ void __launch_bounds__(kThreads, Dq<E, D>::kPerSm) dq_kernel(const __
     wait();
     const float rh = dec.ch[row], rl = dec.cl[row], from_start = ex2(rh + rl);
     float tok = 0.f;
-    Held<NL> a1;
+    Held<NL, W> a1;
     // Lane: token i = row; columns: tokens j <= i. A1 = D * (dy V^T).
-    masked_blocks<NL>(wg, [&](int j0) {
+    masked_blocks<NL, W>(wg, [&](int bk_, int j0) {
       float x[16], z[16];
       if (j0 > 32 * q + 31) {  // after every row of the warp
 #pragma unroll
@@ -1204,12 +1257,13 @@ __global__ void __launch_bounds__(kThreads, Dq<E, D>::kPerSm) dq_kernel(const __
           }
         }
       }
-      a1.put(j0, lb, z);
+      a1.put(bk_, j0, lb, z);
     });
-    if constexpr (NL > 1) {
+    if constexpr (NL > 1)
       sync();  // both products have been read
-      a1.store(lb, wg);
-    }
+    else if constexpr (W == 4)
+      half_read(q, wg);
+    a1.store(lb, wg);
     st_wait();
     sync();
     if (warp == kDecayWarp && more) dw.table<false>(dec);
@@ -1221,8 +1275,8 @@ __global__ void __launch_bounds__(kThreads, Dq<E, D>::kPerSm) dq_kernel(const __
     wait();
     float aq = 0.f;
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k) {
-      const int j0 = wg * (D / 2) + 16 * k;
+    for (int k = 0; k < D / (16 * W); ++k) {
+      const int j0 = wg * (D / W) + 16 * k;
       uint32_t r1[16], r2[16];
       float x[16], z[16], qr[16];
       um::ld16_async(lb + F::kDq + j0, r1);
@@ -1243,14 +1297,14 @@ __global__ void __launch_bounds__(kThreads, Dq<E, D>::kPerSm) dq_kernel(const __
         store_row16<E>(p.dQ, a.b, a.h, p.H, a.t0 + row, p.T, j0, p.dk, x);
     }
     aq *= from_start;
-    sm.a[wg][row] = aq + tok;
+    token_share<W>(sm.a, q, wg, row, aq + tok);
     const float ws = warp_sum(aq);
     if (lane == 0) sm.red[warp] = ws;
     sync();
     if (ok && tid < a.n) p.tq[a.bh * p.T + a.t0 + tid] = sm.a[0][tid] + sm.a[1][tid];
     if (ok && tid == kC) {
       float s = 0.f;
-      for (int i = 0; i < 8; ++i) s += sm.red[i];
+      for (int i = 0; i < NT / 32; ++i) s += sm.red[i];
       p.aq[a.bh * p.nchunks + a.c] = s;
     }
     if (tma && ok && tid == 0) {
@@ -1291,14 +1345,16 @@ struct Dkv {
   static constexpr size_t kSmem =
       kSmallB + 2 * ((4 * NL + (kE ? 1 : 0)) * (size_t)kTileE + 3 * (size_t)D * D);
   static constexpr int kPerSm = 2 * (kSmem + 1024) <= 228 * 1024 && kCols <= 256 ? 2 : 1;
+  static constexpr int kThreads = kPerSm == 1 ? 512 : 256;
   static_assert(kSmem <= 227 * 1024, "");
 };
 
 template <typename E, int D>
-__global__ void __launch_bounds__(kThreads, Dkv<E, D>::kPerSm) dkv_kernel(const __grid_constant__ Args<E> p) {
+__global__ void __launch_bounds__(Dkv<E, D>::kThreads, Dkv<E, D>::kPerSm) dkv_kernel(const __grid_constant__ Args<E> p) {
   using F = Dkv<E, D>;
-  constexpr int NL = F::NL, kTileE = F::kTileE;
+  constexpr int NL = F::NL, kTileE = F::kTileE, NT = F::kThreads, W = NT / 128;
   extern __shared__ __align__(1024) unsigned char smem[];
+  using Ev = Even<NT>;
   SmallB& sm = *reinterpret_cast<SmallB*>(smem);
   bf16* Q = reinterpret_cast<bf16*>(smem + kSmallB);
   bf16 *K = Q + NL * kTileE, *V = K + NL * kTileE, *G = V + NL * kTileE, *X = G + NL * kTileE;
@@ -1336,26 +1392,26 @@ __global__ void __launch_bounds__(kThreads, Dkv<E, D>::kPerSm) dkv_kernel(const 
     dw.load(lg + (long long)(c1 - 1) * kC * p.lst, p.lst, rows(c1 - 1));
     dw.table<true>(dec);
   }
-  float dSe[16];  // kE
-  State<D> dS;    // otherwise
+  float dSe[Ev::kN];  // kE
+  State<D, NT> dS;    // otherwise
   {
     const float* end = s + 1 < p.nseg ? p.seg + (bh * p.nsub + (s + 1) * p.r - 1) * (D * D) : nullptr;
     const float* S_end = p.saved + (bh * (p.nchunks + 1) + c1) * (D * D);
     float d = 0.f;  // <S, dS> at the segment's end
     if constexpr (F::kE) {
-      const int er = Even::row(), ec = Even::col();
+      const int er = Ev::row(), ec = Ev::col();
       if (end) {
-        Even::load_own(end, dSe);
+        Ev::load_own(end, dSe);
       } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
+        for (int i = 0; i < Ev::kN; ++i)
           dSe[i] = p.dHT && er < p.dk && ec + i < p.dv ? p.dHT[bh * p.sbh + er * p.sld + ec + i] : 0.f;
       }
-      float v[16];
-      Even::load_own(S_end, v);
+      float v[Ev::kN];
+      Ev::load_own(S_end, v);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) d = fmaf(v[i], dSe[i], d);
-      Even::to_smem(X, dSe);
+      for (int i = 0; i < Ev::kN; ++i) d = fmaf(v[i], dSe[i], d);
+      Ev::to_smem(X, dSe);
     } else {
       if (end)
         dS.load_own(end);
@@ -1363,10 +1419,10 @@ __global__ void __launch_bounds__(kThreads, Dkv<E, D>::kPerSm) dkv_kernel(const 
         dS.load(p.dHT + bh * p.sbh, p.dk, p.dv, p.sld);
       else
         dS.zero();
-      State<D> S;
+      State<D, NT> S;
       S.load_own(S_end);
 #pragma unroll
-      for (int i = 0; i < State<D>::kCols; ++i) d = fmaf(S.v[i], dS.v[i], d);
+      for (int i = 0; i < State<D, NT>::kCols; ++i) d = fmaf(S.v[i], dS.v[i], d);
       dS.template to_smem<3>(X);
     }
     d = warp_sum(d);
@@ -1389,7 +1445,7 @@ __global__ void __launch_bounds__(kThreads, Dkv<E, D>::kPerSm) dkv_kernel(const 
   double Fend = 0.0;  // kSumWarp: <S, dS> at the end of the chunk being summed
   float tq[4], lgs[4], aqs = 0.f;
   if (warp == kSumWarp)
-    for (int i = 0; i < 8; ++i) Fend += (double)sm.red[i];
+    for (int i = 0; i < NT / 32; ++i) Fend += (double)sm.red[i];
   // What chunk c's dlog_gamma needs from memory, and its sums once sm.a is complete:
   // four tokens to a lane, from the end, in fp64.
   auto sums_load = [&](int c) {
@@ -1430,7 +1486,7 @@ __global__ void __launch_bounds__(kThreads, Dkv<E, D>::kPerSm) dkv_kernel(const 
       }
     }
     double bk = 0.0;
-    for (int i = 0; i < 8; ++i) bk += (double)sm.red2[i];
+    for (int i = 0; i < NT / 32; ++i) bk += (double)sm.red2[i];
     Fend += (double)aqs - bk;
   };
   const int row = 32 * q + lane;
@@ -1441,10 +1497,10 @@ __global__ void __launch_bounds__(kThreads, Dkv<E, D>::kPerSm) dkv_kernel(const 
     if (tma) {
       if (ok) ok = mbar_wait(&sm.full, turn, &g_sticky_err, kPolls);
     } else {
-      load_tile<E, D>(K, p.K, b, h, t0, n, p.dk);
-      load_tile<E, D>(Q, p.Q, b, h, t0, n, p.dk);
-      load_tile<E, D>(V, p.V, b, h, t0, n, p.dv);
-      load_tile<E, D>(G, p.dy, b, h, t0, n, p.dv);
+      load_tile<E, D, NT>(K, p.K, b, h, t0, n, p.dk);
+      load_tile<E, D, NT>(Q, p.Q, b, h, t0, n, p.dk);
+      load_tile<E, D, NT>(V, p.V, b, h, t0, n, p.dv);
+      load_tile<E, D, NT>(G, p.dy, b, h, t0, n, p.dv);
     }
     sync();
     const uint32_t tb = sm.tbase, lb = tb + ((uint32_t)(32 * q) << 16);
@@ -1476,8 +1532,8 @@ __global__ void __launch_bounds__(kThreads, Dkv<E, D>::kPerSm) dkv_kernel(const 
     float tok = 0.f;  // this half's part of what token `row` takes from t <= row
     {
       // Lane: token j = row; columns: tokens i >= j. A2 = D * (K Q^T), A1 = D * (V dy^T).
-      Held<NL> a1, a2;
-      masked_blocks<NL>(wg, [&](int i0) {
+      Held<NL, W> a1, a2;
+      masked_blocks<NL, W>(wg, [&](int bk_, int i0) {
         float x[16], z[16];
         if (i0 + 15 < 32 * q) {  // before every row of the warp
 #pragma unroll
@@ -1509,11 +1565,11 @@ __global__ void __launch_bounds__(kThreads, Dkv<E, D>::kPerSm) dkv_kernel(const 
             }
           }
         }
-        a2.put(i0, lb, x);
-        a1.put(i0, lb + F::kA1, z);
+        a2.put(bk_, i0, lb, x);
+        a1.put(bk_, i0, lb + F::kA1, z);
       });
       if constexpr (F::kE) {  // decayed K rows, one level: they end in dV alone
-        using I = Items<D>;
+        using I = Items<D, NT>;
 #pragma unroll
         for (int i = 0; i < I::kN; ++i) {
           float x[8];
@@ -1524,11 +1580,12 @@ __global__ void __launch_bounds__(kThreads, Dkv<E, D>::kPerSm) dkv_kernel(const 
           store_levels8<1>(Ex, 0, I::offset(i), x);
         }
       }
-      if constexpr (NL > 1) {
+      if constexpr (NL > 1)
         sync();  // both products have been read
-        a2.store(lb, wg);
-        a1.store(lb + F::kA1, wg);
-      }
+      else if constexpr (W == 4)
+        half_read(q, wg);
+      a2.store(lb, wg);
+      a1.store(lb + F::kA1, wg);
       st_wait();
     }
     sync();
@@ -1549,7 +1606,7 @@ __global__ void __launch_bounds__(kThreads, Dkv<E, D>::kPerSm) dkv_kernel(const 
       }
       um::commit(&sm.bar2);
     }
-    auto scale = [&]() { scale_rows<NL, D>(Q, lv, [&](int r) { return ex2(dec.ch[r] + dec.cl[r]); }); };
+    auto scale = [&]() { scale_rows<NL, D, NT>(Q, lv, [&](int r) { return ex2(dec.ch[r] + dec.cl[r]); }); };
     auto sum_states = [&]() {
       if (ok && tid == 0) {
         product_rows<NL, D>(tb + F::kU, lv, G, false);
@@ -1565,10 +1622,10 @@ __global__ void __launch_bounds__(kThreads, Dkv<E, D>::kPerSm) dkv_kernel(const 
       sum_states();
     }
     float bk = 0.f;  // k . its gradient's state part
-    uint32_t dvp[F::kE ? 16 : 1];
+    uint32_t dvp[F::kE ? 8 * (D / (16 * W)) : 1];
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k) {
-      const int j0 = wg * (D / 2) + 16 * k;
+    for (int k = 0; k < D / (16 * W); ++k) {
+      const int j0 = wg * (D / W) + 16 * k;
       uint32_t r1[16], r2[16];
       float x[16], z[16];
       um::ld16_async(lb + F::kDv + j0, r1);
@@ -1585,7 +1642,7 @@ __global__ void __launch_bounds__(kThreads, Dkv<E, D>::kPerSm) dkv_kernel(const 
       else if (ok && row < n)
         store_row16<E>(p.dV, b, h, p.H, t0 + row, p.T, j0, p.dv, x);
       um::ld16_async(lb + F::kDk + j0, r1);
-      um::ld16_async(lb + (F::kE ? (wg == 0 ? 0 : 192) : F::kIk) + j0, r2);
+      um::ld16_async(lb + (F::kE ? (j0 < 32 ? 0 : 192) : F::kIk) + j0, r2);
       float kr[16];
       load_levels8<NL>(K, kTileE, sw<kC>(row, j0), kr);
       load_levels8<NL>(K, kTileE, sw<kC>(row, j0 + 8), kr + 8);
@@ -1603,7 +1660,7 @@ __global__ void __launch_bounds__(kThreads, Dkv<E, D>::kPerSm) dkv_kernel(const 
         store_row16<E>(p.dK, b, h, p.H, t0 + row, p.T, j0, p.dk, x);
     }
     bk *= to_end;
-    sm.a[wg][row] = tok - bk;
+    token_share<W>(sm.a, q, wg, row, tok - bk);
     bk = warp_sum(bk);
     if (lane == 0) sm.red2[warp] = bk;
     if (!F::kE) {  // over Q and what else has been read
@@ -1617,10 +1674,10 @@ __global__ void __launch_bounds__(kThreads, Dkv<E, D>::kPerSm) dkv_kernel(const 
     if constexpr (F::kE) {
       // the sum goes over the extra tile in its own order, then to all threads
       if (tma) {
-        packed16_to_tile(V, row, wg * 32, dvp);
-        packed16_to_tile(V, row, wg * 32 + 16, dvp + 8);
+#pragma unroll
+        for (int k = 0; k < D / (16 * W); ++k) packed16_to_tile(V, row, wg * (D / W) + 16 * k, dvp + 8 * k);
       }
-      State<D> u;
+      State<D, NT> u;
       u.zero();
       u.update(0.f, tb, F::kU);
       u.store_own(reinterpret_cast<float*>(Ex));
@@ -1637,11 +1694,11 @@ __global__ void __launch_bounds__(kThreads, Dkv<E, D>::kPerSm) dkv_kernel(const 
           tma_load<D>(V, &p.mV, t0 - kC, h, b, &sm.full);
         }
       }
-      float v[16];
-      Even::load_own(reinterpret_cast<const float*>(Ex), v);
+      float v[Ev::kN];
+      Ev::load_own(reinterpret_cast<const float*>(Ex), v);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) dSe[i] = fmaf(g, dSe[i], v[i]);
-      Even::to_smem(X, dSe);
+      for (int i = 0; i < Ev::kN; ++i) dSe[i] = fmaf(g, dSe[i], v[i]);
+      Ev::to_smem(X, dSe);
     } else {
       if (tma && ok && tid == 0 && more) {
         mbar_arrive_expect_tx(&sm.full, 4 * tile_bytes(D));
@@ -1660,9 +1717,9 @@ __global__ void __launch_bounds__(kThreads, Dkv<E, D>::kPerSm) dkv_kernel(const 
   if (tma && tid == 0) bulk_wait_read();
   if (ok && s == 0 && p.dH0) {
     if constexpr (F::kE) {
-      const int er = Even::row(), ec = Even::col();
+      const int er = Ev::row(), ec = Ev::col();
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
+      for (int i = 0; i < Ev::kN; ++i)
         if (er < p.dk && ec + i < p.dv) p.dH0[bh * p.sbh + er * p.sld + ec + i] = dSe[i];
     } else {
       dS.store(p.dH0 + bh * p.sbh, p.dk, p.dv, p.sld);
@@ -1793,7 +1850,7 @@ int run_segments(const Args<E>& a, cudaStream_t st) {
   constexpr size_t smem = Sums<E, D>::kSmem;
   auto k1 = state_kernel<E, D, kBwd>;
   if (int r = set_smem(k1, smem)) return r;
-  k1<<<(unsigned)(a.BH * (a.nseg - 1) * a.r), kThreads, smem, st>>>(a);
+  k1<<<(unsigned)(a.BH * (a.nseg - 1) * a.r), Sums<E, D>::kThreads, smem, st>>>(a);
   if (int r = launched()) return r;
   const long long n = a.BH * (D * D / 4);
   scan_kernel<D, kBwd><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(
@@ -1809,13 +1866,13 @@ int run_main(bool fwd, const Args<E>& a, cudaStream_t st) {
     using F = Dq<E, D>;
     if (int r = set_smem(dq_kernel<E, D>, F::kSmem)) return r;
     const long long n = a.BH * a.nchunks, places = (long long)sm_count() * F::kPerSm;
-    dq_kernel<E, D><<<(unsigned)(n < places ? n : places), kThreads, F::kSmem, st>>>(a);
+    dq_kernel<E, D><<<(unsigned)(n < places ? n : places), F::kThreads, F::kSmem, st>>>(a);
     if (int r = launched()) return r;
   }
   auto k = fwd ? fwd_kernel<E, D> : dkv_kernel<E, D>;
   const size_t smem = fwd ? Fwd<E, D>::kSmem : Dkv<E, D>::kSmem;
   if (int r = set_smem(k, smem)) return r;
-  k<<<(unsigned)(a.BH * a.nseg), kThreads, smem, st>>>(a);
+  k<<<(unsigned)(a.BH * a.nseg), fwd ? Fwd<E, D>::kThreads : Dkv<E, D>::kThreads, smem, st>>>(a);
   return launched();
 }
 
