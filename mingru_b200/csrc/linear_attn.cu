@@ -399,11 +399,25 @@ __device__ __forceinline__ Op<D> state_k(const bf16* t) { return operand<D>(t, f
 template <int D>
 __device__ __forceinline__ Op<D> state_mn(const bf16* t) { return operand<D>(t, true, D * D); }
 
+// One warp issues the products, by a thread that it elects: warp-uniform control
+// flow lets descriptors stay in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(r));
+  return r != 0;
+}
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+      : "memory");
+}
 __device__ __forceinline__ void mma_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
   asm volatile(
       "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc), "r"(0), "r"(0), "r"(0), "r"(0)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
       : "memory");
 }
 
@@ -413,8 +427,8 @@ __device__ __forceinline__ void mma_ta(uint32_t d, uint32_t a, uint64_t b, uint3
 constexpr int kMaxPair = 2;
 
 // D (M x N) (+)= A B over K = 16 ks. One thread.
-template <int NA, int NB, int M, int N, int RA, int RB>
-__device__ __forceinline__ void product(uint32_t d, const Op<RA>& a, const Op<RB>& b, int ks, bool acc = false) {
+template <int NA, int NB, int M, int N, int KS, int RA, int RB>
+__device__ __forceinline__ void product(uint32_t d, const Op<RA>& a, const Op<RB>& b, bool acc = false) {
   const uint32_t id = um::idesc64(a.mn, b.mn, M == 128, N);
 #pragma unroll
   for (int o = kMaxPair; o >= 0; --o)
@@ -422,9 +436,9 @@ __device__ __forceinline__ void product(uint32_t d, const Op<RA>& a, const Op<RB
     for (int i = 0; i < NA; ++i) {
       const int j = o - i;
       if (j < 0 || j >= NB) continue;
-#pragma unroll 4
-      for (int k = 0; k < ks; ++k) {
-        um::mma(d, a.d + a.at(k) + i * a.level, b.d + b.at(k) + j * b.level, id, acc);
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        mma(d, a.d + a.at(k) + i * a.level, b.d + b.at(k) + j * b.level, id, acc);
         acc = true;
       }
     }
@@ -447,7 +461,7 @@ __device__ __forceinline__ void product_ta(uint32_t d, uint32_t a, const Op<kC>&
     for (int i = 0; i < NA; ++i) {
       const int j = o - i;
       if (j < 0 || j >= NB) continue;
-#pragma unroll 4
+#pragma unroll
       for (int k = 0; k < kC / 16; ++k) {
         mma_ta(d, a + packed_at<NA>(16 * k) + i * 64, b.d + b.at(k) + j * b.level, id, acc);
         acc = true;
@@ -660,9 +674,9 @@ __device__ __forceinline__ void product_rows(uint32_t d, bf16* const (&a)[3], co
     for (int i = 0; i < 3; ++i) {
       const int j = r - i;
       if (j < 0 || j >= NL) continue;
-#pragma unroll 4
+#pragma unroll
       for (int k = 0; k < kC / 16; ++k) {
-        um::mma(d, da[i] + o.at(k), o.d + o.at(k) + j * o.level, id, acc);
+        mma(d, da[i] + o.at(k), o.d + o.at(k) + j * o.level, id, acc);
         acc = true;
       }
     }
@@ -702,7 +716,7 @@ __global__ void __launch_bounds__(Sums<E, D>::kThreads, Sums<E, D>::kPerSm) stat
   Small& sm = *reinterpret_cast<Small*>(smem);
   bf16* A = reinterpret_cast<bf16*>(smem + kSmallBytes);  // three levels (NL on arrival)
   bf16* Bt = A + 3 * kTileE;
-  const int tid = threadIdx.x, warp = tid >> 5;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const long long bh = blockIdx.x % p.BH;
   const int s = (int)(blockIdx.x / p.BH) + (kBwd ? p.r : 0);
   const int b = (int)(bh / p.H), h = (int)(bh % p.H);
@@ -757,7 +771,7 @@ __global__ void __launch_bounds__(Sums<E, D>::kThreads, Sums<E, D>::kPerSm) stat
     });
     run += (double)th + (double)tl;
     sync();
-    if (ok && tid == 0) {
+    if (warp == 0 && elect_one() && ok) {
       product_rows<NL, D>(sm.tbase, lv, Bt, false);
       um::commit(&sm.bar);
     }
@@ -835,7 +849,7 @@ __global__ void __launch_bounds__(Fwd<E, D>::kThreads, Fwd<E, D>::kPerSm) fwd_ke
   bf16* const Q0 = reinterpret_cast<bf16*>(smem + kSmallBytes);
   bf16 *const K0 = Q0 + F::kBufs * NL * kTileE, *const V = K0 + F::kBufs * NL * kTileE,
               *const X = V + (NL + F::kExtra) * kTileE;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q = warp & 3, wg = warp >> 2;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, q = warp & 3, wg = warp >> 2;
   const long long bh = blockIdx.x % p.BH;
   const int s = (int)(blockIdx.x / p.BH);
   const int b = (int)(bh / p.H), h = (int)(bh % p.H);
@@ -909,16 +923,16 @@ __global__ void __launch_bounds__(Fwd<E, D>::kThreads, Fwd<E, D>::kPerSm) fwd_ke
     }
     sync();
     const uint32_t tb = sm.tbase;
-    if (ok && tid == 0) {
-      product<NL, NL, 128, 128>(tb, op_k<D>(Q), op_k<D>(K), D / 16);
-      product<NL, NL, 128, D>(tb + F::kY, op_k<D>(Q), state_mn<D>(X), D / 16);
+    if (warp == 0 && elect_one() && ok) {
+      product<NL, NL, 128, 128, D / 16>(tb, op_k<D>(Q), op_k<D>(K));
+      product<NL, NL, 128, D, D / 16>(tb + F::kY, op_k<D>(Q), state_mn<D>(X));
       um::commit(&sm.bar);
-      if (tma) {
-        if (c > c0) tma_store<D>(&p.my, t0 - kC, h, b, p.dv, Qn);  // the last chunk's y
-        if (more) {
-          mbar_arrive_expect_tx(&sm.full[buf ^ 1], 2 * tile_bytes(D));
-          tma_load<D>(Kn, &p.mK, t0 + kC, h, b, &sm.full[buf ^ 1]);
-        }
+    }
+    if (tma && ok && tid == 0) {
+      if (c > c0) tma_store<D>(&p.my, t0 - kC, h, b, p.dv, Qn);  // the last chunk's y
+      if (more) {
+        mbar_arrive_expect_tx(&sm.full[buf ^ 1], 2 * tile_bytes(D));
+        tma_load<D>(Kn, &p.mK, t0 + kC, h, b, &sm.full[buf ^ 1]);
       }
     }
     if (warp == kDecayWarp && more) dw.load(lg + (t0 + kC) * p.lst, p.lst, rows(c + 1));
@@ -930,7 +944,7 @@ __global__ void __launch_bounds__(Fwd<E, D>::kThreads, Fwd<E, D>::kPerSm) fwd_ke
     if (add) {  // its products run while the masked product is read
       scale_rows<NL, D, NT>(K, lv, [&](int r) { return dec.to(th, tl, r); });
       sync();
-      if (ok && tid == 0) {
+      if (warp == 0 && elect_one() && ok) {
         if (tma) ok = mbar_wait(&sm.full[2], i_ & 1, &g_sticky_err, kPolls);
         if (ok) {
           product_rows<NL, D>(tb + F::kU, lv, V, false);
@@ -989,7 +1003,7 @@ __global__ void __launch_bounds__(Fwd<E, D>::kThreads, Fwd<E, D>::kPerSm) fwd_ke
     }
     st_wait();
     sync();
-    if (ok && tid == 0) {
+    if (warp == 0 && elect_one() && ok) {
       product_ta<NL, NL, D>(tb + F::kY, tb + F::kP, op_mn<D>(V), true);
       um::commit(&sm.bar);
     }
@@ -1054,7 +1068,10 @@ struct SmallB {
 };
 constexpr int kSmallB = 3072;
 static_assert(sizeof(SmallB) <= kSmallB, "");
-constexpr int kSumWarp = 5;  // puts dlog_gamma together, during the next chunk's first products
+// In dkv_kernel the first rows have most masked blocks, so the last quarter's warps
+// do the sundries: kSumWarp puts dlog_gamma together during the next chunk's first
+// products.
+constexpr int kSumWarp = 7, kDkvDecayWarp = 3;
 
 // D = 64: 16 or 8 entries of one row of a state to each thread, all lanes busy.
 template <int NT>
@@ -1128,7 +1145,7 @@ __global__ void __launch_bounds__(Dq<E, D>::kThreads, Dq<E, D>::kPerSm) dq_kerne
   SmallB& sm = *reinterpret_cast<SmallB*>(smem);
   bf16* Q = reinterpret_cast<bf16*>(smem + kSmallB);
   bf16 *K = Q + NL * kTileE, *V = K + NL * kTileE, *G = V + NL * kTileE, *X = G + NL * kTileE;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q = warp & 3, wg = warp >> 2;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, q = warp & 3, wg = warp >> 2;
   const int row = 32 * q + lane;
   const long long total = p.BH * p.nchunks;
   struct At {  // a chunk's place
@@ -1208,16 +1225,16 @@ __global__ void __launch_bounds__(Dq<E, D>::kThreads, Dq<E, D>::kPerSm) dq_kerne
     }
     sync();
     const uint32_t tb = sm.tbase, lb = tb + ((uint32_t)(32 * q) << 16);
-    if (ok && tid == 0) {
-      product<NL, NL, 128, 128>(tb, op_k<D>(G), op_k<D>(V), D / 16);
-      product<NL, NL, 128, 128>(tb + 128, op_k<D>(Q), op_k<D>(K), D / 16);
+    if (warp == 0 && elect_one() && ok) {
+      product<NL, NL, 128, 128, D / 16>(tb, op_k<D>(G), op_k<D>(V));
+      product<NL, NL, 128, 128, D / 16>(tb + 128, op_k<D>(Q), op_k<D>(K));
       um::commit(&sm.bar);
-      if (tma && more) {
-        tma_prefetch<D>(&p.mdy, next.t0, next.h, next.b, p.dv);
-        tma_prefetch<D>(&p.mV, next.t0, next.h, next.b, p.dv);
-        tma_prefetch<D>(&p.mQ, next.t0, next.h, next.b, p.dk);
-        tma_prefetch<D>(&p.mK, next.t0, next.h, next.b, p.dk);
-      }
+    }
+    if (tma && more && ok && tid == 0) {
+      tma_prefetch<D>(&p.mdy, next.t0, next.h, next.b, p.dv);
+      tma_prefetch<D>(&p.mV, next.t0, next.h, next.b, p.dv);
+      tma_prefetch<D>(&p.mQ, next.t0, next.h, next.b, p.dk);
+      tma_prefetch<D>(&p.mK, next.t0, next.h, next.b, p.dk);
     }
     if (tid < D * D / 32)  // the next state's lines
       asm volatile("prefetch.global.L2 [%0];" ::"l"(
@@ -1267,9 +1284,9 @@ __global__ void __launch_bounds__(Dq<E, D>::kThreads, Dq<E, D>::kPerSm) dq_kerne
     st_wait();
     sync();
     if (warp == kDecayWarp && more) dw.table<false>(dec);
-    if (ok && tid == 0) {
+    if (warp == 0 && elect_one() && ok) {
       product_ta<NL, NL, D>(tb + F::kDq, tb, op_mn<D>(K), false);
-      product<NL, 3, 128, D>(tb + F::kIq, op_k<D>(G), state_k<D>(X), D / 16);
+      product<NL, 3, 128, D, D / 16>(tb + F::kIq, op_k<D>(G), state_k<D>(X));
       um::commit(&sm.bar);
     }
     wait();
@@ -1362,7 +1379,7 @@ __global__ void __launch_bounds__(Dkv<E, D>::kThreads, Dkv<E, D>::kPerSm) dkv_ke
   // the scaled Q rows go over Q and, below three levels, over what has been read by then
   bf16* const lv[3] = {Q, F::kE ? V : NL == 1 ? K : Q + kTileE,
                        F::kE ? Ex : NL == 1 ? V : NL == 2 ? K : Q + 2 * kTileE};
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q = warp & 3, wg = warp >> 2;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, q = warp & 3, wg = warp >> 2;
   const long long bh = blockIdx.x % p.BH;
   const int s = p.nseg - 1 - (int)(blockIdx.x / p.BH);
   const int b = (int)(bh / p.H), h = (int)(bh % p.H);
@@ -1388,7 +1405,7 @@ __global__ void __launch_bounds__(Dkv<E, D>::kThreads, Dkv<E, D>::kPerSm) dkv_ke
     }
   }
   DecayWarp dw;
-  if (warp == kDecayWarp) {
+  if (warp == kDkvDecayWarp) {
     dw.load(lg + (long long)(c1 - 1) * kC * p.lst, p.lst, rows(c1 - 1));
     dw.table<true>(dec);
   }
@@ -1504,16 +1521,16 @@ __global__ void __launch_bounds__(Dkv<E, D>::kThreads, Dkv<E, D>::kPerSm) dkv_ke
     }
     sync();
     const uint32_t tb = sm.tbase, lb = tb + ((uint32_t)(32 * q) << 16);
-    if (ok && tid == 0) {
-      product<NL, NL, 128, 128>(tb, op_k<D>(K), op_k<D>(Q), D / 16);
-      product<NL, NL, 128, 128>(tb + 128, op_k<D>(V), op_k<D>(G), D / 16);
+    if (warp == 0 && elect_one() && ok) {
+      product<NL, NL, 128, 128, D / 16>(tb, op_k<D>(K), op_k<D>(Q));
+      product<NL, NL, 128, 128, D / 16>(tb + 128, op_k<D>(V), op_k<D>(G));
       um::commit(&sm.bar);
-      if (tma && more) {  // the next chunk's rows on their way into L2
-        tma_prefetch<D>(&p.mK, t0 - kC, h, b, p.dk);
-        tma_prefetch<D>(&p.mQ, t0 - kC, h, b, p.dk);
-        tma_prefetch<D>(&p.mV, t0 - kC, h, b, p.dv);
-        tma_prefetch<D>(&p.mdy, t0 - kC, h, b, p.dv);
-      }
+    }
+    if (tma && more && ok && tid == 0) {  // the next chunk's rows on their way into L2
+      tma_prefetch<D>(&p.mK, t0 - kC, h, b, p.dk);
+      tma_prefetch<D>(&p.mQ, t0 - kC, h, b, p.dk);
+      tma_prefetch<D>(&p.mV, t0 - kC, h, b, p.dv);
+      tma_prefetch<D>(&p.mdy, t0 - kC, h, b, p.dv);
     }
     if (!tma && more) {
       prefetch_rows(p.Q, b, h, t0 - kC, kC, p.dk);
@@ -1521,7 +1538,7 @@ __global__ void __launch_bounds__(Dkv<E, D>::kThreads, Dkv<E, D>::kPerSm) dkv_ke
       prefetch_rows(p.V, b, h, t0 - kC, kC, p.dv);
       prefetch_rows(p.dy, b, h, t0 - kC, kC, p.dv);
     }
-    if (warp == kDecayWarp && more) dw.load(lg + (t0 - kC) * p.lst, p.lst, kC);
+    if (warp == kDkvDecayWarp && more) dw.load(lg + (t0 - kC) * p.lst, p.lst, kC);
     if (warp == kSumWarp) {
       if (c + 1 < c1) sums(c + 1);
       sums_load(c);
@@ -1589,30 +1606,30 @@ __global__ void __launch_bounds__(Dkv<E, D>::kThreads, Dkv<E, D>::kPerSm) dkv_ke
       st_wait();
     }
     sync();
-    if (ok && tid == 0) {
+    if (warp == 0 && elect_one() && ok) {
       product_ta<NL, NL, D>(tb + F::kDv, tb, op_mn<D>(G), false);
-      if (F::kE) product<1, 2, 128, D>(tb + F::kDv, op_k<D>(Ex), state_mn<D>(X), D / 16, true);
+      if (F::kE) product<1, 2, 128, D, D / 16>(tb + F::kDv, op_k<D>(Ex), state_mn<D>(X), true);
       product_ta<NL, NL, D>(tb + F::kDk, tb + F::kA1, op_mn<D>(Q), false);
       um::commit(&sm.bar);
     }
     wait();
-    if (ok && tid == 0) {
+    if (warp == 0 && elect_one() && ok) {
       if constexpr (F::kE) {  // in two halves of its columns: rows of dS
-        product<NL, 3, 128, 32>(tb, op_k<D>(V), state_k<D>(X), D / 16);
-        product<NL, 3, 128, 32>(tb + 224, op_k<D>(V), state_k<D>(X + 32 * 64), D / 16);
+        product<NL, 3, 128, 32, D / 16>(tb, op_k<D>(V), state_k<D>(X));
+        product<NL, 3, 128, 32, D / 16>(tb + 224, op_k<D>(V), state_k<D>(X + 32 * 64));
       } else {
-        product<NL, 3, 128, D>(tb, op_k<D>(K), state_mn<D>(X), D / 16);
-        product<NL, 3, 128, D>(tb + F::kIk, op_k<D>(V), state_k<D>(X), D / 16);
+        product<NL, 3, 128, D, D / 16>(tb, op_k<D>(K), state_mn<D>(X));
+        product<NL, 3, 128, D, D / 16>(tb + F::kIk, op_k<D>(V), state_k<D>(X));
       }
       um::commit(&sm.bar2);
     }
     auto scale = [&]() { scale_rows<NL, D, NT>(Q, lv, [&](int r) { return ex2(dec.ch[r] + dec.cl[r]); }); };
     auto sum_states = [&]() {
-      if (ok && tid == 0) {
+      if (warp == 0 && elect_one() && ok) {
         product_rows<NL, D>(tb + F::kU, lv, G, false);
         um::commit(&sm.bar);
       }
-      if (warp == kDecayWarp && more) dw.table<true>(dec);  // the table has been used
+      if (warp == kDkvDecayWarp && more) dw.table<true>(dec);  // the table has been used
     };
     if (ok) ok = mbar_wait(&sm.bar2, turn, &g_sticky_err, kPolls);
     um::fence_after();
