@@ -18,8 +18,8 @@
 // with R = D * Q K^T * dy V^T and dQ', dK' the state parts of dQ and dK: every
 // term is one whose span of decays holds token t.
 //
-// Decays. The sums are formed in base 2 and fp64 and kept as ch + cl, ch a
-// multiple of 2^-9 (exact differences in fp32) and cl the small rest, so that
+// Decays. The sums are formed in base 2 and kept as ch + cl, ch a multiple of
+// 2^-9 (exact sums and differences in fp32) and cl the small rest, so that
 // exp(c_i - c_j) is as good for two tokens late in a chunk of strong decays
 // as for the first two. A token's log2 decay is held to >= -128: 2^-128 is
 // below what fp32 keeps, so the state is wiped exactly (log_gamma = -inf, the
@@ -324,7 +324,9 @@ struct Decays {
   __device__ __forceinline__ float from(float h, float l, int t) const { return ex2((ch[t] - h) + (cl[t] - l)); }
 };
 
-// By one warp, four tokens to a lane, in fp64. Tokens from n on add nothing.
+// By one warp, four tokens to a lane. Tokens from n on add nothing. A token's log2
+// decay is split into a multiple of 2^-9, whose sums fp32 holds exactly, and the
+// rest, below 2^-10, whose sums stay below 1/8.
 struct DecayWarp {
   float lg[4];
   __device__ __forceinline__ void load(const float* p, long long st, int n) {
@@ -334,39 +336,54 @@ struct DecayWarp {
   }
   template <bool kStart>
   __device__ __forceinline__ void table(Decays& o) const {
+    constexpr float kLog2e = 1.44269502f, kLog2eLow = 1.92596299e-8f;  // their sum is log2(e) to 2^-49
     const int lane = threadIdx.x & 31;
-    double s[4];
-    double run = 0.0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      double v = (double)lg[i] * 1.4426950408889634;
-      if (v < (double)kMinLog2) v = (double)kMinLog2;
-      run += v;
-      s[i] = run;
-    }
-    double inc = run;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const double x = __shfl_up_sync(0xffffffffu, inc, d);
-      if (lane >= d) inc += x;
-    }
-    const double before = inc - run;
     float h[4], l[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const double c = before + s[i];
-      h[i] = rintf((float)c * 512.f) * (1.f / 512.f);
-      l[i] = (float)(c - (double)h[i]);
+      float v = lg[i] * kLog2e;
+      float rest = fmaf(lg[i], kLog2eLow, fmaf(lg[i], kLog2e, -v));
+      if (v < kMinLog2) v = kMinLog2, rest = 0.f;
+      h[i] = rintf(v * 512.f) * (1.f / 512.f);
+      l[i] = (v - h[i]) + rest;
+      if (i > 0) h[i] += h[i - 1], l[i] += l[i - 1];
     }
+    float ih = h[3], il = l[3];
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const float x = __shfl_up_sync(0xffffffffu, ih, d), y = __shfl_up_sync(0xffffffffu, il, d);
+      if (lane >= d) ih += x, il += y;
+    }
+    const float bh = ih - h[3], bl = il - l[3];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] += bh, l[i] += bl;
     const int edge = kStart ? lane & ~3 : lane | 3;
     const float eh = __shfl_sync(0xffffffffu, kStart ? h[0] : h[3], edge);
     const float el = __shfl_sync(0xffffffffu, kStart ? l[0] : l[3], edge);
+    float4 ch, cl, cf;
+    float *ph = &ch.x, *pl = &cl.x, *pf = &cf.x;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      o.ch[4 * lane + i] = h[i];
-      o.cl[4 * lane + i] = l[i];
-      o.cf[4 * lane + i] = kStart ? ex2((h[i] - eh) + (l[i] - el)) : ex2((eh - h[i]) + (el - l[i]));
+      ph[i] = h[i], pl[i] = l[i];
+      pf[i] = kStart ? ex2((h[i] - eh) + (l[i] - el)) : ex2((eh - h[i]) + (el - l[i]));
     }
+    *reinterpret_cast<float4*>(o.ch + 4 * lane) = ch;
+    *reinterpret_cast<float4*>(o.cl + 4 * lane) = cl;
+    *reinterpret_cast<float4*>(o.cf + 4 * lane) = cf;
+  }
+};
+
+// A sum as two fp32 numbers, the second what the first's roundings lost (Knuth).
+struct Two {
+  float s, e;
+  __device__ __forceinline__ void add(float x) {
+    const float t = s + x, b = t - s;
+    e += (s - (t - b)) + (x - b);
+    s = t;
+  }
+  __device__ __forceinline__ void add(const Two& o) {
+    add(o.s);
+    e += o.e;
   }
 };
 
@@ -701,7 +718,9 @@ constexpr int kDecayWarp = 4;  // builds the next chunk's table, during the prod
 template <typename E, int D>
 struct Sums {
   static constexpr int NL = kLevels<E>, kTileE = kC * D;
-  static constexpr size_t kSmem = kSmallBytes + 2 * (3 + NL) * (size_t)kTileE;
+  // bf16: two buffers, the next chunk's tiles on their way during this one
+  static constexpr int kBufs = NL == 1 ? 2 : 1;
+  static constexpr size_t kSmem = kSmallBytes + 2 * (NL == 1 ? 6 : 3 + NL) * (size_t)kTileE;
   static constexpr int kPerSm = (int)(228 * 1024 / (kSmem + 1024)) < 3 ? (int)(228 * 1024 / (kSmem + 1024)) : 3;
   static constexpr int kThreads = kPerSm == 1 ? 512 : 256;
 };
@@ -714,30 +733,37 @@ __global__ void __launch_bounds__(Sums<E, D>::kThreads, Sums<E, D>::kPerSm) stat
   constexpr int NL = kLevels<E>, kTileE = kC * D, NT = Sums<E, D>::kThreads;
   extern __shared__ __align__(1024) unsigned char smem[];
   Small& sm = *reinterpret_cast<Small*>(smem);
-  bf16* A = reinterpret_cast<bf16*>(smem + kSmallBytes);  // three levels (NL on arrival)
-  bf16* Bt = A + 3 * kTileE;
+  constexpr int kBufs = Sums<E, D>::kBufs;
+  // one buffer: three levels of rows (NL on arrival) and the other tile; two: rows, the
+  // other tiles, and the second and third levels
+  bf16* const tiles = reinterpret_cast<bf16*>(smem + kSmallBytes);
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const long long bh = blockIdx.x % p.BH;
   const int s = (int)(blockIdx.x / p.BH) + (kBwd ? p.r : 0);
   const int b = (int)(bh / p.H), h = (int)(bh % p.H);
   const float* lg = p.lg + b * p.lsb + h * p.lsh;
-  bf16* const lv[3] = {A, A + kTileE, A + 2 * kTileE};
-  const int c0 = s * p.ms, c1 = min(c0 + p.ms, p.nchunks), count = c1 - c0;
+  const int seg = s / p.r, c0 = seg * p.m + (s % p.r) * p.ms;
+  const int c1 = min(min(c0 + p.ms, (seg + 1) * p.m), p.nchunks), count = c1 - c0;
   const int first = kBwd ? c0 : c1 - 1, step = kBwd ? 1 : -1;
   auto rows = [&](int c) { return (int)min((long long)kC, p.T - (long long)c * kC); };
   const bool tma = NL == 1 && p.tma;
-  auto load = [&](int c) {  // by one thread
-    mbar_arrive_expect_tx(&sm.full[0], 2 * tile_bytes(D));
-    tma_load<D>(A, kBwd ? &p.mQ : &p.mK, (long long)c * kC, h, b, &sm.full[0]);
-    tma_load<D>(Bt, kBwd ? &p.mdy : &p.mV, (long long)c * kC, h, b, &sm.full[0]);
+  auto rows_tile = [&](int i) { return tiles + (kBufs == 2 ? (i & 1) : 0) * kTileE; };
+  auto other_tile = [&](int i) { return tiles + (kBufs == 2 ? 2 + (i & 1) : 3) * kTileE; };
+  auto load = [&](int i) {  // the part's i-th chunk, by one thread
+    const long long t0 = (long long)(first + i * step) * kC;
+    uint64_t* full = &sm.full[i & 1];
+    mbar_arrive_expect_tx(full, 2 * tile_bytes(D));
+    tma_load<D>(rows_tile(i), kBwd ? &p.mQ : &p.mK, t0, h, b, full);
+    tma_load<D>(other_tile(i), kBwd ? &p.mdy : &p.mV, t0, h, b, full);
   };
 
   if (warp == 0) um::alloc(&sm.tbase, D);
   if (tid == 0) {
     mbar_init(&sm.bar, 1);
     mbar_init(&sm.full[0], 1);
+    mbar_init(&sm.full[1], 1);
     mbar_fence_init();
-    if (tma && count > 0) load(first);
+    if (tma && count > 0) load(0);
   }
   bool ok = true;
   auto sync = [&]() {
@@ -754,22 +780,26 @@ __global__ void __launch_bounds__(Sums<E, D>::kThreads, Sums<E, D>::kPerSm) stat
     dw.table<false>(sm.dec);
   }
   sync();
-  double run = 0.0;  // log2 decay of the chunks already summed
+  Two run{0.f, 0.f};  // log2 decay of the chunks already summed
   for (int i = 0, c = first; i < count; ++i, c += step) {
     const bool more = i + 1 < count;
+    bf16 *const A = rows_tile(i), *const Bt = other_tile(i);
+    bf16* const lv[3] = {A, kBufs == 2 ? tiles + 4 * kTileE : A + kTileE,
+                         kBufs == 2 ? tiles + 5 * kTileE : A + 2 * kTileE};
     if (tma) {
-      if (ok) ok = mbar_wait(&sm.full[0], i & 1, &g_sticky_err, kPolls);
+      if (ok && tid == 0 && more) load(i + 1);  // the products of i - 1 are done
+      if (ok) ok = mbar_wait(&sm.full[i & 1], (i >> 1) & 1, &g_sticky_err, kPolls);
     } else {
       load_tile<E, D, NT>(A, kBwd ? p.Q : p.K, b, h, (long long)c * kC, rows(c), p.dk);
       load_tile<E, D, NT>(Bt, kBwd ? p.dy : p.V, b, h, (long long)c * kC, rows(c), p.dv);
     }
     if (warp == kDecayWarp && more) dw.load(lg + (long long)(c + step) * kC * p.lst, p.lst, rows(c + step));
-    const float rh = (float)run, th = sm.dec.ch[kC - 1], tl = sm.dec.cl[kC - 1];
+    const float rh = run.s, rl = run.e, th = sm.dec.ch[kC - 1], tl = sm.dec.cl[kC - 1];
     scale_rows<NL, D, NT>(A, lv, [&](int r) {  // a thread's own items, in place
       const Decays& d = sm.dec;
-      return kBwd ? ex2((d.ch[r] + rh) + d.cl[r]) : ex2(((th - d.ch[r]) + rh) + (tl - d.cl[r]));
+      return kBwd ? ex2((d.ch[r] + rh) + (d.cl[r] + rl)) : ex2(((th - d.ch[r]) + rh) + ((tl - d.cl[r]) + rl));
     });
-    run += (double)th + (double)tl;
+    run.add(th), run.add(tl);
     sync();
     if (warp == 0 && elect_one() && ok) {
       product_rows<NL, D>(sm.tbase, lv, Bt, false);
@@ -778,14 +808,13 @@ __global__ void __launch_bounds__(Sums<E, D>::kThreads, Sums<E, D>::kPerSm) stat
     if (warp == kDecayWarp && more) dw.table<false>(sm.dec);
     if (ok) ok = mbar_wait(&sm.bar, i & 1, &g_sticky_err, kPolls);
     um::fence_after();
-    if (tma && ok && tid == 0 && more) load(c + step);
     st.update(1.f, sm.tbase, 0);  // in registers: round to nearest
     sync();                       // the next table; the sum has been read
   }
   // forward: the state that enters part s + 1; backward: the gradient that leaves s - 1
   if (ok) {
     st.store_own(p.seg + (bh * p.nsub + s + (kBwd ? -1 : 1)) * (D * D));
-    if (tid == 0) p.segl[bh * p.nsub + s] = (float)run;
+    if (tid == 0) p.segl[bh * p.nsub + s] = run.s + run.e;
   }
   um::fence_before();
   __syncthreads();
@@ -810,14 +839,28 @@ __global__ void __launch_bounds__(256) scan_kernel(float* seg, const float* segl
     x[i] = init && row < dk && col + i < dv ? init[bh * sbh + row * sld + col + i] : 0.f;
   float4* sp = reinterpret_cast<float4*>(seg + bh * nsub * (long long)(D * D)) + e;
   const float* lp = segl + bh * nsub;
-#pragma unroll 4
-  for (int i = 0; i < steps; ++i) {
-    const int s = kBwd ? nsub - 1 - i : i, to = kBwd ? s - 1 : s + 1;
-    const float f = ex2(lp[s]);
-    float4 u = sp[(long long)to * (D * D / 4)];
-    x[0] = fmaf(f, x[0], u.x), x[1] = fmaf(f, x[1], u.y);
-    x[2] = fmaf(f, x[2], u.z), x[3] = fmaf(f, x[3], u.w);
-    sp[(long long)to * (D * D / 4)] = make_float4(x[0], x[1], x[2], x[3]);
+  constexpr int kN = 8;  // loads on their way together
+  for (int i0 = 0; i0 < steps; i0 += kN) {
+    float4 u[kN];
+    float f[kN];
+#pragma unroll
+    for (int k = 0; k < kN; ++k) {
+      const int i = i0 + k, s = kBwd ? nsub - 1 - i : i, to = kBwd ? s - 1 : s + 1;
+      if (i < steps) {
+        f[k] = lp[s];
+        u[k] = sp[(long long)to * (D * D / 4)];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kN; ++k) {
+      const int i = i0 + k, s = kBwd ? nsub - 1 - i : i, to = kBwd ? s - 1 : s + 1;
+      if (i < steps) {
+        const float e = ex2(f[k]);
+        x[0] = fmaf(e, x[0], u[k].x), x[1] = fmaf(e, x[1], u[k].y);
+        x[2] = fmaf(e, x[2], u[k].z), x[3] = fmaf(e, x[3], u[k].w);
+        sp[(long long)to * (D * D / 4)] = make_float4(x[0], x[1], x[2], x[3]);
+      }
+    }
   }
 }
 
@@ -1459,12 +1502,12 @@ __global__ void __launch_bounds__(Dkv<E, D>::kThreads, Dkv<E, D>::kPerSm) dkv_ke
     um::fence_after();
   };
   sync();
-  double Fend = 0.0;  // kSumWarp: <S, dS> at the end of the chunk being summed
+  Two Fend{0.f, 0.f};  // kSumWarp: <S, dS> at the end of the chunk being summed
   float tq[4], lgs[4], aqs = 0.f;
   if (warp == kSumWarp)
-    for (int i = 0; i < NT / 32; ++i) Fend += (double)sm.red[i];
+    for (int i = 0; i < NT / 32; ++i) Fend.add(sm.red[i]);
   // What chunk c's dlog_gamma needs from memory, and its sums once sm.a is complete:
-  // four tokens to a lane, from the end, in fp64.
+  // four tokens to a lane, from the end.
   auto sums_load = [&](int c) {
     const long long t0 = (long long)c * kC;
     const int n = rows(c);
@@ -1479,32 +1522,35 @@ __global__ void __launch_bounds__(Dkv<E, D>::kThreads, Dkv<E, D>::kPerSm) dkv_ke
   auto sums = [&](int c) {
     const long long t0 = (long long)c * kC;
     const int n = rows(c);
-    double v[4], run = 0.0;
+    const float4 a0 = *reinterpret_cast<const float4*>(sm.a[0] + 4 * lane);
+    const float4 a1 = *reinterpret_cast<const float4*>(sm.a[1] + 4 * lane);
+    const float *p0 = &a0.x, *p1 = &a1.x;
+    Two v[4], run{0.f, 0.f};
 #pragma unroll
     for (int i = 3; i >= 0; --i) {
-      const int t = 4 * lane + i;
-      run += (double)tq[i] + (double)sm.a[0][t] + (double)sm.a[1][t];
+      run.add(tq[i]), run.add(p0[i]), run.add(p1[i]);
       v[i] = run;
     }
-    double inc = run;
+    Two inc = run;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const double x = __shfl_down_sync(0xffffffffu, inc, o);
-      if (lane + o < 32) inc += x;
+      const Two x{__shfl_down_sync(0xffffffffu, inc.s, o), __shfl_down_sync(0xffffffffu, inc.e, o)};
+      if (lane + o < 32) inc.add(x);
     }
-    const double rest = inc - run + Fend;
+    inc.add(Two{-run.s, -run.e});  // the lanes after this one
+    inc.add(Fend);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int t = 4 * lane + i;
       if (t < n && ok) {
         float* o = p.dlg + bh * p.T + t0 + t;
-        const double all = v[i] + rest + (p.dlg_add ? (double)*o : 0.0);
-        *o = lgs[i] * 1.4426950408889634f <= kMinLog2 ? 0.f : (float)all;
+        v[i].add(inc);
+        if (p.dlg_add) v[i].add(*o);
+        *o = lgs[i] * 1.4426950408889634f <= kMinLog2 ? 0.f : v[i].s + v[i].e;
       }
     }
-    double bk = 0.0;
-    for (int i = 0; i < NT / 32; ++i) bk += (double)sm.red2[i];
-    Fend += (double)aqs - bk;
+    Fend.add(aqs);
+    for (int i = 0; i < NT / 32; ++i) Fend.add(-sm.red2[i]);
   };
   const int row = 32 * q + lane;
   for (int c = c1 - 1; c >= c0; --c) {
@@ -1764,8 +1810,9 @@ int sm_count() {
 }
 
 // Segments: as many as there are places for CTAs of the main kernel, whole
-// chunks to each. For the state sums, whose CTAs are smaller, segments split
-// again while the parts have places.
+// chunks to each. For the state sums, which go through a chunk in less time than
+// they take to fill the SMs evenly, segments split again, for some waves of CTAs.
+constexpr int kSumsWaves = 2;
 Plan plan_for(long long BH, long long T, int D, int per_sm, int sums_per_sm) {
   Plan pl{};
   pl.D = D;
@@ -1777,10 +1824,11 @@ Plan plan_for(long long BH, long long T, int D, int per_sm, int sums_per_sm) {
   pl.nseg = (pl.nchunks + pl.m - 1) / pl.m;
   pl.ms = pl.m, pl.r = 1, pl.nsub = pl.nseg;
   if (pl.nseg > 1) {
-    long long r = (long long)sm_count() * sums_per_sm / (BH * (pl.nseg - 1));
+    const long long ctas = BH * (pl.nseg - 1);
+    long long r = (kSumsWaves * (long long)sm_count() * sums_per_sm + ctas / 2) / ctas;
     r = r < 1 ? 1 : r > pl.m ? pl.m : r;
-    while (pl.m % r) --r;  // equal parts, so that segments begin where parts do
-    pl.r = (int)r, pl.ms = pl.m / pl.r, pl.nsub = pl.nseg * pl.r;
+    pl.ms = (int)((pl.m + r - 1) / r);
+    pl.r = (pl.m + pl.ms - 1) / pl.ms, pl.nsub = pl.nseg * pl.r;
   }
   return pl;
 }
