@@ -19,6 +19,8 @@
 // the forward. Sums over rows stay in the threads' registers while a CTA walks
 // its rows, then go through shared memory to one partial row per CTA and, in
 // order, to the result: the same bits on every run.
+#include <utility>
+
 #include "common.cuh"
 
 namespace mgs {
@@ -36,37 +38,44 @@ struct Args {
   long long ldx, ldres, ldgate, lddy, lddh;  // row strides of the inputs; outputs are dense
   long long rows;
   int D, G, n, tpg, gpc, rpc;  // threads to a group, groups and rows to a CTA
-  int rms;
+  int rms, w32;  // weights in fp32
   float eps;
 };
 
-// A thread's K vectors of VEC elements, tpg vectors apart, as fp32; zeros from
-// column n on. One loop of loads and nothing else, so that they are all under
-// way before the first is used.
+// A thread's K vectors of VEC elements, tpg vectors apart, zeros from column n on:
+// loaded in one go, a row ahead of their use, and widened then.
 template <typename T, int VEC, int K>
-__device__ __forceinline__ void ldrow(const void* p, long long i, int t, int tpg, int n, float (&v)[K * VEC]) {
-  const T* q = static_cast<const T*>(p) + i + t * VEC;
-  constexpr int kBytes = VEC * (int)sizeof(T);
-  using U = std::conditional_t<VEC == 1, T, uint4>;
-  constexpr int kN = VEC == 1 ? 1 : kBytes / 16;
-  U raw[K][kN];
+struct Raw {
+  static constexpr int kN = VEC == 1 ? 1 : VEC * (int)sizeof(T) / 16;
+  std::conditional_t<VEC == 1, T, uint4> r[K][kN];
+  __device__ __forceinline__ void load(const void* p, long long i, int t, int tpg, int n) {
+    const T* q = static_cast<const T*>(p) + i + t * VEC;
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const bool in = (k * tpg + t) * VEC < n;
+    for (int k = 0; k < K; ++k) {
+      const bool in = (k * tpg + t) * VEC < n;
 #pragma unroll
-    for (int j = 0; j < kN; ++j) {
-      if constexpr (VEC == 1)
-        raw[k][j] = in ? q[k * tpg] : from_f32<T>(0.f);
-      else
-        raw[k][j] = in ? __ldg(reinterpret_cast<const uint4*>(q + k * tpg * VEC) + j) : make_uint4(0, 0, 0, 0);
+      for (int j = 0; j < kN; ++j) {
+        if constexpr (VEC == 1)
+          r[k][j] = in ? q[k * tpg] : from_f32<T>(0.f);
+        else
+          r[k][j] = in ? __ldg(reinterpret_cast<const uint4*>(q + k * tpg * VEC) + j) : make_uint4(0, 0, 0, 0);
+      }
     }
   }
+  __device__ __forceinline__ void get(float (&v)[K * VEC]) const {
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const T* e = reinterpret_cast<const T*>(raw[k]);
+    for (int k = 0; k < K; ++k) {
+      const T* e = reinterpret_cast<const T*>(r[k]);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) v[k * VEC + j] = to_f32<T>(e[j]);
+      for (int j = 0; j < VEC; ++j) v[k * VEC + j] = to_f32<T>(e[j]);
+    }
   }
+};
+template <typename T, int VEC, int K>
+__device__ __forceinline__ void ldrow(const void* p, long long i, int t, int tpg, int n, float (&v)[K * VEC]) {
+  Raw<T, VEC, K> r;
+  r.load(p, i, t, tpg, n);
+  r.get(v);
 }
 template <typename T, int VEC, int K>
 __device__ __forceinline__ void strow(void* p, long long i, int t, int tpg, int n, const float (&v)[K * VEC]) {
@@ -88,7 +97,8 @@ __device__ __forceinline__ void strow(void* p, long long i, int t, int tpg, int 
 
 // Sums over the tpg threads of a group: a segment of a warp, or whole warps
 // that meet at a named barrier of the group's own. `buf` alternates, so that
-// one barrier is enough for each sum.
+// one barrier is enough for each sum. What the threads wrote to shared memory
+// before is visible to the group after.
 struct Reduce {
   float2 (*red)[32];
   int tpg, slot, buf;
@@ -103,21 +113,25 @@ struct Reduce {
   __device__ __forceinline__ float2 operator()(float a, float b) {
     const int lane = threadIdx.x & 31;
     if (tpg == 8) {
+      __syncwarp(0xffu << (lane & 24));
       lanes<8>(0xffu << (lane & 24), a, b);
     } else if (tpg == 16) {
+      __syncwarp(0xffffu << (lane & 16));
       lanes<16>(0xffffu << (lane & 16), a, b);
     } else {
+      __syncwarp();
       lanes<32>(0xffffffffu, a, b);
       if (tpg > 32) {
         const int nw = tpg / 32, w0 = slot * nw;
         if (lane == 0) red[buf][threadIdx.x >> 5] = make_float2(a, b);
         named_bar(1 + slot, tpg);
-        a = b = 0.f;
-        for (int w = 0; w < nw; ++w) {
-          const float2 f = red[buf][w0 + w];
-          a += f.x;
-          b += f.y;
-        }
+        const float2 f = lane < nw ? red[buf][w0 + lane] : make_float2(0.f, 0.f);
+        a = f.x, b = f.y;
+        if (nw <= 4)
+          lanes<4>(0xffffffffu, a, b);
+        else
+          lanes<32>(0xffffffffu, a, b);
+        a = __shfl_sync(0xffffffffu, a, 0), b = __shfl_sync(0xffffffffu, b, 0);
         buf ^= 1;
       }
     }
@@ -151,6 +165,9 @@ struct Place {
 // way, 1024 threads' worth forward and 768 backward.
 constexpr int fwd_ctas(int threads) { return 1024 / threads; }
 constexpr int bwd_ctas(int threads) { return threads == 256 ? 3 : 1; }
+// Odd rows, a row ahead in registers as well: 80 registers, up to 128 backward.
+constexpr int odd_fwd_ctas(int threads) { return threads == 256 ? 3 : threads == 384 ? 2 : 1; }
+constexpr int odd_bwd_ctas(int threads) { return threads == 256 ? 2 : 1; }
 
 template <typename E, typename W, int VEC, int K, int MAXT>
 __global__ void __launch_bounds__(MAXT, fwd_ctas(MAXT)) fwd_kernel(const Args p) {
@@ -162,12 +179,32 @@ __global__ void __launch_bounds__(MAXT, fwd_ctas(MAXT)) fwd_kernel(const Args p)
   const float inv_n = 1.f / (float)p.n;
   const int col = at.g * p.n;
   auto in = [&](int i) { return ((i / VEC) * p.tpg + at.t) * VEC < p.n; };
-  for (long long row = (long long)blockIdx.x * p.rpc + at.rs; row < p.rows;
-       row += (long long)gridDim.x * p.rpc) {
+  const long long step = (long long)gridDim.x * p.rpc;
+  Raw<E, VEC, K> rx, ra;  // x, and the residual or else the gate, of the next row where there is room
+  constexpr bool kAhead = K == 1;  // 16 values to a thread leave no registers for it
+  auto fetch = [&](long long row) {
+    if (row >= p.rows) return;
+    rx.load(p.x, row * p.ldx + col, at.t, p.tpg, p.n);
+    if (p.res)
+      ra.load(p.res, row * p.ldres + col, at.t, p.tpg, p.n);
+    else if (p.gate)
+      ra.load(p.gate, row * p.ldgate + col, at.t, p.tpg, p.n);
+  };
+  if (kAhead) fetch((long long)blockIdx.x * p.rpc + at.rs);
+  for (long long row = (long long)blockIdx.x * p.rpc + at.rs; row < p.rows; row += step) {
     float h[N], a[N], w[N];
-    ldrow<E, VEC, K>(p.x, row * p.ldx + col, at.t, p.tpg, p.n, h);
+    if constexpr (kAhead) {
+      rx.get(h);
+      ra.get(a);
+      fetch(row + step);
+    } else {
+      ldrow<E, VEC, K>(p.x, row * p.ldx + col, at.t, p.tpg, p.n, h);
+      if (p.res)
+        ldrow<E, VEC, K>(p.res, row * p.ldres + col, at.t, p.tpg, p.n, a);
+      else if (p.gate)
+        ldrow<E, VEC, K>(p.gate, row * p.ldgate + col, at.t, p.tpg, p.n, a);
+    }
     if (p.res) {
-      ldrow<E, VEC, K>(p.res, row * p.ldres + col, at.t, p.tpg, p.n, a);
       if (p.s) {
         ldrow<W, VEC, K>(p.s, col, at.t, p.tpg, p.n, w);
 #pragma unroll
@@ -177,7 +214,7 @@ __global__ void __launch_bounds__(MAXT, fwd_ctas(MAXT)) fwd_kernel(const Args p)
         for (int i = 0; i < N; ++i) h[i] += a[i];
       }
     }
-    if (p.gate) ldrow<E, VEC, K>(p.gate, row * p.ldgate + col, at.t, p.tpg, p.n, a);
+    if (p.res && p.gate) ldrow<E, VEC, K>(p.gate, row * p.ldgate + col, at.t, p.tpg, p.n, a);
     ldrow<W, VEC, K>(p.w, col, at.t, p.tpg, p.n, w);
     float acc = 0.f;
 #pragma unroll
@@ -335,6 +372,345 @@ __global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT)) bwd_kernel(const Args p)
   }
 }
 
+// ------------------------------------------------------------ odd rows --
+//
+// Rows that do not start on 16 bytes (an odd D). Element by element they cost a
+// memory instruction for every 32 elements of every tensor, which is what bounds
+// them; but rows of all tensors lie the same way, so a thread takes the 16-byte
+// vectors of memory, from the one that the group's first element is in, and only
+// what goes by column -- weights in, their gradients' sums -- is shifted with the
+// row: these are fp32 in shared memory, column c in plane c % V, so that a warp's
+// access to one element of its vectors is to consecutive words.
+
+template <int V>
+struct Planes {
+  int len;  // every column that a thread's vectors can hold, and the vector before: zeros outside
+  __host__ __device__ explicit Planes(int vectors) : len(vectors + 2) {}
+  __host__ __device__ int size() const { return V * len; }
+  __device__ __forceinline__ int at(int c) const {  // c >= -V
+    return (c & (V - 1)) * len + ((c + V) / V);
+  }
+};
+
+// Where a thread's K vectors lie in a row whose first element is `sh` past the
+// aligned one: columns, the places in the planes, and whether all its vectors are
+// inside the group (most threads') or need a look at each element.
+template <int V, int K>
+struct OddRow {
+  int sh, n, t, tpg;
+  int off[V];  // element i of vector 0, in the planes
+  bool edge;
+  __device__ __forceinline__ OddRow(const Planes<V>& pl, int sh_, int n_, int t_, int tpg_)
+      : sh(sh_), n(n_), t(t_), tpg(tpg_) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) off[i] = ((i - sh) & (V - 1)) * pl.len + ((i - sh + V) / V) + t;
+    edge = t * V < sh || ((K - 1) * tpg + t + 1) * V > sh + n;
+  }
+  __device__ __forceinline__ int plane(int i) const { return off[i % V] + (i / V) * tpg; }
+  __device__ __forceinline__ bool in(int i) const {
+    return (unsigned)(((i / V) * tpg + t) * V + i % V - sh) < (unsigned)n;
+  }
+  // f(i) for the thread's elements inside the group, where zeros will not do
+  template <class F>
+  __device__ __forceinline__ void each(F&& f) const {
+    if (!edge) {
+#pragma unroll
+      for (int i = 0; i < K * V; ++i) f(i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < K * V; ++i)
+        if (in(i)) f(i);
+    }
+  }
+  // The vectors of one tensor whose group starts at element `start`: loaded whole,
+  // the neighbours' elements in them too, where another row follows; and as values,
+  // zeros outside the group.
+  template <typename T>
+  __device__ __forceinline__ static void load(const void* p, long long start, bool last, int sh, int n, int t,
+                                              int tpg, uint4 (&raw)[K]) {
+    const T* q = static_cast<const T*>(p) + (start - sh) + t * V;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int pos = (k * tpg + t) * V;
+      raw[k] = make_uint4(0, 0, 0, 0);
+      if (pos < sh + n) {
+        if (!last || pos + V <= sh + n) {
+          raw[k] = __ldg(reinterpret_cast<const uint4*>(q + k * tpg * V));
+        } else {
+          T e[V];
+#pragma unroll
+          for (int i = 0; i < V; ++i) e[i] = pos + i < sh + n ? q[k * tpg * V + i] : from_f32<T>(0.f);
+          raw[k] = *reinterpret_cast<const uint4*>(e);
+        }
+      }
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ void get(const uint4 (&raw)[K], float (&v)[K * V]) const {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const T* e = reinterpret_cast<const T*>(&raw[k]);
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[k * V + i] = to_f32<T>(e[i]);
+    }
+    if (edge) {
+#pragma unroll
+      for (int i = 0; i < K * V; ++i)
+        if (!in(i)) v[i] = 0.f;
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ void store(void* p, long long start, const float (&v)[K * V]) const {
+    T* q = static_cast<T*>(p) + (start - sh) + t * V;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * tpg + t) * V - sh;
+      uint4 u;
+      T* e = reinterpret_cast<T*>(&u);
+#pragma unroll
+      for (int i = 0; i < V; ++i) e[i] = from_f32<T>(v[k * V + i]);
+      if (c >= 0 && c + V <= n) {
+        *reinterpret_cast<uint4*>(q + k * tpg * V) = u;
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if ((unsigned)(c + i) < (unsigned)n) q[k * tpg * V + i] = e[i];
+      }
+    }
+  }
+};
+
+// The CTA's groups' columns of a weight as planes, one group after the other.
+template <typename E, int V>
+__device__ __forceinline__ void stage_planes(float* o, const void* w, const Args& p, const Planes<V>& pl) {
+  const int first = blockIdx.y * p.gpc;
+  for (int i = threadIdx.x; i < p.gpc * pl.size(); i += blockDim.x) o[i] = 0.f;
+  __syncthreads();
+  for (int i = threadIdx.x; i < p.gpc * p.n; i += blockDim.x) {
+    const int g = i / p.n, c = i % p.n;
+    const long long e = (long long)(first + g) * p.n + c;
+    if (first + g < p.G)
+      o[g * pl.size() + pl.at(c)] = p.w32 ? static_cast<const float*>(w)[e] : to_f32<E>(static_cast<const E*>(w)[e]);
+  }
+}
+
+template <typename E, int K, int MAXT>
+__global__ void __launch_bounds__(MAXT, odd_fwd_ctas(MAXT)) fwd_odd_kernel(const Args p) {
+  constexpr int V = 16 / (int)sizeof(E), N = K * V;
+  __shared__ float2 red[2][32];
+  extern __shared__ float cols[];
+  const Planes<V> pl(K * p.tpg);
+  const Place at(p);
+  const int width = p.gpc * pl.size(), g0 = (at.slot % p.gpc) * pl.size();
+  float *w = cols, *b = w + width, *sc = b + (p.b ? width : 0);
+  stage_planes<E, V>(w, p.w, p, pl);
+  if (p.b) stage_planes<E, V>(b, p.b, p, pl);
+  if (p.s) stage_planes<E, V>(sc, p.s, p, pl);
+  __syncthreads();
+  if (!at.on) return;
+  w += g0, b += g0, sc += g0;
+  Reduce sum{red, p.tpg, at.slot, 0};
+  const float inv_n = 1.f / (float)p.n;
+  const int col = at.g * p.n;
+  const long long step = (long long)gridDim.x * p.rpc;
+  using R = OddRow<V, K>;
+  auto shift = [&](long long row) { return (int)((row * p.ldx + col) & (V - 1)); };
+  uint4 rx[K], ra[K];  // of the next row: x, and the residual or else the gate
+  auto ahead = [&](long long row) {
+    if (row >= p.rows) return;
+    const bool last = row + 1 == p.rows;
+    const int sh = shift(row);
+    R::template load<E>(p.x, row * p.ldx + col, last, sh, p.n, at.t, p.tpg, rx);
+    if (p.res)
+      R::template load<E>(p.res, row * p.ldres + col, last, sh, p.n, at.t, p.tpg, ra);
+    else if (p.gate)
+      R::template load<E>(p.gate, row * p.ldgate + col, last, sh, p.n, at.t, p.tpg, ra);
+  };
+  ahead((long long)blockIdx.x * p.rpc + at.rs);
+  for (long long row = (long long)blockIdx.x * p.rpc + at.rs; row < p.rows; row += step) {
+    const R at_row(pl, shift(row), p.n, at.t, p.tpg);
+    float h[N], a[N];
+    at_row.template get<E>(rx, h);
+    at_row.template get<E>(ra, a);
+    ahead(row + step);
+    if (p.s) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) h[i] = fmaf(sc[at_row.plane(i)], h[i], a[i]);
+    } else if (p.res) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) h[i] += a[i];
+    }
+    if (p.res && p.gate) {
+      uint4 rg[K];
+      R::template load<E>(p.gate, row * p.ldgate + col, row + 1 == p.rows, at_row.sh, p.n, at.t, p.tpg, rg);
+      at_row.template get<E>(rg, a);
+    }
+    float acc = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc += h[i];
+    const float mean = p.rms ? 0.f : sum(acc, 0.f).x * inv_n;
+    float sq = 0.f, rs = 0.f;
+    at_row.each([&](int i) {
+      const float d = h[i] - mean;
+      sq = fmaf(d, d, sq);
+      rs += d;
+    });
+    const float2 m = sum(sq, rs);
+    const float rest = p.rms ? 0.f : m.y * inv_n;
+    const float r = inv_sqrt(fmaxf(fmaf(-rest, rest, m.x * inv_n), 0.f) + p.eps);
+    if (p.stats && at.t == 0) {
+      float* st = p.stats + (row * p.G + at.g) * 3;
+      st[0] = mean, st[1] = rest, st[2] = r;
+    }
+    const long long o = row * p.D + col;
+    if (p.h) at_row.template store<E>(p.h, o, h);
+#pragma unroll
+    for (int i = 0; i < N; ++i) h[i] = ((h[i] - mean) - rest) * r * w[at_row.plane(i)];
+    if (p.b) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) h[i] += b[at_row.plane(i)];
+    }
+    if (p.gate) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) h[i] *= a[i] * sigm(a[i]);
+    }
+    at_row.template store<E>(p.y, o, h);
+  }
+}
+
+template <typename E, int K, int MAXT, bool GATE, bool SCALE>
+__global__ void __launch_bounds__(MAXT, odd_bwd_ctas(MAXT)) bwd_odd_kernel(const Args p) {
+  constexpr int V = 16 / (int)sizeof(E), N = K * V;
+  __shared__ float2 red[2][32];
+  extern __shared__ float cols[];
+  const Planes<V> pl(K * p.tpg);
+  const Place at(p);
+  const int width = p.gpc * pl.size(), g0 = (at.slot % p.gpc) * pl.size(), all = p.rpc * width;
+  float *w = cols, *b = w + width, *sc = b + (p.b ? width : 0), *gw = sc + (SCALE ? width : 0);
+  float *gb = gw + all, *gs = gb + (p.b ? all : 0);
+  stage_planes<E, V>(w, p.w, p, pl);
+  if (p.b) stage_planes<E, V>(b, p.b, p, pl);
+  if (SCALE) stage_planes<E, V>(sc, p.s, p, pl);
+  for (int i = threadIdx.x; i < all * (1 + (p.b ? 1 : 0) + SCALE); i += blockDim.x) gw[i] = 0.f;
+  __syncthreads();
+  if (at.on) {
+    const float *ws = w + g0, *bs = b + g0, *ss = sc + g0;
+    const int mine = at.rs * width + g0;
+    Reduce sum{red, p.tpg, at.slot, 0};
+    const float inv_n = 1.f / (float)p.n;
+    const int col = at.g * p.n;
+    const long long step = (long long)gridDim.x * p.rpc;
+    using R = OddRow<V, K>;
+    auto shift = [&](long long row) { return (int)((row * p.ldx + col) & (V - 1)); };
+    uint4 rx[K], rd[K], ra[K], rh[K];  // of the next row: x, dy, the gate or else the residual, dh
+    float stats[3];
+    auto ahead = [&](long long row) {
+      if (row >= p.rows) return;
+      const bool last = row + 1 == p.rows;
+      const int sh = shift(row);
+      R::template load<E>(p.x, row * p.ldx + col, last, sh, p.n, at.t, p.tpg, rx);
+      R::template load<E>(p.dy, row * p.lddy + col, last, sh, p.n, at.t, p.tpg, rd);
+      if (GATE)
+        R::template load<E>(p.gate, row * p.ldgate + col, last, sh, p.n, at.t, p.tpg, ra);
+      else if (SCALE || p.res)
+        R::template load<E>(p.res, row * p.ldres + col, last, sh, p.n, at.t, p.tpg, ra);
+      if (p.dh) R::template load<E>(p.dh, row * p.lddh + col, last, sh, p.n, at.t, p.tpg, rh);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) stats[i] = p.stats[(row * p.G + at.g) * 3 + i];
+    };
+    ahead((long long)blockIdx.x * p.rpc + at.rs);
+    for (long long row = (long long)blockIdx.x * p.rpc + at.rs; row < p.rows; row += step) {
+      const R at_row(pl, shift(row), p.n, at.t, p.tpg);
+      const long long o = row * p.D + col;
+      float x[N], d[N], z[N], g[GATE ? N : 1], hh[N];
+      at_row.template get<E>(rx, x);
+      at_row.template get<E>(rd, d);
+      if constexpr (GATE)
+        at_row.template get<E>(ra, g);
+      else
+        at_row.template get<E>(ra, z);
+      uint4 keep[K];  // dh, until it is wanted
+#pragma unroll
+      for (int k = 0; k < K; ++k) keep[k] = rh[k];
+      const float mean = stats[0], rest = stats[1], r = stats[2];
+      ahead(row + step);
+      if (SCALE || p.res) {
+        if (GATE) {
+          uint4 rr[K];
+          R::template load<E>(p.res, row * p.ldres + col, row + 1 == p.rows, at_row.sh, p.n, at.t, p.tpg, rr);
+          at_row.template get<E>(rr, z);
+        }
+        if constexpr (SCALE) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) z[i] = fmaf(ss[at_row.plane(i)], x[i], z[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < N; ++i) z[i] += x[i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) z[i] = x[i];
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i) z[i] = ((z[i] - mean) - rest) * r;
+      if constexpr (GATE) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int e = at_row.plane(i);
+          const float sg = sigm(g[i]), a = fmaf(z[i], ws[e], p.b ? bs[e] : 0.f), dd = d[i];
+          d[i] = dd * g[i] * sg;
+          g[i] = dd * a * sg * fmaf(g[i], 1.f - sg, 1.f);
+        }
+        at_row.template store<E>(p.dgate, o, g);
+      }
+      float s1 = 0.f, s2 = 0.f;
+      float *gwr = gw + mine, *gbr = gb + mine, *gsr = gs + mine;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {  // outside the group d and the weights are zeros
+        const int e = at_row.plane(i);
+        gwr[e] = fmaf(d[i], z[i], gwr[e]);
+        if (p.b) gbr[e] += d[i];
+        d[i] *= ws[e];
+        s1 += d[i];
+        s2 = fmaf(d[i], z[i], s2);
+      }
+      const float2 m = sum(s1, s2);
+      const float m1 = p.rms ? 0.f : m.x * inv_n, m2 = m.y * inv_n;
+#pragma unroll
+      for (int i = 0; i < N; ++i) d[i] = r * (d[i] - m1 - z[i] * m2);
+      if (p.dh) {
+        at_row.template get<E>(keep, hh);
+#pragma unroll
+        for (int i = 0; i < N; ++i) d[i] += hh[i];
+      }
+      if constexpr (SCALE) {
+        at_row.template store<E>(p.dres, o, d);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int e = at_row.plane(i);
+          gsr[e] = fmaf(d[i], x[i], gsr[e]);
+          d[i] *= ss[e];
+        }
+      }
+      at_row.template store<E>(p.dx, o, d);
+    }
+  }
+  // the CTA's rows: one partial row of each sum
+  __syncthreads();
+  const int first = blockIdx.y * p.gpc;
+  for (int q = 0; q < 2 + SCALE; ++q) {
+    if (q == 1 && !p.b) continue;
+    const float* s = q == 0 ? gw : q == 1 ? gb : gs;
+    for (int i = threadIdx.x; i < p.gpc * p.n; i += blockDim.x) {
+      const int g = i / p.n, c = i % p.n;
+      if (first + g >= p.G) break;
+      float a = 0.f;
+      for (int k = 0; k < p.rpc; ++k) a += s[k * width + g * pl.size() + pl.at(c)];
+      p.part[((long long)q * gridDim.x + blockIdx.x) * p.D + (first + g) * p.n + c] = a;
+    }
+  }
+}
+
 // Partial rows -> dweight, dbias, dscale (blockIdx.y), 32 columns to a CTA.
 template <typename W>
 __global__ void __launch_bounds__(1024) sum_kernel(const float* part, W* dw, W* db, W* ds, int n, int D) {
@@ -364,9 +740,13 @@ int sm_count() {
   return n;
 }
 
+enum Way { kElements, kVectors, kOdd };  // how rows are read
+
 struct Plan {
+  Way way;
   int vec, k, tpg, gpc, rpc, threads;
   unsigned gx, gy;
+  size_t odd_smem;
 };
 
 // Threads to a group: as few as hold it at `values` each (a row's sums then need
@@ -374,12 +754,14 @@ struct Plan {
 // groups side by side in a CTA as they lie in a row. 16 values forward; 8
 // backward, which keeps seven arrays of them in registers, while a CTA of 1024
 // threads holds the group at that.
-bool make_plan(Plan& pl, long long rows, int D, int G, int size, bool vec, bool fwd) {
+bool make_plan(Plan& pl, long long rows, int D, int G, int size, Way way, bool fwd, int weights) {
   const int n = D / G;
   if (n > kMaxGroup) return false;
+  const bool vec = way != kElements, odd = way == kOdd;
   const int values = fwd || n > kMaxGroup / 2 ? 16 : 8;
+  pl.way = way;
   pl.vec = vec ? 16 / size : 1;
-  const int need = (n + pl.vec - 1) / pl.vec, most = values / pl.vec;
+  const int need = (n + (odd ? pl.vec - 1 : 0) + pl.vec - 1) / pl.vec, most = values / pl.vec;
   pl.k = 1;
   while (pl.k < most && pl.k * 8 < need) pl.k *= 2;
   if (!vec && pl.k < 4) pl.k = 4;
@@ -389,8 +771,14 @@ bool make_plan(Plan& pl, long long rows, int D, int G, int size, bool vec, bool 
   pl.gpc = pl.threads / pl.tpg < G ? pl.threads / pl.tpg : G;
   pl.rpc = pl.threads / (pl.tpg * pl.gpc);
   pl.gy = (unsigned)((G + pl.gpc - 1) / pl.gpc);
+  if (odd) {  // planes of the weights, and backward of their gradients' sums
+    const size_t planes = (size_t)pl.vec * (pl.k * pl.tpg + 2) * pl.gpc * sizeof(float);
+    pl.odd_smem = planes * weights * (fwd ? 1 : 1 + pl.rpc);
+    if (pl.odd_smem > 200 * 1024 || pl.threads > 1024 || n > (fwd ? kMaxGroup : kMaxGroup / 2) - 8) return false;
+  }
   // a few CTAs to an SM, each walking rows
-  const int per_sm = fwd ? 1024 / pl.threads : pl.threads > 512 ? 1 : pl.threads > 256 ? 2 : 3;
+  int per_sm = fwd ? 1024 / pl.threads : pl.threads > 512 ? 1 : pl.threads > 256 ? 2 : 3;
+  if (odd) per_sm = fwd ? (pl.threads > 384 ? 1 : pl.threads > 256 ? 2 : 3) : pl.threads > 256 ? 1 : 2;
   const long long most_x = ((long long)sm_count() * per_sm + pl.gy - 1) / pl.gy;
   const long long want = (rows + pl.rpc - 1) / pl.rpc;
   pl.gx = (unsigned)(want < most_x ? (want < 1 ? 1 : want) : most_x);
@@ -403,9 +791,24 @@ bool make_plan(Plan& pl, long long rows, int D, int G, int size, bool vec, bool 
   if (pl.vec == v && pl.k == kk && pl.threads <= maxt) return MGS_NORM_KERNEL(v, kk, maxt);
 #define MGS_NORM_SIZES(v, kk) MGS_NORM_CASE(v, kk, 256) MGS_NORM_CASE(v, kk, 512) MGS_NORM_CASE(v, kk, 1024)
 
+#define MGS_NORM_ODD(kk, maxt) \
+  if (pl.k == kk && pl.threads <= maxt) return MGS_NORM_ODD_KERNEL(kk, maxt);
+#define MGS_NORM_ODD_SIZES(kk, mid) \
+  MGS_NORM_ODD(kk, 256) MGS_NORM_ODD(kk, mid) MGS_NORM_ODD(kk, 768) MGS_NORM_ODD(kk, 1024)
+
 template <typename E, typename W, class F>
 int by_plan_fwd(const Plan& pl, F&& f) {
   constexpr int V = 16 / (int)sizeof(E);
+  if (pl.way == kOdd) {
+#define MGS_NORM_ODD_KERNEL(kk, maxt) f(fwd_odd_kernel<E, kk, maxt>)
+    MGS_NORM_ODD(1, 256)
+    if constexpr (V == 4) {
+      MGS_NORM_ODD(2, 256)
+    }
+    MGS_NORM_ODD_SIZES(16 / V, 384)
+#undef MGS_NORM_ODD_KERNEL
+    return MGS_UNSUPPORTED;
+  }
 #define MGS_NORM_KERNEL(v, kk, maxt) f(fwd_kernel<E, W, v, kk, maxt>)
   MGS_NORM_CASE(V, 1, 256)
   if constexpr (V == 4) {
@@ -422,6 +825,15 @@ int by_plan_fwd(const Plan& pl, F&& f) {
 template <typename E, typename W, bool GATE, bool SCALE, class F>
 int by_plan_bwd(const Plan& pl, F&& f) {
   constexpr int V = 16 / (int)sizeof(E);
+  if (pl.way == kOdd) {
+#define MGS_NORM_ODD_KERNEL(kk, maxt) f(bwd_odd_kernel<E, kk, maxt, GATE, SCALE>)
+    if constexpr (V == 4) {
+      MGS_NORM_ODD(1, 256)
+    }
+    MGS_NORM_ODD_SIZES(8 / V, 512)
+#undef MGS_NORM_ODD_KERNEL
+    return MGS_UNSUPPORTED;
+  }
 #define MGS_NORM_KERNEL(v, kk, maxt) f(bwd_kernel<E, W, v, kk, maxt, GATE, SCALE>)
   if constexpr (V == 4) {
     MGS_NORM_CASE(V, 1, 256)
@@ -436,6 +848,8 @@ int by_plan_bwd(const Plan& pl, F&& f) {
 }
 #undef MGS_NORM_SIZES
 #undef MGS_NORM_CASE
+#undef MGS_NORM_ODD_SIZES
+#undef MGS_NORM_ODD
 
 template <class F>
 int by_dtypes(int dtype, int wdtype, F&& f) {
@@ -453,15 +867,33 @@ bool shape_ok(int64_t rows, int64_t D, int groups) {
   return rows >= 0 && D >= 1 && D <= 0x3fffffff && groups >= 1 && D % groups == 0;
 }
 
-// Whole 16-byte vectors everywhere: addresses, row strides, group starts.
-bool vec_ok(const Args& a, int size, int wsize) {
+// How a call's rows can be read: whole 16-byte vectors everywhere (addresses, row
+// strides, group starts); vectors of memory with the columns shifted from row to
+// row, where that shift is the same for all tensors; or element by element.
+Way way_of(const Args& a, int size, int wsize) {
   const int v = 16 / size;
-  bool ok = a.n % v == 0 && (long long)a.n * wsize % 16 == 0;
-  for (const void* q : {a.x, a.res, a.gate, a.w, a.b, a.s, a.dy, a.dh, (const void*)a.y, (const void*)a.h,
-                        (const void*)a.dx, (const void*)a.dres, (const void*)a.dgate})
-    ok = ok && aligned(q, 16);
-  for (long long s : {a.ldx, a.ldres, a.ldgate, a.lddy, a.lddh}) ok = ok && s % v == 0;
-  return ok;
+  bool vec = a.n % v == 0 && (long long)a.n * wsize % 16 == 0, odd = true;
+  for (const void* q : {a.x, a.res, a.gate, a.dy, a.dh, (const void*)a.y, (const void*)a.h, (const void*)a.dx,
+                        (const void*)a.dres, (const void*)a.dgate})
+    odd = odd && aligned(q, 16);
+  vec = vec && odd;
+  for (const void* q : {a.w, a.b, a.s}) vec = vec && aligned(q, 16);
+  const long long out = a.D % v;  // of the dense outputs
+  for (auto [q, ld] : {std::pair(a.x, a.ldx), std::pair(a.res, a.ldres), std::pair(a.gate, a.ldgate),
+                       std::pair(a.dy, a.lddy), std::pair(a.dh, a.lddh)})
+    if (q) {
+      vec = vec && ld % v == 0;
+      odd = odd && ld % v == out;
+    }
+  vec = vec && (out == 0 || a.rows == 1);
+  return vec ? kVectors : odd ? kOdd : kElements;
+}
+
+// The plan of a call's way, or of single elements where that does not fit.
+bool plan_call(Plan& pl, const Args& a, int size, int wsize, bool fwd) {
+  const int weights = 1 + (a.b ? 1 : 0) + (a.s ? 1 : 0);
+  return make_plan(pl, a.rows, a.D, a.G, size, way_of(a, size, wsize), fwd, weights) ||
+         make_plan(pl, a.rows, a.D, a.G, size, kElements, fwd, weights);
 }
 
 void set_plan(Args& a, const Plan& pl) { a.tpg = pl.tpg, a.gpc = pl.gpc, a.rpc = pl.rpc; }
@@ -479,9 +911,12 @@ size_t mgs_block_norm_workspace_size(int64_t rows, int64_t D, int groups, int dt
   const int size = mgs::dtype_size(dtype);
   if (!shape_ok(rows, D, groups) || size == 0) return 0;
   size_t most = 0;
-  for (bool vec : {false, true}) {
+  for (Way way : {kElements, kVectors, kOdd}) {
     Plan pl;
-    if (!make_plan(pl, rows, (int)D, groups, size, vec, false)) return 0;
+    if (!make_plan(pl, rows, (int)D, groups, size, way, false, 1)) {
+      if (way == kOdd) continue;
+      return 0;
+    }
     const size_t n = 3 * (size_t)pl.gx * (size_t)D * sizeof(float);
     most = n > most ? n : most;
   }
@@ -503,12 +938,16 @@ int mgs_block_norm_fwd(const void* x, const void* residual, const void* gate, co
     a.h = residual ? h : nullptr, a.stats = stats;
     a.ldx = row_strides[0], a.ldres = row_strides[1], a.ldgate = row_strides[2];
     a.rows = rows, a.D = (int)D, a.G = groups, a.n = (int)D / groups, a.rms = rms, a.eps = eps;
+    a.w32 = std::is_same_v<W, float>;
     Plan pl;
-    if (!make_plan(pl, rows, (int)D, groups, sizeof(E), vec_ok(a, sizeof(E), sizeof(W)), true)) return MGS_UNSUPPORTED;
+    if (!plan_call(pl, a, sizeof(E), sizeof(W), true)) return MGS_UNSUPPORTED;
     if (pl.gy > 65535) return MGS_UNSUPPORTED;
     set_plan(a, pl);
     return by_plan_fwd<E, W>(pl, [&](auto fwd) -> int {
-      fwd<<<dim3(pl.gx, pl.gy), pl.threads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+      const size_t smem = pl.way == kOdd ? pl.odd_smem : 0;
+      if (smem > 40 * 1024)
+        MGS_CUDA_OK(cudaFuncSetAttribute(fwd, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+      fwd<<<dim3(pl.gx, pl.gy), pl.threads, smem, static_cast<cudaStream_t>(stream)>>>(a);
       return launched();
     });
   });
@@ -540,14 +979,15 @@ int mgs_block_norm_bwd(const void* x, const void* residual, const void* gate, co
     a.ldx = row_strides[0], a.ldres = row_strides[1], a.ldgate = row_strides[2], a.lddy = row_strides[3],
     a.lddh = row_strides[4];
     a.rows = rows, a.D = (int)D, a.G = groups, a.n = (int)D / groups, a.rms = rms;
+    a.w32 = std::is_same_v<W, float>;
     Plan pl;
-    if (!make_plan(pl, rows, (int)D, groups, sizeof(E), vec_ok(a, sizeof(E), sizeof(W)), false)) return MGS_UNSUPPORTED;
+    if (!plan_call(pl, a, sizeof(E), sizeof(W), false)) return MGS_UNSUPPORTED;
     if (pl.gy > 65535) return MGS_UNSUPPORTED;
     if (workspace_bytes < 3 * (size_t)pl.gx * (size_t)D * sizeof(float)) return MGS_WORKSPACE_TOO_SMALL;
     set_plan(a, pl);
     auto launch = [&](auto bwd) -> int {
-      const size_t smem = (size_t)pl.rpc * pl.gpc * a.n * sizeof(float);
-      if (smem > 48 * 1024)
+      const size_t smem = pl.way == kOdd ? pl.odd_smem : (size_t)pl.rpc * pl.gpc * a.n * sizeof(float);
+      if (smem > 40 * 1024)
         MGS_CUDA_OK(cudaFuncSetAttribute(bwd, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
       bwd<<<dim3(pl.gx, pl.gy), pl.threads, smem, st>>>(a);
       return launched();
