@@ -14,6 +14,7 @@ from .modules import (
     MinGRU,
     MinGRUBlock,
     MinGRUStack,
+    RetentionMinGRU,
     RotationMinGRU,
     SignedMinGRU,
     g,
@@ -42,6 +43,7 @@ __all__ = [
     "RotationMinGRU",
     "GivensMinGRU",
     "DeltaMinGRU",
+    "RetentionMinGRU",
     "MinGRUBlock",
     "MinGRUStack",
     "delta_scan_impl",

@@ -16,6 +16,7 @@ DeltaMinGRU        min_gru.py:2827-3695        ``delta_scan_impl`` (with decay:
                                                ``delta_gated_scan_impl``)
 MinGRUBlock        min_gru.py:3698-3922        (pre-norm residual wrapper)
 MinGRUStack        min_gru.py:4019-4336        (stack of blocks)
+RetentionMinGRU    (none: this package's own)  ``linear_attention``
 =================  ==========================  =====================================
 
 The coefficient heads (``nn.Linear`` + elementwise activations) are plain
@@ -37,6 +38,8 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import step_ops
+from .attn_ops import linear_attention
+from .norm_ops import block_norm
 from .scan_ops import (
     angle_scan_impl,
     brickwall_meta,
@@ -511,11 +514,110 @@ class DeltaMinGRU(DecayMixin, nn.Module):
                 f"chunk_size={self.chunk_size}")
 
 
+class RetentionMinGRU(DecayMixin, nn.Module):
+    """minGRU with a matrix state, its memory plain linear attention: per head
+
+    ``H_t = (1 - z_t) H_{t-1} + z_t k_t v_t^T``, ``y_t = H_t^T q_t``, ``z_t = sigmoid(a_t)``
+
+    with a scalar gate for each head and unit-norm keys, then an RMS norm of each
+    head's readout times ``silu`` of a gate (``block_norm``) and the output
+    projection. It is DeltaMinGRU without the correction of ``v`` by what the memory
+    holds under ``k``. ``forward`` runs on ``linear_attention``, ``step()`` on
+    ``step_ops.linear_attention_step``; the state, ``(B, 1, n_heads * d_k * d_v)``
+    from ``forward(return_state=True)``, is fp32 whatever the inputs' dtype."""
+
+    carries_matrix_state: bool = True
+
+    def __init__(self, input_size, hidden_size, bias=True, n_heads=4, d_k=None, d_v=None,
+                 decay: Decay = None, decay_rate=1.0, log1p_delta=False):
+        super().__init__()
+        if n_heads <= 0:
+            raise ValueError(f"n_heads must be positive (got {n_heads})")
+        if d_k is None and hidden_size % n_heads != 0:
+            raise ValueError(
+                f"hidden_size ({hidden_size}) must be divisible by n_heads ({n_heads}) when d_k is "
+                "not given explicitly"
+            )
+        self.input_size = input_size
+        self.hidden_size = hidden_size
+        self.n_heads = n_heads
+        self.d_k = d_k if d_k is not None else hidden_size // n_heads
+        self.d_v = d_v if d_v is not None else self.d_k
+        self.linear_q = nn.Linear(input_size, n_heads * self.d_k, bias=bias)
+        self.linear_k = nn.Linear(input_size, n_heads * self.d_k, bias=bias)
+        self.linear_v = nn.Linear(input_size, n_heads * self.d_v, bias=bias)
+        self.linear_z = nn.Linear(input_size, n_heads, bias=bias)
+        self.linear_g = nn.Linear(input_size, n_heads * self.d_v, bias=bias)
+        self.norm_weight = nn.Parameter(torch.ones(n_heads * self.d_v))
+        self.out_proj = nn.Linear(n_heads * self.d_v, hidden_size, bias=bias)
+        self._init_decay(decay, decay_rate, log1p_delta, num_channels=self.n_heads)
+
+    def _coeffs(self, x, dt):
+        lead = x.shape[:-1]
+        q = self.linear_q(x).view(*lead, self.n_heads, self.d_k) * self.d_k**-0.5
+        k = F.normalize(self.linear_k(x).view(*lead, self.n_heads, self.d_k), dim=-1)
+        a = self.linear_z(x)
+        v = torch.sigmoid(a).unsqueeze(-1) * self.linear_v(x).view(*lead, self.n_heads, self.d_v)
+        log_gamma = -F.softplus(a.float())  # log(1 - z)
+        if dt is not None:
+            log_gamma = log_gamma - self._decay_lambda() * dt.unsqueeze(-1)
+        return q, k, v, log_gamma
+
+    def _read(self, y, x):
+        y = block_norm(y, self.norm_weight, gate=self.linear_g(x), groups=self.n_heads, rms=True)
+        return self.out_proj(y)
+
+    def _state(self, h, expected, name):
+        if h is None:
+            return None
+        if tuple(h.shape) != expected:
+            raise ValueError(f"{name} must have shape {expected} (got {tuple(h.shape)})")
+        return h.reshape(expected[0], self.n_heads, self.d_k, self.d_v).float()
+
+    def forward(self, x, h_0=None, delta_t=None, return_state=False):
+        dt = self._prepare_decay(_match_delta_t_dtype(delta_t, self), canonical_ndim=2)
+        B, T, _ = x.shape
+        expected = (B, 1, self.n_heads * self.d_k * self.d_v)
+        H = self._state(h_0, expected, "h_0")
+        q, k, v, log_gamma = self._coeffs(x, dt)
+        heads = lambda t: t.transpose(1, 2)  # noqa: E731  (read in place)
+        y, H = linear_attention(heads(q), heads(k), heads(v), heads(log_gamma), H)
+        y = self._read(heads(y).reshape(B, T, self.n_heads * self.d_v), x)
+        return (y, H.reshape(expected)) if return_state else y
+
+    @torch.no_grad()
+    def step(self, x_t, h_prev=None, delta_t=None):
+        dt = self._prepare_decay(_match_delta_t_dtype(delta_t, self), canonical_ndim=1)
+        B = x_t.size(0)
+        expected = (B, self.n_heads * self.d_k * self.d_v)
+        H = self._state(h_prev, expected, "h_prev")
+        if H is None:
+            H = torch.zeros(B, self.n_heads, self.d_k, self.d_v, dtype=torch.float32, device=x_t.device)
+        q, k, v, log_gamma = self._coeffs(x_t, dt)
+        y, H = step_ops.linear_attention_step(q, k, v, log_gamma, H)
+        return self._read(y.reshape(B, self.n_heads * self.d_v), x_t), H.reshape(expected)
+
+    def extra_repr(self):
+        return (f"input_size={self.input_size}, hidden_size={self.hidden_size}, "
+                f"n_heads={self.n_heads}, d_k={self.d_k}, d_v={self.d_v}")
+
+
 # ------------------------------------------------------ block / stack -----
 
 
+def _add_norm(x, branch, norm):
+    """``(norm(x + branch), x + branch)`` by one kernel; ``branch`` may be ``None``."""
+    if branch is None:
+        return block_norm(x, norm.weight, norm.bias, eps=norm.eps), x
+    return block_norm(branch, norm.weight, norm.bias, residual=x, eps=norm.eps)
+
+
 class MinGRUBlock(nn.Module):
-    """Pre-norm residual block: ``x + mixer(LN(x))`` then ``x + MLP(LN(x))``."""
+    """Pre-norm residual block: ``x + mixer(LN(x))`` then ``x + MLP(LN(x))``.
+
+    ``fused_norms``: each residual add and the LayerNorm that follows it are one
+    kernel (``block_norm``), in a stack those between blocks too; the same weights
+    and the same function, rounded once where the two ops round twice."""
 
     _MIXER_CLASSES: dict[str, tuple[type[nn.Module], bool]] = {
         "log": (MinGRU, True),
@@ -523,11 +625,13 @@ class MinGRUBlock(nn.Module):
         "rotation": (RotationMinGRU, False),
         "givens": (GivensMinGRU, False),
         "delta": (DeltaMinGRU, False),
+        "retention": (RetentionMinGRU, False),
     }
 
     def __init__(self, d_model, mlp_expansion=4, dropout=0.0, learnable_h0=False, mixer="log",
-                 mixer_kwargs=None):
+                 mixer_kwargs=None, fused_norms=False):
         super().__init__()
+        self.fused_norms = fused_norms
         if mixer not in self._MIXER_CLASSES:
             raise ValueError(f"unknown mixer {mixer!r}; expected one of {sorted(self._MIXER_CLASSES)}")
         kwargs = dict(mixer_kwargs) if mixer_kwargs else {}
@@ -550,6 +654,9 @@ class MinGRUBlock(nn.Module):
             self.mlp = None
 
     def forward(self, x, h_0=None, delta_t=None):
+        if self.fused_norms:
+            x, branch, state = self._fused(x, None, h_0, delta_t)
+            return x + branch, state
         delta_t = _match_delta_t_dtype(delta_t, self.mingru)
         if getattr(self.mingru, "carries_matrix_state", False):
             h_seq, state = self.mingru(self.norm1(x), h_0, delta_t, return_state=True)
@@ -561,8 +668,29 @@ class MinGRUBlock(nn.Module):
             x = x + self.mlp(self.norm2(x))
         return x, state
 
+    def _fused(self, x, branch, h_0, delta_t, step=False):
+        """The block on a stream ``x`` that ``branch`` has yet to be added to (``None``:
+        nothing); returns the stream, the branch to add to it, and the state."""
+        delta_t = _match_delta_t_dtype(delta_t, self.mingru)
+        y, x = _add_norm(x, branch, self.norm1)
+        matrix = getattr(self.mingru, "carries_matrix_state", False)
+        if step:
+            h = self.mingru.step(y, h_0, delta_t)
+            h, state = h if matrix else (h, h)
+        else:
+            h = self.mingru(y, h_0, delta_t, **({"return_state": True} if matrix else {}))
+            h, state = h if matrix else (h, h[:, -1:])
+            h = self.drop(h)
+        if self.mlp is None:
+            return x, h, state
+        y, x = _add_norm(x, h, self.norm2)
+        return x, self.mlp(y), state
+
     @torch.no_grad()
     def step(self, x_t, h_prev, delta_t=None):
+        if self.fused_norms:
+            x_t, branch, state = self._fused(x_t, None, h_prev, delta_t, step=True)
+            return x_t + branch, state
         delta_t = _match_delta_t_dtype(delta_t, self.mingru)
         if getattr(self.mingru, "carries_matrix_state", False):
             y_t, state = self.mingru.step(self.norm1(x_t), h_prev, delta_t)
@@ -611,11 +739,15 @@ def _resolve_stack_mixer_spec(mixer, mixer_kwargs, n_layers):
 
 
 class MinGRUStack(nn.Module):
-    """``in_proj`` -> ``n_layers`` MinGRUBlocks -> LayerNorm, with per-block state."""
+    """``in_proj`` -> ``n_layers`` MinGRUBlocks -> LayerNorm, with per-block state.
+
+    ``fused_norms``: residual adds and LayerNorms in one kernel each (MinGRUBlock)."""
 
     def __init__(self, input_size, d_model, n_layers, mlp_expansion=4, dropout=0.0,
-                 learnable_h0=False, mixer="log", mixer_kwargs=None, decay_layers="all"):
+                 learnable_h0=False, mixer="log", mixer_kwargs=None, decay_layers="all",
+                 fused_norms=False):
         super().__init__()
+        self.fused_norms = fused_norms
         if decay_layers not in ("all", "last"):
             raise ValueError(f"decay_layers must be 'all' or 'last' (got {decay_layers!r})")
         self.decay_layers = decay_layers
@@ -635,7 +767,7 @@ class MinGRUStack(nn.Module):
             )
         self.blocks = nn.ModuleList(
             MinGRUBlock(d_model, mlp_expansion, dropout, learnable_h0, name,
-                        by_type[name] if i == n_layers - 1 else no_decay[name])
+                        by_type[name] if i == n_layers - 1 else no_decay[name], fused_norms)
             for i, name in enumerate(names)
         )
         self.norm_out = nn.LayerNorm(d_model)
@@ -652,6 +784,8 @@ class MinGRUStack(nn.Module):
             state = self.init_state()
         self._check_delta_t_has_decay(delta_t)
         x = self.in_proj(x)
+        if self.fused_norms:
+            return self._fused(x, state, delta_t)
         new_state = []
         for blk, h0 in zip(self.blocks, state):
             x, h_last = blk(x, h0, delta_t if blk.mingru.decay is not None else None)
@@ -662,8 +796,18 @@ class MinGRUStack(nn.Module):
     def step(self, x_t, state, delta_t=None):
         self._check_delta_t_has_decay(delta_t)
         x_t = self.in_proj(x_t)
+        if self.fused_norms:
+            return self._fused(x_t, state, delta_t, step=True)
         new_state = []
         for blk, h_prev in zip(self.blocks, state):
             x_t, h = blk.step(x_t, h_prev, delta_t if blk.mingru.decay is not None else None)
             new_state.append(h)
         return self.norm_out(x_t), new_state
+
+    def _fused(self, x, state, delta_t, step=False):
+        branch, new_state = None, []
+        for blk, h in zip(self.blocks, state):
+            x, branch, h = blk._fused(x, branch, h, delta_t if blk.mingru.decay is not None else None,
+                                      step=step)
+            new_state.append(h)
+        return _add_norm(x, branch, self.norm_out)[0], new_state
