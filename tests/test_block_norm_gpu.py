@@ -270,3 +270,19 @@ def test_refusals(cuda):
     a = torch.randn(3, 24, device=cuda, requires_grad=True)
     with pytest.raises(RuntimeError, match="second-order"):
         torch.autograd.grad(mb.block_norm(a, w).sum(), a, create_graph=True)
+
+
+def test_under_compile(cuda):
+    """torch.compile sees opaque ops, forward and backward."""
+    import mingru_b200 as mb
+
+    t, dy, dh = inputs((20,), 96, torch.float32, torch.float32, cuda, ("bias", "residual", "scale", "gate"), 7)
+    x = [a.requires_grad_(True) for a in t.values()]
+
+    def run(x, w, b, r, s, g):
+        return mb.block_norm(x, w, b, residual=r, scale=s, gate=g, groups=4)
+
+    got, want = torch.compile(run, backend="aot_eager", fullgraph=True)(*x), run(*x)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for a, b in zip(torch.autograd.grad(got, x, (dy, dh)), torch.autograd.grad(want, x, (dy, dh))):
+        assert torch.equal(a, b)

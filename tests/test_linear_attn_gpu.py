@@ -329,3 +329,17 @@ def test_c_entry_refuses(cuda):
     assert name(call(1, 1, 1, 8, 8, 0, saved=p + 4)) == "MGS_BAD_ALIGNMENT"
     assert name(call(0, 1, 5, 8, 8, 0)) == "MGS_OK"
     assert lib.mgs_linear_attn_saved_size(1, 1, 128, 129, 8, 1) == 0
+
+
+def test_under_compile(cuda):
+    """torch.compile sees opaque ops, forward and backward."""
+    import mingru_b200 as mb
+
+    Q, K, V, lg, H0, dy, dH = inputs(1, 2, 150, 32, 32, torch.float32, cuda)
+    x = [t.requires_grad_(True) for t in (Q, K, V, lg, H0)]
+    f = torch.compile(lambda *a: mb.linear_attention(*a), backend="aot_eager", fullgraph=True)
+    got = f(*x)
+    want = mb.linear_attention(*x)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for a, b in zip(torch.autograd.grad(got, x, (dy, dH)), torch.autograd.grad(want, x, (dy, dH))):
+        assert torch.equal(a, b)
