@@ -24,7 +24,7 @@ import functools
 import torch
 
 from . import _lib
-from .scan_ops import _dense, _dtype_code, _ptr, _require_cuda, _workspace, on_device, raw_stream
+from .scan_ops import _dense, _dtype_code, _ptr, _require_cuda, on_device, raw_stream
 
 __all__ = ["linear_attention"]
 
@@ -38,7 +38,9 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _strides(*ts: torch.Tensor):
-    flat = [s for t in ts for s in t.stride()[:3]]
+    flat = []
+    for t in ts:
+        flat += t.stride()[:3]
     return (ctypes.c_int64 * len(flat))(*flat)
 
 
@@ -59,17 +61,17 @@ def _forward(Q, K, V, lg, H0, save):
         code = _dtype_code(_OP, Q)
         n, nsaved = _sizes(dev.index, B, H, T, dk, dv, code)
         y = torch.empty_like(V)
-        HT = torch.empty((B, H, dk, dv), dtype=torch.float32, device=dev)
-        saved = torch.empty(nsaved, dtype=torch.float32, device=dev) if save else HT.new_empty(0)
+        HT = lg.new_empty((B, H, dk, dv))  # log_gamma is fp32 and on the same device
+        saved = lg.new_empty(nsaved) if save else None
         if T == 0:  # no token: the state passes through
             HT.zero_() if H0 is None else HT.copy_(H0)
             return y, HT, saved
         if H0 is not None:
             H0 = _dense(H0)
-        ws = _workspace(n, dev) if n else None
+        ws = lg.new_empty(n // 4) if n else None
         st = _lib.load().mgs_linear_attn_fwd(
             Q.data_ptr(), K.data_ptr(), V.data_ptr(), lg.data_ptr(), _ptr(H0), y.data_ptr(), HT.data_ptr(),
-            saved.data_ptr() if save else None, _strides(Q, K, V, lg, y), B, H, T, dk, dv, code, _ptr(ws), n,
+            _ptr(saved), _strides(Q, K, V, lg, y), B, H, T, dk, dv, code, _ptr(ws), n,
             raw_stream(dev),
         )
         if st:
@@ -82,7 +84,8 @@ def _linear_attn_fwd(
     Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, lg: torch.Tensor, H0: torch.Tensor | None,
     save: bool,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return _forward(Q, K, V, lg, H0, save)
+    y, HT, saved = _forward(Q, K, V, lg, H0, save)
+    return y, HT, lg.new_empty(0) if saved is None else saved
 
 
 @_linear_attn_fwd.register_fake
@@ -101,8 +104,8 @@ def _gradients(Q, K, V, lg, saved, dy, dHT, want_dH0):
         dv = V.shape[3]
         code = _dtype_code(_OP, Q)
         dQ, dK, dV = torch.empty_like(Q), torch.empty_like(K), torch.empty_like(V)
-        dlg = torch.empty((B, H, T), dtype=torch.float32, device=dev)
-        dH0 = torch.empty((B, H, dk, dv) if want_dH0 else (0,), dtype=torch.float32, device=dev)
+        dlg = lg.new_empty((B, H, T))
+        dH0 = lg.new_empty((B, H, dk, dv)) if want_dH0 else None
         if dHT is not None:
             dHT = _dense(dHT.float())
         if T == 0:
@@ -110,11 +113,11 @@ def _gradients(Q, K, V, lg, saved, dy, dHT, want_dH0):
                 dH0.zero_() if dHT is None else dH0.copy_(dHT)
             return dQ, dK, dV, dlg, dH0
         n, _ = _sizes(dev.index, B, H, T, dk, dv, code)
-        ws = _workspace(n, dev) if n else None
+        ws = lg.new_empty(n // 4) if n else None
         st = _lib.load().mgs_linear_attn_bwd(
             Q.data_ptr(), K.data_ptr(), V.data_ptr(), lg.data_ptr(), saved.data_ptr(), dy.data_ptr(),
             _ptr(dHT), dQ.data_ptr(), dK.data_ptr(), dV.data_ptr(), dlg.data_ptr(),
-            dH0.data_ptr() if want_dH0 else None, _strides(Q, K, V, lg, dy, dQ, dK, dV), B, H, T, dk, dv,
+            _ptr(dH0), _strides(Q, K, V, lg, dy, dQ, dK, dV), B, H, T, dk, dv,
             code, _ptr(ws), n, raw_stream(dev),
         )
         if st:
@@ -127,7 +130,8 @@ def _linear_attn_bwd(
     Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, lg: torch.Tensor, saved: torch.Tensor,
     dy: torch.Tensor, dHT: torch.Tensor | None, want_dH0: bool,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    return _gradients(Q, K, V, lg, saved, dy, dHT, want_dH0)
+    *grads, dH0 = _gradients(Q, K, V, lg, saved, dy, dHT, want_dH0)
+    return *grads, lg.new_empty(0) if dH0 is None else dH0
 
 
 @_linear_attn_bwd.register_fake

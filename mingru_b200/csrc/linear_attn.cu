@@ -1326,6 +1326,10 @@ __global__ void __launch_bounds__(Dq<E, D>::kThreads, Dq<E, D>::kPerSm) dq_kerne
     a1.store(lb, wg);
     st_wait();
     sync();
+    if (tma && ok && tid == 0 && more) {  // V has been used
+      mbar_arrive_expect_tx(&sm.full, 4 * tile_bytes(D));
+      tma_load<D>(V, &p.mV, next.t0, next.h, next.b, &sm.full);
+    }
     if (warp == kDecayWarp && more) dw.table<false>(dec);
     if (warp == 0 && elect_one() && ok) {
       product_ta<NL, NL, D>(tb + F::kDq, tb, op_mn<D>(K), false);
@@ -1333,6 +1337,10 @@ __global__ void __launch_bounds__(Dq<E, D>::kThreads, Dq<E, D>::kPerSm) dq_kerne
       um::commit(&sm.bar);
     }
     wait();
+    if (tma && ok && tid == 0 && more) {  // and so have dy and K
+      tma_load<D>(G, &p.mdy, next.t0, next.h, next.b, &sm.full);
+      tma_load<D>(K, &p.mK, next.t0, next.h, next.b, &sm.full);
+    }
     float aq = 0.f;
 #pragma unroll
     for (int k = 0; k < D / (16 * W); ++k) {
@@ -1352,7 +1360,7 @@ __global__ void __launch_bounds__(Dq<E, D>::kThreads, Dq<E, D>::kPerSm) dq_kerne
         x[i] = fmaf(from_start, z[i], x[i]);
       }
       if (tma)
-        row16_to_tile(V, row, j0, x);  // V has been used
+        row16_to_tile(Q, row, j0, x);  // over what this thread has read
       else if (ok && row < a.n)
         store_row16<E>(p.dQ, a.b, a.h, p.H, a.t0 + row, p.T, j0, p.dk, x);
     }
@@ -1368,14 +1376,10 @@ __global__ void __launch_bounds__(Dq<E, D>::kThreads, Dq<E, D>::kPerSm) dq_kerne
       p.aq[a.bh * p.nchunks + a.c] = s;
     }
     if (tma && ok && tid == 0) {
-      tma_store<D>(&p.mdQ, a.t0, a.h, a.b, p.dk, V);
+      tma_store<D>(&p.mdQ, a.t0, a.h, a.b, p.dk, Q);
       if (more) {
-        mbar_arrive_expect_tx(&sm.full, 4 * tile_bytes(D));
-        tma_load<D>(G, &p.mdy, next.t0, next.h, next.b, &sm.full);
-        tma_load<D>(Q, &p.mQ, next.t0, next.h, next.b, &sm.full);
-        tma_load<D>(K, &p.mK, next.t0, next.h, next.b, &sm.full);
         bulk_wait_read();
-        tma_load<D>(V, &p.mV, next.t0, next.h, next.b, &sm.full);
+        tma_load<D>(Q, &p.mQ, next.t0, next.h, next.b, &sm.full);
       }
     }
     a = next;
@@ -1734,6 +1738,11 @@ __global__ void __launch_bounds__(Dkv<E, D>::kThreads, Dkv<E, D>::kPerSm) dkv_ke
     }
     wait();
     const float g = ex2(th + tl);
+    if (F::kE && tma && ok && tid == 0 && more) {  // these two have been used
+      mbar_arrive_expect_tx(&sm.full, 4 * tile_bytes(D));
+      tma_load<D>(Q, &p.mQ, t0 - kC, h, b, &sm.full);
+      tma_load<D>(G, &p.mdy, t0 - kC, h, b, &sm.full);
+    }
     if constexpr (F::kE) {
       // the sum goes over the extra tile in its own order, then to all threads
       if (tma) {
@@ -1749,9 +1758,6 @@ __global__ void __launch_bounds__(Dkv<E, D>::kThreads, Dkv<E, D>::kPerSm) dkv_ke
         tma_store<D>(&p.mdV, t0, h, b, p.dv, V);
         tma_store<D>(&p.mdK, t0, h, b, p.dk, K);
         if (more) {
-          mbar_arrive_expect_tx(&sm.full, 4 * tile_bytes(D));
-          tma_load<D>(Q, &p.mQ, t0 - kC, h, b, &sm.full);
-          tma_load<D>(G, &p.mdy, t0 - kC, h, b, &sm.full);
           bulk_wait_read();
           tma_load<D>(K, &p.mK, t0 - kC, h, b, &sm.full);
           tma_load<D>(V, &p.mV, t0 - kC, h, b, &sm.full);
