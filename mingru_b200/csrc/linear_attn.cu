@@ -1109,7 +1109,7 @@ struct SmallB {
   float a[2][kC];           // a token's share of the sums above, in two parts
   Decays dec;
 };
-constexpr int kSmallB = 3072;
+constexpr int kSmallB = 3 * 1024;
 static_assert(sizeof(SmallB) <= kSmallB, "");
 // In dkv_kernel the first rows have most masked blocks, so the last quarter's warps
 // do the sundries: kSumWarp puts dlog_gamma together during the next chunk's first
@@ -1815,28 +1815,52 @@ int sm_count() {
   return n;
 }
 
-// Segments: as many as there are places for CTAs of the main kernel, whole
-// chunks to each. For the state sums, which go through a chunk in less time than
-// they take to fill the SMs evenly, segments split again, for some waves of CTAs.
-constexpr int kSumsWaves = 2;
-Plan plan_for(long long BH, long long T, int D, int per_sm, int sums_per_sm) {
-  Plan pl{};
-  pl.D = D;
-  pl.nchunks = (int)((T + kC - 1) / kC);
-  if (BH <= 0 || pl.nchunks <= 0) return pl;
-  long long want = (long long)sm_count() * per_sm / BH;
-  want = want < 1 ? 1 : want > pl.nchunks ? pl.nchunks : want;
-  pl.m = (int)((pl.nchunks + want - 1) / want);
-  pl.nseg = (pl.nchunks + pl.m - 1) / pl.m;
-  pl.ms = pl.m, pl.r = 1, pl.nsub = pl.nseg;
-  if (pl.nseg > 1) {
-    const long long ctas = BH * (pl.nseg - 1);
-    long long r = (kSumsWaves * (long long)sm_count() * sums_per_sm + ctas / 2) / ctas;
-    r = r < 1 ? 1 : r > pl.m ? pl.m : r;
-    pl.ms = (int)((pl.m + r - 1) / r);
-    pl.r = (pl.m + pl.ms - 1) / pl.ms, pl.nsub = pl.nseg * pl.r;
+// Segments of m chunks for the main kernel, each in r parts of ms chunks for the
+// state sums. CTAs of a kernel take equally long, so its time goes by whole waves
+// of them: the plan is the cheapest of one segment and of as many as fill 1 to 8
+// waves, in units of a chunk of the state sums (2.6 us, bf16 heads of 64). In these
+// a chunk of the forward is 2.1 to 4 and one of dkv_kernel 4 to 6.4, by type and
+// width; a wave starts and ends in some 0.6 of a chunk; a part's state costs 0.04
+// in scan_kernel, more with many heads; the two further launches are worth 2.
+// Parts, state and scan together, bf16: 8 heads, T = 65536, 37 segments: r = 1 takes
+// 47 us, 2 takes 53, 4 takes 68; 64 heads, T = 8192, 4 segments: r = 1 takes 44, 3
+// takes 42, 6 takes 47. Segments, forward and backward, this rule against as many
+// as fill one wave in parts for two: 104 heads, T = 4096 of 64: 361 us, 374; 16,
+// T = 4096 of 128: 196, 209; 4, T = 256: 17 forward, 24. Heads that fill a wave by
+// themselves are not split: a last wave of few CTAs is quicker than the model's
+// (200 heads, T = 2048 of 128: forward 185 us, 214 in segments; 320 of 64: 136, 159).
+Plan plan_for(long long BH, long long T, int D, bool fwd, int per_sm, int sums_per_sm) {
+  Plan best{};
+  best.D = D;
+  const int n = (int)((T + kC - 1) / kC);
+  best.nchunks = n;
+  if (BH <= 0 || n <= 0) return best;
+  const long long sms = sm_count(), places = sms * per_sm, sums_places = sms * sums_per_sm;
+  const float main = fwd ? 2.5f : 5.f, slot = 0.04f + 0.001f * (float)BH;
+  auto waves = [](long long ctas, long long at_once) { return (float)((ctas + at_once - 1) / at_once); };
+  float least = 0.f;
+  for (int w = 0; w <= (BH < places ? 8 : 0); ++w) {
+    const long long fill = w == 0 ? 1 : w * places / BH;
+    if (w > 0 && fill < 2) continue;
+    Plan pl = best;
+    pl.m = (int)(fill < n ? (n + fill - 1) / fill : 1);
+    pl.nseg = (n + pl.m - 1) / pl.m;
+    pl.ms = pl.m, pl.r = 1;
+    float cost = main * waves(BH * pl.nseg, places) * (pl.m + 0.5f);
+    if (pl.nseg > 1) {
+      float sums = 0.f;
+      for (int r = 1; r <= 4 && r <= pl.m; ++r) {
+        const int ms = (pl.m + r - 1) / r, rr = (pl.m + ms - 1) / ms;
+        const float c = waves(BH * (pl.nseg - 1) * rr, sums_places) * (ms + 0.6f) + slot * (float)(rr * pl.nseg);
+        if (r == 1 || c < sums) sums = c, pl.ms = ms, pl.r = rr;
+      }
+      cost += sums + 2.f;
+    }
+    pl.nsub = pl.nseg * pl.r;
+    if (w == 0 || cost < least) least = cost, best = pl;
+    if (fill >= n) break;
   }
-  return pl;
+  return best;
 }
 
 // Element type and the width that kernels run at. bf16 heads up to 128 run
@@ -1863,7 +1887,7 @@ size_t seg_bytes(const Plan& pl, long long BH) {
 
 template <typename E, int D>
 Plan plan_of(bool fwd, long long BH, long long T) {
-  return plan_for(BH, T, D, fwd ? Fwd<E, D>::kPerSm : Dkv<E, D>::kPerSm, Sums<E, D>::kPerSm);
+  return plan_for(BH, T, D, fwd, fwd ? Fwd<E, D>::kPerSm : Dkv<E, D>::kPerSm, Sums<E, D>::kPerSm);
 }
 
 bool shape_ok(int64_t B, int H, int64_t T, int dk, int dv) {
