@@ -139,7 +139,14 @@ struct Reduce {
   }
 };
 
-__device__ __forceinline__ float sigm(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+// 1 / (1 + e^-x) in four instructions: denormals of the hardware's 2^x and 1 / x are
+// flushed, which nothing sees next to the 1, or below 2^-126.
+__device__ __forceinline__ float sigm(float x) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.44269504f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return r;
+}
 
 // 1 / sqrt(v) to the last place, by a step of Newton's on the hardware's: the
 // gradient takes differences of z * z and 1.
@@ -191,6 +198,8 @@ __global__ void __launch_bounds__(MAXT, fwd_ctas(MAXT)) fwd_kernel(const Args p)
       ra.load(p.gate, row * p.ldgate + col, at.t, p.tpg, p.n);
   };
   if (kAhead) fetch((long long)blockIdx.x * p.rpc + at.rs);
+  float wk[kAhead ? N : 1];  // the weight, for all rows
+  if constexpr (kAhead) ldrow<W, VEC, K>(p.w, col, at.t, p.tpg, p.n, wk);
   for (long long row = (long long)blockIdx.x * p.rpc + at.rs; row < p.rows; row += step) {
     float h[N], a[N], w[N];
     if constexpr (kAhead) {
@@ -215,19 +224,23 @@ __global__ void __launch_bounds__(MAXT, fwd_ctas(MAXT)) fwd_kernel(const Args p)
       }
     }
     if (p.res && p.gate) ldrow<E, VEC, K>(p.gate, row * p.ldgate + col, at.t, p.tpg, p.n, a);
-    ldrow<W, VEC, K>(p.w, col, at.t, p.tpg, p.n, w);
-    float acc = 0.f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) acc += h[i];
+    const long long o = row * p.D + col;
+    if (p.h) strow<E, VEC, K>(p.h, o, at.t, p.tpg, p.n, h);
     // The fp32 mean is off by up to half a unit of its last place: what it leaves in the
     // differences, `rest`, is their own mean, and comes with the sum of their squares.
-    const float mean = p.rms ? 0.f : sum(acc, 0.f).x * inv_n;
+    float mean = 0.f;
+    if (!p.rms) {
+      float acc = 0.f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc += h[i];
+      mean = sum(acc, 0.f).x * inv_n;
+    }
     float sq = 0.f, rs = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float d = in(i) ? h[i] - mean : 0.f;
-      sq = fmaf(d, d, sq);
-      rs += d;
+      h[i] = in(i) ? h[i] - mean : 0.f;
+      sq = fmaf(h[i], h[i], sq);
+      rs += h[i];
     }
     const float2 m = sum(sq, rs);
     const float rest = p.rms ? 0.f : m.y * inv_n;
@@ -236,10 +249,10 @@ __global__ void __launch_bounds__(MAXT, fwd_ctas(MAXT)) fwd_kernel(const Args p)
       float* st = p.stats + (row * p.G + at.g) * 3;
       st[0] = mean, st[1] = rest, st[2] = r;
     }
-    const long long o = row * p.D + col;
-    if (p.h) strow<E, VEC, K>(p.h, o, at.t, p.tpg, p.n, h);
+    const float shift = -rest * r;
+    if constexpr (!kAhead) ldrow<W, VEC, K>(p.w, col, at.t, p.tpg, p.n, w);
 #pragma unroll
-    for (int i = 0; i < N; ++i) h[i] = ((h[i] - mean) - rest) * r * w[i];
+    for (int i = 0; i < N; ++i) h[i] = fmaf(h[i], r, shift) * (kAhead ? wk[i % (kAhead ? N : 1)] : w[i]);
     if (p.b) {
       ldrow<W, VEC, K>(p.b, col, at.t, p.tpg, p.n, w);
 #pragma unroll
@@ -277,7 +290,7 @@ __global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT)) bwd_kernel(const Args p)
       float x[N], d[N], z[N], w[N];
       ldrow<E, VEC, K>(p.x, row * p.ldx + col, at.t, p.tpg, p.n, x);
       ldrow<E, VEC, K>(p.dy, row * p.lddy + col, at.t, p.tpg, p.n, d);
-      const float mean = st[0], rest = st[1], r = st[2];
+      const float mean = st[0], r = st[2], shift = -st[1] * r;
       if (SCALE || p.res) {
         ldrow<E, VEC, K>(p.res, row * p.ldres + col, at.t, p.tpg, p.n, z);
         if constexpr (SCALE) {
@@ -294,7 +307,7 @@ __global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT)) bwd_kernel(const Args p)
       }
       ldrow<W, VEC, K>(p.w, col, at.t, p.tpg, p.n, w);
 #pragma unroll
-      for (int i = 0; i < N; ++i) z[i] = ((z[i] - mean) - rest) * r;
+      for (int i = 0; i < N; ++i) z[i] = fmaf(z[i] - mean, r, shift);
       if constexpr (GATE) {
         float g[N], b[N];
         ldrow<E, VEC, K>(p.gate, row * p.ldgate + col, at.t, p.tpg, p.n, g);
