@@ -39,6 +39,7 @@ struct Args {
   long long rows;
   int D, G, n, tpg, gpc, rpc;  // threads to a group, groups and rows to a CTA
   int rms, w32;  // weights in fp32
+  int staged;    // backward: the inputs that come through shared memory, a row ahead; 0: straight
   float eps;
 };
 
@@ -95,6 +96,33 @@ __device__ __forceinline__ void strow(void* p, long long i, int t, int tpg, int 
   }
 }
 
+// The same K vectors into 16-byte places of the thread's own in shared memory, `stride`
+// apart: on their way without registers. Out of the row they become zeros.
+template <typename T, int VEC, int K>
+__device__ __forceinline__ void stage_row(uint4* to, int stride, const void* p, long long i, int t, int tpg, int n) {
+  constexpr int kN = VEC * (int)sizeof(T) / 16;
+  const T* q = static_cast<const T*>(p);
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = (k * tpg + t) * VEC;
+    const T* from = c < n ? q + i + c : q;
+#pragma unroll
+    for (int j = 0; j < kN; ++j)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to + (k * kN + j) * stride)),
+                   "l"(reinterpret_cast<const uint4*>(from) + (c < n ? j : 0)), "r"(c < n ? 16 : 0)
+                   : "memory");
+  }
+}
+template <typename T, int VEC, int K>
+__device__ __forceinline__ void staged_row(const uint4* from, int stride, float (&v)[K * VEC]) {
+  Raw<T, VEC, K> r;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int j = 0; j < r.kN; ++j) r.r[k][j] = from[(k * r.kN + j) * stride];
+  r.get(v);
+}
+
 // Sums over the tpg threads of a group: a segment of a warp, or whole warps
 // that meet at a named barrier of the group's own. `buf` alternates, so that
 // one barrier is enough for each sum. What the threads wrote to shared memory
@@ -102,25 +130,26 @@ __device__ __forceinline__ void strow(void* p, long long i, int t, int tpg, int 
 struct Reduce {
   float2 (*red)[32];
   int tpg, slot, buf;
-  template <int W>
+  template <int W, bool TWO>
   __device__ __forceinline__ static void lanes(unsigned mask, float& a, float& b) {
 #pragma unroll
     for (int o = W / 2; o > 0; o >>= 1) {
       a += __shfl_xor_sync(mask, a, o);
-      b += __shfl_xor_sync(mask, b, o);
+      if constexpr (TWO) b += __shfl_xor_sync(mask, b, o);
     }
   }
-  __device__ __forceinline__ float2 operator()(float a, float b) {
+  template <bool TWO>
+  __device__ __forceinline__ float2 go(float a, float b) {
     const int lane = threadIdx.x & 31;
     if (tpg == 8) {
       __syncwarp(0xffu << (lane & 24));
-      lanes<8>(0xffu << (lane & 24), a, b);
+      lanes<8, TWO>(0xffu << (lane & 24), a, b);
     } else if (tpg == 16) {
       __syncwarp(0xffffu << (lane & 16));
-      lanes<16>(0xffffu << (lane & 16), a, b);
+      lanes<16, TWO>(0xffffu << (lane & 16), a, b);
     } else {
       __syncwarp();
-      lanes<32>(0xffffffffu, a, b);
+      lanes<32, TWO>(0xffffffffu, a, b);
       if (tpg > 32) {
         const int nw = tpg / 32, w0 = slot * nw;
         if (lane == 0) red[buf][threadIdx.x >> 5] = make_float2(a, b);
@@ -128,15 +157,18 @@ struct Reduce {
         const float2 f = lane < nw ? red[buf][w0 + lane] : make_float2(0.f, 0.f);
         a = f.x, b = f.y;
         if (nw <= 4)
-          lanes<4>(0xffffffffu, a, b);
+          lanes<4, TWO>(0xffffffffu, a, b);
         else
-          lanes<32>(0xffffffffu, a, b);
-        a = __shfl_sync(0xffffffffu, a, 0), b = __shfl_sync(0xffffffffu, b, 0);
+          lanes<32, TWO>(0xffffffffu, a, b);
+        a = __shfl_sync(0xffffffffu, a, 0);
+        if constexpr (TWO) b = __shfl_sync(0xffffffffu, b, 0);
         buf ^= 1;
       }
     }
     return make_float2(a, b);
   }
+  __device__ __forceinline__ float2 operator()(float a, float b) { return go<true>(a, b); }
+  __device__ __forceinline__ float operator()(float a) { return go<false>(a, 0.f).x; }
 };
 
 // 1 / (1 + e^-x) in four instructions: denormals of the hardware's 2^x and 1 / x are
@@ -228,23 +260,28 @@ __global__ void __launch_bounds__(MAXT, fwd_ctas(MAXT)) fwd_kernel(const Args p)
     if (p.h) strow<E, VEC, K>(p.h, o, at.t, p.tpg, p.n, h);
     // The fp32 mean is off by up to half a unit of its last place: what it leaves in the
     // differences, `rest`, is their own mean, and comes with the sum of their squares.
-    float mean = 0.f;
-    if (!p.rms) {
-      float acc = 0.f;
+    float mean = 0.f, rest = 0.f, sq = 0.f;
+    if (p.rms) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) acc += h[i];
-      mean = sum(acc, 0.f).x * inv_n;
-    }
-    float sq = 0.f, rs = 0.f;
+      for (int i = 0; i < N; ++i) sq = fmaf(h[i], h[i], sq);  // zeros from column n on
+      sq = sum(sq) * inv_n;
+    } else {
+      // The fp32 mean is off by up to half a unit of its last place: what it leaves in the
+      // differences, `rest`, is their own mean, and comes with the sum of their squares.
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      h[i] = in(i) ? h[i] - mean : 0.f;
-      sq = fmaf(h[i], h[i], sq);
-      rs += h[i];
+      for (int i = 0; i < N; ++i) mean += h[i];
+      mean = sum(mean) * inv_n;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        h[i] = in(i) ? h[i] - mean : 0.f;
+        sq = fmaf(h[i], h[i], sq);
+        rest += h[i];
+      }
+      const float2 m = sum(sq, rest);
+      rest = m.y * inv_n;
+      sq = fmaxf(fmaf(-rest, rest, m.x * inv_n), 0.f);
     }
-    const float2 m = sum(sq, rs);
-    const float rest = p.rms ? 0.f : m.y * inv_n;
-    const float r = inv_sqrt(fmaxf(fmaf(-rest, rest, m.x * inv_n), 0.f) + p.eps);
+    const float r = inv_sqrt(sq + p.eps);
     if (p.stats && at.t == 0) {
       float* st = p.stats + (row * p.G + at.g) * 3;
       st[0] = mean, st[1] = rest, st[2] = r;
@@ -266,7 +303,13 @@ __global__ void __launch_bounds__(MAXT, fwd_ctas(MAXT)) fwd_kernel(const Args p)
   }
 }
 
-// GATE and SCALE: whether they are there, so that a call without them keeps no registers for them.
+// GATE and SCALE: whether they are there, so that a call without them keeps no
+// registers for them. The seven arrays leave no registers for a row ahead, so rows
+// come through shared memory, the next on its way during this one, where the SM has
+// room for two rows' inputs of all its CTAs (groups up to 2048 in bf16 with few
+// inputs, or wider with one CTA): 16384 x 2048 bf16 with a residual 77 us, straight
+// 112; 65536 x 512 in 8 gated groups 78, 116 (0.41 GB: 4.3 TB/s, by its 450
+// instructions to 8 elements); 8192 x 512 fp32 14.1, 14.5.
 template <typename E, typename W, int VEC, int K, int MAXT, bool GATE, bool SCALE>
 __global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT)) bwd_kernel(const Args p) {
   constexpr int N = K * VEC;
@@ -282,17 +325,50 @@ __global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT)) bwd_kernel(const Args p)
     gw[i] = gb[i] = 0.f;
     if constexpr (SCALE) gs[i] = 0.f;
   }
+  const long long step = (long long)gridDim.x * p.rpc;
+  const bool staged = VEC > 1 && p.staged;
+  constexpr int kPieces = VEC > 1 ? K * VEC * (int)sizeof(E) / 16 : 1;  // of 16 bytes to an input
+  const int NT = blockDim.x, i_gate = 2 + (p.res != nullptr), i_dh = i_gate + GATE;
+  auto place = [&](int buf, int i) {
+    return reinterpret_cast<uint4*>(cols) + ((buf * p.staged + i) * kPieces * NT + (int)threadIdx.x);
+  };
+  auto fetch = [&](long long row, int buf) {
+    if constexpr (VEC > 1) {
+      if (row < p.rows) {
+        auto go = [&](int i, const void* t, long long ld) {
+          stage_row<E, VEC, K>(place(buf, i), NT, t, row * ld + col, at.t, p.tpg, p.n);
+        };
+        go(0, p.x, p.ldx);
+        go(1, p.dy, p.lddy);
+        if (p.res) go(2, p.res, p.ldres);
+        if constexpr (GATE) go(i_gate, p.gate, p.ldgate);
+        if (p.dh) go(i_dh, p.dh, p.lddh);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  };
+  int buf = 0;
+  auto take = [&](int i, const void* t, long long at_row, float (&v)[N]) {
+    if constexpr (VEC > 1) {
+      if (staged) return staged_row<E, VEC, K>(place(buf, i), NT, v);
+    }
+    ldrow<E, VEC, K>(t, at_row, at.t, p.tpg, p.n, v);
+  };
   if (at.on) {
-    for (long long row = (long long)blockIdx.x * p.rpc + at.rs; row < p.rows;
-         row += (long long)gridDim.x * p.rpc) {
+    if (staged) fetch((long long)blockIdx.x * p.rpc + at.rs, 0);
+    for (long long row = (long long)blockIdx.x * p.rpc + at.rs; row < p.rows; row += step, buf ^= staged) {
+      if (staged) {  // a thread reads what it copied itself
+        fetch(row + step, buf ^ 1);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+      }
       const float* st = p.stats + (row * p.G + at.g) * 3;
       const long long o = row * p.D + col;
       float x[N], d[N], z[N], w[N];
-      ldrow<E, VEC, K>(p.x, row * p.ldx + col, at.t, p.tpg, p.n, x);
-      ldrow<E, VEC, K>(p.dy, row * p.lddy + col, at.t, p.tpg, p.n, d);
+      take(0, p.x, row * p.ldx + col, x);
+      take(1, p.dy, row * p.lddy + col, d);
       const float mean = st[0], r = st[2], shift = -st[1] * r;
       if (SCALE || p.res) {
-        ldrow<E, VEC, K>(p.res, row * p.ldres + col, at.t, p.tpg, p.n, z);
+        take(2, p.res, row * p.ldres + col, z);
         if constexpr (SCALE) {
           ldrow<W, VEC, K>(p.s, col, at.t, p.tpg, p.n, w);
 #pragma unroll
@@ -310,7 +386,7 @@ __global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT)) bwd_kernel(const Args p)
       for (int i = 0; i < N; ++i) z[i] = fmaf(z[i] - mean, r, shift);
       if constexpr (GATE) {
         float g[N], b[N];
-        ldrow<E, VEC, K>(p.gate, row * p.ldgate + col, at.t, p.tpg, p.n, g);
+        take(i_gate, p.gate, row * p.ldgate + col, g);
         if (p.b) {
           ldrow<W, VEC, K>(p.b, col, at.t, p.tpg, p.n, b);
         } else {
@@ -319,27 +395,36 @@ __global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT)) bwd_kernel(const Args p)
         }
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          const float sg = sigm(g[i]), a = fmaf(z[i], w[i], b[i]);
-          b[i] = d[i] * a * sg * fmaf(g[i], 1.f - sg, 1.f);
-          d[i] *= g[i] * sg;
+          const float sg = sigm(g[i]), u = g[i] * sg;
+          b[i] = d[i] * fmaf(z[i], w[i], b[i]) * fmaf(-u, sg, sg + u);  // silu' = sg + u - u sg
+          d[i] *= u;
         }
         strow<E, VEC, K>(p.dgate, o, at.t, p.tpg, p.n, b);
       }
       float s1 = 0.f, s2 = 0.f;  // columns past n have d = w = 0
+      if (p.b) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) gb[i] += d[i];
+      }
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         gw[i] = fmaf(d[i], z[i], gw[i]);
-        gb[i] += d[i];
         d[i] *= w[i];
-        s1 += d[i];
         s2 = fmaf(d[i], z[i], s2);
       }
-      const float2 m = sum(s1, s2);
-      const float m1 = p.rms ? 0.f : m.x * inv_n, m2 = m.y * inv_n;
+      if (p.rms) {
+        s2 = sum(s2);
+      } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i) d[i] = r * (d[i] - m1 - z[i] * m2);
+        for (int i = 0; i < N; ++i) s1 += d[i];
+        const float2 m = sum(s1, s2);
+        s1 = m.x, s2 = m.y;
+      }
+      s1 *= inv_n, s2 *= -inv_n;  // differences first: they cancel in small groups
+#pragma unroll
+      for (int i = 0; i < N; ++i) d[i] = r * fmaf(z[i], s2, d[i] - s1);
       if (p.dh) {
-        ldrow<E, VEC, K>(p.dh, row * p.lddh + col, at.t, p.tpg, p.n, w);
+        take(i_dh, p.dh, row * p.lddh + col, w);
 #pragma unroll
         for (int i = 0; i < N; ++i) d[i] += w[i];
       }
@@ -355,6 +440,7 @@ __global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT)) bwd_kernel(const Args p)
       strow<E, VEC, K>(p.dx, o, at.t, p.tpg, p.n, d);
     }
   }
+  if (staged) asm volatile("cp.async.wait_group 0;" ::: "memory");  // cols takes the places
   // the CTA's rows: one partial row of each sum
   const int width = p.gpc * p.n;  // columns of this CTA
   for (int q = 0; q < 2 + SCALE; ++q) {
@@ -999,7 +1085,16 @@ int mgs_block_norm_bwd(const void* x, const void* residual, const void* gate, co
     if (workspace_bytes < 3 * (size_t)pl.gx * (size_t)D * sizeof(float)) return MGS_WORKSPACE_TOO_SMALL;
     set_plan(a, pl);
     auto launch = [&](auto bwd) -> int {
-      const size_t smem = pl.way == kOdd ? pl.odd_smem : (size_t)pl.rpc * pl.gpc * a.n * sizeof(float);
+      size_t smem = pl.way == kOdd ? pl.odd_smem : (size_t)pl.rpc * pl.gpc * a.n * sizeof(float);
+      if (pl.way == kVectors) {  // two rows' inputs, where the SM has room for its CTAs
+        const int inputs = 2 + (residual != nullptr) + (gate != nullptr) + (dh != nullptr);
+        const size_t places = (size_t)2 * inputs * pl.k * pl.vec * sizeof(E) * pl.threads;
+        const int ctas = pl.threads > 512 ? 1 : pl.threads > 256 ? 2 : 3;
+        if (ctas * (places + 2048) <= 224 * 1024) {
+          a.staged = inputs;
+          smem = smem > places ? smem : places;
+        }
+      }
       if (smem > 40 * 1024)
         MGS_CUDA_OK(cudaFuncSetAttribute(bwd, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
       bwd<<<dim3(pl.gx, pl.gy), pl.threads, smem, st>>>(a);
