@@ -415,7 +415,8 @@ int mgs_delta_step(const void* q, const void* k, const void* v, const void* beta
  * of 64: the recurrence is linear in q and k and separate in the columns of v).
  * The size queries return 0 outside it, the entry points MGS_UNSUPPORTED.
  * `saved` (mgs_linear_attn_saved_size bytes, 16-byte aligned) takes the states
- * at the chunks' starts for the backward; NULL: no backward follows.        */
+ * at the chunks' starts for the backward; NULL: no backward follows. T = 0: no
+ * output is written, H_T included (it is H0). */
 size_t mgs_linear_attn_workspace_size(int64_t B, int H, int64_t T, int dk, int dv, int dtype);
 size_t mgs_linear_attn_saved_size(int64_t B, int H, int64_t T, int dk, int dv, int dtype);
 int mgs_linear_attn_fwd(const void* Q, const void* K, const void* V, const float* log_gamma,

@@ -38,6 +38,13 @@
 // (batch, head) pairs than CTAs fit the GPU: state_kernel sums what a segment
 // adds to the state, scan_kernel joins these along the sequence, and the main
 // kernels then run all segments at once, chunk by chunk inside each.
+//
+// What bounds them (8 x 8 heads of 64, T = 8192, bf16, 0.54 GB for forward and
+// backward: 84 us at copy speed; 415 are taken): neither DRAM (24 to 49% of its peak)
+// nor the tensor pipe (22 to 25%) but the chain inside a chunk -- products, mask,
+// products that use it, sums that read those -- of which an SM has two under way, and
+// the instructions of masking, scaling and rounding (38 to 47% of the issue slots).
+// So the work on this chain is what each choice below is about.
 #include <type_traits>
 
 #include "common.cuh"
@@ -727,9 +734,14 @@ struct Sums {
 
 // What part s of a sequence (ms chunks) adds to the state: forward
 // sum_j e^{c_end - c_j} k_j v_j^T, backward (kBwd) sum_i e^{c_i} q_i dy_i^T with
-// c from the part's start. Every factor is <= 1, so the chunks just add up.
+// c from the part's start. Every factor is <= 1, so the chunks just add up, in
+// registers, without a chain through a state; the scaled rows take three levels since
+// their sum is an fp32 state. Two CTAs to an SM (bf16 heads of 64), each with the next
+// chunk on its way: 64 heads, T = 8192: 36 us (2.8 TB/s). One buffer and three CTAs
+// to an SM: 35, but heads of 128 then 22 instead of 20.
 template <typename E, int D, bool kBwd>
-__global__ void __launch_bounds__(Sums<E, D>::kThreads, Sums<E, D>::kPerSm) state_kernel(const __grid_constant__ Args<E> p) {
+__global__ void __launch_bounds__(Sums<E, D>::kThreads, Sums<E, D>::kPerSm)
+    state_kernel(const __grid_constant__ Args<E> p) {
   constexpr int NL = kLevels<E>, kTileE = kC * D, NT = Sums<E, D>::kThreads;
   extern __shared__ __align__(1024) unsigned char smem[];
   Small& sm = *reinterpret_cast<Small*>(smem);
@@ -823,8 +835,10 @@ __global__ void __launch_bounds__(Sums<E, D>::kThreads, Sums<E, D>::kPerSm) stat
 
 // Joins the parts along the sequence: slot s + 1 = e^{L_s} slot s + what s
 // added, from H0 (backward: slot s - 1 from slot s, from dH_T). One thread to
-// four elements of one (batch, head). Parts before the first segment's end
-// (backward: after the last one's start) have nobody to add for.
+// four elements of one (batch, head), eight parts' loads under way together: with few
+// heads it is their latency that counts (8 heads of 64, 37 parts: 6.8 us; 74: 10.8,
+// with sixteen under way 15.7, or 13.7 at one element to a thread). Parts before the
+// first segment's end (backward: after the last one's start) have nobody to add for.
 template <int D, bool kBwd>
 __global__ void __launch_bounds__(256) scan_kernel(float* seg, const float* segl, const float* init,
                                                    long long BH, int nsub, int steps, int dk, int dv,
@@ -866,6 +880,15 @@ __global__ void __launch_bounds__(256) scan_kernel(float* seg, const float* segl
 
 // ---------------------------------------------------------------- forward --
 
+// A segment, chunk by chunk: P = D * Q K^T in TMEM, y = P V + decayed Q S, then S for
+// the next chunk, whose sum over the scaled K rows runs during P's masking and whose
+// tiles load meanwhile. Bound by that chain, with two CTAs to an SM (bf16 heads of 64)
+// to fill it; one level of P where the output is 16 bits: its rounding is of the size
+// of the output's. 64 heads, T = 8192, bf16: 86 us, 3.1 TB/s, 8 heads, T = 65536: 70;
+// heads of 128 (16, T = 4096): 43; fp32 (64 heads, T = 1024, 512 threads and one CTA
+// to an SM): 52, where three levels make each product six. 512 threads at 64
+// registers with two CTAs to an SM took 115.
+//
 // TMEM columns: Q K^T 0..127 (one level: P packed in its place), y 128.., the
 // states' sum after it, P's levels after that.
 template <typename E, int D>
@@ -884,7 +907,8 @@ struct Fwd {
 };
 
 template <typename E, int D>
-__global__ void __launch_bounds__(Fwd<E, D>::kThreads, Fwd<E, D>::kPerSm) fwd_kernel(const __grid_constant__ Args<E> p) {
+__global__ void __launch_bounds__(Fwd<E, D>::kThreads, Fwd<E, D>::kPerSm)
+    fwd_kernel(const __grid_constant__ Args<E> p) {
   using F = Fwd<E, D>;
   constexpr int NL = F::NL, kTileE = F::kTileE, NT = F::kThreads, W = NT / 128;
   extern __shared__ __align__(1024) unsigned char smem[];
@@ -892,7 +916,8 @@ __global__ void __launch_bounds__(Fwd<E, D>::kThreads, Fwd<E, D>::kPerSm) fwd_ke
   bf16* const Q0 = reinterpret_cast<bf16*>(smem + kSmallBytes);
   bf16 *const K0 = Q0 + F::kBufs * NL * kTileE, *const V = K0 + F::kBufs * NL * kTileE,
               *const X = V + (NL + F::kExtra) * kTileE;
-  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, q = warp & 3, wg = warp >> 2;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  const int q = warp & 3, wg = warp >> 2;
   const long long bh = blockIdx.x % p.BH;
   const int s = (int)(blockIdx.x / p.BH);
   const int b = (int)(bh / p.H), h = (int)(bh % p.H);
@@ -932,7 +957,8 @@ __global__ void __launch_bounds__(Fwd<E, D>::kThreads, Fwd<E, D>::kPerSm) fwd_ke
     S.zero();
   S.template to_smem<NL>(X);
   // After a wait that runs out (recorded in the sticky word) the CTA issues no
-  // MMA or copy, waits on nothing and writes no output; sync makes the flag common.
+  // MMA or copy, waits on nothing and writes no output; sync makes the flag common. That
+  // wait is over a second, by when the CTA's other copies have long arrived.
   bool ok = true;
   auto sync = [&]() {
     fence_proxy_async_smem();
@@ -1166,6 +1192,13 @@ __device__ __forceinline__ void packed16_to_tile(bf16* tile, int r, int c0, cons
   *reinterpret_cast<uint4*>(tile + sw<kC>(r, c0 + 8)) = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
+// dQ = A1 K + decayed dy S^T with A1 = D * dy V^T, and a token's tq, from A1 and Q K^T.
+// Chunks are independent, so that CTAs fill all SMs and take every so many; the next
+// chunk's tiles load as each becomes free. Reads most of all kernels (four tiles and a
+// state to a chunk) and comes nearest to DRAM's limit, 49%. 64 heads, T = 8192, bf16:
+// 80 us (512 threads at 64 registers: 124); heads of 128 (16, T = 4096): 33; fp32 (64
+// heads, T = 1024): 55.
+//
 // TMEM columns: (dy V^T) 0..127 and (Q K^T) 128..255. One level: the masked A1 in
 // the former's place, and once both are read dQ and its state part in the latter's;
 // more levels: A1 at 0, the others after it.
@@ -1180,7 +1213,8 @@ struct Dq {
 };
 
 template <typename E, int D>
-__global__ void __launch_bounds__(Dq<E, D>::kThreads, Dq<E, D>::kPerSm) dq_kernel(const __grid_constant__ Args<E> p) {
+__global__ void __launch_bounds__(Dq<E, D>::kThreads, Dq<E, D>::kPerSm)
+    dq_kernel(const __grid_constant__ Args<E> p) {
   using F = Dq<E, D>;
   constexpr int NL = F::NL, kTileE = F::kTileE, NT = F::kThreads, W = NT / 128;
   extern __shared__ __align__(1024) unsigned char smem[];
@@ -1188,7 +1222,8 @@ __global__ void __launch_bounds__(Dq<E, D>::kThreads, Dq<E, D>::kPerSm) dq_kerne
   SmallB& sm = *reinterpret_cast<SmallB*>(smem);
   bf16* Q = reinterpret_cast<bf16*>(smem + kSmallB);
   bf16 *K = Q + NL * kTileE, *V = K + NL * kTileE, *G = V + NL * kTileE, *X = G + NL * kTileE;
-  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, q = warp & 3, wg = warp >> 2;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  const int q = warp & 3, wg = warp >> 2;
   const int row = 32 * q + lane;
   const long long total = p.BH * p.nchunks;
   struct At {  // a chunk's place
@@ -1390,6 +1425,14 @@ __global__ void __launch_bounds__(Dq<E, D>::kThreads, Dq<E, D>::kPerSm) dq_kerne
   if (warp == 0) um::dealloc(sm.tbase, F::kCols);
 }
 
+// A segment from its end: both masked products transposed, so that a thread has a key's
+// row; dV = A2 dy + decayed K dS, dK = A1 Q + decayed V dS^T; then dS, in three levels
+// as an operand, since dlog_gamma (fp32) is made from it. Its chain is the longest, four
+// waits for products to a chunk, and bounds it: 64 heads, T = 8192, bf16: 160 us;
+// heads of 128 (16, T = 4096): 80; fp32 (64 heads, T = 1024): 84. Outputs through
+// staged tiles by TMA: stored from registers in 32-byte pieces 176. 512 threads at 64
+// registers, two CTAs to an SM: 238.
+//
 // TMEM columns: (K Q^T) 0..127 and (V dy^T) 128..255. One level: their masked forms
 // A2 and A1 in their places, dV and dK (D = 64) in the columns these leave free
 // (D = 128: from 256 on); more levels: A2 at 0 and A1 at 64 NL once both are read, dV
@@ -1414,7 +1457,8 @@ struct Dkv {
 };
 
 template <typename E, int D>
-__global__ void __launch_bounds__(Dkv<E, D>::kThreads, Dkv<E, D>::kPerSm) dkv_kernel(const __grid_constant__ Args<E> p) {
+__global__ void __launch_bounds__(Dkv<E, D>::kThreads, Dkv<E, D>::kPerSm)
+    dkv_kernel(const __grid_constant__ Args<E> p) {
   using F = Dkv<E, D>;
   constexpr int NL = F::NL, kTileE = F::kTileE, NT = F::kThreads, W = NT / 128;
   extern __shared__ __align__(1024) unsigned char smem[];
@@ -1426,7 +1470,8 @@ __global__ void __launch_bounds__(Dkv<E, D>::kThreads, Dkv<E, D>::kPerSm) dkv_ke
   // the scaled Q rows go over Q and, below three levels, over what has been read by then
   bf16* const lv[3] = {Q, F::kE ? V : NL == 1 ? K : Q + kTileE,
                        F::kE ? Ex : NL == 1 ? V : NL == 2 ? K : Q + 2 * kTileE};
-  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, q = warp & 3, wg = warp >> 2;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  const int q = warp & 3, wg = warp >> 2;
   const long long bh = blockIdx.x % p.BH;
   const int s = p.nseg - 1 - (int)(blockIdx.x / p.BH);
   const int b = (int)(bh / p.H), h = (int)(bh % p.H);

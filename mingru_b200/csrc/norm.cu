@@ -12,8 +12,8 @@
 //   dx = scale * dh, dresidual = dh, dgate = dy * (z * weight + bias) * silu'(gate)
 //   dweight = sum da z, dbias = sum da, dscale = sum dh x     (over rows)
 //
-// Memory bound: the forward reads each input once and writes each output once,
-// a group's values staying in its threads' registers between the two
+// Memory bound on paper: the forward reads each input once and writes each output
+// once, a group's values staying in its threads' registers between the two
 // reductions; the backward reads the inputs again instead of z (and h is taken
 // in fp32 from x and residual, not from its rounded copy), with mean and r from
 // the forward. Sums over rows stay in the threads' registers while a CTA walks
@@ -208,6 +208,11 @@ constexpr int bwd_ctas(int threads) { return threads == 256 ? 3 : 1; }
 constexpr int odd_fwd_ctas(int threads) { return threads == 256 ? 3 : threads == 384 ? 2 : 1; }
 constexpr int odd_bwd_ctas(int threads) { return threads == 256 ? 2 : 1; }
 
+// Values of the next row are on their way where 8 to a thread leave registers for them
+// (16: 64 registers are full without; 8192 x 512 fp32 takes 23 us with, 15 without).
+// 16384 x 2048 bf16 with a residual: 55 us, 4.9 TB/s; 65536 x 512 bf16 in 8 gated
+// groups: 40 us, 5.0 TB/s, bound by the instructions of the gate (75% of the issue
+// slots before the sums that only a mean needs were left out of RMS rows: 47 us).
 template <typename E, typename W, int VEC, int K, int MAXT>
 __global__ void __launch_bounds__(MAXT, fwd_ctas(MAXT)) fwd_kernel(const Args p) {
   constexpr int N = K * VEC;
@@ -479,7 +484,10 @@ __global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT)) bwd_kernel(const Args p)
 // vectors of memory, from the one that the group's first element is in, and only
 // what goes by column -- weights in, their gradients' sums -- is shifted with the
 // row: these are fp32 in shared memory, column c in plane c % V, so that a warp's
-// access to one element of its vectors is to consecutive words.
+// access to one element of its vectors is to consecutive words. 4097 x 5001 fp16 with
+// a residual and a scale, forward and backward: 202 us (0.33 GB), element by element
+// 290. The planes' accesses, three or four to an element, and the barriers of rows of
+// 5000 bound them: both take half the issue slots.
 
 template <int V>
 struct Planes {
@@ -852,7 +860,8 @@ struct Plan {
 // few steps, and more rows are under way), a part of a warp or whole warps;
 // groups side by side in a CTA as they lie in a row. 16 values forward; 8
 // backward, which keeps seven arrays of them in registers, while a CTA of 1024
-// threads holds the group at that.
+// threads holds the group at that (odd rows, backward: 16 values took 235 us where 8
+// take 125).
 bool make_plan(Plan& pl, long long rows, int D, int G, int size, Way way, bool fwd, int weights) {
   const int n = D / G;
   if (n > kMaxGroup) return false;
@@ -1100,8 +1109,11 @@ int mgs_block_norm_bwd(const void* x, const void* residual, const void* gate, co
       bwd<<<dim3(pl.gx, pl.gy), pl.threads, smem, st>>>(a);
       return launched();
     };
-    const int r = gate ? (scale ? by_plan_bwd<E, W, true, true>(pl, launch) : by_plan_bwd<E, W, true, false>(pl, launch))
-                       : (scale ? by_plan_bwd<E, W, false, true>(pl, launch) : by_plan_bwd<E, W, false, false>(pl, launch));
+    int r;
+    if (gate)
+      r = scale ? by_plan_bwd<E, W, true, true>(pl, launch) : by_plan_bwd<E, W, true, false>(pl, launch);
+    else
+      r = scale ? by_plan_bwd<E, W, false, true>(pl, launch) : by_plan_bwd<E, W, false, false>(pl, launch);
     if (r) return r;
     sum_kernel<W><<<dim3((unsigned)((D + 31) / 32), 3), dim3(32, 32), 0, st>>>(
         a.part, static_cast<W*>(dweight), bias ? static_cast<W*>(dbias) : nullptr,
