@@ -40,7 +40,7 @@
 // kernels then run all segments at once, chunk by chunk inside each.
 //
 // What bounds them (8 x 8 heads of 64, T = 8192, bf16, 0.54 GB for forward and
-// backward: 84 us at copy speed; 415 are taken): neither DRAM (24 to 49% of its peak)
+// backward: 84 us at copy speed; 430 are taken): neither DRAM (24 to 49% of its peak)
 // nor the tensor pipe (22 to 25%) but the chain inside a chunk -- products, mask,
 // products that use it, sums that read those -- of which an SM has two under way, and
 // the instructions of masking, scaling and rounding (38 to 47% of the issue slots).
@@ -99,11 +99,12 @@ struct Args {
   const float* dHT;  // (B, H, dk, dv) or null: zeros
   float* dH0;        // (B, H, dk, dv) or null: not wanted
   float* dlg;        // (B, H, T)
-  float* saved;      // (BH, nchunks + 1, D * D) states at the chunks' starts and the end, or null: no backward
+  float* saved;      // (BH, nchunks, D * D) states at the chunks' starts, or null: no backward
   float* seg;        // (BH, nsub, D * D) states at the parts' starts (backward: ends) (workspace)
   float* segl;       // (BH, nsub) log2 of each part's total decay (workspace)
-  float* tq;         // (BH, T) a token's row sums and q . its gradient's state part (workspace)
-  float* aq;         // (BH, nchunks) sums of the latter over a chunk (workspace)
+  float* rows_R;     // (BH, T) a token's sum of R over the tokens before it in its chunk (workspace)
+  float* state_q;    // (BH, T) q . the state part of its gradient (workspace)
+  float* quarters;   // (BH, nchunks, 16) sums of R over quarters of rows (4) and of columns (workspace)
   long long T;
   int H, dk, dv, nchunks, m, nseg;  // m chunks to a segment
   int ms, r, nsub;                  // segments in r parts of ms chunks for the state sums, nsub in all
@@ -1005,7 +1006,7 @@ __global__ void __launch_bounds__(Fwd<E, D>::kThreads, Fwd<E, D>::kPerSm)
       }
     }
     if (warp == kDecayWarp && more) dw.load(lg + (t0 + kC) * p.lst, p.lst, rows(c + 1));
-    if (p.saved) S.store_own(p.saved + (bh * (p.nchunks + 1) + c) * (D * D));
+    if (p.saved) S.store_own(p.saved + (bh * p.nchunks + c) * (D * D));
     wait();
     const uint32_t lb = tb + ((uint32_t)(32 * q) << 16);
     const float rh = dec.ch[row], rl = dec.cl[row], th = dec.ch[kC - 1], tl = dec.cl[kC - 1];
@@ -1104,10 +1105,7 @@ __global__ void __launch_bounds__(Fwd<E, D>::kThreads, Fwd<E, D>::kPerSm)
       bulk_wait_read();
     }
   }
-  if (ok && s + 1 == p.nseg) {
-    S.store(p.HT + bh * p.sbh, p.dk, p.dv, p.sld);
-    if (p.saved) S.store_own(p.saved + (bh * (p.nchunks + 1) + c1) * (D * D));
-  }
+  if (ok && s + 1 == p.nseg) S.store(p.HT + bh * p.sbh, p.dk, p.dv, p.sld);
   um::fence_before();
   __syncthreads();
   if (warp == 0) um::dealloc(sm.tbase, F::kCols);
@@ -1120,19 +1118,20 @@ __global__ void __launch_bounds__(Fwd<E, D>::kThreads, Fwd<E, D>::kPerSm)
 // states' gradient go through a segment's chunks from its end: dkv_kernel. Both
 // form the masked products anew, each as its own rows want them.
 //
-// dlog_gamma. Token i's row of R and its state part add to every t <= i, token
-// j's column of R takes the pairs with i, j >= t out again, and its state part
-// bk_j = k_j . dK'_j adds to every t > j. The part that passes through a chunk
-// whole, e^{c_C} <S, dS'>, follows from chunk to chunk: with F = <S, dS> at a
-// chunk's end it is F - sum_j bk_j, and F at its start that plus sum_i q_i .
-// dQ'_i. So with tq_i = sum_j R_ij + q_i . dQ'_i, from dq_kernel,
-//   dlog_gamma_t = sum_{i >= t} (tq_i - sum_{i' > i} R_i'i - bk_i) + F.
+// dlog_gamma is the sum of all that crosses token t. What has come through the state
+// is added up as it is: q_i . dQ'_i for i >= t, k_j . dK'_j for j < t (prime: the state
+// parts) and e^{c_C} <S, dS>. Pairs inside the chunk, X_t = sum_{i >= t > j} R_ij, go
+// from row sums less column sums, X_t = X_{t+1} + sum_{j < t} R_tj - sum_{i > t} R_it,
+// but only over the 16 tokens to the next edge of a quarter, where X is summed anew
+// from the quarters' sums: dq_kernel's rows and dkv_kernel's columns round R
+// differently, and with a decay of a few tokens X is no larger than what 100 tokens
+// of that leave (2e-6 to 5e-6 of a head's summed gradient, now below 1e-6).
 
 struct SmallB {
   uint64_t bar, bar2, full;
   uint32_t tbase, pad;
-  float red[16], red2[16];  // by warp
-  float a[2][kC];           // a token's share of the sums above, in two parts
+  float red[2][16];  // by warp
+  float a[2][kC];    // a token's two sums
   Decays dec;
 };
 constexpr int kSmallB = 3 * 1024;
@@ -1167,16 +1166,23 @@ __device__ __forceinline__ float warp_sum(float x) {
   return x;
 }
 
-// a[0][row] + a[1][row], after the next barrier: the sum of all parts' shares.
+// A token's two values, summed over the parts, to a[0] and a[1]; 32 tokens, the warps
+// of all parts that share them, at a barrier of their own.
 template <int W>
-__device__ __forceinline__ void token_share(float (&a)[2][kC], int q, int part, int row, float x) {
+__device__ __forceinline__ void token_sums(float (&a)[2][kC], int q, int part, int row, float x, float y) {
   if constexpr (W == 4) {
     if (part >= 2) a[part - 2][row] = x;
     named_bar(9 + q, 128);
-    if (part >= 2) return;
-    x += a[part][row];
+    if (part < 2) x += a[part][row];
+    named_bar(9 + q, 128);
+    if (part >= 2) a[part - 2][row] = y;
+    named_bar(9 + q, 128);
+    if (part < 2) y += a[part][row];
+    named_bar(9 + q, 128);
   }
-  a[part][row] = x;
+  if (part == 1) a[0][row] = x, a[1][row] = y;
+  named_bar(9 + q, 32 * W);
+  if (part == 0) a[0][row] += x, a[1][row] += y;
 }
 
 // 16 values, rounded to bf16 and packed, and back into a tile's row.
@@ -1192,7 +1198,7 @@ __device__ __forceinline__ void packed16_to_tile(bf16* tile, int r, int c0, cons
   *reinterpret_cast<uint4*>(tile + sw<kC>(r, c0 + 8)) = make_uint4(w[4], w[5], w[6], w[7]);
 }
 
-// dQ = A1 K + decayed dy S^T with A1 = D * dy V^T, and a token's tq, from A1 and Q K^T.
+// dQ = A1 K + decayed dy S^T with A1 = D * dy V^T, and R's rows, from A1 and Q K^T.
 // Chunks are independent, so that CTAs fill all SMs and take every so many; the next
 // chunk's tiles load as each becomes free. Reads most of all kernels (four tiles and a
 // state to a chunk) and comes nearest to DRAM's limit, 49%. 64 heads, T = 8192, bf16:
@@ -1282,7 +1288,7 @@ __global__ void __launch_bounds__(Dq<E, D>::kThreads, Dq<E, D>::kPerSm)
     const bool more = id + gridDim.x < total;
     const At next = at(more ? id + gridDim.x : id);
     {  // the state that entered the chunk
-      const float* src = p.saved + (a.bh * (p.nchunks + 1) + a.c) * (D * D);
+      const float* src = p.saved + (a.bh * p.nchunks + a.c) * (D * D);
       if constexpr (D == 64) {
         float v[Ev::kN];
         Ev::load_own(src, v);
@@ -1316,11 +1322,11 @@ __global__ void __launch_bounds__(Dq<E, D>::kThreads, Dq<E, D>::kPerSm)
     }
     if (tid < D * D / 32)  // the next state's lines
       asm volatile("prefetch.global.L2 [%0];" ::"l"(
-          p.saved + (next.bh * (p.nchunks + 1) + next.c) * (D * D) + tid * 32));
+          p.saved + (next.bh * p.nchunks + next.c) * (D * D) + tid * 32));
     if (warp == kDecayWarp && more) load_decay(next);
     wait();
     const float rh = dec.ch[row], rl = dec.cl[row], from_start = ex2(rh + rl);
-    float tok = 0.f;
+    float tok = 0.f, left = 0.f, right = 0.f;  // R's row: in the diagonal quarter, in two quarters before it
     Held<NL, W> a1;
     // Lane: token i = row; columns: tokens j <= i. A1 = D * (dy V^T).
     masked_blocks<NL, W>(wg, [&](int bk_, int j0) {
@@ -1337,11 +1343,13 @@ __global__ void __launch_bounds__(Dq<E, D>::kThreads, Dq<E, D>::kPerSm)
         um::ld_bind(r2, x);
         if (j0 + 15 < 32 * q) {  // before every row
           const float f0 = dec.to(rh, rl, j0 + 15);
+          float r = 0.f;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             z[i] *= f0 * dec.cf[j0 + i];
-            tok = fmaf(z[i], x[i], tok);
+            r = fmaf(z[i], x[i], r);
           }
+          (j0 & 32 ? right : left) += r;
         } else {
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
@@ -1400,15 +1408,19 @@ __global__ void __launch_bounds__(Dq<E, D>::kThreads, Dq<E, D>::kPerSm)
         store_row16<E>(p.dQ, a.b, a.h, p.H, a.t0 + row, p.T, j0, p.dk, x);
     }
     aq *= from_start;
-    token_share<W>(sm.a, q, wg, row, aq + tok);
-    const float ws = warp_sum(aq);
-    if (lane == 0) sm.red[warp] = ws;
+    token_sums<W>(sm.a, q, wg, row, tok + left + right, aq);
+    left = warp_sum(left), right = warp_sum(right);
+    if (lane == 0) sm.red[0][warp] = left, sm.red[1][warp] = right;
     sync();
-    if (ok && tid < a.n) p.tq[a.bh * p.T + a.t0 + tid] = sm.a[0][tid] + sm.a[1][tid];
-    if (ok && tid == kC) {
-      float s = 0.f;
-      for (int i = 0; i < NT / 32; ++i) s += sm.red[i];
-      p.aq[a.bh * p.nchunks + a.c] = s;
+    if (ok && tid < a.n) {
+      p.rows_R[a.bh * p.T + a.t0 + tid] = sm.a[0][tid];
+      p.state_q[a.bh * p.T + a.t0 + tid] = sm.a[1][tid];
+    }
+    if (ok && tid >= kC && tid < kC + 16) {  // rows' quarter i / 4, columns' quarter i % 4
+      const int i = tid - kC, w = (i >> 2) + 4 * ((i >> 1) & 1) * (W / 2);
+      float s = sm.red[i & 1][w];
+      if (W == 4) s += sm.red[i & 1][w + 4];
+      p.quarters[(a.bh * p.nchunks + a.c) * 16 + i] = s;
     }
     if (tma && ok && tid == 0) {
       tma_store<D>(&p.mdQ, a.t0, a.h, a.b, p.dk, Q);
@@ -1428,10 +1440,11 @@ __global__ void __launch_bounds__(Dq<E, D>::kThreads, Dq<E, D>::kPerSm)
 // A segment from its end: both masked products transposed, so that a thread has a key's
 // row; dV = A2 dy + decayed K dS, dK = A1 Q + decayed V dS^T; then dS, in three levels
 // as an operand, since dlog_gamma (fp32) is made from it. Its chain is the longest, four
-// waits for products to a chunk, and bounds it: 64 heads, T = 8192, bf16: 160 us;
-// heads of 128 (16, T = 4096): 80; fp32 (64 heads, T = 1024): 84. Outputs through
-// staged tiles by TMA: stored from registers in 32-byte pieces 176. 512 threads at 64
-// registers, two CTAs to an SM: 238.
+// waits for products to a chunk, and bounds it: 64 heads, T = 8192, bf16: 168 us;
+// heads of 128 (16, T = 4096): 84; fp32 (64 heads, T = 1024): 84. Outputs through
+// staged tiles by TMA: stored from registers in 32-byte pieces 15 us more. 512 threads
+// at 64 registers, two CTAs to an SM: a quarter more. The entering states, for
+// dlog_gamma alone, take 8 us, loaded with the tiles (16 when loaded at their use).
 //
 // TMEM columns: (K Q^T) 0..127 and (V dy^T) 128..255. One level: their masked forms
 // A2 and A1 in their places, dV and dK (D = 64) in the columns these leave free
@@ -1505,8 +1518,6 @@ __global__ void __launch_bounds__(Dkv<E, D>::kThreads, Dkv<E, D>::kPerSm)
   State<D, NT> dS;    // otherwise
   {
     const float* end = s + 1 < p.nseg ? p.seg + (bh * p.nsub + (s + 1) * p.r - 1) * (D * D) : nullptr;
-    const float* S_end = p.saved + (bh * (p.nchunks + 1) + c1) * (D * D);
-    float d = 0.f;  // <S, dS> at the segment's end
     if constexpr (F::kE) {
       const int er = Ev::row(), ec = Ev::col();
       if (end) {
@@ -1516,10 +1527,6 @@ __global__ void __launch_bounds__(Dkv<E, D>::kThreads, Dkv<E, D>::kPerSm)
         for (int i = 0; i < Ev::kN; ++i)
           dSe[i] = p.dHT && er < p.dk && ec + i < p.dv ? p.dHT[bh * p.sbh + er * p.sld + ec + i] : 0.f;
       }
-      float v[Ev::kN];
-      Ev::load_own(S_end, v);
-#pragma unroll
-      for (int i = 0; i < Ev::kN; ++i) d = fmaf(v[i], dSe[i], d);
       Ev::to_smem(X, dSe);
     } else {
       if (end)
@@ -1528,14 +1535,8 @@ __global__ void __launch_bounds__(Dkv<E, D>::kThreads, Dkv<E, D>::kPerSm)
         dS.load(p.dHT + bh * p.sbh, p.dk, p.dv, p.sld);
       else
         dS.zero();
-      State<D, NT> S;
-      S.load_own(S_end);
-#pragma unroll
-      for (int i = 0; i < State<D, NT>::kCols; ++i) d = fmaf(S.v[i], dS.v[i], d);
       dS.template to_smem<3>(X);
     }
-    d = warp_sum(d);
-    if (lane == 0) sm.red[warp] = d;
   }
   bool ok = true;
   auto sync = [&]() {
@@ -1551,61 +1552,96 @@ __global__ void __launch_bounds__(Dkv<E, D>::kThreads, Dkv<E, D>::kPerSm)
     um::fence_after();
   };
   sync();
-  Two Fend{0.f, 0.f};  // kSumWarp: <S, dS> at the end of the chunk being summed
-  float tq[4], lgs[4], aqs = 0.f;
-  if (warp == kSumWarp)
-    for (int i = 0; i < NT / 32; ++i) Fend.add(sm.red[i]);
+  // <the state that enters chunk c, dS> by warps, as the chunk begins; dS has passed the
+  // chunk's decay in dlog_gamma. The state loads with the tiles.
+  using Entry = std::conditional_t<F::kE, float[Ev::kN], State<D, NT>>;
+  auto entry_load = [&](int c, Entry& S) {
+    const float* S_in = p.saved + (bh * p.nchunks + c) * (D * D);
+    if constexpr (F::kE)
+      Ev::load_own(S_in, S);
+    else
+      S.load_own(S_in);
+  };
+  auto through = [&](int c, const Entry& S) {
+    float d = 0.f;
+    if constexpr (F::kE) {
+#pragma unroll
+      for (int i = 0; i < Ev::kN; ++i) d = fmaf(S[i], dSe[i], d);
+    } else {
+#pragma unroll
+      for (int i = 0; i < State<D, NT>::kCols; ++i) d = fmaf(S.v[i], dS.v[i], d);
+    }
+    d = warp_sum(d);
+    if (lane == 0) sm.red[c & 1][warp] = d * ex2(dec.ch[kC - 1] + dec.cl[kC - 1]);
+  };
+  float rq[4], sq[4], lgs[4], edge = 0.f;
   // What chunk c's dlog_gamma needs from memory, and its sums once sm.a is complete:
-  // four tokens to a lane, from the end.
+  // four tokens to a lane, four lanes to an edge of a quarter.
   auto sums_load = [&](int c) {
     const long long t0 = (long long)c * kC;
     const int n = rows(c);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int t = 4 * lane + i;
-      tq[i] = t < n ? p.tq[bh * p.T + t0 + t] : 0.f;
+      rq[i] = t < n ? p.rows_R[bh * p.T + t0 + t] : 0.f;
+      sq[i] = t < n ? p.state_q[bh * p.T + t0 + t] : 0.f;
       lgs[i] = t < n ? lg[(t0 + t) * p.lst] : 0.f;
     }
-    aqs = p.aq[bh * p.nchunks + c];
+    // this lane's edge is e quarters from the start: rows' quarters from e on, columns' before it
+    const int e = (lane + 4) >> 3;
+    const float4* x = reinterpret_cast<const float4*>(p.quarters + (bh * p.nchunks + c) * 16);
+    edge = 0.f;
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {
+      const float4 f = x[i];
+      if (i >= e) edge += (e > 0 ? f.x : 0.f) + (e > 1 ? f.y : 0.f) + (e > 2 ? f.z : 0.f);
+    }
   };
   auto sums = [&](int c) {
     const long long t0 = (long long)c * kC;
     const int n = rows(c);
     const float4 a0 = *reinterpret_cast<const float4*>(sm.a[0] + 4 * lane);
     const float4 a1 = *reinterpret_cast<const float4*>(sm.a[1] + 4 * lane);
-    const float *p0 = &a0.x, *p1 = &a1.x;
-    Two v[4], run{0.f, 0.f};
+    const float *col = &a0.x, *bk = &a1.x;
+    float past = 0.f;
+    for (int i = 0; i < NT / 32; ++i) past += sm.red[c & 1][i];
+    float x = 0.f, y = 0.f, z = 0.f;  // this lane's: rows less columns, q's and k's state parts
 #pragma unroll
-    for (int i = 3; i >= 0; --i) {
-      run.add(tq[i]), run.add(p0[i]), run.add(p1[i]);
-      v[i] = run;
+    for (int i = 0; i < 4; ++i) x += rq[i] - col[i], y += sq[i], z += bk[i];
+    const bool after = lane & 4;  // the edge is after these tokens
+    float nx = 0.f, iy = y, iz = z;
+#pragma unroll
+    for (int o = 1; o < 4; ++o) {  // lanes between this one and the edge
+      const float u = __shfl_sync(0xffffffffu, x, after ? lane + o : lane - o);
+      if (after ? (lane & 3) + o < 4 : (lane & 3) >= o) nx += u;
     }
-    Two inc = run;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const Two x{__shfl_down_sync(0xffffffffu, inc.s, o), __shfl_down_sync(0xffffffffu, inc.e, o)};
-      if (lane + o < 32) inc.add(x);
+      const float u = __shfl_down_sync(0xffffffffu, iy, o), w = __shfl_up_sync(0xffffffffu, iz, o);
+      if (lane + o < 32) iy += u;
+      if (lane >= o) iz += w;
     }
-    inc.add(Two{-run.s, -run.e});  // the lanes after this one
-    inc.add(Fend);
+    float in = after ? nx + x : -nx, sy = iy, sz = iz - z;  // at the lane's first token
+    past += edge;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int t = 4 * lane + i;
       if (t < n && ok) {
         float* o = p.dlg + bh * p.T + t0 + t;
-        v[i].add(inc);
-        if (p.dlg_add) v[i].add(*o);
-        *o = lgs[i] * 1.4426950408889634f <= kMinLog2 ? 0.f : v[i].s + v[i].e;
+        float v = (in + past) + (sy + sz);
+        if (p.dlg_add) v += *o;
+        *o = lgs[i] * 1.4426950408889634f <= kMinLog2 ? 0.f : v;
       }
+      in -= rq[i] - col[i], sy -= sq[i], sz += bk[i];
     }
-    Fend.add(aqs);
-    for (int i = 0; i < NT / 32; ++i) Fend.add(-sm.red2[i]);
   };
   const int row = 32 * q + lane;
   for (int c = c1 - 1; c >= c0; --c) {
     const long long t0 = (long long)c * kC;
     const int n = rows(c), turn = (c1 - 1 - c) & 1;
     const bool more = c > c0;
+    Entry S_in;
+    entry_load(c, S_in);
     if (tma) {
       if (ok) ok = mbar_wait(&sm.full, turn, &g_sticky_err, kPolls);
     } else {
@@ -1638,10 +1674,13 @@ __global__ void __launch_bounds__(Dkv<E, D>::kThreads, Dkv<E, D>::kPerSm)
       if (c + 1 < c1) sums(c + 1);
       sums_load(c);
     }
+    through(c, S_in);  // while the products run
+    if (more && tid < D * D / 32)  // the next state's lines
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(p.saved + (bh * p.nchunks + c - 1) * (D * D) + tid * 32));
     wait();
     const float rh = dec.ch[row], rl = dec.cl[row], th = dec.ch[kC - 1], tl = dec.cl[kC - 1];
     const float to_end = dec.to(th, tl, row);
-    float tok = 0.f;  // this half's part of what token `row` takes from t <= row
+    float tok = 0.f;  // this part's share of R's column `row`
     {
       // Lane: token j = row; columns: tokens i >= j. A2 = D * (K Q^T), A1 = D * (V dy^T).
       Held<NL, W> a1, a2;
@@ -1663,7 +1702,7 @@ __global__ void __launch_bounds__(Dkv<E, D>::kThreads, Dkv<E, D>::kPerSm)
             for (int i = 0; i < 16; ++i) {
               const float f = f0 * dec.cf[i0 + i];
               x[i] *= f;
-              tok = fmaf(-x[i], z[i], tok);
+              tok = fmaf(x[i], z[i], tok);
               z[i] *= f;
             }
           } else {
@@ -1671,7 +1710,7 @@ __global__ void __launch_bounds__(Dkv<E, D>::kThreads, Dkv<E, D>::kPerSm)
             for (int i = 0; i < 16; ++i) {
               const float f = dec.from(rh, rl, i0 + i);
               const float pf = x[i] * f;
-              tok -= i0 + i > row ? pf * z[i] : 0.f;
+              tok += i0 + i > row ? pf * z[i] : 0.f;
               x[i] = i0 + i >= row ? pf : 0.f;
               z[i] = i0 + i >= row ? z[i] * f : 0.f;
             }
@@ -1772,9 +1811,7 @@ __global__ void __launch_bounds__(Dkv<E, D>::kThreads, Dkv<E, D>::kPerSm)
         store_row16<E>(p.dK, b, h, p.H, t0 + row, p.T, j0, p.dk, x);
     }
     bk *= to_end;
-    token_share<W>(sm.a, q, wg, row, tok - bk);
-    bk = warp_sum(bk);
-    if (lane == 0) sm.red2[warp] = bk;
+    token_sums<W>(sm.a, q, wg, row, tok, bk);
     if (!F::kE) {  // over Q and what else has been read
       sync();
       scale();
@@ -2027,7 +2064,7 @@ size_t part_floats(const Blocks& n, bool fwd) {
 }
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
-size_t sums_floats(const Plan& pl, long long BH, long long T) { return (size_t)BH * (T + pl.nchunks); }
+size_t sums_floats(const Plan& pl, long long BH, long long T) { return (size_t)BH * (2 * T + 16 * (size_t)pl.nchunks); }
 
 template <typename E, int D>
 size_t workspace_bytes_of(bool fwd, int64_t B, int H, int64_t T, int dk, int dv) {
@@ -2056,7 +2093,8 @@ int run_blocks(Args<E>& a, bool fwd, const float* lg, const int64_t* s, int64_t 
   const size_t rows = (size_t)BH * T * 64;
   char* rest = static_cast<char*>(ws) + up256(seg_bytes(pl, BH));
   if (!fwd) {
-    a.tq = reinterpret_cast<float*>(rest), a.aq = a.tq + (size_t)BH * T;
+    a.quarters = reinterpret_cast<float*>(rest);  // aligned
+    a.rows_R = a.quarters + (size_t)BH * 16 * pl.nchunks, a.state_q = a.rows_R + (size_t)BH * T;
     rest += up256(sums_floats(pl, BH, T) * sizeof(float));
   }
   float* part = reinterpret_cast<float*>(rest);
@@ -2089,7 +2127,7 @@ int run_blocks(Args<E>& a, bool fwd, const float* lg, const int64_t* s, int64_t 
         if (whole.dH0) a.dH0 = whole.dH0 + s0;
         a.dlg_add = i + j > 0;
       }
-      if (whole.saved) a.saved = whole.saved + (size_t)(j * n.nk + i) * BH * (pl.nchunks + 1) * D * D;
+      if (whole.saved) a.saved = whole.saved + (size_t)(j * n.nk + i) * BH * pl.nchunks * D * D;
       if constexpr (std::is_same_v<E, bf16>) {
         bool ok = map_of(&a.mQ, a.Q, dk, T, H, B) && map_of(&a.mK, a.K, dk, T, H, B) &&
                   map_of(&a.mV, a.V, dv, T, H, B);
@@ -2136,8 +2174,7 @@ size_t mgs_linear_attn_saved_size(int64_t B, int H, int64_t T, int dk, int dv, i
   (void)by_shape(dtype, dk, dv, [&](auto, auto d) -> int {
     constexpr int D = decltype(d)::value;
     const Blocks blocks(dk, dv, D);
-    n = (size_t)blocks.nk * blocks.nv * (size_t)(B * H) * (size_t)((T + kC - 1) / kC + 1) * D * D *
-        sizeof(float);
+    n = (size_t)blocks.nk * blocks.nv * (size_t)(B * H) * (size_t)((T + kC - 1) / kC) * D * D * sizeof(float);
     return MGS_OK;
   });
   return n;

@@ -343,3 +343,43 @@ def test_under_compile(cuda):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     for a, b in zip(torch.autograd.grad(got, x, (dy, dH)), torch.autograd.grad(want, x, (dy, dH))):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("T", [1, 5, 33, 128, 200, 700])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_first_token_without_a_state_has_no_decay_gradient(T, dtype):
+    """dlog_gamma_0 = gamma_0 <H0, dS_0>: exactly zero when nothing enters, not what sums cancel to."""
+    import mingru_b200 as mb
+
+    g = torch.Generator(device="cuda").manual_seed(T)
+    q, k, v, dy = (torch.randn(2, 3, T, 40, device="cuda", generator=g).to(dtype) for _ in range(4))
+    lg = (-0.2 * torch.rand(2, 3, T, device="cuda", generator=g)).requires_grad_(True)
+    y, H = mb.linear_attention(q, k, v, lg)
+    (dlg,) = torch.autograd.grad((y, H), (lg,), (dy, torch.ones_like(H)))
+    assert dlg[..., 0].abs().max().item() == 0.0
+
+
+@pytest.mark.parametrize("T", [260, 500, 1000])
+def test_decay_gradient_of_a_short_memory(T):
+    """A decay of a few tokens: dlog_gamma_t is a sum over few pairs, and is as exact as these.
+
+    R_ij = e^{c_i - c_j} (q_i . k_j)(dy_i . v_j), each within 2^-19 of its size (products of 64 in fp32,
+    factors within some 2^-21); a token takes the pairs of 16 tokens' rows and columns at most twice:
+    within 32 * 2 * 2^-19 of the largest row's or column's sum of sizes.
+    """
+    import mingru_b200 as mb
+
+    g = torch.Generator(device="cuda").manual_seed(T)
+    q, k, v, dy = (torch.randn(2, 2, T, 64, device="cuda", generator=g).bfloat16() for _ in range(4))
+    lg = torch.full((2, 2, T), -0.2, device="cuda", requires_grad=True)
+    y, _ = mb.linear_attention(q, k, v, lg)
+    (dlg,) = torch.autograd.grad(y, (lg,), dy)
+    qd, kd, vd, dyd = (t.double() for t in (q, k, v, dy))
+    i = torch.arange(T, device="cuda")
+    D = torch.where(i[:, None] >= i, torch.exp(-0.2 * (i[:, None] - i).clamp_min(0).double()), 0.0)
+    R = D * (qd @ kd.mT) * (dyd @ vd.mT)
+    # over pairs i >= t > j: the suffix over rows of the prefix over columns before t
+    before = torch.cat((torch.zeros_like(R[..., :1]), R.cumsum(-1)[..., :-1]), -1)
+    ref = torch.stack([before[..., t:, t].sum(-1) for t in range(T)], -1)
+    most = torch.maximum(R.abs().sum(-1).amax(), R.abs().sum(-2).amax())
+    assert (dlg.double() - ref).abs().max() <= 64 * 2**-19 * most
