@@ -11,11 +11,11 @@ def test_sizes():
     from mingru_b200 import _lib
 
     lib = _lib.load()
-    # states at each chunk of 128 tokens and at the end, 64 x 64 or 128 x 128 in fp32
-    assert lib.mgs_linear_attn_saved_size(2, 3, 300, 64, 40, 1) == 6 * 4 * 64 * 64 * 4
-    assert lib.mgs_linear_attn_saved_size(2, 3, 300, 65, 40, 1) == 6 * 4 * 128 * 128 * 4
+    # states at each chunk of 128 tokens, 64 x 64 or 128 x 128 in fp32
+    assert lib.mgs_linear_attn_saved_size(2, 3, 300, 64, 40, 1) == 6 * 3 * 64 * 64 * 4
+    assert lib.mgs_linear_attn_saved_size(2, 3, 300, 65, 40, 1) == 6 * 3 * 128 * 128 * 4
     # fp32 heads of 130 x 70: three blocks by two
-    assert lib.mgs_linear_attn_saved_size(1, 1, 128, 130, 70, 0) == 6 * 2 * 64 * 64 * 4
+    assert lib.mgs_linear_attn_saved_size(1, 1, 128, 130, 70, 0) == 6 * 1 * 64 * 64 * 4
     assert lib.mgs_linear_attn_saved_size(1, 1, 128, 129, 8, 1) == 0
     assert lib.mgs_linear_attn_saved_size(-1, 1, 128, 8, 8, 1) == 0
     assert lib.mgs_linear_attn_workspace_size(1, 1, 128, 8, 8, 9) == 0
