@@ -40,10 +40,10 @@
 // kernels then run all segments at once, chunk by chunk inside each.
 //
 // What bounds them (8 x 8 heads of 64, T = 8192, bf16, 0.54 GB for forward and
-// backward: 84 us at copy speed; 430 are taken): neither DRAM (24 to 49% of its peak)
-// nor the tensor pipe (22 to 25%) but the chain inside a chunk -- products, mask,
+// backward: 84 us at copy speed; 430 are taken): neither DRAM (27 to 48% of its peak)
+// nor the tensor pipe (22 to 26%) but the chain inside a chunk -- products, mask,
 // products that use it, sums that read those -- of which an SM has two under way, and
-// the instructions of masking, scaling and rounding (38 to 47% of the issue slots).
+// the instructions of masking, scaling and rounding (37 to 47% of the issue slots).
 // So the work on this chain is what each choice below is about.
 #include <type_traits>
 
@@ -1201,8 +1201,8 @@ __device__ __forceinline__ void packed16_to_tile(bf16* tile, int r, int c0, cons
 // dQ = A1 K + decayed dy S^T with A1 = D * dy V^T, and R's rows, from A1 and Q K^T.
 // Chunks are independent, so that CTAs fill all SMs and take every so many; the next
 // chunk's tiles load as each becomes free. Reads most of all kernels (four tiles and a
-// state to a chunk) and comes nearest to DRAM's limit, 49%. 64 heads, T = 8192, bf16:
-// 80 us (512 threads at 64 registers: 124); heads of 128 (16, T = 4096): 33; fp32 (64
+// state to a chunk) and comes nearest to DRAM's limit, 48%. 64 heads, T = 8192, bf16:
+// 81 us (512 threads at 64 registers: 124); heads of 128 (16, T = 4096): 33; fp32 (64
 // heads, T = 1024): 55.
 //
 // TMEM columns: (dy V^T) 0..127 and (Q K^T) 128..255. One level: the masked A1 in

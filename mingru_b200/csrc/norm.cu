@@ -311,10 +311,10 @@ __global__ void __launch_bounds__(MAXT, fwd_ctas(MAXT)) fwd_kernel(const Args p)
 // GATE and SCALE: whether they are there, so that a call without them keeps no
 // registers for them. The seven arrays leave no registers for a row ahead, so rows
 // come through shared memory, the next on its way during this one, where the SM has
-// room for two rows' inputs of all its CTAs (groups up to 2048 in bf16 with few
-// inputs, or wider with one CTA): 16384 x 2048 bf16 with a residual 77 us, straight
-// 112; 65536 x 512 in 8 gated groups 78, 116 (0.41 GB: 4.3 TB/s, by its 450
-// instructions to 8 elements); 8192 x 512 fp32 14.1, 14.5.
+// room for two rows' inputs of all its CTAs: 16384 x 2048 bf16 with a residual takes
+// 77 us so and 112 straight, 65536 x 512 in 8 gated groups 78 and 116 (0.34 GB, 4.3
+// TB/s: 440 instructions to 8 elements of a warp's lanes, 69% of the issue slots),
+// 8192 x 512 fp32 14.1 and 14.5.
 template <typename E, typename W, int VEC, int K, int MAXT, bool GATE, bool SCALE>
 __global__ void __launch_bounds__(MAXT, bwd_ctas(MAXT)) bwd_kernel(const Args p) {
   constexpr int N = K * VEC;
