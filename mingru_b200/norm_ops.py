@@ -28,14 +28,10 @@ def _rows(t: torch.Tensor | None, D: int):
     if t.is_contiguous():
         return t, D
     if t.stride(-1) == 1 or D == 1:
-        if t.dim() == 1:
-            return t, D
-        # one stride from row to row over all the leading dimensions
-        s, ok = t.stride(-2), True
-        for i in range(t.dim() - 2):
-            ok = ok and (t.shape[i] == 1 or t.stride(i) == t.stride(i + 1) * t.shape[i + 1])
-        if ok and all(n > 0 for n in t.shape):
-            return t, s
+        # one stride from row to row over all the leading dimensions; one of size 1 has none that counts
+        lead = [(n, s) for n, s in zip(t.shape[:-1], t.stride()) if n != 1]
+        if all(s == inner * n for (_, s), (n, inner) in zip(lead, lead[1:])):
+            return t, lead[-1][1] if lead else D
     return t.contiguous(), D
 
 
