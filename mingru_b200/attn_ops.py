@@ -37,6 +37,14 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """An output in ``t``'s memory order, its last dimension dense, as the kernels
+    write it: PyTorch puts another one innermost where it is as dense in ``t``
+    (overlapping windows, heads)."""
+    o = torch.empty_like(t)
+    return o if o.stride(-1) == 1 or o.shape[-1] == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _strides(*ts: torch.Tensor):
     flat = []
     for t in ts:
@@ -60,7 +68,7 @@ def _forward(Q, K, V, lg, H0, save):
         dv = V.shape[3]
         code = _dtype_code(_OP, Q)
         n, nsaved = _sizes(dev.index, B, H, T, dk, dv, code)
-        y = torch.empty_like(V)
+        y = _like(V)
         HT = lg.new_empty((B, H, dk, dv))  # log_gamma is fp32 and on the same device
         saved = lg.new_empty(nsaved) if save else None
         if T == 0:  # no token: the state passes through
@@ -103,7 +111,7 @@ def _gradients(Q, K, V, lg, saved, dy, dHT, want_dH0):
         B, H, T, dk = Q.shape
         dv = V.shape[3]
         code = _dtype_code(_OP, Q)
-        dQ, dK, dV = torch.empty_like(Q), torch.empty_like(K), torch.empty_like(V)
+        dQ, dK, dV = _like(Q), _like(K), _like(V)
         dlg = lg.new_empty((B, H, T))
         dH0 = lg.new_empty((B, H, dk, dv)) if want_dH0 else None
         if dHT is not None:

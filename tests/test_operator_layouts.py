@@ -42,3 +42,47 @@ def test_rows_are_read_in_place():
                   (torch.zeros(4, 6, 8)[..., 1:5], 8)):
         t, got = _rows(x, x.shape[-1])
         assert t is x and got == ld
+
+
+def _attention_views():
+    """(1, 1, T, d) views and what is to be dense of them: the last dimension, for every output."""
+    line = torch.zeros(937)
+    yield line.as_strided((1, 1, 8, 64), (937, 937, 1, 1))  # sliding windows: time is as dense
+    yield line.as_strided((1, 4, 8, 64), (937, 1, 64, 1))  # heads that overlap
+    yield line.as_strided((4, 1, 8, 64), (1, 937, 64, 1))
+    yield torch.zeros(2, 3, 64, 8).transpose(2, 3)
+    yield torch.zeros(2, 8, 3, 64).transpose(1, 2)
+    yield torch.zeros(2, 1, 8, 64).expand(2, 3, 8, 64)
+    yield torch.zeros(2, 3, 8, 1).expand(2, 3, 8, 64)
+    yield torch.zeros(2, 3, 8, 65)[..., 1:]
+    yield torch.zeros(1, 1, 1, 64)
+    yield torch.zeros(3, 8, 2, 1).permute(2, 0, 1, 3)
+
+
+def _one_place_each(t):
+    """Every element in a place of its own, rows dense: what a kernel writes row by row."""
+    places = torch.zeros(t.shape, dtype=torch.int64)
+    for n, s, d in zip(t.shape, t.stride(), range(t.dim())):
+        places += (torch.arange(n) * s).view([-1 if i == d else 1 for i in range(t.dim())])
+    return places.unique().numel() == t.numel() and (t.stride(-1) == 1 or t.shape[-1] == 1)
+
+
+@pytest.mark.parametrize("x", list(_attention_views()), ids=lambda x: f"{tuple(x.shape)}-{x.stride()}")
+def test_outputs_of_attention_are_dense_rows(x, monkeypatch):
+    """The C entry takes no stride of the last dimension: outputs have 1 there, whatever the inputs' order."""
+    import contextlib
+
+    from mingru_b200 import attn_ops
+
+    class Library:
+        mgs_linear_attn_fwd = mgs_linear_attn_bwd = staticmethod(lambda *a: 0)
+
+    monkeypatch.setattr(attn_ops._lib, "load", lambda: Library)
+    monkeypatch.setattr(attn_ops, "_sizes", lambda *a: (0, 0))
+    monkeypatch.setattr(attn_ops, "on_device", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(attn_ops, "raw_stream", lambda d: 0)
+    lg = torch.zeros(x.shape[:3])
+    y, HT, saved = attn_ops._forward(x, x, x, lg, None, True)
+    assert _one_place_each(y) and _one_place_each(HT)
+    for g in attn_ops._gradients(x, x, x, lg, saved, y, None, True):
+        assert _one_place_each(g)
