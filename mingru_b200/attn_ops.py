@@ -63,6 +63,13 @@ def _sizes(device: int, B: int, H: int, T: int, dk: int, dv: int, code: int) -> 
             lib.mgs_linear_attn_saved_size(B, H, T, dk, dv, code) // 4)
 
 
+def _saved_floats(B, H, T, dk, dv, dtype):
+    """What ``mgs_linear_attn_saved_size`` asks for, of sizes that may be a compiler's
+    symbols: a D x D state at every chunk of 128 tokens of every block of a head."""
+    D = 128 if dtype == torch.bfloat16 and (dk > 64 or dv > 64) else 64
+    return B * H * ((T + 127) // 128) * (-(-dk // D)) * (-(-dv // D)) * D * D
+
+
 def _forward(Q, K, V, lg, H0, save):
     dev = Q.device
     with on_device(dev):  # sizes are queried on the launch device
@@ -102,9 +109,9 @@ def _linear_attn_fwd(
 @_linear_attn_fwd.register_fake
 def _(Q, K, V, lg, H0, save):
     B, H, T, dk = Q.shape
-    return (_like(V), Q.new_empty((B, H, dk, V.shape[3]), dtype=torch.float32),
-            Q.new_empty((_sizes(Q.device.index, B, H, T, dk, V.shape[3], _dtype_code(_OP, Q))[1] if save else 0,),
-                        dtype=torch.float32))
+    dv = V.shape[3]
+    return (_like(V), Q.new_empty((B, H, dk, dv), dtype=torch.float32),
+            Q.new_empty((_saved_floats(B, H, T, dk, dv, Q.dtype) if save else 0,), dtype=torch.float32))
 
 
 def _gradients(Q, K, V, lg, saved, dy, dHT, want_dH0):

@@ -33,3 +33,40 @@ def test_strides_that_the_fakes_give(fake):
     assert dK.stride() == (450 * 32, 150 * 32, 32, 1)
     assert y.stride() == dV.stride() and y.stride(-1) == 1
     assert H.stride() == dH0.stride() == (3 * 32 * 40, 32 * 40, 40, 1) and dlg.stride() == (450, 150, 1)
+
+
+def test_saved_states_of_the_fake_are_the_librarys(fake):
+    from mingru_b200 import _lib
+
+    size = _lib.load().mgs_linear_attn_saved_size
+    for code, dtype in enumerate((torch.float32, torch.bfloat16, torch.float16)):
+        for B, H, T, dk, dv in [(2, 3, 300, 64, 40), (1, 1, 1, 1, 1), (1, 2, 128, 65, 3), (3, 1, 129, 7, 128),
+                                (2, 2, 0, 8, 8), (0, 2, 5, 8, 8), (1, 3, 5000, 128, 128), (2, 1, 257, 130, 70)]:
+            if dtype == torch.bfloat16 and max(dk, dv) > 128:
+                continue  # not a call of the op's
+            Q, V, lg = _cuda(B, H, T, dk, dtype=dtype), _cuda(B, H, T, dv, dtype=dtype), _cuda(B, H, T)
+            saved = torch.ops.mingru_b200.linear_attn_fwd(Q, Q, V, lg, None, True)[2]
+            assert 4 * saved.numel() == size(B, H, T, dk, dv, code)
+
+
+def test_lengths_that_are_symbols():
+    """Dynamic shapes: batch and length are not numbers while a compiler looks at the op."""
+    import mingru_b200  # noqa: F401
+    from torch._dynamo.source import ConstantSource
+    from torch.fx.experimental.symbolic_shapes import DimDynamic, StatelessSymbolicContext
+
+    mode = FakeTensorMode(shape_env=ShapeEnv())
+
+    def symbolic(name, *shape):
+        kinds = [DimDynamic.DYNAMIC if i in (0, 2) else DimDynamic.STATIC for i in range(len(shape))]
+        return mode.from_tensor(torch.empty(*shape, device="meta"), source=ConstantSource(name),
+                                symbolic_context=StatelessSymbolicContext(kinds))
+
+    q, g = symbolic("q", 2, 3, 300, 64), symbolic("g", 2, 3, 300)
+    assert not isinstance(q.shape[2], int)
+    with mode:
+        y, H, saved = torch.ops.mingru_b200.linear_attn_fwd(q, q, q, g, None, True)
+        assert y.shape == q.shape
+        assert saved.shape[0].node.expr.free_symbols == (q.shape[0] * q.shape[2]).node.expr.free_symbols
+        grads = torch.ops.mingru_b200.linear_attn_bwd(q, q, q, g, saved, y, None, False)
+        assert all(t.shape == q.shape for t in grads[:3]) and grads[4].numel() == 0
