@@ -24,7 +24,7 @@ import functools
 import torch
 
 from . import _lib
-from .scan_ops import _dense, _dtype_code, _ptr, _require_cuda, on_device, raw_stream
+from .scan_ops import _dense, _dtype_code, _ptr, _require_cuda, _wants_grad, on_device, raw_stream
 
 __all__ = ["linear_attention"]
 
@@ -207,10 +207,10 @@ def _run(Q, K, V, lg, H0):
         # the fp32 kernels take blocks of any number, added before the one rounding
         y, HT = _run(Q.float(), K.float(), V.float(), lg, H0)
         return y.to(Q.dtype), HT
+    save = _wants_grad(Q, K, V, lg, H0)
     if torch.compiler.is_compiling():
-        return _linear_attn_fwd(Q, K, V, lg, H0, True)[:2]
-    if torch.is_grad_enabled() and (Q.requires_grad or K.requires_grad or V.requires_grad
-                                    or lg.requires_grad or (H0 is not None and H0.requires_grad)):
+        return _linear_attn_fwd(Q, K, V, lg, H0, save)[:2]
+    if save:
         return _Eager.apply(Q, K, V, lg, H0)
     return _forward(Q, K, V, lg, H0, False)[:2]
 

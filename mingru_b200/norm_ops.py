@@ -14,7 +14,7 @@ import functools
 import torch
 
 from . import _lib
-from .scan_ops import _dense, _dtype_code, _ptr, _require_cuda, _workspace, on_device, raw_stream
+from .scan_ops import _dense, _dtype_code, _ptr, _require_cuda, _wants_grad, _workspace, on_device, raw_stream
 
 __all__ = ["block_norm"]
 
@@ -72,16 +72,18 @@ def _forward(x, weight, bias, residual, scale, gate, groups, eps, rms, save):
 def _block_norm_fwd(
     x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, residual: torch.Tensor | None,
     scale: torch.Tensor | None, gate: torch.Tensor | None, groups: int, eps: float, rms: bool,
+    save: bool,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    y, h, stats = _forward(x, weight, bias, residual, scale, gate, groups, eps, rms, True)
-    return y, x.new_empty(0) if h is None else h, stats
+    y, h, stats = _forward(x, weight, bias, residual, scale, gate, groups, eps, rms, save)
+    return (y, x.new_empty(0) if h is None else h,
+            x.new_empty(0, dtype=torch.float32) if stats is None else stats)
 
 
 @_block_norm_fwd.register_fake
-def _(x, weight, bias, residual, scale, gate, groups, eps, rms):
+def _(x, weight, bias, residual, scale, gate, groups, eps, rms, save):
     y = x.new_empty(x.shape)
     h = x.new_empty(x.shape) if residual is not None else x.new_empty((0,))
-    return y, h, x.new_empty((x.numel() // x.shape[-1] * groups * 3,), dtype=torch.float32)
+    return y, h, x.new_empty((x.numel() // x.shape[-1] * groups * 3 if save else 0,), dtype=torch.float32)
 
 
 def _gradients(x, weight, bias, residual, scale, gate, stats, dy, dh, groups, rms):
@@ -128,7 +130,7 @@ def _(x, weight, bias, residual, scale, gate, stats, dy, dh, groups, rms):
 
 
 def _setup(ctx, inputs, output):
-    x, weight, bias, residual, scale, gate, groups, _eps, rms = inputs
+    x, weight, bias, residual, scale, gate, groups, _eps, rms, _save = inputs
     ctx.save_for_backward(x, weight, bias, residual, scale, gate, output[2])
     ctx.groups, ctx.rms = groups, rms
     ctx.mark_non_differentiable(output[2], *(() if residual is not None else (output[1],)))
@@ -140,14 +142,14 @@ def _backward(ctx, dy, dh, _gstats=None, run=_block_norm_bwd):
         raise RuntimeError(f"{_OP} does not support second-order autograd (create_graph=True)")
     x, weight, bias, residual, scale, gate, stats = ctx.saved_tensors
     if dy is None and dh is None:
-        return (None,) * 9
+        return (None,) * 10
     if dy is None:
         dy = torch.zeros_like(x)
     dx, dw, db, dres, ds, dgate = run(x, weight, bias, residual, scale, gate, stats, dy,
                                       dh if residual is not None else None, ctx.groups, ctx.rms)
     return (dx, dw, db if bias is not None else None,
             None if residual is None else dx if scale is None else dres,
-            ds if scale is not None else None, dgate if gate is not None else None, None, None, None)
+            ds if scale is not None else None, dgate if gate is not None else None, None, None, None, None)
 
 
 torch.library.register_autograd("mingru_b200::block_norm_fwd", _backward, setup_context=_setup)
@@ -166,7 +168,7 @@ class _Eager(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy, dh=None):
-        return _backward(ctx, dy, dh, run=_gradients)
+        return _backward(ctx, dy, dh, run=_gradients)[:9]
 
 
 def block_norm(
@@ -209,9 +211,10 @@ def block_norm(
     given = [t for t in (x, weight, bias, residual, scale, gate) if t is not None]
     _require_cuda(_OP, *given)
     args = (x, weight, bias, residual, scale, gate, groups, float(eps), bool(rms))
+    save = _wants_grad(*given)
     if torch.compiler.is_compiling():
-        y, h, _ = _block_norm_fwd(*args)
-    elif torch.is_grad_enabled() and any(t.requires_grad for t in given):
+        y, h, _ = _block_norm_fwd(*args, save)
+    elif save:
         return _Eager.apply(*args)
     else:
         y, h, _ = _forward(*args, False)

@@ -76,6 +76,10 @@ def raw_stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+def _wants_grad(*ts: torch.Tensor | None) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
 def _ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 

@@ -70,3 +70,38 @@ def test_lengths_that_are_symbols():
         assert saved.shape[0].node.expr.free_symbols == (q.shape[0] * q.shape[2]).node.expr.free_symbols
         grads = torch.ops.mingru_b200.linear_attn_bwd(q, q, q, g, saved, y, None, False)
         assert all(t.shape == q.shape for t in grads[:3]) and grads[4].numel() == 0
+
+
+def _compiled_calls(f, *args):
+    """Name and arguments of every op that a compiler sees in f(*args)."""
+    calls = []
+
+    def backend(gm, _):
+        calls.extend((str(n.target), n.args) for n in gm.graph.nodes if "mingru_b200" in str(n.target))
+        return gm.forward
+
+    torch._dynamo.reset()
+    torch.compile(f, backend=backend, fullgraph=True)(*args)
+    return dict(calls)
+
+
+def test_compiled_inference_saves_nothing(fake):
+    """States and statistics are for a backward: written only where one can follow, compiled as eager."""
+    import mingru_b200 as mb
+
+    q, lg, w = _cuda(1, 2, 300, 32), _cuda(1, 2, 300), _cuda(32)
+
+    def f(q, lg, w):
+        return mb.linear_attention(q, q, q, lg), mb.block_norm(q, w)
+
+    def saves():
+        calls = _compiled_calls(f, q, lg, w)
+        return (calls["mingru_b200.linear_attn_fwd.default"][-1], calls["mingru_b200.block_norm_fwd.default"][-1])
+
+    assert saves() == (False, False)  # no tensor wants a gradient
+    q.requires_grad_(True)
+    assert saves() == (True, True)
+    with torch.no_grad():
+        assert saves() == (False, False)
+    stats = torch.ops.mingru_b200.block_norm_fwd(q.detach(), w, None, None, None, None, 1, 1e-5, False, False)[2]
+    assert stats.numel() == 0
