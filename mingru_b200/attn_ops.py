@@ -24,7 +24,7 @@ import functools
 import torch
 
 from . import _lib
-from .scan_ops import _dense, _dtype_code, _ptr, _require_cuda, _wants_grad, on_device, raw_stream
+from .scan_ops import _dense, _dtype_code, _ptr, _require_cuda, _traced, _wants_grad, on_device, raw_stream
 
 __all__ = ["linear_attention"]
 
@@ -208,7 +208,7 @@ def _run(Q, K, V, lg, H0):
         y, HT = _run(Q.float(), K.float(), V.float(), lg, H0)
         return y.to(Q.dtype), HT
     save = _wants_grad(Q, K, V, lg, H0)
-    if torch.compiler.is_compiling():
+    if _traced(Q, K, V, lg, H0):
         return _linear_attn_fwd(Q, K, V, lg, H0, save)[:2]
     if save:
         return _Eager.apply(Q, K, V, lg, H0)

@@ -14,7 +14,8 @@ import functools
 import torch
 
 from . import _lib
-from .scan_ops import _dense, _dtype_code, _ptr, _require_cuda, _wants_grad, _workspace, on_device, raw_stream
+from .scan_ops import (_dense, _dtype_code, _ptr, _require_cuda, _traced, _wants_grad, _workspace, on_device,
+                       raw_stream)
 
 __all__ = ["block_norm"]
 
@@ -212,7 +213,7 @@ def block_norm(
     _require_cuda(_OP, *given)
     args = (x, weight, bias, residual, scale, gate, groups, float(eps), bool(rms))
     save = _wants_grad(*given)
-    if torch.compiler.is_compiling():
+    if _traced(*given):
         y, h, _ = _block_norm_fwd(*args, save)
     elif save:
         return _Eager.apply(*args)

@@ -76,6 +76,14 @@ def raw_stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+def _traced(*ts: torch.Tensor | None) -> bool:
+    """Whether a compiler, a dispatch mode, a tensor subclass or a function transform
+    is to see a call: then it goes through its custom op and not straight to the kernels."""
+    return (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
+            or torch._C._are_functorch_transforms_active()
+            or any(t is not None and type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter for t in ts))
+
+
 def _wants_grad(*ts: torch.Tensor | None) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 

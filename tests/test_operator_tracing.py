@@ -105,3 +105,35 @@ def test_compiled_inference_saves_nothing(fake):
         assert saves() == (False, False)
     stats = torch.ops.mingru_b200.block_norm_fwd(q.detach(), w, None, None, None, None, 1, 1e-5, False, False)[2]
     assert stats.numel() == 0
+
+
+def test_calls_under_dispatch_modes(fake):
+    """Fake tensors, tracers and dispatch modes see the ops, as they see the scans'."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    import mingru_b200 as mb
+
+    class Seen(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.names = set()
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.names.add(str(func))
+            return func(*args, **(kwargs or {}))
+
+    q, lg, w = _cuda(1, 2, 300, 32), _cuda(1, 2, 300), _cuda(32)
+    ops = {"mingru_b200.linear_attn_fwd.default", "mingru_b200.block_norm_fwd.default"}
+
+    def f(q, lg, w):
+        y, H = mb.linear_attention(q, q, q, lg)
+        return mb.block_norm(y, w), H
+
+    for grad in (False, True):
+        q.requires_grad_(grad)
+        with Seen() as seen:
+            y, H = f(q, lg, w)
+        assert y.shape == q.shape and H.shape == (1, 2, 32, 32) and y.requires_grad == grad
+        assert ops <= seen.names
+        assert ops <= {str(n.target) for n in make_fx(f)(q, lg, w).graph.nodes}

@@ -70,3 +70,33 @@ def test_fakes_against_the_op(cuda, transposed, save):
         y, H, saved = torch.ops.mingru_b200.linear_attn_fwd(*args)
         torch.library.opcheck(torch.ops.mingru_b200.linear_attn_bwd, (*args[:4], saved, y, H, True),
                               test_utils=("test_schema", "test_faketensor"))
+
+
+def test_under_a_dispatch_mode(cuda):
+    """A mode sees the ops, forward and backward, and results are those of calls without one."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    import mingru_b200 as mb
+
+    class Seen(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.names = set()
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.names.add(str(func))
+            return func(*args, **(kwargs or {}))
+
+    def f(q, lg, w):
+        y = mb.block_norm(mb.linear_attention(q, q, q, lg)[0], w)
+        return [y, *torch.autograd.grad(y, (q, lg, w), y.detach())]
+
+    g = torch.Generator(device=cuda).manual_seed(0)
+    x = [torch.randn(1, 2, 300, 32, device=cuda, generator=g), -torch.rand(1, 2, 300, device=cuda, generator=g),
+         1 + torch.rand(32, device=cuda, generator=g)]
+    x = [t.requires_grad_(True) for t in x]
+    with Seen() as seen:
+        got = f(*x)
+    assert {f"mingru_b200.{n}.default" for n in ("linear_attn_fwd", "linear_attn_bwd", "block_norm_fwd",
+                                                 "block_norm_bwd")} <= seen.names
+    assert all(torch.equal(a, b) for a, b in zip(got, f(*x)))
