@@ -609,6 +609,8 @@ def _add_norm(x, branch, norm):
     """``(norm(x + branch), x + branch)`` by one kernel; ``branch`` may be ``None``."""
     if branch is None:
         return block_norm(x, norm.weight, norm.bias, eps=norm.eps), x
+    if branch.dtype != x.dtype:  # as the sum promotes them
+        x, branch = (t.to(torch.promote_types(x.dtype, branch.dtype)) for t in (x, branch))
     return block_norm(branch, norm.weight, norm.bias, residual=x, eps=norm.eps)
 
 
