@@ -558,7 +558,8 @@ class RetentionMinGRU(DecayMixin, nn.Module):
         k = F.normalize(self.linear_k(x).view(*lead, self.n_heads, self.d_k), dim=-1)
         a = self.linear_z(x)
         v = torch.sigmoid(a).unsqueeze(-1) * self.linear_v(x).view(*lead, self.n_heads, self.d_v)
-        log_gamma = -F.softplus(a.float())  # log(1 - z)
+        # log(1 - z); softplus's backward has other strides under a compiler than it has
+        log_gamma = F.logsigmoid(-a.float())
         if dt is not None:
             log_gamma = log_gamma - self._decay_lambda() * dt.unsqueeze(-1)
         return q, k, v, log_gamma

@@ -43,12 +43,13 @@ def test_attention_at_several_lengths(cuda, dynamic, dtype):
         _same(f, mb.linear_attention, x, w)
 
 
-def test_retention_at_several_lengths(cuda):
+@pytest.mark.parametrize("dynamic", [True, False])
+def test_retention_at_several_lengths(cuda, dynamic):
     import mingru_b200 as mb
 
     torch.manual_seed(0)
     mod = mb.RetentionMinGRU(24, 64, n_heads=2).to(cuda)
-    compiled = torch.compile(mod, backend="aot_eager", dynamic=True)
+    compiled = torch.compile(mod, backend="aot_eager", dynamic=dynamic)
     for T in (140, 260):
         x = torch.randn(2, T, 24, device=cuda, requires_grad=True)
         want, got = mod(x), compiled(x)
