@@ -20,3 +20,13 @@ def test_stream_and_branch_of_two_types(stream, branch):
         x, b = torch.empty(3, 32, device="cuda", dtype=stream), torch.empty(3, 32, device="cuda", dtype=branch)
         y, h = _add_norm(x, b, norm)
     assert y.dtype == h.dtype == (x + b).dtype == torch.float32
+
+
+def test_keys_of_zeros_in_fp16():
+    """A token whose keys are zeros (padding, no bias) has no direction, and writes nothing."""
+    from mingru_b200 import RetentionMinGRU
+
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        mod = RetentionMinGRU(16, 32, bias=False, n_heads=2).to(dtype)
+        q, k, v, log_gamma = mod._coeffs(torch.zeros(2, 3, 16, dtype=dtype), None)
+        assert not k.any() and torch.isfinite(log_gamma).all()
