@@ -556,7 +556,8 @@ class RetentionMinGRU(DecayMixin, nn.Module):
         lead = x.shape[:-1]
         q = self.linear_q(x).view(*lead, self.n_heads, self.d_k) * self.d_k**-0.5
         k = self.linear_k(x).view(*lead, self.n_heads, self.d_k)
-        k = F.normalize(k, dim=-1, eps=max(1e-12, torch.finfo(k.dtype).tiny))  # 1e-12 is 0 in fp16
+        # 1e-12 is 0 in fp16; under autocast a norm is 32 bits
+        k = F.normalize(k, dim=-1, eps=max(1e-12, torch.finfo(k.dtype).tiny)).to(q.dtype)
         a = self.linear_z(x)
         v = torch.sigmoid(a).unsqueeze(-1) * self.linear_v(x).view(*lead, self.n_heads, self.d_v)
         # log(1 - z); softplus's backward has other strides under a compiler than it has

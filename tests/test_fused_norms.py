@@ -30,3 +30,16 @@ def test_keys_of_zeros_in_fp16():
         mod = RetentionMinGRU(16, 32, bias=False, n_heads=2).to(dtype)
         q, k, v, log_gamma = mod._coeffs(torch.zeros(2, 3, 16, dtype=dtype), None)
         assert not k.any() and torch.isfinite(log_gamma).all()
+
+
+def test_coefficients_share_a_type_under_autocast(monkeypatch):
+    """Where normalising comes out in 32 bits, as under autocast, keys take the queries' type."""
+    import torch.nn.functional as F
+
+    from mingru_b200 import RetentionMinGRU
+
+    normalize = F.normalize
+    monkeypatch.setattr(F, "normalize", lambda x, **kw: normalize(x.float(), **kw))
+    mod = RetentionMinGRU(16, 32, n_heads=2).bfloat16()
+    q, k, v, _ = mod._coeffs(torch.randn(2, 3, 16).bfloat16(), None)
+    assert q.dtype == k.dtype == v.dtype == torch.bfloat16
