@@ -610,10 +610,13 @@ class RetentionMinGRU(DecayMixin, nn.Module):
 
 def _add_norm(x, branch, norm):
     """``(norm(x + branch), x + branch)`` by one kernel; ``branch`` may be ``None``."""
+    dtype = x.dtype if branch is None else torch.promote_types(x.dtype, branch.dtype)  # the sum's
+    if torch.is_autocast_enabled(x.device.type) and not dtype == norm.weight.dtype == torch.float32:
+        x = x if branch is None else x + branch
+        return norm(x), x  # comes out in 32 bits there, whatever it is given
     if branch is None:
         return block_norm(x, norm.weight, norm.bias, eps=norm.eps), x
-    if branch.dtype != x.dtype:  # as the sum promotes them
-        x, branch = (t.to(torch.promote_types(x.dtype, branch.dtype)) for t in (x, branch))
+    x, branch = x.to(dtype), branch.to(dtype)
     return block_norm(branch, norm.weight, norm.bias, residual=x, eps=norm.eps)
 
 

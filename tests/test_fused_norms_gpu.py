@@ -32,3 +32,28 @@ def test_retention_under_autocast(cuda):
             _near(out.float(), want[:, 0])
         g = torch.autograd.grad(got.float().sum(), x)[0]
     assert torch.isfinite(g).all()
+
+
+@pytest.mark.parametrize("mixer", ["log", "signed", "retention"])
+@pytest.mark.parametrize("width", [32, 20])
+def test_stack_under_autocast(cuda, mixer, width):
+    """The stream is 32 bits where there is no input projection (width = d_model), 16 where there is."""
+    import mingru_b200 as mb
+
+    torch.manual_seed(1)
+    a = mb.MinGRUStack(width, 32, 2, mixer=mixer).to(cuda)
+    b = mb.MinGRUStack(width, 32, 2, mixer=mixer, fused_norms=True).to(cuda)
+    b.load_state_dict(a.state_dict())
+    x = torch.randn(2, 40, width, device=cuda)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        ya, sa = a(x)
+        yb, sb = b(x)
+        _near(yb, ya)
+        for u, v in zip(sb, sa):
+            _near(u, v)
+        block = a.blocks[0]
+        h = torch.randn(2, 40, 32, device=cuda)
+        want = block(h)
+        block.fused_norms = True
+        for u, v in zip(block(h), want):
+            _near(u, v)
