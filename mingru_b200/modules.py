@@ -608,8 +608,20 @@ class RetentionMinGRU(DecayMixin, nn.Module):
 # ------------------------------------------------------ block / stack -----
 
 
+def _is_plain(m, cls):
+    """Whether calling ``m`` is ``cls.forward`` and nothing else -- no subclass or wrapper,
+    no hooks, no other or compiled forward -- so that its parts may run without the call."""
+    return (type(m) is cls and "forward" not in m.__dict__ and m._compiled_call_impl is None
+            and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
+            and not nn.modules.module._has_any_global_hook())
+
+
 def _add_norm(x, branch, norm):
-    """``(norm(x + branch), x + branch)`` by one kernel; ``branch`` may be ``None``."""
+    """``(norm(x + branch), x + branch)`` by one kernel; ``branch`` may be ``None``.
+    A norm that is more than a LayerNorm is called as it is."""
+    if not _is_plain(norm, nn.LayerNorm) or norm.weight is None:
+        x = x if branch is None else x + branch
+        return norm(x), x
     dtype = x.dtype if branch is None else torch.promote_types(x.dtype, branch.dtype)  # the sum's
     if torch.is_autocast_enabled(x.device.type) and not dtype == norm.weight.dtype == torch.float32:
         x = x if branch is None else x + branch
@@ -625,7 +637,8 @@ class MinGRUBlock(nn.Module):
 
     ``fused_norms``: each residual add and the LayerNorm that follows it are one
     kernel (``block_norm``), in a stack those between blocks too; the same weights
-    and the same function, rounded once where the two ops round twice."""
+    and the same function, rounded once where the two ops round twice. Blocks and
+    norms that are wrapped, replaced or hooked are called, one op after the other."""
 
     _MIXER_CLASSES: dict[str, tuple[type[nn.Module], bool]] = {
         "log": (MinGRU, True),
@@ -815,7 +828,11 @@ class MinGRUStack(nn.Module):
     def _fused(self, x, state, delta_t, step=False):
         branch, new_state = None, []
         for blk, h in zip(self.blocks, state):
-            x, branch, h = blk._fused(x, branch, h, delta_t if blk.mingru.decay is not None else None,
-                                      step=step)
+            dt = delta_t if blk.mingru.decay is not None else None
+            if _is_plain(blk, MinGRUBlock) and blk.fused_norms:
+                x, branch, h = blk._fused(x, branch, h, dt, step=step)
+            else:  # called, so that what is around it runs
+                x, branch = x if branch is None else x + branch, None
+                x, h = blk.step(x, h, dt) if step else blk(x, h, dt)
             new_state.append(h)
         return _add_norm(x, branch, self.norm_out)[0], new_state

@@ -43,3 +43,91 @@ def test_coefficients_share_a_type_under_autocast(monkeypatch):
     mod = RetentionMinGRU(16, 32, n_heads=2).bfloat16()
     q, k, v, _ = mod._coeffs(torch.randn(2, 3, 16).bfloat16(), None)
     assert q.dtype == k.dtype == v.dtype == torch.bfloat16
+
+
+def _stack():
+    """On fake CUDA tensors, in a FakeTensorMode."""
+    from mingru_b200 import MinGRUStack
+
+    with torch.device("cuda"):
+        return MinGRUStack(16, 32, 3, mixer="retention", mixer_kwargs=dict(n_heads=2), fused_norms=True)
+
+
+def test_hooks_of_blocks_and_norms_run(monkeypatch):
+    """What is hooked to a block, a norm or every module runs with fused_norms too."""
+    from mingru_b200 import step_ops
+
+    monkeypatch.setattr(step_ops, "linear_attention_step", lambda q, k, v, lg, H: (v, H))
+    with FakeTensorMode():
+        stack = _stack()
+        x = torch.empty(2, 5, 16, device="cuda")
+        seen = []
+        hooked = [*stack.blocks, stack.blocks[1].norm1, stack.blocks[2].norm2, stack.norm_out]
+        handles = [m.register_forward_hook(lambda m, a, out: seen.append(m)) for m in hooked]
+        y, _ = stack(x)
+        assert len(seen) == len(hooked) and set(seen) == set(hooked) and y.shape == (2, 5, 32)
+        for h in handles:
+            h.remove()
+        seen.clear()
+        stack.blocks[0].norm1.register_forward_pre_hook(lambda m, a: seen.append(m))
+        stack.step(x[:, 0], stack.init_state())
+        assert seen == [stack.blocks[0].norm1]
+        seen.clear()
+        handle = nn.modules.module.register_module_forward_hook(lambda m, a, out: seen.append(m))
+        stack(x)
+        handle.remove()
+        assert {*stack.blocks, *(b.norm1 for b in stack.blocks), *(b.norm2 for b in stack.blocks), stack.norm_out} <= set(seen)
+
+
+def test_replaced_parts_run():
+    """Wrapped blocks, other norms and replaced forwards are called, not gone past."""
+
+    class Wrapper(nn.Module):  # as checkpointing or sharding wraps a block
+        def __init__(self, inner):
+            super().__init__()
+            self.inner, self.calls = inner, 0
+
+        def forward(self, *args):
+            self.calls += 1
+            return self.inner(*args)
+
+        def __getattr__(self, name):
+            try:
+                return super().__getattr__(name)
+            except AttributeError:
+                return getattr(self.inner, name)
+
+    class Half(nn.LayerNorm):
+        def forward(self, x):
+            return 0.5 * super().forward(x)
+
+    with FakeTensorMode():
+        stack = _stack()
+        x = torch.empty(2, 5, 16, device="cuda")
+        stack.blocks[1] = Wrapper(stack.blocks[1])
+        calls = []
+        forward = stack.blocks[2].forward
+        stack.blocks[2].forward = lambda *a: calls.append(2) or forward(*a)
+        stack.blocks[0].norm2 = Half(32, device="cuda")
+        half = stack.blocks[0].norm2
+        half.forward = lambda t: calls.append(0) or Half.forward(half, t)
+        stack.norm_out = nn.Identity()
+        y, state = stack(x)
+        assert stack.blocks[1].calls == 1 and calls == [0, 2] and y.shape == (2, 5, 32) and len(state) == 3
+
+
+def test_fused_calls_stay_few():
+    """Without hooks every norm of a stack is one op with its sum: 3 blocks of two norms, and the last."""
+    import mingru_b200  # noqa: F401
+
+    calls = []
+
+    def backend(gm, _):
+        calls.extend(n for n in gm.graph.nodes if "block_norm_fwd" in str(n.target))
+        return gm.forward
+
+    with FakeTensorMode():
+        stack = _stack()
+        torch._dynamo.reset()
+        torch.compile(stack, backend=backend, fullgraph=True)(torch.empty(2, 5, 16, device="cuda"))
+    assert len(calls) == 7 + 3  # and the mixers' own
