@@ -640,6 +640,8 @@ class MinGRUBlock(nn.Module):
     and the same function, rounded once where the two ops round twice. Blocks and
     norms that are wrapped, replaced or hooked are called, one op after the other."""
 
+    fused_norms: bool = False  # of blocks pickled before the option
+
     _MIXER_CLASSES: dict[str, tuple[type[nn.Module], bool]] = {
         "log": (MinGRU, True),
         "signed": (SignedMinGRU, True),
@@ -763,6 +765,8 @@ class MinGRUStack(nn.Module):
     """``in_proj`` -> ``n_layers`` MinGRUBlocks -> LayerNorm, with per-block state.
 
     ``fused_norms``: residual adds and LayerNorms in one kernel each (MinGRUBlock)."""
+
+    fused_norms: bool = False
 
     def __init__(self, input_size, d_model, n_layers, mlp_expansion=4, dropout=0.0,
                  learnable_h0=False, mixer="log", mixer_kwargs=None, decay_layers="all",

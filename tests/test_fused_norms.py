@@ -131,3 +131,16 @@ def test_fused_calls_stay_few():
         torch._dynamo.reset()
         torch.compile(stack, backend=backend, fullgraph=True)(torch.empty(2, 5, 16, device="cuda"))
     assert len(calls) == 7 + 3  # and the mixers' own
+
+
+def test_modules_pickled_before_the_option():
+    """Blocks and stacks that were pickled whole before fused_norms existed have no such attribute."""
+    import copy
+
+    import mingru_b200 as mb
+
+    stack = mb.MinGRUStack(8, 16, 2)
+    for m in (stack, *stack.blocks):
+        del m.__dict__["fused_norms"]
+    old = copy.deepcopy(stack)
+    assert not old.fused_norms and not old.blocks[0].fused_norms
