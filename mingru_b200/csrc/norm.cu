@@ -181,10 +181,11 @@ __device__ __forceinline__ float sigm(float x) {
 }
 
 // 1 / sqrt(v) to the last place, by a step of Newton's on the hardware's: the
-// gradient takes differences of z * z and 1.
+// gradient takes differences of z * z and 1. 0 of an infinite sum of squares (finite
+// values past 2^64), as 1 / sqrt has it; the step would make that inf * 0.
 __device__ __forceinline__ float inv_sqrt(float v) {
   const float r = rsqrtf(v);
-  return fmaf(0.5f * r, fmaf(-v * r, r, 1.f), r);
+  return r == 0.f ? r : fmaf(0.5f * r, fmaf(-v * r, r, 1.f), r);
 }
 
 // Where a thread stands: its group (of the row), row slot and first column.
