@@ -188,6 +188,10 @@ __device__ __forceinline__ float inv_sqrt(float v) {
   return r == 0.f ? r : fmaf(0.5f * r, fmaf(-v * r, r, 1.f), r);
 }
 
+// A mean of squares that cancellation took below zero; NaN stays (fmaxf drops it, and
+// a row with a NaN came out finite but for that element).
+__device__ __forceinline__ float at_least_zero(float v) { return v < 0.f ? 0.f : v; }
+
 // Where a thread stands: its group (of the row), row slot and first column.
 struct Place {
   int slot, rs, g, t;
@@ -285,7 +289,7 @@ __global__ void __launch_bounds__(MAXT, fwd_ctas(MAXT)) fwd_kernel(const Args p)
       }
       const float2 m = sum(sq, rest);
       rest = m.y * inv_n;
-      sq = fmaxf(fmaf(-rest, rest, m.x * inv_n), 0.f);
+      sq = at_least_zero(fmaf(-rest, rest, m.x * inv_n));
     }
     const float r = inv_sqrt(sq + p.eps);
     if (p.stats && at.t == 0) {
@@ -665,7 +669,7 @@ __global__ void __launch_bounds__(MAXT, odd_fwd_ctas(MAXT)) fwd_odd_kernel(const
     });
     const float2 m = sum(sq, rs);
     const float rest = p.rms ? 0.f : m.y * inv_n;
-    const float r = inv_sqrt(fmaxf(fmaf(-rest, rest, m.x * inv_n), 0.f) + p.eps);
+    const float r = inv_sqrt(at_least_zero(fmaf(-rest, rest, m.x * inv_n)) + p.eps);
     if (p.stats && at.t == 0) {
       float* st = p.stats + (row * p.G + at.g) * 3;
       st[0] = mean, st[1] = rest, st[2] = r;

@@ -29,3 +29,32 @@ def test_squares_beyond_fp32(cuda, rms, D):
     norm.close(y[~big], want, norm.TOL[torch.float32], "y")
     dx = torch.autograd.grad(y.sum(), xl)[0]
     assert not dx[big].any() and torch.isfinite(dx).all()
+
+
+@pytest.mark.parametrize("D", [64, 512, 63, 5001])
+@pytest.mark.parametrize("rms", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_what_is_not_finite_stays_in_its_row(cuda, value, dtype, rms, D):
+    import mingru_b200 as mb
+
+    g = torch.Generator(device=cuda).manual_seed(D)
+    x, r, gate = (torch.randn(9, D, device=cuda, generator=g).to(dtype) for _ in range(3))
+    w, b, s = (1 + torch.rand(D, device=cuda, generator=g) for _ in range(3))
+    good = torch.ones(9, dtype=torch.bool, device=cuda)
+    good[3] = good[8] = False
+    x[3, D // 2] = r[8, -1] = value
+    leaves = [t.requires_grad_(True) for t in (x, r, gate)]
+    y, h = mb.block_norm(x, w, b, residual=r, scale=s, gate=gate, rms=rms)
+    d = [t.detach()[good].double().requires_grad_(True) for t in leaves]
+    want = norm.plain(d[0], w.double(), b.double(), d[1], s.double(), d[2], 1, 1e-5, rms)
+    for n, a, e in zip("yh", (y, h), want):
+        norm.close(a[good], e, norm.TOL[dtype], n)
+    bad = y[~good].detach().float()
+    assert bad.isnan().any(-1).all()  # at least where the value was; all of a row that has no mean
+    assert rms and value == float("inf") or bad.isnan().all()
+    dy = torch.randn(9, D, device=cuda, generator=g).to(dtype)
+    got = torch.autograd.grad((y, h), leaves, (dy, dy))
+    ref = torch.autograd.grad(want, d, (dy[good].double(), dy[good].double()))
+    for n, a, e in zip(("dx", "dresidual", "dgate"), got, ref):
+        norm.close(a[good], e, 3 * norm.TOL[dtype] if dtype == torch.float32 else norm.TOL[dtype], n)
