@@ -46,7 +46,7 @@ def nvcc_path() -> str:
 
 
 def _deps(src: Path) -> list[Path]:
-    return [src, *CSRC.glob("*.cuh"), *INCLUDE.glob("*.h")]
+    return [src, *CSRC.glob("*.cuh"), *CSRC.glob("*.h"), *INCLUDE.glob("*.h")]
 
 
 def _compile(src: Path, force: bool, verbose: bool) -> Path:

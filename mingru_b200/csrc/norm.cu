@@ -19,9 +19,11 @@
 // the forward. Sums over rows stay in the threads' registers while a CTA walks
 // its rows, then go through shared memory to one partial row per CTA and, in
 // order, to the result: the same bits on every run.
+#include <algorithm>
 #include <utility>
 
 #include "common.cuh"
+#include "odd_rows.h"
 
 namespace mgs {
 namespace norm {
@@ -39,6 +41,7 @@ struct Args {
   long long rows;
   int D, G, n, tpg, gpc, rpc;  // threads to a group, groups and rows to a CTA
   int rms, w32;  // weights in fp32
+  int tail;      // odd rows: the last rows, whose vectors may pass the tensors' ends
   int staged;    // backward: the inputs that come through shared memory, a row ahead; 0: straight
   float eps;
 };
@@ -535,10 +538,10 @@ struct OddRow {
     }
   }
   // The vectors of one tensor whose group starts at element `start`: loaded whole,
-  // the neighbours' elements in them too, where another row follows; and as values,
+  // the neighbours' elements in them too, where the tensor goes on; and as values,
   // zeros outside the group.
   template <typename T>
-  __device__ __forceinline__ static void load(const void* p, long long start, bool last, int sh, int n, int t,
+  __device__ __forceinline__ static void load(const void* p, long long start, bool tail, int sh, int n, int t,
                                               int tpg, uint4 (&raw)[K]) {
     const T* q = static_cast<const T*>(p) + (start - sh) + t * V;
 #pragma unroll
@@ -546,7 +549,7 @@ struct OddRow {
       const int pos = (k * tpg + t) * V;
       raw[k] = make_uint4(0, 0, 0, 0);
       if (pos < sh + n) {
-        if (!last || pos + V <= sh + n) {
+        if (odd::whole(pos, sh + n, V, tail)) {
           raw[k] = __ldg(reinterpret_cast<const uint4*>(q + k * tpg * V));
         } else {
           T e[V];
@@ -630,13 +633,13 @@ __global__ void __launch_bounds__(MAXT, odd_fwd_ctas(MAXT)) fwd_odd_kernel(const
   uint4 rx[K], ra[K];  // of the next row: x, and the residual or else the gate
   auto ahead = [&](long long row) {
     if (row >= p.rows) return;
-    const bool last = row + 1 == p.rows;
+    const bool tail = row + p.tail >= p.rows;
     const int sh = shift(row);
-    R::template load<E>(p.x, row * p.ldx + col, last, sh, p.n, at.t, p.tpg, rx);
+    R::template load<E>(p.x, row * p.ldx + col, tail, sh, p.n, at.t, p.tpg, rx);
     if (p.res)
-      R::template load<E>(p.res, row * p.ldres + col, last, sh, p.n, at.t, p.tpg, ra);
+      R::template load<E>(p.res, row * p.ldres + col, tail, sh, p.n, at.t, p.tpg, ra);
     else if (p.gate)
-      R::template load<E>(p.gate, row * p.ldgate + col, last, sh, p.n, at.t, p.tpg, ra);
+      R::template load<E>(p.gate, row * p.ldgate + col, tail, sh, p.n, at.t, p.tpg, ra);
   };
   ahead((long long)blockIdx.x * p.rpc + at.rs);
   for (long long row = (long long)blockIdx.x * p.rpc + at.rs; row < p.rows; row += step) {
@@ -654,7 +657,7 @@ __global__ void __launch_bounds__(MAXT, odd_fwd_ctas(MAXT)) fwd_odd_kernel(const
     }
     if (p.res && p.gate) {
       uint4 rg[K];
-      R::template load<E>(p.gate, row * p.ldgate + col, row + 1 == p.rows, at_row.sh, p.n, at.t, p.tpg, rg);
+      R::template load<E>(p.gate, row * p.ldgate + col, row + p.tail >= p.rows, at_row.sh, p.n, at.t, p.tpg, rg);
       at_row.template get<E>(rg, a);
     }
     float acc = 0.f;
@@ -718,15 +721,15 @@ __global__ void __launch_bounds__(MAXT, odd_bwd_ctas(MAXT)) bwd_odd_kernel(const
     float stats[3];
     auto ahead = [&](long long row) {
       if (row >= p.rows) return;
-      const bool last = row + 1 == p.rows;
+      const bool tail = row + p.tail >= p.rows;
       const int sh = shift(row);
-      R::template load<E>(p.x, row * p.ldx + col, last, sh, p.n, at.t, p.tpg, rx);
-      R::template load<E>(p.dy, row * p.lddy + col, last, sh, p.n, at.t, p.tpg, rd);
+      R::template load<E>(p.x, row * p.ldx + col, tail, sh, p.n, at.t, p.tpg, rx);
+      R::template load<E>(p.dy, row * p.lddy + col, tail, sh, p.n, at.t, p.tpg, rd);
       if (GATE)
-        R::template load<E>(p.gate, row * p.ldgate + col, last, sh, p.n, at.t, p.tpg, ra);
+        R::template load<E>(p.gate, row * p.ldgate + col, tail, sh, p.n, at.t, p.tpg, ra);
       else if (SCALE || p.res)
-        R::template load<E>(p.res, row * p.ldres + col, last, sh, p.n, at.t, p.tpg, ra);
-      if (p.dh) R::template load<E>(p.dh, row * p.lddh + col, last, sh, p.n, at.t, p.tpg, rh);
+        R::template load<E>(p.res, row * p.ldres + col, tail, sh, p.n, at.t, p.tpg, ra);
+      if (p.dh) R::template load<E>(p.dh, row * p.lddh + col, tail, sh, p.n, at.t, p.tpg, rh);
 #pragma unroll
       for (int i = 0; i < 3; ++i) stats[i] = p.stats[(row * p.G + at.g) * 3 + i];
     };
@@ -749,7 +752,7 @@ __global__ void __launch_bounds__(MAXT, odd_bwd_ctas(MAXT)) bwd_odd_kernel(const
       if (SCALE || p.res) {
         if (GATE) {
           uint4 rr[K];
-          R::template load<E>(p.res, row * p.ldres + col, row + 1 == p.rows, at_row.sh, p.n, at.t, p.tpg, rr);
+          R::template load<E>(p.res, row * p.ldres + col, row + p.tail >= p.rows, at_row.sh, p.n, at.t, p.tpg, rr);
           at_row.template get<E>(rr, z);
         }
         if constexpr (SCALE) {
@@ -1009,7 +1012,12 @@ bool plan_call(Plan& pl, const Args& a, int size, int wsize, bool fwd) {
          make_plan(pl, a.rows, a.D, a.G, size, kElements, fwd, weights);
 }
 
-void set_plan(Args& a, const Plan& pl) { a.tpg = pl.tpg, a.gpc = pl.gpc, a.rpc = pl.rpc; }
+void set_plan(Args& a, const Plan& pl) {
+  a.tpg = pl.tpg, a.gpc = pl.gpc, a.rpc = pl.rpc, a.tail = 1;
+  for (auto [q, ld] : {std::pair(a.x, a.ldx), std::pair(a.res, a.ldres), std::pair(a.gate, a.ldgate),
+                       std::pair(a.dy, a.lddy), std::pair(a.dh, a.lddh)})
+    if (q) a.tail = std::max(a.tail, odd::tail_rows(ld, pl.vec));
+}
 
 int launched() { return cudaGetLastError() == cudaSuccess ? MGS_OK : MGS_LAUNCH_FAILED; }
 

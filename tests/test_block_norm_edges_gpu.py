@@ -58,3 +58,27 @@ def test_what_is_not_finite_stays_in_its_row(cuda, value, dtype, rms, D):
     ref = torch.autograd.grad(want, d, (dy[good].double(), dy[good].double()))
     for n, a, e in zip(("dx", "dresidual", "dgate"), got, ref):
         norm.close(a[good], e, 3 * norm.TOL[dtype] if dtype == torch.float32 else norm.TOL[dtype], n)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D", [1, 2, 3, 5])
+def test_rows_shorter_than_a_vector(cuda, D, dtype):
+    norm.check(cuda, (37,), D, dtype, ("residual", "gate", "bias"), rms=True)
+
+
+def test_rows_that_overlap(cuda):
+    """Windows of one line, an element apart: rows of 9 that start everywhere."""
+    import mingru_b200 as mb
+
+    g = torch.Generator(device=cuda).manual_seed(0)
+    line = torch.randn(28, device=cuda, generator=g).bfloat16()
+    x = line.unfold(0, 9, 1)
+    w = 1 + torch.rand(9, device=cuda, generator=g)
+    xl = x.detach().requires_grad_(True)
+    y = mb.block_norm(xl, w)
+    d = x.double().requires_grad_(True)
+    want = norm.plain(d, w.double(), None, None, None, None, 1, 1e-5, False)
+    norm.close(y, want, norm.TOL[torch.bfloat16], "y")
+    dy = torch.randn(20, 9, device=cuda, generator=g).bfloat16()
+    got = torch.autograd.grad(y, xl, dy)[0]
+    norm.close(got, torch.autograd.grad(want, d, dy.double())[0], norm.TOL[torch.bfloat16], "dx")
