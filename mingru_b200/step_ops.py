@@ -138,6 +138,8 @@ def linear_attention_step(q, k, v, log_gamma, H_prev, out=None):
             raise ValueError(f"{op}: log_gamma must broadcast to {shape[:2]} (got "
                              f"{tuple(lg.shape)})") from None
     H_prev = H_prev.contiguous()
+    if 0 < abs(H_prev.data_ptr() - out.data_ptr()) < 4 * out.numel():
+        H_prev = H_prev.clone()  # out lies over a part of it: in place is every element on itself
     y = torch.empty_like(v)
     _run(op, _lib.load().mgs_linear_attn_step, q.device, _p(q), _p(k), _p(v), _p(lg), lg.stride(0),
          lg.stride(1), _p(H_prev), _p(y), _p(out), B, nH, dk, dv, _dtype_code(op, q))

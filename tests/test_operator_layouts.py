@@ -86,3 +86,24 @@ def test_outputs_of_attention_are_dense_rows(x, monkeypatch):
     assert _one_place_each(y) and _one_place_each(HT)
     for g in attn_ops._gradients(x, x, x, lg, saved, y, None, True):
         assert _one_place_each(g)
+
+
+def test_step_reads_no_state_that_it_is_writing(monkeypatch):
+    """A buffer that lies over a part of H_prev: the kernel gets a copy; in place it gets the one buffer."""
+    from mingru_b200 import step_ops
+
+    got = []
+    monkeypatch.setattr(step_ops, "_require_cuda", lambda *a: None)
+    monkeypatch.setattr(step_ops._lib, "load", lambda: type("L", (), {"mgs_linear_attn_step": None}))
+    monkeypatch.setattr(step_ops, "_run", lambda op, fn, dev, *a: got.append((a[6], a[8])))
+    q, lg = torch.zeros(2, 3, 4), torch.zeros(2, 3)
+    n = 2 * 3 * 4 * 4
+    line = torch.zeros(2 * n)
+    state = lambda i: line[i:i + n].view(2, 3, 4, 4)  # noqa: E731
+    for prev, out in ((state(0), state(16)), (state(16), state(0)), (state(1), state(0)), (state(0), state(n - 1))):
+        step_ops.linear_attention_step(q, q, q, lg, prev, out=out)
+        a, b = got.pop()
+        assert b == out.data_ptr() and abs(a - b) >= 4 * n
+    for prev, out in ((state(0), state(0)), (state(0), state(n)), (state(n), state(0))):
+        step_ops.linear_attention_step(q, q, q, lg, prev, out=out)
+        assert got.pop() == (prev.data_ptr(), out.data_ptr())
