@@ -239,6 +239,13 @@ def linear_attention(
     and its ``log_gamma`` gets no gradient. The products run on the tensor
     cores over chunks of 128 tokens, so a non-finite value spreads to earlier
     tokens of its own chunk (and to all later ones, as the recurrence has it).
+
+    States, sums and the gradients of ``log_gamma`` and ``H0`` are fp32. In
+    bf16 the masked products, and the states where they meet a query, are
+    rounded once to bf16 before their second product: ``y`` and the gradients
+    of Q, K and V are off by 0.0023 of their norm, where an fp32 computation
+    rounded at the end is off by 0.0017. fp16 and fp32 inputs are held to 16
+    and 24 bits throughout; pass those for more.
     """
     if Q.ndim != 4 or K.ndim != 4 or V.ndim != 4:
         raise ValueError(

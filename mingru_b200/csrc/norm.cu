@@ -271,8 +271,6 @@ __global__ void __launch_bounds__(MAXT, fwd_ctas(MAXT)) fwd_kernel(const Args p)
     if (p.res && p.gate) ldrow<E, VEC, K>(p.gate, row * p.ldgate + col, at.t, p.tpg, p.n, a);
     const long long o = row * p.D + col;
     if (p.h) strow<E, VEC, K>(p.h, o, at.t, p.tpg, p.n, h);
-    // The fp32 mean is off by up to half a unit of its last place: what it leaves in the
-    // differences, `rest`, is their own mean, and comes with the sum of their squares.
     float mean = 0.f, rest = 0.f, sq = 0.f;
     if (p.rms) {
 #pragma unroll
