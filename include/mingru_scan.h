@@ -168,11 +168,15 @@ int mgs_log_scan_bwd_fixup(const void* log_coeffs, const void* log_values, const
  * Returns MGS_UNSUPPORTED for shapes that do not take that path. Outputs of
  * the first tile are left unwritten.
  * mgs_test_mbarrier_timeout: one CTA waits on an mbarrier nothing arrives on;
- * `err_word` (device u32) receives the bit.                                   */
+ * `err_word` (device u32) receives the bit.
+ * mgs_test_linear_attn_timeout: the same in linear attention's library part,
+ * which has a sticky word of its own, by a CTA that holds tensor memory and
+ * leaves as its kernels do.                                                   */
 int mgs_test_lookback_timeout(const void* a, const void* b, void* A, void* Bc, int64_t B,
                               int64_t T, int64_t D, void* workspace, size_t workspace_bytes,
                               int64_t spin_limit, void* stream);
 int mgs_test_mbarrier_timeout(void* err_word, int64_t spin_limit, void* stream);
+int mgs_test_linear_attn_timeout(int64_t spin_limit, void* stream);
 
 /* ------------------------------------------------------------------------ */
 /* parallel_scan_log: h_t = a_t h_{t-1} + b_t in log space, a_t =

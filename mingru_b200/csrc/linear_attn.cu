@@ -1881,6 +1881,30 @@ __global__ void __launch_bounds__(Dkv<E, D>::kThreads, Dkv<E, D>::kPerSm)
   if (warp == 0) um::dealloc(sm.tbase, F::kCols);
 }
 
+// How the kernels above leave a wait that runs out, on a barrier that nothing arrives on.
+__global__ void __launch_bounds__(256) stall_kernel(long long polls) {
+  __shared__ Small sm;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  if (warp == 0) um::alloc(&sm.tbase, 64);
+  if (tid == 0) {
+    mbar_init(&sm.bar, 1);
+    mbar_fence_init();
+  }
+  bool ok = true;
+  auto sync = [&]() {
+    um::fence_before();
+    ok = !__syncthreads_or(!ok);
+    um::fence_after();
+  };
+  sync();
+  if (tid < 32) ok = mbar_wait(&sm.bar, 0, &g_sticky_err, polls);
+  sync();  // now for all threads: the second wait is not begun
+  if (ok) ok = mbar_wait(&sm.bar, 0, &g_sticky_err, kPolls);
+  um::fence_before();
+  __syncthreads();
+  if (warp == 0) um::dealloc(sm.tbase, 64);
+}
+
 // ------------------------------------------------------------------- host --
 
 struct Plan {
@@ -2178,6 +2202,12 @@ size_t mgs_linear_attn_saved_size(int64_t B, int H, int64_t T, int dk, int dv, i
     return MGS_OK;
   });
   return n;
+}
+
+int mgs_test_linear_attn_timeout(int64_t spin_limit, void* stream) {
+  if (spin_limit < 1) return MGS_BAD_SHAPE;
+  mgs::lattn::stall_kernel<<<1, 256, 0, static_cast<cudaStream_t>(stream)>>>(spin_limit);
+  return mgs::lattn::launched();
 }
 
 int mgs_linear_attn_fwd(const void* Q, const void* K, const void* V, const float* log_gamma,
