@@ -38,14 +38,11 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _like(t: torch.Tensor) -> torch.Tensor:
-    """An output in ``t``'s memory order, its last dimension dense, as the kernels
-    write it: PyTorch puts another one innermost where it is as dense in ``t``
-    (overlapping windows, heads). Of a tensor as given or of its ``_rows``, alike."""
-    if t.stride(-1) == 1 or t.shape[-1] == 1:
-        o = torch.empty_like(t)
-        if o.stride(-1) == 1 or o.shape[-1] == 1:
-            return o
-    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    """An output in the memory order of ``t``, one of the ``_rows``, its last dimension
+    dense, as the kernels write it: PyTorch puts another one innermost where it is as
+    dense in ``t`` (overlapping windows, heads)."""
+    o = torch.empty_like(t)
+    return o if o.stride(-1) == 1 or o.shape[-1] == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _strides(*ts: torch.Tensor):
@@ -110,7 +107,7 @@ def _linear_attn_fwd(
 def _(Q, K, V, lg, H0, save):
     B, H, T, dk = Q.shape
     dv = V.shape[3]
-    return (_like(V), Q.new_empty((B, H, dk, dv), dtype=torch.float32),
+    return (_like(_rows(V)), Q.new_empty((B, H, dk, dv), dtype=torch.float32),
             Q.new_empty((_saved_floats(B, H, T, dk, dv, Q.dtype) if save else 0,), dtype=torch.float32))
 
 
@@ -156,7 +153,7 @@ def _linear_attn_bwd(
 def _(Q, K, V, lg, saved, dy, dHT, want_dH0):
     B, H, T, dk = Q.shape
     f32 = dict(dtype=torch.float32)
-    return (_like(Q), _like(K), _like(V), Q.new_empty((B, H, T), **f32),
+    return (_like(_rows(Q)), _like(_rows(K)), _like(_rows(V)), Q.new_empty((B, H, T), **f32),
             Q.new_empty((B, H, dk, V.shape[3]) if want_dH0 else (0,), **f32))
 
 

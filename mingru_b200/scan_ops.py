@@ -79,13 +79,24 @@ def raw_stream(device: torch.device) -> int:
 def _traced(*ts: torch.Tensor | None) -> bool:
     """Whether a compiler, a dispatch mode, a tensor subclass or a function transform
     is to see a call: then it goes through its custom op and not straight to the kernels."""
-    return (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
-            or torch._C._are_functorch_transforms_active()
-            or any(t is not None and type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter for t in ts))
+    if torch.compiler.is_compiling() or _modes() > 0 or _transforms():
+        return True
+    for t in ts:
+        if type(t) not in _PLAIN:
+            return True
+    return False
+
+
+_modes, _transforms = torch._C._len_torch_dispatch_stack, torch._C._are_functorch_transforms_active
+_PLAIN = (torch.Tensor, torch.nn.Parameter, type(None))
 
 
 def _wants_grad(*ts: torch.Tensor | None) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _ptr(t: torch.Tensor | None):
