@@ -19,7 +19,6 @@
 // the forward. Sums over rows stay in the threads' registers while a CTA walks
 // its rows, then go through shared memory to one partial row per CTA and, in
 // order, to the result: the same bits on every run.
-#include <algorithm>
 #include <utility>
 
 #include "common.cuh"
@@ -41,7 +40,6 @@ struct Args {
   long long rows;
   int D, G, n, tpg, gpc, rpc;  // threads to a group, groups and rows to a CTA
   int rms, w32;  // weights in fp32
-  int tail;      // odd rows: the last rows, whose vectors may pass the tensors' ends
   int staged;    // backward: the inputs that come through shared memory, a row ahead; 0: straight
   float eps;
 };
@@ -184,16 +182,20 @@ __device__ __forceinline__ float sigm(float x) {
 }
 
 // 1 / sqrt(v) to the last place, by a step of Newton's on the hardware's: the
-// gradient takes differences of z * z and 1. 0 of an infinite sum of squares (finite
-// values past 2^64), as 1 / sqrt has it; the step would make that inf * 0.
+// gradient takes differences of z * z and 1. The step of an infinite sum of squares
+// (finite values past 2^64) would be inf * 0; fminf makes it 1, and the result 0.
 __device__ __forceinline__ float inv_sqrt(float v) {
   const float r = rsqrtf(v);
-  return r == 0.f ? r : fmaf(0.5f * r, fmaf(-v * r, r, 1.f), r);
+  return fmaf(0.5f * r, fminf(fmaf(-v * r, r, 1.f), 1.f), r);
 }
 
 // A mean of squares that cancellation took below zero; NaN stays (fmaxf drops it, and
 // a row with a NaN came out finite but for that element).
-__device__ __forceinline__ float at_least_zero(float v) { return v < 0.f ? 0.f : v; }
+__device__ __forceinline__ float at_least_zero(float v) {
+  float r;
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(v));
+  return r;
+}
 
 // Where a thread stands: its group (of the row), row slot and first column.
 struct Place {
@@ -536,10 +538,10 @@ struct OddRow {
     }
   }
   // The vectors of one tensor whose group starts at element `start`: loaded whole,
-  // the neighbours' elements in them too, where the tensor goes on; and as values,
+  // the neighbours' elements in them too, where another row follows; and as values,
   // zeros outside the group.
   template <typename T>
-  __device__ __forceinline__ static void load(const void* p, long long start, bool tail, int sh, int n, int t,
+  __device__ __forceinline__ static void load(const void* p, long long start, bool last, int sh, int n, int t,
                                               int tpg, uint4 (&raw)[K]) {
     const T* q = static_cast<const T*>(p) + (start - sh) + t * V;
 #pragma unroll
@@ -547,7 +549,7 @@ struct OddRow {
       const int pos = (k * tpg + t) * V;
       raw[k] = make_uint4(0, 0, 0, 0);
       if (pos < sh + n) {
-        if (odd::whole(pos, sh + n, V, tail)) {
+        if (odd::whole(pos, sh + n, V, last)) {
           raw[k] = __ldg(reinterpret_cast<const uint4*>(q + k * tpg * V));
         } else {
           T e[V];
@@ -631,13 +633,13 @@ __global__ void __launch_bounds__(MAXT, odd_fwd_ctas(MAXT)) fwd_odd_kernel(const
   uint4 rx[K], ra[K];  // of the next row: x, and the residual or else the gate
   auto ahead = [&](long long row) {
     if (row >= p.rows) return;
-    const bool tail = row + p.tail >= p.rows;
+    const bool last = row + 1 == p.rows;
     const int sh = shift(row);
-    R::template load<E>(p.x, row * p.ldx + col, tail, sh, p.n, at.t, p.tpg, rx);
+    R::template load<E>(p.x, row * p.ldx + col, last, sh, p.n, at.t, p.tpg, rx);
     if (p.res)
-      R::template load<E>(p.res, row * p.ldres + col, tail, sh, p.n, at.t, p.tpg, ra);
+      R::template load<E>(p.res, row * p.ldres + col, last, sh, p.n, at.t, p.tpg, ra);
     else if (p.gate)
-      R::template load<E>(p.gate, row * p.ldgate + col, tail, sh, p.n, at.t, p.tpg, ra);
+      R::template load<E>(p.gate, row * p.ldgate + col, last, sh, p.n, at.t, p.tpg, ra);
   };
   ahead((long long)blockIdx.x * p.rpc + at.rs);
   for (long long row = (long long)blockIdx.x * p.rpc + at.rs; row < p.rows; row += step) {
@@ -655,7 +657,7 @@ __global__ void __launch_bounds__(MAXT, odd_fwd_ctas(MAXT)) fwd_odd_kernel(const
     }
     if (p.res && p.gate) {
       uint4 rg[K];
-      R::template load<E>(p.gate, row * p.ldgate + col, row + p.tail >= p.rows, at_row.sh, p.n, at.t, p.tpg, rg);
+      R::template load<E>(p.gate, row * p.ldgate + col, row + 1 == p.rows, at_row.sh, p.n, at.t, p.tpg, rg);
       at_row.template get<E>(rg, a);
     }
     float acc = 0.f;
@@ -719,15 +721,15 @@ __global__ void __launch_bounds__(MAXT, odd_bwd_ctas(MAXT)) bwd_odd_kernel(const
     float stats[3];
     auto ahead = [&](long long row) {
       if (row >= p.rows) return;
-      const bool tail = row + p.tail >= p.rows;
+      const bool last = row + 1 == p.rows;
       const int sh = shift(row);
-      R::template load<E>(p.x, row * p.ldx + col, tail, sh, p.n, at.t, p.tpg, rx);
-      R::template load<E>(p.dy, row * p.lddy + col, tail, sh, p.n, at.t, p.tpg, rd);
+      R::template load<E>(p.x, row * p.ldx + col, last, sh, p.n, at.t, p.tpg, rx);
+      R::template load<E>(p.dy, row * p.lddy + col, last, sh, p.n, at.t, p.tpg, rd);
       if (GATE)
-        R::template load<E>(p.gate, row * p.ldgate + col, tail, sh, p.n, at.t, p.tpg, ra);
+        R::template load<E>(p.gate, row * p.ldgate + col, last, sh, p.n, at.t, p.tpg, ra);
       else if (SCALE || p.res)
-        R::template load<E>(p.res, row * p.ldres + col, tail, sh, p.n, at.t, p.tpg, ra);
-      if (p.dh) R::template load<E>(p.dh, row * p.lddh + col, tail, sh, p.n, at.t, p.tpg, rh);
+        R::template load<E>(p.res, row * p.ldres + col, last, sh, p.n, at.t, p.tpg, ra);
+      if (p.dh) R::template load<E>(p.dh, row * p.lddh + col, last, sh, p.n, at.t, p.tpg, rh);
 #pragma unroll
       for (int i = 0; i < 3; ++i) stats[i] = p.stats[(row * p.G + at.g) * 3 + i];
     };
@@ -750,7 +752,7 @@ __global__ void __launch_bounds__(MAXT, odd_bwd_ctas(MAXT)) bwd_odd_kernel(const
       if (SCALE || p.res) {
         if (GATE) {
           uint4 rr[K];
-          R::template load<E>(p.res, row * p.ldres + col, row + p.tail >= p.rows, at_row.sh, p.n, at.t, p.tpg, rr);
+          R::template load<E>(p.res, row * p.ldres + col, row + 1 == p.rows, at_row.sh, p.n, at.t, p.tpg, rr);
           at_row.template get<E>(rr, z);
         }
         if constexpr (SCALE) {
@@ -983,7 +985,8 @@ bool shape_ok(int64_t rows, int64_t D, int groups) {
 
 // How a call's rows can be read: whole 16-byte vectors everywhere (addresses, row
 // strides, group starts); vectors of memory with the columns shifted from row to
-// row, where that shift is the same for all tensors; or element by element.
+// row, where that shift is the same for all tensors and nothing past their ends is
+// read; or element by element.
 Way way_of(const Args& a, int size, int wsize) {
   const int v = 16 / size;
   bool vec = a.n % v == 0 && (long long)a.n * wsize % 16 == 0, odd = true;
@@ -997,7 +1000,7 @@ Way way_of(const Args& a, int size, int wsize) {
                        std::pair(a.dy, a.lddy), std::pair(a.dh, a.lddh)})
     if (q) {
       vec = vec && ld % v == 0;
-      odd = odd && ld % v == out;
+      odd = odd && ld % v == out && (a.rows == 1 || odd::steps_far_enough(ld, v));
     }
   vec = vec && (out == 0 || a.rows == 1);
   return vec ? kVectors : odd ? kOdd : kElements;
@@ -1010,12 +1013,7 @@ bool plan_call(Plan& pl, const Args& a, int size, int wsize, bool fwd) {
          make_plan(pl, a.rows, a.D, a.G, size, kElements, fwd, weights);
 }
 
-void set_plan(Args& a, const Plan& pl) {
-  a.tpg = pl.tpg, a.gpc = pl.gpc, a.rpc = pl.rpc, a.tail = 1;
-  for (auto [q, ld] : {std::pair(a.x, a.ldx), std::pair(a.res, a.ldres), std::pair(a.gate, a.ldgate),
-                       std::pair(a.dy, a.lddy), std::pair(a.dh, a.lddh)})
-    if (q) a.tail = std::max(a.tail, odd::tail_rows(ld, pl.vec));
-}
+void set_plan(Args& a, const Plan& pl) { a.tpg = pl.tpg, a.gpc = pl.gpc, a.rpc = pl.rpc; }
 
 int launched() { return cudaGetLastError() == cudaSuccess ? MGS_OK : MGS_LAUNCH_FAILED; }
 

@@ -21,17 +21,18 @@ int main() {
     for (int D = 1; D <= 41; ++D)
       for (long long ld = 0; ld <= 2 * D + 16; ++ld) {
         if (ld % v != D % v) continue;  // what the kernels take as odd rows
-        for (int rows : {1, 2, 3, 9, 37})
+        for (int rows : {1, 2, 3, 9, 37}) {
+          if (rows > 1 && !mgs::odd::steps_far_enough(ld, v)) continue;  // read element by element
           for (int groups = 1; groups <= D; ++groups) {
             if (D % groups) continue;
-            const int n = D / groups, tail = mgs::odd::tail_rows(ld, v);
+            const int n = D / groups;
             const long long extent = (rows - 1) * ld + D;
             for (int r = 0; r < rows; ++r)
               for (int g = 0; g < groups; ++g) {
                 const long long start = r * ld + g * n;
                 const int sh = (int)(start & (v - 1));
                 for (int pos = 0; pos < sh + n; pos += v) {
-                  const bool all = mgs::odd::whole(pos, sh + n, v, r + tail >= rows);
+                  const bool all = mgs::odd::whole(pos, sh + n, v, r + 1 == rows);
                   const long long first = start - sh + pos, end = all ? first + v : start + n;
                   ++loads;
                   if (first < 0 || end > extent) {
@@ -42,6 +43,7 @@ int main() {
                 }
               }
           }
+        }
       }
   std::printf("%lld\\n", loads);
   return loads > 100000 ? 0 : 2;
