@@ -439,7 +439,7 @@ int mgs_linear_attn_bwd(const void* Q, const void* K, const void* V, const float
 /* One token of linear attention for every (b, head): S = exp(log_gamma) S_prev
  * + k v^T, y = S^T q. q, k (B, H, dk), v, y (B, H, dv) op dtype and S, S_prev
  * (B, H, dk, dv) fp32, C-contiguous; log_gamma fp32 with the given batch and
- * head strides. S may be S_prev. */
+ * head strides. S may be S_prev, but not lie over a part of it. */
 int mgs_linear_attn_step(const void* q, const void* k, const void* v, const float* log_gamma,
                          int64_t lg_stride_b, int64_t lg_stride_h, const float* S_prev, void* y, float* S,
                          int64_t B, int heads, int dk, int dv, int dtype, void* stream);
