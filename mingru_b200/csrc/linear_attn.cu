@@ -884,8 +884,9 @@ __global__ void __launch_bounds__(256) scan_kernel(float* seg, const float* segl
 // A segment, chunk by chunk: P = D * Q K^T in TMEM, y = P V + decayed Q S, then S for
 // the next chunk, whose sum over the scaled K rows runs during P's masking and whose
 // tiles load meanwhile. Bound by that chain, with two CTAs to an SM (bf16 heads of 64)
-// to fill it; one level of P where the output is 16 bits: its rounding is of the size
-// of the output's. 64 heads, T = 8192, bf16: 86 us, 3.1 TB/s, 8 heads, T = 65536: 70;
+// to fill it; one level of P, and of S as an operand, where the output is 16 bits: each
+// rounding is of the size of the output's (bf16 errors of 0.0023 for 0.0017), and a second
+// level of either, 64 TMEM columns or 8 KB, would leave one CTA to an SM. 64 heads, T = 8192, bf16: 86 us, 3.1 TB/s, 8 heads, T = 65536: 70;
 // heads of 128 (16, T = 4096): 43; fp32 (64 heads, T = 1024, 512 threads and one CTA
 // to an SM): 52, where three levels make each product six. 512 threads at 64
 // registers with two CTAs to an SM took 115.
@@ -1455,7 +1456,8 @@ template <typename E, int D>
 struct Dkv {
   static constexpr int NL = kLevels<E>, kTileE = kC * D;
   // Two CTAs to an SM: dS is spread over all threads, and one tile more holds the
-  // decayed K rows, so that dV's state part adds up in dV's own accumulator.
+  // decayed K rows, so that dV's state part adds up in dV's own accumulator. One
+  // level of these rows and two of dS: they end in dV's 16 bits alone.
   static constexpr bool kE = NL == 1 && D == 64;
   static constexpr int kA1 = NL == 1 ? 128 : 64 * NL;
   static constexpr int kDv = kE ? 32 : NL == 1 ? 256 : 128 * NL, kDk = kE ? 160 : kDv + D;
