@@ -39,7 +39,7 @@ import torch.nn.functional as F
 
 from . import step_ops
 from .attn_ops import linear_attention
-from .norm_ops import block_norm
+from .norm_ops import MAX_GROUP, block_norm
 from .scan_ops import (
     angle_scan_impl,
     brickwall_meta,
@@ -618,8 +618,8 @@ def _is_plain(m, cls):
 
 def _add_norm(x, branch, norm):
     """``(norm(x + branch), x + branch)`` by one kernel; ``branch`` may be ``None``.
-    A norm that is more than a LayerNorm is called as it is."""
-    if not _is_plain(norm, nn.LayerNorm) or norm.weight is None:
+    A norm that is more than a LayerNorm, or wider than the kernel's, is called as it is."""
+    if not _is_plain(norm, nn.LayerNorm) or norm.weight is None or x.shape[-1] > MAX_GROUP:
         x = x if branch is None else x + branch
         return norm(x), x
     dtype = x.dtype if branch is None else torch.promote_types(x.dtype, branch.dtype)  # the sum's

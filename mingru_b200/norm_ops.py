@@ -20,6 +20,7 @@ from .scan_ops import (_dense, _dtype_code, _ptr, _require_cuda, _traced, _wants
 __all__ = ["block_norm"]
 
 _OP = "block_norm"
+MAX_GROUP = 16384  # channels of a group that the kernels take
 
 
 def _rows(t: torch.Tensor | None, D: int):

@@ -144,3 +144,21 @@ def test_modules_pickled_before_the_option():
         del m.__dict__["fused_norms"]
     old = copy.deepcopy(stack)
     assert not old.fused_norms and not old.blocks[0].fused_norms
+
+
+def test_rows_beyond_the_kernels(monkeypatch):
+    """block_norm takes up to 16384 channels; wider streams keep the norm's own call."""
+    from mingru_b200 import modules
+
+    def refuse(x, *a, **kw):
+        assert x.shape[-1] <= 16384, "MGS_UNSUPPORTED"
+        return x if kw.get("residual") is None else (x, x)
+
+    monkeypatch.setattr(modules, "block_norm", refuse)
+    for D in (16384, 16385):
+        norm, x = nn.LayerNorm(D), torch.randn(2, D)
+        y, h = modules._add_norm(x, x, norm)
+        if D > 16384:
+            torch.testing.assert_close(y, norm(x + x))
+            torch.testing.assert_close(h, x + x)
+        modules._add_norm(x, None, norm)
